@@ -217,6 +217,78 @@ int dmh_adamw_step(dmh_stream_t stream, const dmh_adamw_param* table, int count,
                    const int* chunk_start, int nchunks, float w1, float w2, float eps,
                    float decay, float alpha);
 
+/* ---- training operators beside the optimizer -------------------------------------
+ * What a GPT-2 training step computes outside its matrix products and the optimizer: the
+ * embedding and its gradient, dropout, and the loss.  No counterpart in the reference, whose
+ * training loop takes them from torch.
+ *
+ * dtype codes: 0 fp32, 1 bf16, 2 fp16.  Computed in fp32, rounded once.  Rows are contiguous;
+ * strides between them are in elements and may be any that is not negative.  Row widths and
+ * addresses need the element's alignment alone.
+ *
+ * Dropout: element e of the output (flat index) takes half (e & 1) of word (e >> 1) & 3 of
+ * the Philox4x32-10 block with counter (e >> 3, offset) and key seed, low words first; it is
+ * kept if these 16 bits are at least `cut` (0 .. 65536), and then scaled by
+ * 65536 / (65536 - cut).  rng_state: {seed, offset} as two int64 in device memory, read when
+ * the kernel runs, instead of the arguments (a captured graph draws a new mask at each
+ * replay); NULL for none.
+ *
+ * dmh_dropout: out = dropout(x) [+ residual], (rows, cols); the residual has out's type, out
+ * is contiguous.  The gradient of x is the same call on out's gradient, without residual. */
+int dmh_dropout(dmh_stream_t stream, const void* x, int x_dtype, long long rows, long long cols,
+                long long x_rstride, const void* residual, long long res_rstride, void* out,
+                int out_dtype, int cut, unsigned long long seed, unsigned long long offset,
+                const void* rng_state);
+
+/* out[i, :] = dropout(scale * weight[ids[i], :] + pos_weight[pos_i, :]) over `tokens` rows of
+ * `dim`; pos_i = positions[i], or i % seq where positions is NULL; pos_weight NULL for none.
+ * ids and positions are int64 (ids_64) or int32.  Both tables have `dtype`.  An id or position
+ * outside its table gives a row of NaN.  out is contiguous. */
+int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long tokens, int seq,
+                  const void* weight, int dtype, long long vocab, int dim, long long w_rstride,
+                  const void* pos_weight, long long pos_rows, long long p_rstride,
+                  const void* positions, float scale, int cut, unsigned long long seed,
+                  unsigned long long offset, const void* rng_state, void* out, int out_dtype);
+
+/* The gradient of a table of `rows` rows: out[v, :] (+)= scale * sum over i with ids[i] = v of
+ * dropout(grad)[i, :], summed in fp32 in an order that the ids alone decide.  ids NULL:
+ * ids[i] = i % seq (a position table).  Every row of out is written, those of ids that do not
+ * occur with zero; with `accumulate` the sums are added to what out holds and other rows stay
+ * untouched.  padding_idx (-1: none) and ids outside the table take no gradient.
+ * tokens, rows < 2^31 - 65536. */
+int dmh_embedding_grad_workspace_size(long long tokens, long long rows, int dim, size_t* bytes);
+int dmh_embedding_grad(dmh_stream_t stream, const void* ids, int ids_64, long long tokens,
+                       int seq, const void* grad, int dtype, long long g_rstride,
+                       long long rows, int dim, long long padding_idx, float scale, int cut,
+                       unsigned long long seed, unsigned long long offset,
+                       const void* rng_state, void* out, int out_dtype, int accumulate,
+                       void* ws, size_t ws_bytes);
+
+/* Cross entropy of logits (rows, classes) against targets (int64 if targets_64, else int32):
+ *   lse = log sum exp z;  loss = lse - (1 - s) z_y - s mean(z) + z_loss lse^2
+ * with s the label smoothing.  Rows whose target is ignore_index count for nothing and get a
+ * gradient of zero; other targets outside [0, classes) give NaN.
+ *   reduction  0 none: loss has `rows` values; 1 mean over the rows that have a target (their
+ *              number goes to `count`); 2 sum
+ *   lse        (rows), kept for dmh_cross_entropy_grad; may be NULL
+ *   dlogits    the gradient of grad_scale * loss (of the sum, for reduction 0), in the
+ *              logits' type; may be the logits themselves; NULL for the loss alone
+ * dmh_cross_entropy_grad: the gradient from a forward call's lse (and count, for a mean; NULL
+ * otherwise), times *grad_out, or grad_out[row] if grad_out_rows.
+ * 1 <= classes < 2^31 - 65536, rows < 2^23. */
+int dmh_cross_entropy_workspace_size(long long rows, long long classes, size_t* bytes);
+int dmh_cross_entropy(dmh_stream_t stream, const void* logits, int dtype, long long rows,
+                      long long classes, long long z_rstride, const void* targets,
+                      int targets_64, long long ignore_index, float smoothing, float z_loss,
+                      int reduction, float grad_scale, float* loss, float* count, float* lse,
+                      void* dlogits, long long d_rstride, void* ws, size_t ws_bytes);
+int dmh_cross_entropy_grad(dmh_stream_t stream, const void* logits, int dtype, long long rows,
+                           long long classes, long long z_rstride, const void* targets,
+                           int targets_64, long long ignore_index, float smoothing,
+                           float z_loss, const float* lse, const float* count,
+                           const float* grad_out, int grad_out_rows, void* dlogits,
+                           long long d_rstride);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,7 @@ _lib = None
 
 c_int, c_ll, c_sz, c_vp, c_float = (ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t,
                                     ctypes.c_void_p, ctypes.c_float)
+c_ull = ctypes.c_ulonglong
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -66,6 +67,21 @@ _SIGS = {
     "dmh_adamw_chunks": (c_int, [c_ll]),
     "dmh_adamw_step": (c_int, [c_vp, c_vp, c_int, c_vp, c_int, c_float, c_float, c_float,
                                c_float, c_float]),
+    "dmh_dropout": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_ll, c_vp, c_int, c_int,
+                            c_ull, c_ull, c_vp]),
+    "dmh_embedding": (c_int, [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll, c_int, c_ll,
+                              c_vp, c_ll, c_ll, c_vp, c_float, c_int, c_ull, c_ull, c_vp, c_vp,
+                              c_int]),
+    "dmh_embedding_grad_workspace_size": (c_int, [c_ll, c_ll, c_int, ctypes.POINTER(c_sz)]),
+    "dmh_embedding_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll, c_ll,
+                                   c_int, c_ll, c_float, c_int, c_ull, c_ull, c_vp, c_vp, c_int,
+                                   c_int, c_vp, c_sz]),
+    "dmh_cross_entropy_workspace_size": (c_int, [c_ll, c_ll, ctypes.POINTER(c_sz)]),
+    "dmh_cross_entropy": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
+                                  c_float, c_float, c_int, c_float, c_vp, c_vp, c_vp, c_vp, c_ll,
+                                  c_vp, c_sz]),
+    "dmh_cross_entropy_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
+                                       c_float, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_ll]),
 }
 
 
@@ -431,3 +447,84 @@ def adamw_step(tab, w1, w2, eps, decay, alpha):
                                  _ptr(tab.chunks), tab.nchunks, float(w1), float(w2),
                                  float(eps), float(decay), float(alpha)),
            "dmh_adamw_step")
+
+
+# ---- training operators (their checks of arguments are train_ops') --------------------------
+# element types of the training operators and their codes (include/defmuon_hip.h)
+FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def dropout(x, residual, out, cut, rng, rows):
+    """out = dropout(x) [+ residual]; rows: (rows, cols, x's row stride, the residual's)."""
+    n, cols, xs, rs = rows
+    seed, offset, state = rng
+    _check(load().dmh_dropout(_stream(x.device), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
+                              0 if residual is None else residual.data_ptr(), rs,
+                              out.data_ptr(), FLOATS[out.dtype], cut, seed, offset, state),
+           "dmh_dropout")
+
+
+def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
+    """Token rows times scale plus position rows through dropout into out (tokens, dim)."""
+    seed, offset, state = rng
+    vocab, dim = weight.shape
+    seq = ids.shape[-1] if ids.ndim else 1
+    pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr(), pos_weight.shape[0],
+                                                pos_weight.stride(0))
+    _check(load().dmh_embedding(_stream(weight.device), ids.data_ptr(),
+                                ids.dtype == torch.int64, ids.numel(), seq, weight.data_ptr(),
+                                FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
+                                0 if positions is None else positions.data_ptr(), scale, cut,
+                                seed, offset, state, out.data_ptr(), FLOATS[out.dtype]),
+           "dmh_embedding")
+
+
+def embedding_grad(ids, tokens, seq, grad, gstride, padding_idx, scale, cut, rng, out,
+                   accumulate):
+    """The gradient of a table, out (rows, dim); ids None: i % seq."""
+    seed, offset, state = rng
+    rows, dim = out.shape
+    lib = load()
+    nbytes = c_sz()
+    _check(lib.dmh_embedding_grad_workspace_size(tokens, rows, dim, ctypes.byref(nbytes)),
+           "dmh_embedding_grad_workspace_size")
+    ws = _workspace(nbytes.value, out.device)
+    _check(lib.dmh_embedding_grad(_stream(out.device), 0 if ids is None else ids.data_ptr(),
+                                  ids is not None and ids.dtype == torch.int64, tokens, seq,
+                                  grad.data_ptr(), FLOATS[grad.dtype], gstride, rows, dim,
+                                  padding_idx, scale, cut, seed, offset, state, out.data_ptr(),
+                                  FLOATS[out.dtype], accumulate, ws.data_ptr(), nbytes.value),
+           "dmh_embedding_grad")
+
+
+def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
+                  count, lse, dlogits, dstride):
+    """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
+    stride) of the logits."""
+    n, classes, zs = rows
+    lib = load()
+    nbytes = 4 * n
+    ws = _workspace(nbytes, logits.device) if reduction else None
+    _check(lib.dmh_cross_entropy(_stream(logits.device), logits.data_ptr(),
+                                 FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
+                                 targets.dtype == torch.int64, ignore, smoothing, z_loss,
+                                 reduction, grad_scale, loss.data_ptr(),
+                                 0 if count is None else count.data_ptr(),
+                                 0 if lse is None else lse.data_ptr(),
+                                 0 if dlogits is None else dlogits.data_ptr(), dstride,
+                                 0 if ws is None else ws.data_ptr(), nbytes),
+           "dmh_cross_entropy")
+
+
+def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, lse, count, grad_out,
+                       per_row, dlogits, dstride):
+    """The gradient of the logits from a forward pass's lse, times grad_out."""
+    n, classes, zs = rows
+    _check(load().dmh_cross_entropy_grad(_stream(logits.device), logits.data_ptr(),
+                                         FLOATS[logits.dtype], n, classes, zs,
+                                         targets.data_ptr(), targets.dtype == torch.int64,
+                                         ignore, smoothing, z_loss, lse.data_ptr(),
+                                         0 if count is None else count.data_ptr(),
+                                         grad_out.data_ptr(), per_row, dlogits.data_ptr(),
+                                         dstride),
+           "dmh_cross_entropy_grad")

@@ -1,0 +1,417 @@
+"""The operators of a GPT-2 training step beside its matrix products and the optimizer: the
+embedding with its gradient, dropout, and the loss with its gradient.
+
+    x = embedding(tokens, wte, wpe, dropout_p=0.1, rng=draw_rng())
+    x = dropout(attn(x), 0.1, draw_rng(), residual=x)
+    loss, dlogits = cross_entropy_step(logits, targets)
+    logits.backward(dlogits)
+
+fp32, bf16 and fp16 tensors; everything is computed in fp32 and rounded once.  All functions
+run through the HIP library on the current stream and synchronise nothing; there is no CPU
+fallback.  embedding, dropout and cross_entropy take part in autograd; the *_backward
+functions and cross_entropy_step are for programs that call the gradients themselves.
+Arguments that do not fit raise NativeError.
+
+Random numbers: `rng` names the mask of a dropout.  It is a pair of integers (seed, offset), or
+an int64 tensor of the two on the GPU, which is read when a kernel runs: a captured graph
+draws a new mask at each replay if the program changes the tensor between its replays (after
+the backward pass, which reads it again).  Two calls with
+the same pair, shape and p drop the same elements, which is how the backward pass has its mask
+without storing it; calls that should differ take different pairs (draw_rng).  p is taken to
+the nearest 1/65536, and kept elements are scaled by the reciprocal of exactly that.  A dropped
+element is replaced by zero, also where it is not finite.
+"""
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from defmuon_amd import _native
+from defmuon_amd._native import FLOATS, NativeError
+
+__all__ = ["embedding", "embedding_backward", "dropout", "dropout_backward", "Dropout",
+           "draw_rng", "cross_entropy", "cross_entropy_step"]
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_NO_RNG = (0, 0, 0)
+
+
+# ---- arguments ------------------------------------------------------------------------------
+
+def _float(t, what, name):
+    if not t.is_cuda:
+        raise NativeError(f"{what}: the HIP path needs a GPU tensor ({name} is on {t.device})")
+    if t.dtype not in FLOATS:
+        raise NativeError(f"{what}: {name} must be fp32, bf16 or fp16, not {t.dtype}")
+
+
+def _ints(t, device, what, name):
+    if t.device != device:
+        raise NativeError(f"{what}: {name} is on {t.device}, not on {device}")
+    if t.dtype not in (torch.int64, torch.int32):
+        raise NativeError(f"{what}: {name} must be int64 or int32, not {t.dtype}")
+
+
+def _out_type(dtype, what):
+    if dtype not in FLOATS:
+        raise NativeError(f"{what}: the result's type must be fp32, bf16 or fp16, not {dtype}")
+
+
+def _rows(t):
+    """(tensor, rows, columns, row stride) of a tensor taken as rows of its last dimension; a
+    copy where its rows are not contiguous or not evenly spaced."""
+    cols = t.shape[-1] if t.ndim else 1
+    rows = t.numel() // cols if cols else 0
+    if t.is_contiguous():
+        return t, rows, cols, cols
+    if t.stride(-1) == 1 or cols == 1:
+        stride = inner = None
+        for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if stride is None:
+                stride, inner = st, st * size
+            elif st == inner:
+                inner = st * size
+            else:
+                break
+        else:
+            return t, rows, cols, cols if stride is None else stride
+    return t.contiguous(), rows, cols, cols
+
+
+def _drop(p, rng, device, what):
+    """(cut, (seed, offset, state address)) of a dropout."""
+    if not 0.0 <= p <= 1.0:
+        raise NativeError(f"{what}: p must be between 0 and 1, not {p}")
+    cut = int(round(p * 65536))
+    if cut == 0:
+        return 0, _NO_RNG
+    if isinstance(rng, torch.Tensor):
+        if (rng.device != device or rng.dtype != torch.int64 or rng.shape != (2,)
+                or not rng.is_contiguous()):
+            raise NativeError(f"{what}: rng must be two int64 on {device}")
+        return cut, (0, 0, rng.data_ptr())
+    try:
+        seed, offset = rng
+        return cut, (int(seed) & (1 << 64) - 1, int(offset) & (1 << 64) - 1, 0)
+    except (TypeError, ValueError):
+        raise NativeError(f"{what}: dropout needs rng=(seed, offset), got {rng!r}") from None
+
+
+def draw_rng():
+    """A fresh (seed, offset) from torch's CPU generator: torch.manual_seed fixes it, and
+    activation checkpointing draws the same one again when it repeats a forward pass."""
+    return tuple(torch.randint(-1 << 63, (1 << 63) - 1, (2,)).tolist())
+
+
+# ---- dropout --------------------------------------------------------------------------------
+
+def _dropout(x, residual, cut, rng, dtype):
+    out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    if out.numel():
+        x, rows, cols, stride = _rows(x)
+        rstride = 0
+        if residual is not None:
+            residual, _, _, rstride = _rows(residual)
+        _native.dropout(x, residual, out, cut, rng, (rows, cols, stride, rstride))
+    return out
+
+
+class _Dropout(Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, rng):
+        ctx.p, ctx.rng, ctx.dtype = p, rng, x.dtype
+        cut, key = _drop(p, rng, x.device, "dropout")
+        return _dropout(x, residual, cut, key, x.dtype if residual is None else residual.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = dropout_backward(grad, ctx.p, ctx.rng, ctx.dtype)
+        return dx, grad if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(x, p, rng, residual=None):
+    """Dropout of x, plus `residual` (same shape; the result then has its type)."""
+    _float(x, "dropout", "x")
+    if residual is not None:
+        _float(residual, "dropout", "residual")
+        if residual.shape != x.shape or residual.device != x.device:
+            raise NativeError(f"dropout: residual is {tuple(residual.shape)} on "
+                              f"{residual.device}, x {tuple(x.shape)} on {x.device}")
+    cut, key = _drop(p, rng, x.device, "dropout")
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or residual is not None and residual.requires_grad):
+        return _Dropout.apply(x, residual, p, rng)
+    return _dropout(x, residual, cut, key, x.dtype if residual is None else residual.dtype)
+
+
+def dropout_backward(grad, p, rng, dtype=None):
+    """The gradient of dropout's x (in `dtype`, the gradient's own by default); that of its
+    residual is `grad` itself."""
+    _float(grad, "dropout_backward", "grad")
+    dtype = dtype or grad.dtype
+    _out_type(dtype, "dropout_backward")
+    return _dropout(grad, None, *_drop(p, rng, grad.device, "dropout_backward"), dtype)
+
+
+class Dropout(torch.nn.Module):
+    """Dropout and an optional residual's addition; a mask of its own at each call in training,
+    x (+ residual) in evaluation."""
+
+    def __init__(self, p=0.1):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise NativeError(f"Dropout: p must be between 0 and 1, not {p}")
+        self.p = p
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+    def forward(self, x, residual=None):
+        p = self.p if self.training else 0.0
+        if p == 0.0 and residual is None:
+            return x
+        return dropout(x, p, draw_rng() if p else None, residual)
+
+
+# ---- embedding ------------------------------------------------------------------------------
+
+def _table(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _positions(positions, ids, what):
+    if positions is None:
+        return None
+    _ints(positions, ids.device, what, "positions")
+    if positions.shape != ids.shape:
+        raise NativeError(f"{what}: positions are {tuple(positions.shape)}, ids "
+                          f"{tuple(ids.shape)}")
+    return positions.to(ids.dtype).contiguous()
+
+
+def _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype):
+    out = torch.empty((*ids.shape, weight.shape[1]), dtype=dtype, device=weight.device)
+    if out.numel():
+        _native.embedding(ids.contiguous(), _table(weight),
+                          None if pos_weight is None else _table(pos_weight), positions, scale,
+                          cut, key, out)
+    return out
+
+
+class _Embedding(Function):
+    @staticmethod
+    def forward(ctx, weight, pos_weight, ids, positions, scale, padding_idx, p, rng, dtype):
+        ctx.save_for_backward(ids, positions)
+        ctx.args = scale, padding_idx, p, rng
+        ctx.weight = weight.shape[0], weight.dtype
+        ctx.pos = None if pos_weight is None else (pos_weight.shape[0], pos_weight.dtype)
+        cut, key = _drop(p, rng, weight.device, "embedding")
+        return _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        ids, positions = ctx.saved_tensors
+        scale, padding_idx, p, rng = ctx.args
+        need_w, need_p = ctx.needs_input_grad[:2]
+        dw, dp = embedding_backward(
+            grad, ids, ctx.weight[0] if need_w else 0, pos_rows=ctx.pos[0] if need_p else 0,
+            positions=positions, scale=scale, padding_idx=padding_idx if need_w else None,
+            dropout_p=p, rng=rng, dtype=ctx.weight[1])
+        return dw if need_w else None, dp if need_p else None, *[None] * 7
+
+
+def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_idx=None,
+              dropout_p=0.0, rng=None, out_dtype=None):
+    """dropout(scale * weight[ids] + pos_weight[positions]): (*ids.shape, dim).
+
+    ids: int64 or int32; positions: of ids' shape, by default the index along its last
+    dimension.  The tables have one type; out_dtype is theirs by default.  padding_idx takes no
+    gradient.  An id or position outside its table gives a row of NaN."""
+    what = "embedding"
+    _float(weight, what, "weight")
+    if weight.ndim != 2:
+        raise NativeError(f"{what}: weight must be (rows, dim), got {tuple(weight.shape)}")
+    _ints(ids, weight.device, what, "ids")
+    positions = _positions(positions, ids, what)
+    if pos_weight is None:
+        if positions is not None:
+            raise NativeError(f"{what}: positions without a position table")
+    else:
+        if (pos_weight.ndim != 2 or pos_weight.shape[1] != weight.shape[1]
+                or pos_weight.dtype != weight.dtype or pos_weight.device != weight.device):
+            raise NativeError(f"{what}: the position table {tuple(pos_weight.shape)} "
+                              f"{pos_weight.dtype} does not fit {tuple(weight.shape)} "
+                              f"{weight.dtype}")
+        if positions is None and (ids.ndim < 1 or ids.shape[-1] > pos_weight.shape[0]):
+            raise NativeError(f"{what}: ids {tuple(ids.shape)} have more positions than the "
+                              f"table's {pos_weight.shape[0]}")
+    _padding(padding_idx, weight.shape[0], what)
+    dtype = out_dtype or weight.dtype
+    _out_type(dtype, what)
+    cut, key = _drop(dropout_p, rng, weight.device, what)
+    if torch.is_grad_enabled() and (weight.requires_grad
+                                    or pos_weight is not None and pos_weight.requires_grad):
+        return _Embedding.apply(weight, pos_weight, ids, positions, scale, padding_idx,
+                                dropout_p, rng, dtype)
+    return _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype)
+
+
+def _padding(padding_idx, rows, what):
+    if padding_idx is not None and not 0 <= padding_idx < rows:
+        raise NativeError(f"{what}: padding_idx {padding_idx} is not one of {rows} rows")
+
+
+def _table_grad(given, rows, dim, dtype, device, what, name):
+    """(tensor, add to it) for the gradient of a table."""
+    if given is None:
+        return torch.empty((rows, dim), dtype=dtype, device=device), False
+    _float(given, what, name)
+    if given.shape != (rows, dim) or given.device != device or not given.is_contiguous():
+        raise NativeError(f"{what}: {name} must be contiguous ({rows}, {dim}) on {device}, got "
+                          f"{tuple(given.shape)} on {given.device}")
+    return given, True
+
+
+def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, padding_idx=None,
+                       dropout_p=0.0, rng=None, dtype=torch.float32, weight_grad=None,
+                       pos_grad=None):
+    """The gradients (rows, dim) and (pos_rows, dim) of embedding's tables from that of its
+    result; None for a table of 0 rows.
+
+    Dense, in `dtype`; or added to weight_grad / pos_grad, which are then returned (the
+    gradient of a tied head, or that of the micro-batches before).  The sums are fp32, in an
+    order that the ids decide: the same inputs give the same bits."""
+    what = "embedding_backward"
+    _float(grad, what, "grad")
+    _ints(ids, grad.device, what, "ids")
+    if grad.ndim != ids.ndim + 1 or grad.shape[:-1] != ids.shape:
+        raise NativeError(f"{what}: grad {tuple(grad.shape)} does not fit ids "
+                          f"{tuple(ids.shape)}")
+    _out_type(dtype, what)
+    if rows < 0 or pos_rows < 0:
+        raise NativeError(f"{what}: {rows} and {pos_rows} rows")
+    _padding(padding_idx, rows, what)
+    positions = _positions(positions, ids, what)
+    if pos_rows and positions is None and (ids.ndim < 1 or ids.shape[-1] > pos_rows):
+        raise NativeError(f"{what}: ids {tuple(ids.shape)} have more positions than {pos_rows}")
+    cut, key = _drop(dropout_p, rng, grad.device, what)
+    dim, tokens = grad.shape[-1], ids.numel()
+    seq = ids.shape[-1] if ids.ndim else 1
+    grad, _, _, stride = _rows(grad)
+    dw = dp = None
+    if rows:
+        dw, add = _table_grad(weight_grad, rows, dim, dtype, grad.device, what, "weight_grad")
+        _native.embedding_grad(ids.contiguous(), tokens, seq, grad, stride,
+                               -1 if padding_idx is None else padding_idx, scale, cut, key, dw,
+                               add)
+    if pos_rows:
+        dp, add = _table_grad(pos_grad, pos_rows, dim, dtype, grad.device, what, "pos_grad")
+        _native.embedding_grad(positions, tokens, seq, grad, stride, -1, 1.0, cut, key, dp, add)
+    return dw, dp
+
+
+# ---- cross entropy --------------------------------------------------------------------------
+
+def _xent_args(logits, targets, label_smoothing, z_loss, reduction, what):
+    _float(logits, what, "logits")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise NativeError(f"{what}: logits must be (..., classes), got {tuple(logits.shape)}")
+    _ints(targets, logits.device, what, "targets")
+    if targets.shape != logits.shape[:-1]:
+        raise NativeError(f"{what}: targets {tuple(targets.shape)} do not fit logits "
+                          f"{tuple(logits.shape)}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise NativeError(f"{what}: label_smoothing must be between 0 and 1, not "
+                          f"{label_smoothing}")
+    if not z_loss >= 0.0:
+        raise NativeError(f"{what}: z_loss must not be negative, got {z_loss}")
+    if reduction not in _REDUCTIONS:
+        raise NativeError(f"{what}: reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
+
+
+def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, keep_lse=False,
+          dlogits=None, grad_scale=1.0):
+    """(loss, count, lse) and, in place, dlogits."""
+    dev = logits.device
+    z, n, classes, stride = _rows(logits)
+    red = _REDUCTIONS[reduction]
+    loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
+    count = torch.empty((), dtype=torch.float32, device=dev) if red == 1 else None
+    lse = torch.empty((n,), dtype=torch.float32, device=dev) if keep_lse else None
+    if n or red:
+        _native.cross_entropy(z, (n, classes, stride), targets.contiguous(), ignore_index,
+                              smoothing, z_loss, red, grad_scale, loss, count, lse, dlogits,
+                              0 if dlogits is None else _rows(dlogits)[3])
+    return loss, count, lse
+
+
+class _CrossEntropy(Function):
+    @staticmethod
+    def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
+        loss, count, lse = _xent(logits, targets, ignore_index, smoothing, z_loss, reduction,
+                                 keep_lse=True)
+        ctx.save_for_backward(logits, targets, count, lse)
+        ctx.args = ignore_index, smoothing, z_loss, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, targets, count, lse = ctx.saved_tensors
+        ignore_index, smoothing, z_loss, reduction = ctx.args
+        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if dz.numel():
+            z, n, classes, stride = _rows(logits)
+            _native.cross_entropy_grad(z, (n, classes, stride), targets.contiguous(),
+                                       ignore_index, smoothing, z_loss, lse, count,
+                                       grad.float().contiguous(), reduction == "none", dz,
+                                       classes)
+        return dz, *[None] * 5
+
+
+def cross_entropy(logits, targets, ignore_index=-100, label_smoothing=0.0, z_loss=0.0,
+                  reduction="mean"):
+    """Cross entropy of logits (..., classes) against integer targets (...), in fp32:
+
+        lse - (1 - s) z_target - s mean(z) + z_loss lse^2,    lse = log sum exp z
+
+    with s the label smoothing; summed, averaged over the rows that have a target, or (for
+    "none") one a row.  Rows whose target is ignore_index count for nothing; another target
+    outside the classes gives NaN, as does a row of logits that are all -inf."""
+    _xent_args(logits, targets, label_smoothing, z_loss, reduction, "cross_entropy")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _CrossEntropy.apply(logits, targets, ignore_index, label_smoothing, z_loss,
+                                   reduction)
+    return _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction)[0]
+
+
+def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, z_loss=0.0,
+                       reduction="mean", grad_scale=1.0, inplace=False):
+    """(loss, dlogits) of cross_entropy ("mean" or "sum") in one pass over the logits, outside
+    autograd: each is read once and its gradient written once.
+
+    dlogits is the gradient of grad_scale * loss (1 / micro-batches, a loss scale) in the
+    logits' type; with inplace it takes the logits' own memory.  logits.backward(dlogits)
+    goes on from there."""
+    what = "cross_entropy_step"
+    logits = logits.detach()
+    _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)
+    if reduction == "none":
+        raise NativeError(f"{what}: the loss must be a mean or a sum")
+    if inplace:
+        if _rows(logits)[0] is not logits or (logits.numel() > logits.shape[-1]
+                                              and _rows(logits)[3] < logits.shape[-1]):
+            raise NativeError(f"{what}: logits of strides {tuple(logits.stride())} have no rows "
+                              "to write a gradient to")
+        dlogits = logits
+    else:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    loss, _, _ = _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction,
+                       dlogits=dlogits, grad_scale=grad_scale)
+    return loss, dlogits

@@ -1,0 +1,158 @@
+"""CPU checks of the training operators: the generator's published vectors, the host's checks
+of arguments (no kernel is launched) and how tensors are taken as rows."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import train_ref as R
+
+
+# counter, key and result: the known-answer vectors published with the generator
+@pytest.mark.parametrize("ctr,key,want", [
+    ([0, 0, 0, 0], [0, 0], [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]),
+    ([0xffffffff] * 4, [0xffffffff] * 2, [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]),
+    ([0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344], [0xa4093822, 0x299f31d0],
+     [0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1]),
+])
+def test_reference_generator_matches_its_published_vectors(ctr, key, want):
+    got = R.philox(np.array([ctr[0] | ctr[1] << 32], dtype=np.uint64), key[0] | key[1] << 32,
+                   ctr[2] | ctr[3] << 32)
+    assert got[0].tolist() == want
+
+
+def test_share_of_kept_elements():
+    # binomial(2^20, 0.9): five standard deviations are 1536
+    k = R.keep(0, 1 << 20, 0.1, (123, 4))
+    assert abs(int(k.sum()) - 0.9 * (1 << 20)) < 1536
+    assert torch.equal(k[24:1000], R.keep(24, 976, 0.1, (123, 4)))
+    assert not torch.equal(k, R.keep(0, 1 << 20, 0.1, (123, 5)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from defmuon_amd import _native
+    return _native.load()
+
+
+def test_entry_points_refuse_without_launching(lib):
+    one = ctypes.c_void_p(256)   # never read: every call below is refused on the host
+
+    def drop(**kw):
+        a = dict(x=one, xt=0, rows=2, cols=3, xs=3, res=None, rs=0, out=one, ot=0, cut=5)
+        a.update(kw)
+        return lib.dmh_dropout(None, a["x"], a["xt"], a["rows"], a["cols"], a["xs"], a["res"],
+                               a["rs"], a["out"], a["ot"], a["cut"], 1, 2, None)
+    for bad in (dict(xt=3), dict(ot=-1), dict(rows=-1), dict(cols=-1), dict(xs=-1), dict(rs=-3),
+                dict(cut=-1), dict(cut=65537), dict(x=None), dict(out=None),
+                dict(rows=1 << 40, cols=1 << 40)):
+        assert drop(**bad) == 1, bad
+        assert b"dmh_dropout" in lib.dmh_last_error()
+    assert drop(rows=0, x=None) == 0 and drop(cols=0, out=None) == 0
+
+    def embed(**kw):
+        a = dict(ids=one, tokens=4, seq=2, w=one, dt=0, vocab=9, dim=8, ws=8, pw=None, pr=0,
+                 ps=0, cut=0, out=one, ot=0)
+        a.update(kw)
+        return lib.dmh_embedding(None, a["ids"], 1, a["tokens"], a["seq"], a["w"], a["dt"],
+                                 a["vocab"], a["dim"], a["ws"], a["pw"], a["pr"], a["ps"], None,
+                                 1.0, a["cut"], 0, 0, None, a["out"], a["ot"])
+    for bad in (dict(ids=None), dict(out=None), dict(w=None), dict(tokens=-1), dict(dim=-1),
+                dict(vocab=-1), dict(dt=7), dict(ot=4), dict(cut=70000), dict(ws=-8),
+                dict(pw=one, pr=2, ps=8, seq=0), dict(tokens=(1 << 40) + 1)):
+        assert embed(**bad) == 1, bad
+        assert b"dmh_embedding" in lib.dmh_last_error()
+    assert embed(tokens=0, ids=None) == 0 and embed(dim=0, w=None) == 0
+
+    def grad(**kw):
+        a = dict(ids=one, tokens=4, seq=2, g=one, dt=0, gs=8, rows=9, dim=8, cut=0, out=one,
+                 ot=0, ws=one, nb=1 << 20)
+        a.update(kw)
+        return lib.dmh_embedding_grad(None, a["ids"], 1, a["tokens"], a["seq"], a["g"], a["dt"],
+                                      a["gs"], a["rows"], a["dim"], -1, 1.0, a["cut"], 0, 0,
+                                      None, a["out"], a["ot"], 0, a["ws"], a["nb"])
+    for bad in (dict(g=None), dict(out=None), dict(tokens=-1), dict(tokens=1 << 31),
+                dict(rows=1 << 31), dict(dim=-1), dict(dim=1 << 30), dict(dt=9), dict(ot=9),
+                dict(gs=-1), dict(cut=-2), dict(ids=None, seq=0)):
+        assert grad(**bad) == 1, bad
+        assert b"dmh_embedding_grad" in lib.dmh_last_error()
+    assert grad(nb=3) == 2 and grad(ws=None) == 2
+    assert b"workspace" in lib.dmh_last_error()
+    assert grad(rows=0, out=None) == 0 and grad(dim=0) == 0
+
+    nb = ctypes.c_size_t()
+    assert lib.dmh_embedding_grad_workspace_size(-1, 5, 8, ctypes.byref(nb)) == 1
+    assert lib.dmh_embedding_grad_workspace_size(5, 5, 8, None) == 1
+    assert lib.dmh_embedding_grad_workspace_size(0, 5, 8, ctypes.byref(nb)) == 0
+
+    def xent(**kw):
+        a = dict(z=one, dt=0, rows=2, v=5, zs=5, y=one, red=1, loss=one, count=one, ds=5, ws=one,
+                 nb=1 << 20)
+        a.update(kw)
+        return lib.dmh_cross_entropy(None, a["z"], a["dt"], a["rows"], a["v"], a["zs"], a["y"], 1,
+                                     -100, 0.0, 0.0, a["red"], 1.0, a["loss"], a["count"], None,
+                                     None, a["ds"], a["ws"], a["nb"])
+    for bad in (dict(z=None), dict(y=None), dict(loss=None), dict(count=None), dict(dt=3),
+                dict(rows=-1), dict(rows=1 << 23), dict(v=0), dict(v=1 << 31), dict(zs=-1),
+                dict(ds=-1), dict(red=3), dict(red=-1)):
+        assert xent(**bad) == 1, bad
+        assert b"dmh_cross_entropy" in lib.dmh_last_error()
+    assert xent(ws=None) == 2 and xent(nb=1) == 2
+    assert xent(rows=0, red=0) == 0
+
+    def xgrad(**kw):
+        a = dict(z=one, dt=0, rows=2, v=5, zs=5, y=one, lse=one, go=one, dz=one, ds=5)
+        a.update(kw)
+        return lib.dmh_cross_entropy_grad(None, a["z"], a["dt"], a["rows"], a["v"], a["zs"],
+                                          a["y"], 1, -100, 0.0, 0.0, a["lse"], None, a["go"], 0,
+                                          a["dz"], a["ds"])
+    for bad in (dict(z=None), dict(y=None), dict(lse=None), dict(go=None), dict(dz=None),
+                dict(dt=5), dict(rows=1 << 23), dict(v=0), dict(zs=-2), dict(ds=-2)):
+        assert xgrad(**bad) == 1, bad
+        assert b"dmh_cross_entropy_grad" in lib.dmh_last_error()
+    assert xgrad(rows=0) == 0
+    assert lib.dmh_cross_entropy_workspace_size(1, 0, ctypes.byref(nb)) == 1
+    assert lib.dmh_cross_entropy_workspace_size(1, 1, None) == 1
+
+
+def test_no_cpu_fallback():
+    from defmuon_amd import train_ops as T
+    from defmuon_amd._native import NativeError
+    x, ids = torch.randn(4, 8), torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: T.dropout(x, 0.1, (1, 2)), lambda: T.dropout_backward(x, 0.1, (1, 2)),
+                 lambda: T.embedding(ids, x), lambda: T.embedding_backward(x, ids, 5),
+                 lambda: T.cross_entropy(x, ids), lambda: T.cross_entropy_step(x, ids)):
+        with pytest.raises(NativeError, match="GPU"):
+            call()
+    with pytest.raises(NativeError):
+        T.Dropout(1.5)
+    assert T.Dropout(0.3).eval()(x) is x
+
+
+def test_tensors_as_rows():
+    from defmuon_amd.train_ops import _rows
+    x = torch.arange(240.0).view(4, 5, 12)
+    for t, rows, stride, same in [
+            (x, 20, 12, True), (x[..., :7], 20, 12, True), (x[:, ::2], 12, 24, False),
+            (x[:, 1:2, 3:], 4, 60, True), (x[::2, :, 1:], 10, 12, False),
+            (x.transpose(0, 1), 20, 12, False), (x.mT, 48, 5, False),
+            (x[0, 0].expand(4, 5, 12), 20, 0, True), (x[:1, :1], 1, 12, True),
+            (torch.ones(()).expand(3, 4), 3, 4, False), (x[..., 3:4], 20, 12, True)]:
+        r, n, cols, st = _rows(t)
+        assert (n, cols) == (rows, t.shape[-1])
+        assert (r is t) == same
+        want = t.reshape(-1, cols)
+        flat = torch.as_strided(r, (n, cols), (st, 1), r.storage_offset())
+        assert torch.equal(flat, want)
+    assert _rows(torch.empty(0, 3))[1:] == (0, 3, 3)
+    assert _rows(torch.empty(3, 0))[1] == 0
+
+
+def test_draws_follow_the_seed():
+    from defmuon_amd.train_ops import draw_rng
+    torch.manual_seed(3)
+    a, b = draw_rng(), draw_rng()
+    torch.manual_seed(3)
+    assert draw_rng() == a != b
