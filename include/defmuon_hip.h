@@ -250,18 +250,23 @@ int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long to
                   const void* positions, float scale, int cut, unsigned long long seed,
                   unsigned long long offset, const void* rng_state, void* out, int out_dtype);
 
-/* The gradient of a table of `rows` rows: out[v, :] (+)= scale * sum over i with ids[i] = v of
- * dropout(grad)[i, :], summed in fp32 in an order that the ids alone decide.  ids NULL:
- * ids[i] = i % seq (a position table).  Every row of out is written, those of ids that do not
- * occur with zero; with `accumulate` the sums are added to what out holds and other rows stay
- * untouched.  padding_idx (-1: none) and ids outside the table take no gradient.
- * tokens, rows < 2^31 - 65536. */
-int dmh_embedding_grad_workspace_size(long long tokens, long long rows, int dim, size_t* bytes);
-int dmh_embedding_grad(dmh_stream_t stream, const void* ids, int ids_64, long long tokens,
-                       int seq, const void* grad, int dtype, long long g_rstride,
-                       long long rows, int dim, long long padding_idx, float scale, int cut,
-                       unsigned long long seed, unsigned long long offset,
-                       const void* rng_state, void* out, int out_dtype, int accumulate,
+/* The gradients of both tables from that of the output, grad (tokens, dim):
+ *   out[v, :]     (+)= scale * sum over i with ids[i] = v of dropout(grad)[i, :]     (rows, dim)
+ *   pos_out[t, :] (+)= sum over i with pos_i = t of dropout(grad)[i, :]          (pos_rows, dim)
+ * summed in fp32 in an order that the ids alone decide.  NULL: that gradient is not wanted.
+ * positions NULL: pos_i = i % seq (tokens a multiple of seq).  Every row of an output is
+ * written, those that no token names with zero; with `accumulate` the sums are added to what
+ * it holds and other rows stay untouched.  padding_idx (-1: none) and ids outside a table
+ * take no gradient.  tokens < 2^27, rows < 2^29.
+ * The workspace depends on how many of the outputs are wanted through ids or positions
+ * (`sorts`, 0 .. 2; implicit positions need no sort). */
+int dmh_embedding_grad_workspace_size(long long tokens, int dim, int sorts, size_t* bytes);
+int dmh_embedding_grad(dmh_stream_t stream, const void* ids, const void* positions, int ids_64,
+                       long long tokens, int seq, const void* grad, int dtype,
+                       long long g_rstride, int dim, long long padding_idx, float scale,
+                       int cut, unsigned long long seed, unsigned long long offset,
+                       const void* rng_state, void* out, long long rows, int accumulate,
+                       void* pos_out, long long pos_rows, int pos_accumulate, int out_dtype,
                        void* ws, size_t ws_bytes);
 
 /* Cross entropy of logits (rows, classes) against targets (int64 if targets_64, else int32):

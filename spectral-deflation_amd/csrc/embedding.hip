@@ -61,49 +61,207 @@ __global__ __launch_bounds__(256) void embed_rows(EmbedArgs a) {
 }
 
 // ---- gradient -----------------------------------------------------------------------------
-// The tokens in the order of (id, index): each token's place is the number of tokens before it
-// in that order.  Ids that take no gradient (padding, outside the table) become `vocab`.
-__device__ __forceinline__ int sort_key(const void* ids, int is64, long long i, long long vocab,
-                                        long long padding) {
-  const long long id = load_index(ids, is64, i);
-  return (unsigned long long)id < (unsigned long long)vocab && id != padding ? (int)id
-                                                                               : (int)vocab;
-}
-
-constexpr int RANK_TILE = 2048;
-
-__global__ __launch_bounds__(256) void embed_rank(const void* ids, int is64, int tokens,
-                                                  long long vocab, long long padding, int* keys,
-                                                  int* order) {
-  __shared__ int tile[RANK_TILE];
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int mine = i < tokens ? sort_key(ids, is64, i, vocab, padding) : 0;
-  int before = 0;
-  for (int t0 = 0; t0 < tokens; t0 += RANK_TILE) {
-    const int n = tokens - t0 < RANK_TILE ? tokens - t0 : RANK_TILE;
-    __syncthreads();
-    for (int j = threadIdx.x; j < n; j += 256)
-      tile[j] = sort_key(ids, is64, t0 + j, vocab, padding);
-    __syncthreads();
-    for (int j = 0; j < n; ++j)
-      before += (tile[j] < mine) | ((tile[j] == mine) & (t0 + j < i));
-  }
-  if (i < tokens) {
-    keys[before] = mine;
-    order[before] = i;
-  }
-}
-
-struct EmbedGradArgs {
-  const int* keys;        // sorted; null for implicit positions (id_i = i % seq)
-  const int* order;
-  const void* g;
+// A table's gradient is a job: its tokens are put in the order of (id, index), the sorted
+// tokens are cut into chunks, and a wave adds up the rows of one chunk and 512 columns, id by
+// id.  What lies in one chunk goes straight to the table; an id that reaches over a chunk's end
+// leaves its parts in the workspace, which a last launch joins.  So the work is even however
+// the ids are distributed, every sum is taken in one order, and there are no atomics on values.
+// Rows that no token names are cleared by the workgroups of the same launch that find no id of
+// theirs in the sorted list.
+//
+// Implicit positions (i % seq) need no sort: sorted place s is token (s % batch) seq + s / batch.
+struct GradJob {
+  const void* ids;     // null: implicit positions
   void* out;
-  long long rows, gstride;
-  int tokens, seq, dim, accumulate;
+  int* keys;           // sorted ids
+  int* order;          // their tokens
+  int* keys2;          // the radix sort's other buffers
+  int* order2;
+  int* hist;
+  float* part;         // two rows of `dimp` a chunk: [0] of an id that began before the chunk,
+                       // [1] of one that begins in it and goes on
+  long long padding;
+  int rows, fill;      // table rows; clear those without tokens
+  int accumulate;
   float scale;
+  int chunks;          // of sorted tokens
+  int reduce_groups, fill_groups;   // workgroups of embed_grad
+  int spans;           // some id may reach over a chunk's end
+};
+struct GradArgs {
+  GradJob job[2];      // the token table's and the position table's
+  const void* g;
+  long long gstride;
+  int is64, tokens, seq, batch, dim, dimp, ctiles, chunk;
   Rng rng;
 };
+
+// Ids that take no gradient (padding, outside the table) sort behind all others, as `rows`.
+__device__ __forceinline__ int sort_key(const GradJob& j, int is64, long long i) {
+  const long long id = load_index(j.ids, is64, i);
+  return (unsigned long long)id < (unsigned long long)j.rows && id != j.padding ? (int)id : j.rows;
+}
+
+// Few tokens: the place of a token is the number of tokens before it in the order of (id,
+// index), counted against all of them.  A workgroup places 32 tokens; the keys lie in LDS, and
+// lane pairs of its waves take a share of them each.
+constexpr int RANK_MAX = 8192, RANK_TOKENS = 32, RANK_THREADS = 512;
+
+__global__ __launch_bounds__(RANK_THREADS) void embed_rank(GradArgs a) {
+  __shared__ __attribute__((aligned(16))) int keys[RANK_MAX];
+  __shared__ int count[RANK_TOKENS];
+  const GradJob& j = a.job[blockIdx.y];
+  if (!j.ids || blockIdx.x * RANK_TOKENS >= a.tokens) return;
+  constexpr int SHARES = RANK_THREADS / RANK_TOKENS;
+  const int n = a.tokens;
+  // padded to a multiple of 4 keys a share with keys that are before none
+  const int len = ((n + SHARES - 1) / SHARES + 3) & ~3;
+  for (int i = threadIdx.x; i < len * SHARES && i < RANK_MAX; i += RANK_THREADS)
+    keys[i] = i < n ? sort_key(j, a.is64, i) : 0x7FFFFFFF;
+  if (threadIdx.x < RANK_TOKENS) count[threadIdx.x] = 0;
+  __syncthreads();
+  const int i = blockIdx.x * RANK_TOKENS + (threadIdx.x & (RANK_TOKENS - 1));
+  const int share = threadIdx.x / RANK_TOKENS;
+  const int mine = i < n ? keys[i] : 0;
+  const int s0 = share * len, s1 = s0 + len < RANK_MAX ? s0 + len : RANK_MAX;
+  int before = 0;
+  for (int s = s0; s < s1; s += 4) {
+    const int4 k = *(const int4*)(keys + s);
+    // equal keys count if their token is before this one
+    before += k.x < mine + (s < i);
+    before += k.y < mine + (s + 1 < i);
+    before += k.z < mine + (s + 2 < i);
+    before += k.w < mine + (s + 3 < i);
+  }
+  atomicAdd(&count[threadIdx.x & (RANK_TOKENS - 1)], before);
+  __syncthreads();
+  if (share == 0 && i < n) {
+    const int at = count[threadIdx.x];
+    j.keys[at] = mine;
+    j.order[at] = i;
+  }
+}
+
+// Many tokens: a stable radix sort, eight bits a pass from the lowest.  At most 256 workgroups
+// take an equal run of the list each: one launch counts the run's digits, the next adds up the
+// counts of the runs before it and moves the run's keys, in order.
+constexpr int RADIX_RUNS = 256, RADIX_ROUND = 1024;
+
+__device__ __forceinline__ int radix_run(int tokens, int runs) {
+  const int len = (tokens + runs - 1) / runs;
+  return (len + RADIX_ROUND - 1) / RADIX_ROUND * RADIX_ROUND;
+}
+
+__global__ __launch_bounds__(256) void radix_count(GradArgs a, int pass, int runs, int parity) {
+  __shared__ int hist[256];
+  const GradJob& j = a.job[blockIdx.y];
+  if (!j.ids) return;
+  const int* src = parity ? j.keys2 : j.keys;   // pass 0 reads the ids
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const long long len = radix_run(a.tokens, runs), i0 = blockIdx.x * len;
+  const long long i1 = i0 + len < a.tokens ? i0 + len : a.tokens;
+  for (long long i = i0 + threadIdx.x; i < i1; i += 256) {
+    const int k = pass ? src[i] : sort_key(j, a.is64, i);
+    atomicAdd(&hist[(unsigned)k >> (8 * pass) & 255], 1);
+  }
+  __syncthreads();
+  j.hist[blockIdx.x * 256 + threadIdx.x] = hist[threadIdx.x];
+}
+
+// A pass of parity 1 reads keys2 / order2 and writes keys / order, the last pass among them;
+// the others the other way.
+__global__ __launch_bounds__(256) void radix_move(GradArgs a, int pass, int runs, int parity) {
+  __shared__ int base[256];       // next place of each digit
+  __shared__ int cnt[4][256];     // keys of each digit in each wave's part of a round
+  __shared__ int wsum[4];
+  const GradJob& j = a.job[blockIdx.y];
+  if (!j.ids) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int* ksrc = parity ? j.keys2 : j.keys;
+  const int* osrc = parity ? j.order2 : j.order;
+  int* kdst = parity ? j.keys : j.keys2;
+  int* odst = parity ? j.order : j.order2;
+  {
+    int total = 0, mine = 0;
+#pragma unroll 8
+    for (int r = 0; r < runs; ++r) {
+      const int c = j.hist[r * 256 + threadIdx.x];
+      total += c;
+      if (r < (int)blockIdx.x) mine += c;
+    }
+    int scan = total;             // over the digits, then without itself
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(scan, d);
+      if (lane >= d) scan += up;
+    }
+    if (lane == 63) wsum[wave] = scan;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) scan += wsum[w];
+    base[threadIdx.x] = scan - total + mine;
+  }
+  const long long len = radix_run(a.tokens, runs), r0 = blockIdx.x * len;
+  const long long r1 = r0 + len < a.tokens ? r0 + len : a.tokens;
+  for (long long i0 = r0; i0 < r1; i0 += RADIX_ROUND) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
+    __syncthreads();
+    int key[4], tok[4], rank[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const long long i = i0 + wave * 256 + q * 64 + lane;
+      key[q] = i >= r1 ? 0 : pass ? ksrc[i] : sort_key(j, a.is64, i);
+      tok[q] = i >= r1 ? 0 : pass ? osrc[i] : (int)i;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool in = i0 + wave * 256 + q * 64 + lane < r1;
+      const int d = (unsigned)key[q] >> (8 * pass) & 255;
+      unsigned long long same = __ballot(in);   // lanes with a key of this digit
+#pragma unroll
+      for (int bit = 0; bit < 8; ++bit) {
+        const unsigned long long set = __ballot(d >> bit & 1);
+        same &= d >> bit & 1 ? set : ~set;
+      }
+      const int below = __popcll(same & ((1ull << lane) - 1));
+      // a wave's LDS accesses are in order; the barriers keep the compiler from moving them
+      const int before = in ? cnt[wave][d] : 0;
+      __builtin_amdgcn_wave_barrier();
+      if (in && below == 0) cnt[wave][d] = before + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      rank[q] = before + below;
+    }
+    __syncthreads();
+    int at = base[threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int c = cnt[w][threadIdx.x];
+      cnt[w][threadIdx.x] = at;
+      at += c;
+    }
+    base[threadIdx.x] = at;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (i0 + wave * 256 + q * 64 + lane < r1) {
+        const int to = cnt[wave][(unsigned)key[q] >> (8 * pass) & 255] + rank[q];
+        kdst[to] = key[q];
+        odst[to] = tok[q];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// sorted ids and their tokens
+__device__ __forceinline__ int key_at(const GradArgs& a, const GradJob& j, int s) {
+  return j.ids ? j.keys[s] : s / a.batch;
+}
+__device__ __forceinline__ int token_at(const GradArgs& a, const GradJob& j, int s) {
+  return j.ids ? j.order[s] : (s % a.batch) * a.seq + s / a.batch;
+}
 
 // first place in the sorted keys that is not below v
 __device__ __forceinline__ int first_at(const int* keys, int n, int v) {
@@ -115,53 +273,161 @@ __device__ __forceinline__ int first_at(const int* keys, int n, int v) {
   return lo;
 }
 
-constexpr int GRAD_ROWS = 16;   // table rows a workgroup
+// the scaled sum of one id into its row of the table
+template <class TO>
+__device__ __forceinline__ void put_row(const GradArgs& a, const GradJob& j, int row, int c, int n,
+                                        const float (&sum)[8]) {
+  TO* o = (TO*)j.out + (long long)row * a.dim + c;
+  float v[8] = {};
+  if (j.accumulate) {
+    if (n == 8) load8(o, v); else load_some(o, n, v);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = fmaf(sum[k], j.scale, v[k]);
+  if (n == 8) store8(o, v); else store_some(o, n, v);
+}
 
-// A wave takes a row of the table and 512 of its columns, eight a lane.
+constexpr int FILL_ROWS = 64;   // table rows a workgroup clears
+constexpr int IN_FLIGHT = 8;    // rows of the gradient that a wave loads ahead
+
+template <class TO>
+__device__ void clear_rows(const GradArgs& a, const GradJob& j, int group) {
+  __shared__ unsigned long long named;
+  const int v0 = group * FILL_ROWS;
+  if (threadIdx.x < 64) {
+    const int v = v0 + threadIdx.x;
+    bool hit = v >= j.rows;
+    if (!hit && j.ids) {
+      const int s = first_at(j.keys, a.tokens, v);
+      hit = s < a.tokens && j.keys[s] == v;
+    } else if (!hit) {
+      hit = a.tokens > 0 && v < a.seq;
+    }
+    const unsigned long long m = __ballot(hit);
+    if (threadIdx.x == 0) named = m;
+  }
+  __syncthreads();
+  const unsigned long long m = named;
+  const float zero[8] = {};
+  const int d8 = (a.dim + 7) / 8;
+  for (int r = 0; r < FILL_ROWS; ++r) {
+    if (m >> r & 1) continue;
+    TO* o = (TO*)j.out + (long long)(v0 + r) * a.dim;
+    for (int c = threadIdx.x; c < d8; c += 256) {
+      const int n = a.dim - c * 8;
+      if (n >= 8) store8(o + c * 8, zero); else store_some(o + c * 8, n, zero);
+    }
+  }
+}
+
 template <class TG, class TO, bool DROP>
-__global__ __launch_bounds__(256) void embed_grad(EmbedGradArgs a) {
-  __shared__ int first[GRAD_ROWS + 1];
-  const long long v0 = (long long)blockIdx.x * GRAD_ROWS;
-  if (a.keys) {
-    if (threadIdx.x <= GRAD_ROWS)
-      first[threadIdx.x] = first_at(a.keys, a.tokens, (int)(v0 + threadIdx.x));
-    __syncthreads();
+__global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
+  int b = blockIdx.x;
+  const int jn = b >= a.job[0].reduce_groups + a.job[1].reduce_groups
+                     ? (b -= a.job[0].reduce_groups + a.job[1].reduce_groups,
+                        b >= a.job[0].fill_groups ? 3 : 2)
+                     : b >= a.job[0].reduce_groups;
+  const GradJob& j = a.job[jn & 1];
+  if (jn >= 2) {
+    clear_rows<TO>(a, j, jn == 3 ? b - a.job[0].fill_groups : b);
+    return;
   }
-  const RngKey key = DROP ? rng_key(a.rng) : RngKey{};
-  const int wave = threadIdx.x >> 6, c = (blockIdx.y * 64 + (threadIdx.x & 63)) * 8;
-  if (c >= a.dim) return;
-  const int n = a.dim - c < 8 ? a.dim - c : 8;
-  for (int r = wave; r < GRAD_ROWS; r += 4) {
-    const long long v = v0 + r;
-    if (v >= a.rows) return;
-    int s0, s1;
-    if (a.keys) {
-      s0 = first[r];
-      s1 = first[r + 1];
-    } else {   // tokens v, v + seq, ...
-      s0 = 0;
-      s1 = v < a.seq ? (a.tokens - (int)v + a.seq - 1) / a.seq : 0;
+  if (jn == 1) b -= a.job[0].reduce_groups;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(b * 4 + (int)(threadIdx.x >> 6));
+  const int chunk = w / a.ctiles, c = ((w - chunk * a.ctiles) * 64 + lane) * 8;
+  if (chunk >= j.chunks) return;
+  const int s0 = chunk * a.chunk, s1 = a.tokens - s0 < a.chunk ? a.tokens : s0 + a.chunk;
+  // lane l has the chunk's entry l
+  int key = j.rows, tok = 0;
+  if (s0 + lane < s1) {
+    key = key_at(a, j, s0 + lane);
+    tok = token_at(a, j, s0 + lane);
+  }
+  const int before = s0 ? key_at(a, j, s0 - 1) : -1;
+  const int after = s1 < a.tokens ? key_at(a, j, s1) : -1;
+  const RngKey rk = DROP ? rng_key(a.rng) : RngKey{};
+  const int n = c >= a.dim ? 0 : a.dim - c < 8 ? a.dim - c : 8;
+  const TG* g = (const TG*)a.g + c;
+  float sum[8] = {};
+  int cur = __builtin_amdgcn_readlane(key, 0);
+  bool began_here = cur != before;
+  for (int e0 = 0; e0 < s1 - s0; e0 += IN_FLIGHT) {
+    float x[IN_FLIGHT][8];
+#pragma unroll
+    for (int q = 0; q < IN_FLIGHT; ++q) {
+      if (e0 + q >= s1 - s0) break;
+      const long long i = __builtin_amdgcn_readlane(tok, e0 + q);
+      if (n == 8)
+        load8(g + i * a.gstride, x[q]);
+      else
+        load_some(g + i * a.gstride, n, x[q]);
     }
-    if (a.accumulate && s0 == s1) continue;
-    float sum[8] = {};
-    for (int s = s0; s < s1; ++s) {
-      const long long i = a.keys ? a.order[s] : v + (long long)s * a.seq;
+#pragma unroll
+    for (int q = 0; q < IN_FLIGHT; ++q) {
+      if (e0 + q >= s1 - s0) break;
+      const int k = __builtin_amdgcn_readlane(key, e0 + q);
+      if (k != cur) {
+        if (began_here)
+          put_row<TO>(a, j, cur, c, n, sum);
+        else if (n)
+          store8(j.part + ((long long)chunk * 2) * a.dimp + c, sum);
+        cur = k;
+        began_here = true;
+#pragma unroll
+        for (int z = 0; z < 8; ++z) sum[z] = 0.f;
+      }
+      if (k >= j.rows) return;   // the rest takes no gradient
+      if (DROP) {
+        const long long i = __builtin_amdgcn_readlane(tok, e0 + q);
+        drop_at(a.rng, rk, (unsigned long long)(i * a.dim + c), x[q]);
+      }
+#pragma unroll
+      for (int z = 0; z < 8; ++z) sum[z] += x[q][z];
+    }
+  }
+  if (cur >= j.rows || !n) return;
+  if (began_here && after != cur)
+    put_row<TO>(a, j, cur, c, n, sum);
+  else
+    store8(j.part + ((long long)chunk * 2 + began_here) * a.dimp + c, sum);
+}
+
+// The ids that reach over a chunk's end: the part in the chunk where an id begins and those of
+// the chunks that it fills or ends in, spread over eight waves and added in their order.
+constexpr int JOIN_WAVES = 8;
+
+template <class TO>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join(GradArgs a) {
+  __shared__ float lds[JOIN_WAVES][64][9];
+  const GradJob& j = a.job[blockIdx.z];
+  const int chunk = blockIdx.x;
+  if (chunk >= j.chunks - 1 || !j.spans) return;
+  const int end = (chunk + 1) * a.chunk, id = key_at(a, j, end - 1);
+  if (id >= j.rows || key_at(a, j, end) != id) return;
+  if (chunk && key_at(a, j, chunk * a.chunk - 1) == id) return;   // began before
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (blockIdx.y * 64 + lane) * 8, n = a.dim - c < 8 ? a.dim - c : 8;
+  float sum[8] = {};
+  // the id has a part in chunk q if it is the first id there
+  for (int q = chunk + 1 + wave; q < j.chunks && key_at(a, j, q * a.chunk) == id;
+       q += JOIN_WAVES) {
+    if (n > 0) {
       float x[8];
-      const TG* g = (const TG*)a.g + i * a.gstride + c;
-      if (n == 8) load8(g, x); else load_some(g, n, x);
-      if (DROP) drop_at(a.rng, key, (unsigned long long)(i * a.dim + c), x);
+      load8(j.part + (long long)q * 2 * a.dimp + c, x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += x[j];
+      for (int z = 0; z < 8; ++z) sum[z] += x[z];
     }
-    TO* o = (TO*)a.out + v * a.dim + c;
-    float old[8] = {};
-    if (a.accumulate) {
-      if (n == 8) load8(o, old); else load_some(o, n, old);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum[j] = fmaf(sum[j], a.scale, old[j]);
-    if (n == 8) store8(o, sum); else store_some(o, n, sum);
   }
+#pragma unroll
+  for (int z = 0; z < 8; ++z) lds[wave][lane][z] = sum[z];
+  __syncthreads();
+  if (wave || n <= 0) return;
+  load8(j.part + ((long long)chunk * 2 + 1) * a.dimp + c, sum);
+  for (int w = 0; w < JOIN_WAVES; ++w)
+#pragma unroll
+    for (int z = 0; z < 8; ++z) sum[z] += lds[w][lane][z];
+  put_row<TO>(a, j, id, c, n, sum);
 }
 
 template <class TW, class TO>
@@ -179,17 +445,74 @@ static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
 }
 
 template <class TG, class TO>
-static void launch_grad(hipStream_t stream, const EmbedGradArgs& a) {
-  const dim3 grid((unsigned)ceil_div(a.rows, GRAD_ROWS), ceil_div(a.dim, 512)), block(256);
+static void launch_grad(hipStream_t stream, const GradArgs& a) {
+  const int groups = a.job[0].reduce_groups + a.job[1].reduce_groups + a.job[0].fill_groups +
+                     a.job[1].fill_groups;
+  if (groups == 0) return;   // no tokens to add
   if (a.rng.cut)
-    hipLaunchKernelGGL((embed_grad<TG, TO, true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((embed_grad<TG, TO, true>), dim3(groups), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((embed_grad<TG, TO, false>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((embed_grad<TG, TO, false>), dim3(groups), dim3(256), 0, stream, a);
 }
 
-static bool grad_shape(long long tokens, long long rows, int dim) {
-  return tokens >= 0 && tokens < (1LL << 31) - 65536 && rows >= 0 && rows < (1LL << 31) - 65536 &&
-         dim >= 0 && dim <= 65535 * 512;
+constexpr int GRAD_CHUNK = 32;
+
+// what a table's gradient takes of the workspace: sorted ids and tokens, the radix sort's other
+// buffers and counts, the parts of ids that reach over chunks
+struct GradSpace {
+  size_t keys, order, keys2, order2, hist, part, bytes;
+};
+static GradSpace grad_space(long long tokens, int dim, bool sorted) {
+  GradSpace g{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return here;
+  };
+  const long long chunks = (tokens + GRAD_CHUNK - 1) / GRAD_CHUNK;
+  if (sorted) {
+    g.keys = take(4 * (size_t)tokens);
+    g.order = take(4 * (size_t)tokens);
+    if (tokens > RANK_MAX) {
+      g.keys2 = take(4 * (size_t)tokens);
+      g.order2 = take(4 * (size_t)tokens);
+      g.hist = take(4 * 256 * RADIX_RUNS);
+    }
+  }
+  g.part = take((size_t)chunks * 2 * ((dim + 7) / 8 * 8) * 4);
+  g.bytes = at;
+  return g;
+}
+
+static bool grad_shape(long long tokens, long long rows, long long pos_rows, int dim) {
+  // launches stay below 2^32 threads
+  return tokens >= 0 && tokens < (1LL << 27) && rows >= 0 && rows < (1LL << 29) &&
+         pos_rows >= 0 && pos_rows < (1LL << 29) && dim >= 0 && dim <= 65535 * 512 &&
+         (tokens / GRAD_CHUNK + 1) * ((dim + 511) / 512) < (1LL << 25);
+}
+
+// One job: its buffers, and how many workgroups it takes.
+static void grad_job(GradJob& j, const GradArgs& a, const void* ids, void* out, long long rows,
+                     long long padding, float scale, int accumulate, char* ws,
+                     const GradSpace& sp) {
+  j.ids = ids;
+  j.out = out;
+  j.keys = (int*)(ws + sp.keys);
+  j.order = (int*)(ws + sp.order);
+  j.keys2 = (int*)(ws + sp.keys2);
+  j.order2 = (int*)(ws + sp.order2);
+  j.hist = (int*)(ws + sp.hist);
+  j.part = (float*)(ws + sp.part);
+  j.padding = padding;
+  j.rows = (int)rows;
+  j.scale = scale;
+  j.accumulate = accumulate;
+  j.chunks = ceil_div(a.tokens, a.chunk);
+  j.reduce_groups = ceil_div((long long)j.chunks * a.ctiles, 4);
+  j.fill_groups = accumulate || (!ids && a.tokens > 0 && a.seq >= rows) ? 0
+                                                                         : ceil_div(rows, FILL_ROWS);
+  j.spans = j.chunks > 1 && (ids || a.chunk % a.batch != 0);
 }
 
 }  // namespace dmh
@@ -237,58 +560,88 @@ int dmh_embedding(hipStream_t stream, const void* ids, int ids_64, long long tok
   return DMH_OK;
 }
 
-int dmh_embedding_grad_workspace_size(long long tokens, long long rows, int dim, size_t* bytes) {
-  if (!bytes || !grad_shape(tokens, rows, dim)) {
-    set_error("dmh_embedding_grad_workspace_size: bad arguments (tokens=%lld rows=%lld dim=%d)",
-              tokens, rows, dim);
+int dmh_embedding_grad_workspace_size(long long tokens, int dim, int sorts, size_t* bytes) {
+  if (!bytes || !grad_shape(tokens, 0, 0, dim) || sorts < 0 || sorts > 2) {
+    set_error("dmh_embedding_grad_workspace_size: bad arguments (tokens=%lld dim=%d sorts=%d)",
+              tokens, dim, sorts);
     return DMH_EINVAL;
   }
-  *bytes = 8 * (size_t)tokens;
+  *bytes = grad_space(tokens, dim, sorts > 0).bytes + grad_space(tokens, dim, sorts > 1).bytes;
   return DMH_OK;
 }
 
-int dmh_embedding_grad(hipStream_t stream, const void* ids, int ids_64, long long tokens, int seq,
-                       const void* grad, int dtype, long long g_rstride, long long rows, int dim,
-                       long long padding_idx, float scale, int cut, unsigned long long seed,
-                       unsigned long long offset, const void* rng_state, void* out,
-                       int out_dtype, int accumulate, void* ws, size_t ws_bytes) {
-  if (!grad_shape(tokens, rows, dim) || g_rstride < 0 || !float_code(dtype) ||
-      !float_code(out_dtype) || cut < 0 || cut > 65536 || (!ids && tokens > 0 && seq < 1)) {
-    set_error("dmh_embedding_grad: bad arguments (tokens=%lld seq=%d rows=%lld dim=%d "
-              "dtypes=%d,%d cut=%d)", tokens, seq, rows, dim, dtype, out_dtype, cut);
+int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* positions, int ids_64,
+                       long long tokens, int seq, const void* grad, int dtype,
+                       long long g_rstride, int dim, long long padding_idx, float scale, int cut,
+                       unsigned long long seed, unsigned long long offset, const void* rng_state,
+                       void* out, long long rows, int accumulate, void* pos_out,
+                       long long pos_rows, int pos_accumulate, int out_dtype, void* ws,
+                       size_t ws_bytes) {
+  const bool pos = pos_out && pos_rows > 0, tok = out && rows > 0;
+  if (!grad_shape(tokens, rows, pos_rows, dim) || g_rstride < 0 || !float_code(dtype) ||
+      !float_code(out_dtype) || cut < 0 || cut > 65536 ||
+      (pos && !positions && tokens > 0 && (seq < 1 || tokens % seq != 0))) {
+    set_error("dmh_embedding_grad: bad arguments (tokens=%lld seq=%d rows=%lld,%lld dim=%d "
+              "dtypes=%d,%d cut=%d)", tokens, seq, rows, pos_rows, dim, dtype, out_dtype, cut);
     return DMH_EINVAL;
   }
-  if (rows == 0 || dim == 0) return DMH_OK;
-  if (!out || (tokens > 0 && !grad)) {
+  if ((!tok && !pos) || dim == 0) return DMH_OK;
+  if (tokens > 0 && (!grad || (tok && !ids))) {
     set_error("dmh_embedding_grad: null tensor");
     return DMH_EINVAL;
   }
-  size_t need;
-  dmh_embedding_grad_workspace_size(tokens, rows, dim, &need);
-  if (ids && need > 0 && (!ws || ws_bytes < need)) {
+  const GradSpace ts = tok ? grad_space(tokens, dim, true) : GradSpace{};
+  const GradSpace ps = pos ? grad_space(tokens, dim, positions != nullptr) : GradSpace{};
+  const size_t need = ts.bytes + ps.bytes;
+  if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("dmh_embedding_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
     return DMH_EWORKSPACE;
   }
-  EmbedGradArgs a;
-  a.keys = ids ? (const int*)ws : nullptr;
-  a.order = ids ? (const int*)ws + tokens : nullptr;
+  GradArgs a{};
   a.g = grad;
-  a.out = out;
-  a.rows = rows;
   a.gstride = g_rstride;
+  a.is64 = ids_64 != 0;
   a.tokens = (int)tokens;
   a.seq = seq < 1 ? 1 : seq;
+  a.batch = a.tokens / a.seq < 1 ? 1 : a.tokens / a.seq;
   a.dim = dim;
-  a.accumulate = accumulate != 0;
-  a.scale = scale;
+  a.dimp = (dim + 7) / 8 * 8;
+  a.ctiles = ceil_div(dim, 512);
+  a.chunk = GRAD_CHUNK;
   a.rng = make_rng(seed, offset, rng_state, cut);
-  if (ids && tokens > 0) {
-    hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, 256)), dim3(256), 0, stream, ids,
-                       ids_64 != 0, (int)tokens, rows, padding_idx, (int*)ws, (int*)ws + tokens);
-    DMH_CHECK_LAUNCH("embed_rank");
+  if (tok)
+    grad_job(a.job[0], a, ids, out, rows, padding_idx, scale, accumulate != 0, (char*)ws, ts);
+  if (pos)
+    grad_job(a.job[1], a, positions, pos_out, pos_rows, -1, 1.f, pos_accumulate != 0,
+             (char*)ws + ts.bytes, ps);
+  if (tokens > 0 && (a.job[0].ids || a.job[1].ids)) {
+    if (tokens <= RANK_MAX) {
+      hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), 2), dim3(RANK_THREADS), 0,
+                         stream, a);
+      DMH_CHECK_LAUNCH("embed_rank");
+    } else {
+      const long long most = rows > pos_rows ? rows : pos_rows;   // the largest key
+      int passes = 1;
+      while (most >> (8 * passes)) ++passes;
+      const int runs = tokens > (long long)RADIX_RUNS * RADIX_ROUND
+                           ? RADIX_RUNS : ceil_div(tokens, RADIX_ROUND);
+      for (int p = 0; p < passes; ++p) {
+        // an odd number of passes starts from the other buffers, so that all end in the first
+        const int parity = (passes - p) & 1;
+        hipLaunchKernelGGL(radix_count, dim3(runs, 2), dim3(256), 0, stream, a, p, runs, parity);
+        hipLaunchKernelGGL(radix_move, dim3(runs, 2), dim3(256), 0, stream, a, p, runs, parity);
+        DMH_CHECK_LAUNCH("radix sort");
+      }
+    }
   }
   DMH_FOR_TYPE(dtype, TG, DMH_FOR_TYPE(out_dtype, TO, (launch_grad<TG, TO>(stream, a))))
   DMH_CHECK_LAUNCH("embed_grad");
+  if (a.job[0].spans || a.job[1].spans) {
+    const int chunks = ceil_div(tokens, a.chunk);
+    DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), dim3(chunks - 1, a.ctiles, 2),
+                                                   dim3(64 * JOIN_WAVES), 0, stream, a))
+    DMH_CHECK_LAUNCH("embed_join");
+  }
   return DMH_OK;
 }
 

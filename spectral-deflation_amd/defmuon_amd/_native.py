@@ -72,10 +72,10 @@ _SIGS = {
     "dmh_embedding": (c_int, [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll, c_int, c_ll,
                               c_vp, c_ll, c_ll, c_vp, c_float, c_int, c_ull, c_ull, c_vp, c_vp,
                               c_int]),
-    "dmh_embedding_grad_workspace_size": (c_int, [c_ll, c_ll, c_int, ctypes.POINTER(c_sz)]),
-    "dmh_embedding_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll, c_ll,
-                                   c_int, c_ll, c_float, c_int, c_ull, c_ull, c_vp, c_vp, c_int,
-                                   c_int, c_vp, c_sz]),
+    "dmh_embedding_grad_workspace_size": (c_int, [c_ll, c_int, c_int, ctypes.POINTER(c_sz)]),
+    "dmh_embedding_grad": (c_int, [c_vp, c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll,
+                                   c_int, c_ll, c_float, c_int, c_ull, c_ull, c_vp, c_vp, c_ll,
+                                   c_int, c_vp, c_ll, c_int, c_int, c_vp, c_sz]),
     "dmh_cross_entropy_workspace_size": (c_int, [c_ll, c_ll, ctypes.POINTER(c_sz)]),
     "dmh_cross_entropy": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
                                   c_float, c_float, c_int, c_float, c_vp, c_vp, c_vp, c_vp, c_ll,
@@ -479,21 +479,30 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
            "dmh_embedding")
 
 
-def embedding_grad(ids, tokens, seq, grad, gstride, padding_idx, scale, cut, rng, out,
-                   accumulate):
-    """The gradient of a table, out (rows, dim); ids None: i % seq."""
-    seed, offset, state = rng
-    rows, dim = out.shape
-    lib = load()
+@functools.lru_cache(maxsize=1024)
+def embedding_grad_workspace_bytes(tokens, dim, sorts):
+    """Workspace of embedding_grad with `sorts` tables whose rows ids or positions name."""
     nbytes = c_sz()
-    _check(lib.dmh_embedding_grad_workspace_size(tokens, rows, dim, ctypes.byref(nbytes)),
+    _check(load().dmh_embedding_grad_workspace_size(tokens, dim, sorts, ctypes.byref(nbytes)),
            "dmh_embedding_grad_workspace_size")
-    ws = _workspace(nbytes.value, out.device)
-    _check(lib.dmh_embedding_grad(_stream(out.device), 0 if ids is None else ids.data_ptr(),
-                                  ids is not None and ids.dtype == torch.int64, tokens, seq,
-                                  grad.data_ptr(), FLOATS[grad.dtype], gstride, rows, dim,
-                                  padding_idx, scale, cut, seed, offset, state, out.data_ptr(),
-                                  FLOATS[out.dtype], accumulate, ws.data_ptr(), nbytes.value),
+    return nbytes.value
+
+
+def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx, scale, cut, rng,
+                   out, add, pos_out, pos_add):
+    """The gradients of the token table (out) and the position table (pos_out), either None."""
+    seed, offset, state = rng
+    some = pos_out if out is None else out
+    nbytes = embedding_grad_workspace_bytes(tokens, dim, 2)
+    ws = _workspace(nbytes, some.device)
+    rows = (0, 0) if out is None else (out.data_ptr(), out.shape[0])
+    prows = (0, 0) if pos_out is None else (pos_out.data_ptr(), pos_out.shape[0])
+    _check(load().dmh_embedding_grad(_stream(some.device), ids.data_ptr(),
+                                     0 if positions is None else positions.data_ptr(),
+                                     ids.dtype == torch.int64, tokens, seq, grad.data_ptr(),
+                                     FLOATS[grad.dtype], gstride, dim, padding_idx, scale, cut,
+                                     seed, offset, state, *rows, add, *prows, pos_add,
+                                     FLOATS[some.dtype], ws.data_ptr(), nbytes),
            "dmh_embedding_grad")
 
 

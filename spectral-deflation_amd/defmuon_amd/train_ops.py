@@ -303,16 +303,24 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     cut, key = _drop(dropout_p, rng, grad.device, what)
     dim, tokens = grad.shape[-1], ids.numel()
     seq = ids.shape[-1] if ids.ndim else 1
+    ids = ids.contiguous()
     grad, _, _, stride = _rows(grad)
     dw = dp = None
+    add = pos_add = False
     if rows:
         dw, add = _table_grad(weight_grad, rows, dim, dtype, grad.device, what, "weight_grad")
-        _native.embedding_grad(ids.contiguous(), tokens, seq, grad, stride,
-                               -1 if padding_idx is None else padding_idx, scale, cut, key, dw,
-                               add)
     if pos_rows:
-        dp, add = _table_grad(pos_grad, pos_rows, dim, dtype, grad.device, what, "pos_grad")
-        _native.embedding_grad(positions, tokens, seq, grad, stride, -1, 1.0, cut, key, dp, add)
+        dp, pos_add = _table_grad(pos_grad, pos_rows, dim, dtype, grad.device, what, "pos_grad")
+    padding_idx = -1 if padding_idx is None else padding_idx
+    if dw is not None and dp is not None and dw.dtype != dp.dtype:
+        # one launch writes one type
+        _native.embedding_grad(ids, None, tokens, seq, grad, stride, dim, padding_idx, scale, cut,
+                               key, dw, add, None, False)
+        _native.embedding_grad(ids, positions, tokens, seq, grad, stride, dim, -1, scale, cut,
+                               key, None, False, dp, pos_add)
+    elif (rows or pos_rows) and dim:
+        _native.embedding_grad(ids, positions, tokens, seq, grad, stride, dim, padding_idx, scale,
+                               cut, key, dw, add, dp, pos_add)
     return dw, dp
 
 

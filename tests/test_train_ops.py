@@ -67,25 +67,29 @@ def test_entry_points_refuse_without_launching(lib):
     assert embed(tokens=0, ids=None) == 0 and embed(dim=0, w=None) == 0
 
     def grad(**kw):
-        a = dict(ids=one, tokens=4, seq=2, g=one, dt=0, gs=8, rows=9, dim=8, cut=0, out=one,
-                 ot=0, ws=one, nb=1 << 20)
+        a = dict(ids=one, pos=None, tokens=4, seq=2, g=one, dt=0, gs=8, rows=9, dim=8, cut=0,
+                 out=one, pout=None, prows=0, ot=0, ws=one, nb=1 << 20)
         a.update(kw)
-        return lib.dmh_embedding_grad(None, a["ids"], 1, a["tokens"], a["seq"], a["g"], a["dt"],
-                                      a["gs"], a["rows"], a["dim"], -1, 1.0, a["cut"], 0, 0,
-                                      None, a["out"], a["ot"], 0, a["ws"], a["nb"])
-    for bad in (dict(g=None), dict(out=None), dict(tokens=-1), dict(tokens=1 << 31),
-                dict(rows=1 << 31), dict(dim=-1), dict(dim=1 << 30), dict(dt=9), dict(ot=9),
-                dict(gs=-1), dict(cut=-2), dict(ids=None, seq=0)):
+        return lib.dmh_embedding_grad(None, a["ids"], a["pos"], 1, a["tokens"], a["seq"], a["g"],
+                                      a["dt"], a["gs"], a["dim"], -1, 1.0, a["cut"], 0, 0, None,
+                                      a["out"], a["rows"], 0, a["pout"], a["prows"], 0, a["ot"],
+                                      a["ws"], a["nb"])
+    for bad in (dict(g=None), dict(ids=None), dict(tokens=-1), dict(tokens=1 << 27),
+                dict(rows=-1), dict(rows=1 << 29), dict(dim=-1), dict(dim=1 << 30), dict(dt=9),
+                dict(ot=9), dict(gs=-1), dict(cut=-2), dict(pout=one, prows=2, seq=0),
+                dict(pout=one, prows=2, seq=3), dict(pout=one, prows=1 << 29)):
         assert grad(**bad) == 1, bad
         assert b"dmh_embedding_grad" in lib.dmh_last_error()
     assert grad(nb=3) == 2 and grad(ws=None) == 2
     assert b"workspace" in lib.dmh_last_error()
-    assert grad(rows=0, out=None) == 0 and grad(dim=0) == 0
+    assert grad(out=None) == 0 and grad(rows=0) == 0 and grad(dim=0) == 0
 
     nb = ctypes.c_size_t()
-    assert lib.dmh_embedding_grad_workspace_size(-1, 5, 8, ctypes.byref(nb)) == 1
-    assert lib.dmh_embedding_grad_workspace_size(5, 5, 8, None) == 1
-    assert lib.dmh_embedding_grad_workspace_size(0, 5, 8, ctypes.byref(nb)) == 0
+    assert lib.dmh_embedding_grad_workspace_size(-1, 8, 1, ctypes.byref(nb)) == 1
+    assert lib.dmh_embedding_grad_workspace_size(5, 8, 1, None) == 1
+    assert lib.dmh_embedding_grad_workspace_size(5, 8, 3, ctypes.byref(nb)) == 1
+    assert lib.dmh_embedding_grad_workspace_size(0, 8, 2, ctypes.byref(nb)) == 0
+    assert nb.value == 0
 
     def xent(**kw):
         a = dict(z=one, dt=0, rows=2, v=5, zs=5, y=one, red=1, loss=one, count=one, ds=5, ws=one,
