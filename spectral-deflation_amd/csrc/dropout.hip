@@ -53,10 +53,11 @@ __global__ __launch_bounds__(256) void dropout(DropArgs a) {
         }
       }
     }
-    drop_block(a.rng, key, (unsigned long long)b, v);
-    if (RES) {
+    const uint32_t bits = a.rng.cut ? keep_bits(a.rng, key, (unsigned long long)b) : ~0u;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += r[j];
+    for (int j = 0; j < 8; ++j) {
+      v[j] = kept(bits, j, v[j] * a.rng.scale);
+      if (RES) v[j] += r[j];
     }
     if (n == 8)
       store8(out + e, v);

@@ -24,39 +24,52 @@ struct EmbedArgs {
   Rng rng;
 };
 
-// Eight columns of one token a thread.
-template <class TW, class TO, bool POS, bool DROP>
+// Eight columns of one token a thread.  The last eight of a row overlap those before them where
+// the width is no multiple of eight (SPLIT), and are written twice with the same values; rows
+// narrower than eight go column by column (NARROW).
+template <class TW, class TO, bool POS, bool DROP, bool SPLIT, bool NARROW>
 __global__ __launch_bounds__(256) void embed_rows(EmbedArgs a) {
-  const int d8 = (a.dim + 7) / 8;
-  const long long items = a.tokens * d8, step = (long long)gridDim.x * 256;
+  constexpr int W = NARROW ? 1 : 8;
+  const int pieces = (a.dim + W - 1) / W;
+  const long long items = a.tokens * pieces, step = (long long)gridDim.x * 256;
   const RngKey key = DROP ? rng_key(a.rng) : RngKey{};
   for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < items; it += step) {
-    const long long i = it / d8;
-    const int c = (int)(it - i * d8) * 8, n = a.dim - c < 8 ? a.dim - c : 8;
+    const bool small = items < (1LL << 32);   // cheaper divisions
+    const long long i = small ? (long long)((unsigned)it / (unsigned)pieces) : it / pieces;
+    int c = (int)(it - i * pieces) * W;
+    if (SPLIT && !NARROW) c = c + 8 > a.dim ? a.dim - 8 : c;
     const long long id = load_index(a.ids, a.is64, i);
-    const long long t = !POS ? 0 : a.pos ? load_index(a.pos, a.is64, i) : i % a.seq;
-    float v[8];
-    if ((unsigned long long)id < (unsigned long long)a.vocab &&
-        (!POS || (unsigned long long)t < (unsigned long long)a.prows)) {
-      const TW* w = (const TW*)a.w + id * a.wstride + c;
-      if (n == 8) load8(w, v); else load_some(w, n, v);
-      if (POS) {
-        float p[8];
-        const TW* pr = (const TW*)a.p + t * a.pstride + c;
-        if (n == 8) load8(pr, p); else load_some(pr, n, p);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], a.scale, p[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= a.scale;
+    const long long t = !POS ? 0 : a.pos   ? load_index(a.pos, a.is64, i)
+                                : small ? (unsigned)i % (unsigned)a.seq
+                                        : i % a.seq;
+    const unsigned long long e = (unsigned long long)i * a.dim + c;
+    const bool ok = (unsigned long long)id < (unsigned long long)a.vocab &&
+                    (!POS || (unsigned long long)t < (unsigned long long)a.prows);
+    TO* o = (TO*)a.out + e;
+    const TW* w = (const TW*)a.w + (ok ? id : 0) * a.wstride + c;
+    const TW* p = (const TW*)a.p + (ok ? t : 0) * a.pstride + c;
+    if (NARROW) {
+      float v = __builtin_nanf("");
+      if (ok) {
+        v = POS ? fmaf((float)*w, a.scale, (float)*p) : (float)*w * a.scale;
+        if (DROP) v = kept(keep_bits_at<true>(a.rng, key, e), 0, v * a.rng.scale);
       }
-      if (DROP) drop_at(a.rng, key, (unsigned long long)(i * a.dim + c), v);
+      *o = (TO)v;
     } else {
+      float v[8], q[8] = {};
+      if (ok) {
+        load8(w, v);
+        if (POS) load8(p, q);
+      }
+      const uint32_t bits = DROP ? keep_bits_at<SPLIT>(a.rng, key, e) : 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __builtin_nanf("");
+      for (int j = 0; j < 8; ++j) {
+        v[j] = POS ? fmaf(v[j], a.scale, q[j]) : v[j] * a.scale;
+        if (DROP) v[j] = kept(bits, j, v[j] * a.rng.scale);
+        if (!ok) v[j] = __builtin_nanf("");
+      }
+      store8(o, v);
     }
-    TO* o = (TO*)a.out + i * a.dim + c;
-    if (n == 8) store8(o, v); else store_some(o, n, v);
   }
 }
 
@@ -92,13 +105,12 @@ struct GradArgs {
   GradJob job[2];      // the token table's and the position table's
   const void* g;
   long long gstride;
-  int is64, tokens, seq, batch, dim, dimp, ctiles, chunk;
+  int is64, tokens, seq, batch, dim, dimp, ctiles, lanes;   // a wave: `lanes` x 8 columns
   Rng rng;
 };
 
 // Ids that take no gradient (padding, outside the table) sort behind all others, as `rows`.
-__device__ __forceinline__ int sort_key(const GradJob& j, int is64, long long i) {
-  const long long id = load_index(j.ids, is64, i);
+__device__ __forceinline__ int sort_key(const GradJob& j, long long id) {
   return (unsigned long long)id < (unsigned long long)j.rows && id != j.padding ? (int)id : j.rows;
 }
 
@@ -110,29 +122,58 @@ constexpr int RANK_MAX = 8192, RANK_TOKENS = 32, RANK_THREADS = 512;
 __global__ __launch_bounds__(RANK_THREADS) void embed_rank(GradArgs a) {
   __shared__ __attribute__((aligned(16))) int keys[RANK_MAX];
   __shared__ int count[RANK_TOKENS];
-  const GradJob& j = a.job[blockIdx.y];
-  if (!j.ids || blockIdx.x * RANK_TOKENS >= a.tokens) return;
-  constexpr int SHARES = RANK_THREADS / RANK_TOKENS;
-  const int n = a.tokens;
-  // padded to a multiple of 4 keys a share with keys that are before none
-  const int len = ((n + SHARES - 1) / SHARES + 3) & ~3;
-  for (int i = threadIdx.x; i < len * SHARES && i < RANK_MAX; i += RANK_THREADS)
-    keys[i] = i < n ? sort_key(j, a.is64, i) : 0x7FFFFFFF;
+  const GradJob& j = a.job[blockIdx.y + !a.job[0].ids];
+  constexpr int SHARES = RANK_THREADS / RANK_TOKENS, ROUNDS = RANK_MAX / RANK_THREADS;
+  const int n = a.tokens, i0 = blockIdx.x * RANK_TOKENS;
+  // padded to a multiple of 16 keys a share (n <= RANK_MAX, a multiple of 16 SHARES)
+  const int len = ((n + SHARES - 1) / SHARES + 15) & ~15;
+  {
+    // all loads on their way before the first is used
+    long long id[ROUNDS];
+    if (a.is64) {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int s = r * RANK_THREADS + threadIdx.x;
+        id[r] = ((const long long*)j.ids)[s < n ? s : 0];
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const int s = r * RANK_THREADS + threadIdx.x;
+        id[r] = ((const int*)j.ids)[s < n ? s : 0];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int s = r * RANK_THREADS + threadIdx.x;
+      keys[s] = s < n ? sort_key(j, id[r]) : 0x7FFFFFFF;   // before none
+    }
+  }
   if (threadIdx.x < RANK_TOKENS) count[threadIdx.x] = 0;
   __syncthreads();
-  const int i = blockIdx.x * RANK_TOKENS + (threadIdx.x & (RANK_TOKENS - 1));
+  const int i = i0 + (threadIdx.x & (RANK_TOKENS - 1));
   const int share = threadIdx.x / RANK_TOKENS;
   const int mine = i < n ? keys[i] : 0;
-  const int s0 = share * len, s1 = s0 + len < RANK_MAX ? s0 + len : RANK_MAX;
+  const int s0 = share * len;
   int before = 0;
-  for (int s = s0; s < s1; s += 4) {
-    const int4 k = *(const int4*)(keys + s);
-    // equal keys count if their token is before this one
-    before += k.x < mine + (s < i);
-    before += k.y < mine + (s + 1 < i);
-    before += k.z < mine + (s + 2 < i);
-    before += k.w < mine + (s + 3 < i);
+  // equal keys count if their token is before this one: all those of 16 keys before this
+  // workgroup's tokens, none of those behind them
+#pragma unroll 2
+  for (int s = s0; s < s0 + len; s += 16) {
+    const int t = mine + (s < i0);
+    int c = 0;
+#pragma unroll
+    for (int q = 0; q < 16; q += 4) {
+      const int4 k = *(const int4*)(keys + s + q);
+      c += (k.x < t) + (k.y < t) + (k.z < t) + (k.w < t);
+    }
+    before += c;
   }
+  if (share < 2)   // the workgroup's own tokens: half of them in each share
+    for (int q = 0; q < RANK_TOKENS / 2; ++q) {
+      const int s = i0 + share * (RANK_TOKENS / 2) + q;
+      before += s < i && keys[s] == mine;
+    }
   atomicAdd(&count[threadIdx.x & (RANK_TOKENS - 1)], before);
   __syncthreads();
   if (share == 0 && i < n) {
@@ -154,15 +195,14 @@ __device__ __forceinline__ int radix_run(int tokens, int runs) {
 
 __global__ __launch_bounds__(256) void radix_count(GradArgs a, int pass, int runs, int parity) {
   __shared__ int hist[256];
-  const GradJob& j = a.job[blockIdx.y];
-  if (!j.ids) return;
+  const GradJob& j = a.job[blockIdx.y + !a.job[0].ids];
   const int* src = parity ? j.keys2 : j.keys;   // pass 0 reads the ids
   hist[threadIdx.x] = 0;
   __syncthreads();
   const long long len = radix_run(a.tokens, runs), i0 = blockIdx.x * len;
   const long long i1 = i0 + len < a.tokens ? i0 + len : a.tokens;
   for (long long i = i0 + threadIdx.x; i < i1; i += 256) {
-    const int k = pass ? src[i] : sort_key(j, a.is64, i);
+    const int k = pass ? src[i] : sort_key(j, load_index(j.ids, a.is64, i));
     atomicAdd(&hist[(unsigned)k >> (8 * pass) & 255], 1);
   }
   __syncthreads();
@@ -175,8 +215,7 @@ __global__ __launch_bounds__(256) void radix_move(GradArgs a, int pass, int runs
   __shared__ int base[256];       // next place of each digit
   __shared__ int cnt[4][256];     // keys of each digit in each wave's part of a round
   __shared__ int wsum[4];
-  const GradJob& j = a.job[blockIdx.y];
-  if (!j.ids) return;
+  const GradJob& j = a.job[blockIdx.y + !a.job[0].ids];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int* ksrc = parity ? j.keys2 : j.keys;
   const int* osrc = parity ? j.order2 : j.order;
@@ -211,7 +250,7 @@ __global__ __launch_bounds__(256) void radix_move(GradArgs a, int pass, int runs
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const long long i = i0 + wave * 256 + q * 64 + lane;
-      key[q] = i >= r1 ? 0 : pass ? ksrc[i] : sort_key(j, a.is64, i);
+      key[q] = i >= r1 ? 0 : pass ? ksrc[i] : sort_key(j, load_index(j.ids, a.is64, i));
       tok[q] = i >= r1 ? 0 : pass ? osrc[i] : (int)i;
     }
 #pragma unroll
@@ -263,199 +302,296 @@ __device__ __forceinline__ int token_at(const GradArgs& a, const GradJob& j, int
   return j.ids ? j.order[s] : (s % a.batch) * a.seq + s / a.batch;
 }
 
-// first place in the sorted keys that is not below v
-__device__ __forceinline__ int first_at(const int* keys, int n, int v) {
-  int lo = 0, hi = n;
+// First of the sorted keys lo .. hi - 1 that is not below v (hi if none): by one lane, and by a
+// wave together, 64 probes a step.
+__device__ __forceinline__ int first_at(const int* keys, int lo, int hi, int v) {
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (keys[mid] < v) lo = mid + 1; else hi = mid;
   }
   return lo;
 }
+__device__ __forceinline__ int wave_first_at(const int* keys, int hi, int v) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) >> 6;
+    const int p = lo + lane * step;          // lane's share: p .. p + step - 1
+    const int last = p + step - 1 < hi ? p + step - 1 : hi - 1;
+    const int full = __popcll(__ballot(p < hi && keys[p < hi ? last : lo] < v));
+    lo = lo + full * step < hi ? lo + full * step : hi;
+    hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+  }
+  return lo;
+}
 
-// the scaled sum of one id into its row of the table
+// the scaled sum of one id into eight columns of its row
 template <class TO>
-__device__ __forceinline__ void put_row(const GradArgs& a, const GradJob& j, int row, int c, int n,
+__device__ __forceinline__ void put_row(const GradArgs& a, const GradJob& j, int row, int c,
                                         const float (&sum)[8]) {
   TO* o = (TO*)j.out + (long long)row * a.dim + c;
   float v[8] = {};
-  if (j.accumulate) {
-    if (n == 8) load8(o, v); else load_some(o, n, v);
-  }
+  if (j.accumulate) load8(o, v);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(sum[k], j.scale, v[k]);
-  if (n == 8) store8(o, v); else store_some(o, n, v);
+  store8(o, v);
 }
 
+constexpr int CHUNK = 32;       // sorted tokens a chunk
 constexpr int FILL_ROWS = 64;   // table rows a workgroup clears
-constexpr int IN_FLIGHT = 8;    // rows of the gradient that a wave loads ahead
+constexpr int IN_FLIGHT = 16;   // rows of the gradient that a wave loads ahead
 
 template <class TO>
 __device__ void clear_rows(const GradArgs& a, const GradJob& j, int group) {
+  __shared__ int bound[2];
   __shared__ unsigned long long named;
   const int v0 = group * FILL_ROWS;
-  if (threadIdx.x < 64) {
-    const int v = v0 + threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (j.ids && wave < 2) {   // the places of this workgroup's rows in the sorted keys
+    const int s = wave_first_at(j.keys, a.tokens, v0 + wave * FILL_ROWS);
+    if (lane == 0) bound[wave] = s;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int v = v0 + lane;
     bool hit = v >= j.rows;
     if (!hit && j.ids) {
-      const int s = first_at(j.keys, a.tokens, v);
-      hit = s < a.tokens && j.keys[s] == v;
+      const int s = first_at(j.keys, bound[0], bound[1], v);
+      hit = s < bound[1] && j.keys[s] == v;
     } else if (!hit) {
       hit = a.tokens > 0 && v < a.seq;
     }
     const unsigned long long m = __ballot(hit);
-    if (threadIdx.x == 0) named = m;
+    if (lane == 0) named = m;
   }
   __syncthreads();
   const unsigned long long m = named;
-  const float zero[8] = {};
-  const int d8 = (a.dim + 7) / 8;
-  for (int r = 0; r < FILL_ROWS; ++r) {
+  constexpr int N = Piece<TO>::N;
+  const typename Piece<TO>::type zero = {};
+  const int whole = a.dim / N;
+  for (int r = wave; r < FILL_ROWS; r += 4) {
     if (m >> r & 1) continue;
     TO* o = (TO*)j.out + (long long)(v0 + r) * a.dim;
-    for (int c = threadIdx.x; c < d8; c += 256) {
-      const int n = a.dim - c * 8;
-      if (n >= 8) store8(o + c * 8, zero); else store_some(o + c * 8, n, zero);
-    }
+    for (int p = lane; p < whole; p += 64) *(typename Piece<TO>::type*)(o + p * N) = zero;
+    if (lane < a.dim - whole * N) o[whole * N + lane] = (TO)0.f;
   }
 }
 
+// A lane has eight columns.  Where the width is no multiple of eight, the last lane of a row takes
+// its last eight columns, some of them its neighbour's too: both write the same values, and lie in
+// one wave (grad_lanes), so that both read before either writes where sums are added.
 template <class TG, class TO, bool DROP>
 __global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
+  // the sums first: their latency is under the writes of the rows cleared behind them
+  const int sums = a.job[0].reduce_groups + a.job[1].reduce_groups;
   int b = blockIdx.x;
-  const int jn = b >= a.job[0].reduce_groups + a.job[1].reduce_groups
-                     ? (b -= a.job[0].reduce_groups + a.job[1].reduce_groups,
-                        b >= a.job[0].fill_groups ? 3 : 2)
-                     : b >= a.job[0].reduce_groups;
-  const GradJob& j = a.job[jn & 1];
-  if (jn >= 2) {
-    clear_rows<TO>(a, j, jn == 3 ? b - a.job[0].fill_groups : b);
+  if (b >= sums) {
+    b -= sums;
+    const int second = b >= a.job[0].fill_groups;
+    clear_rows<TO>(a, a.job[second], second ? b - a.job[0].fill_groups : b);
     return;
   }
-  if (jn == 1) b -= a.job[0].reduce_groups;
+  const int jn = b >= a.job[0].reduce_groups;
+  const GradJob& j = a.job[jn];
+  if (jn) b -= a.job[0].reduce_groups;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(b * 4 + (int)(threadIdx.x >> 6));
-  const int chunk = w / a.ctiles, c = ((w - chunk * a.ctiles) * 64 + lane) * 8;
+  const int chunk = w / a.ctiles;
   if (chunk >= j.chunks) return;
-  const int s0 = chunk * a.chunk, s1 = a.tokens - s0 < a.chunk ? a.tokens : s0 + a.chunk;
-  // lane l has the chunk's entry l
-  int key = j.rows, tok = 0;
-  if (s0 + lane < s1) {
-    key = key_at(a, j, s0 + lane);
-    tok = token_at(a, j, s0 + lane);
-  }
+  int c = ((w - chunk * a.ctiles) * a.lanes + lane) * 8;
+  const bool mine = lane < a.lanes && c < a.dim;
+  c = mine && c + 8 <= a.dim ? c : a.dim - 8;   // lanes without columns read, and write nothing
+  const int s0 = chunk * CHUNK, count = a.tokens - s0 < CHUNK ? a.tokens - s0 : CHUNK;
+  // lane l has the chunk's entry l; behind the last one, that one again
+  const int sl = s0 + (lane < count ? lane : count - 1);
+  const int key = key_at(a, j, sl), tok = token_at(a, j, sl);
   const int before = s0 ? key_at(a, j, s0 - 1) : -1;
-  const int after = s1 < a.tokens ? key_at(a, j, s1) : -1;
+  const int after = s0 + count < a.tokens ? key_at(a, j, s0 + count) : -1;
   const RngKey rk = DROP ? rng_key(a.rng) : RngKey{};
-  const int n = c >= a.dim ? 0 : a.dim - c < 8 ? a.dim - c : 8;
   const TG* g = (const TG*)a.g + c;
+  float* part = j.part + (long long)chunk * 2 * a.dimp + c;
   float sum[8] = {};
   int cur = __builtin_amdgcn_readlane(key, 0);
   bool began_here = cur != before;
-  for (int e0 = 0; e0 < s1 - s0; e0 += IN_FLIGHT) {
-    float x[IN_FLIGHT][8];
+  for (int e0 = 0; e0 < count; e0 += IN_FLIGHT) {
+    Raw8<TG> x[IN_FLIGHT];
 #pragma unroll
-    for (int q = 0; q < IN_FLIGHT; ++q) {
-      if (e0 + q >= s1 - s0) break;
-      const long long i = __builtin_amdgcn_readlane(tok, e0 + q);
-      if (n == 8)
-        load8(g + i * a.gstride, x[q]);
-      else
-        load_some(g + i * a.gstride, n, x[q]);
+    for (int q = 0; q < IN_FLIGHT; ++q)
+      x[q].load(g + (long long)__builtin_amdgcn_readlane(tok, e0 + q) * a.gstride);
+    // the masks of four rows to a word, while the rows are on their way
+    uint32_t bits[IN_FLIGHT / 4];
+    if (DROP) {
+#pragma unroll
+      for (int q4 = 0; q4 < IN_FLIGHT / 4; ++q4) {
+        bits[q4] = 0;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          const unsigned long long e =
+              (unsigned long long)__builtin_amdgcn_readlane(tok, e0 + q4 * 4 + q) * a.dim + c;
+          bits[q4] |= (a.dim & 7 ? keep_bits_at<true>(a.rng, rk, e)
+                                 : keep_bits_at<false>(a.rng, rk, e)) << (4 * q);
+        }
+      }
     }
 #pragma unroll
     for (int q = 0; q < IN_FLIGHT; ++q) {
-      if (e0 + q >= s1 - s0) break;
+      if (e0 + q >= count) break;
       const int k = __builtin_amdgcn_readlane(key, e0 + q);
       if (k != cur) {
-        if (began_here)
-          put_row<TO>(a, j, cur, c, n, sum);
-        else if (n)
-          store8(j.part + ((long long)chunk * 2) * a.dimp + c, sum);
+        if (mine) {
+          if (began_here) put_row<TO>(a, j, cur, c, sum); else store8(part, sum);
+        }
         cur = k;
         began_here = true;
 #pragma unroll
         for (int z = 0; z < 8; ++z) sum[z] = 0.f;
       }
       if (k >= j.rows) return;   // the rest takes no gradient
-      if (DROP) {
-        const long long i = __builtin_amdgcn_readlane(tok, e0 + q);
-        drop_at(a.rng, rk, (unsigned long long)(i * a.dim + c), x[q]);
-      }
 #pragma unroll
-      for (int z = 0; z < 8; ++z) sum[z] += x[q][z];
+      for (int z = 0; z < 8; ++z)
+        sum[z] += DROP ? kept(bits[q / 4] >> (4 * (q & 3)), z, x[q][z]) : x[q][z];
     }
   }
-  if (cur >= j.rows || !n) return;
+  if (cur >= j.rows || !mine) return;
   if (began_here && after != cur)
-    put_row<TO>(a, j, cur, c, n, sum);
+    put_row<TO>(a, j, cur, c, sum);
   else
-    store8(j.part + ((long long)chunk * 2 + began_here) * a.dimp + c, sum);
+    store8(part + (began_here ? a.dimp : 0), sum);
+}
+
+// Tables narrower than eight columns: a thread has one element of the table and walks through
+// its tokens.
+template <class TG, class TO, bool DROP>
+__global__ __launch_bounds__(256) void embed_grad_narrow(GradArgs a, int jn) {
+  const GradJob& j = a.job[jn];
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (long long)j.rows * a.dim) return;
+  const int v = (int)(at / a.dim), c = (int)(at - (long long)v * a.dim);
+  int s0, s1;
+  if (j.ids) {
+    s0 = first_at(j.keys, 0, a.tokens, v);
+    s1 = first_at(j.keys, s0, a.tokens, v + 1);
+  } else {
+    s0 = v < a.seq ? v * a.batch : 0;
+    s1 = v < a.seq && a.tokens ? s0 + a.batch : s0;
+  }
+  const RngKey rk = DROP ? rng_key(a.rng) : RngKey{};
+  float sum = 0.f;
+  for (int s = s0; s < s1; ++s) {
+    const long long i = token_at(a, j, s);
+    const float x = (float)((const TG*)a.g)[i * a.gstride + c];
+    sum += DROP ? kept(keep_bits_at<true>(a.rng, rk, (unsigned long long)(i * a.dim + c)), 0, x) : x;
+  }
+  TO* o = (TO*)j.out + at;
+  if (j.accumulate) {
+    if (s1 > s0) *o = (TO)fmaf(sum, j.scale, (float)*o);
+  } else {
+    *o = (TO)(sum * j.scale);
+  }
 }
 
 // The ids that reach over a chunk's end: the part in the chunk where an id begins and those of
-// the chunks that it fills or ends in, spread over eight waves and added in their order.
-constexpr int JOIN_WAVES = 8;
+// the chunks that it fills or ends in, spread over four waves and added in their order.
+constexpr int JOIN_WAVES = 4;
 
 template <class TO>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join(GradArgs a) {
   __shared__ float lds[JOIN_WAVES][64][9];
-  const GradJob& j = a.job[blockIdx.z];
+  const GradJob& j = a.job[blockIdx.z + !a.job[0].spans];
   const int chunk = blockIdx.x;
-  if (chunk >= j.chunks - 1 || !j.spans) return;
-  const int end = (chunk + 1) * a.chunk, id = key_at(a, j, end - 1);
+  
+  const int end = (chunk + 1) * CHUNK, id = key_at(a, j, end - 1);
   if (id >= j.rows || key_at(a, j, end) != id) return;
-  if (chunk && key_at(a, j, chunk * a.chunk - 1) == id) return;   // began before
+  if (chunk && key_at(a, j, chunk * CHUNK - 1) == id) return;   // began before
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = (blockIdx.y * 64 + lane) * 8, n = a.dim - c < 8 ? a.dim - c : 8;
+  int c = (blockIdx.y * a.lanes + lane) * 8;
+  const bool mine = lane < a.lanes && c < a.dim;
+  c = mine && c + 8 <= a.dim ? c : a.dim - 8;
+  // the id has a part in every chunk from here on whose first id it is; the sorted list says at
+  // once of 64 chunks whether they are
+  int last = chunk + 1;
+  for (;;) {
+    const int q = last + 1 + lane;
+    const unsigned long long m =
+        __ballot(q < j.chunks && key_at(a, j, (q < j.chunks ? q : chunk) * CHUNK) == id);
+    last += m == ~0ull ? 64 : __builtin_ctzll(~m);
+    if (m != ~0ull) break;
+  }
   float sum[8] = {};
-  // the id has a part in chunk q if it is the first id there
-  for (int q = chunk + 1 + wave; q < j.chunks && key_at(a, j, q * a.chunk) == id;
-       q += JOIN_WAVES) {
-    if (n > 0) {
-      float x[8];
-      load8(j.part + (long long)q * 2 * a.dimp + c, x);
+  const float* part = j.part + c;
+#pragma unroll 4
+  for (int q = chunk + 1 + wave; q <= last; q += JOIN_WAVES) {
+    float x[8];
+    load8(part + (long long)q * 2 * a.dimp, x);
 #pragma unroll
-      for (int z = 0; z < 8; ++z) sum[z] += x[z];
-    }
+    for (int z = 0; z < 8; ++z) sum[z] += x[z];
   }
 #pragma unroll
   for (int z = 0; z < 8; ++z) lds[wave][lane][z] = sum[z];
   __syncthreads();
-  if (wave || n <= 0) return;
+  if (wave || !mine) return;
   load8(j.part + ((long long)chunk * 2 + 1) * a.dimp + c, sum);
   for (int w = 0; w < JOIN_WAVES; ++w)
 #pragma unroll
     for (int z = 0; z < 8; ++z) sum[z] += lds[w][lane][z];
-  put_row<TO>(a, j, id, c, n, sum);
+  put_row<TO>(a, j, id, c, sum);
 }
 
+template <class TW, class TO, bool POS, bool DROP>
+static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
+  const int w = a.dim < 8 ? 1 : 8;
+  const long long groups = (a.tokens * ((a.dim + w - 1) / w) + 255) / 256;
+  const dim3 grid((unsigned)(groups < (1 << 22) ? groups : (1 << 22))), block(256);
+  if (a.dim < 8)
+    hipLaunchKernelGGL((embed_rows<TW, TO, POS, DROP, true, true>), grid, block, 0, stream, a);
+  else if (a.dim & 7)
+    hipLaunchKernelGGL((embed_rows<TW, TO, POS, DROP, true, false>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((embed_rows<TW, TO, POS, DROP, false, false>), grid, block, 0, stream, a);
+}
 template <class TW, class TO>
 static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
-  const long long groups = (a.tokens * ((a.dim + 7) / 8) + 255) / 256;
-  const dim3 grid((unsigned)(groups < (1 << 22) ? groups : (1 << 22))), block(256);
   if (a.p && a.rng.cut)
-    hipLaunchKernelGGL((embed_rows<TW, TO, true, true>), grid, block, 0, stream, a);
+    launch_rows<TW, TO, true, true>(stream, a);
   else if (a.p)
-    hipLaunchKernelGGL((embed_rows<TW, TO, true, false>), grid, block, 0, stream, a);
+    launch_rows<TW, TO, true, false>(stream, a);
   else if (a.rng.cut)
-    hipLaunchKernelGGL((embed_rows<TW, TO, false, true>), grid, block, 0, stream, a);
+    launch_rows<TW, TO, false, true>(stream, a);
   else
-    hipLaunchKernelGGL((embed_rows<TW, TO, false, false>), grid, block, 0, stream, a);
+    launch_rows<TW, TO, false, false>(stream, a);
 }
 
-template <class TG, class TO>
+template <class TG, class TO, bool DROP>
 static void launch_grad(hipStream_t stream, const GradArgs& a) {
+  if (a.dim < 8) {
+    for (int jn = 0; jn < 2; ++jn)
+      if (a.job[jn].rows)
+        hipLaunchKernelGGL((embed_grad_narrow<TG, TO, DROP>),
+                           dim3(ceil_div((long long)a.job[jn].rows * a.dim, 256)), dim3(256), 0,
+                           stream, a, jn);
+    return;
+  }
   const int groups = a.job[0].reduce_groups + a.job[1].reduce_groups + a.job[0].fill_groups +
                      a.job[1].fill_groups;
   if (groups == 0) return;   // no tokens to add
+  hipLaunchKernelGGL((embed_grad<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
+}
+template <class TG, class TO>
+static void launch_grad(hipStream_t stream, const GradArgs& a) {
   if (a.rng.cut)
-    hipLaunchKernelGGL((embed_grad<TG, TO, true>), dim3(groups), dim3(256), 0, stream, a);
+    launch_grad<TG, TO, true>(stream, a);
   else
-    hipLaunchKernelGGL((embed_grad<TG, TO, false>), dim3(groups), dim3(256), 0, stream, a);
+    launch_grad<TG, TO, false>(stream, a);
 }
 
-constexpr int GRAD_CHUNK = 32;
+// Lanes of a wave that take columns: such that the last wave of a row has two at least where the
+// last lane's columns overlap its neighbour's.
+static int grad_lanes(int dim) {
+  const int pieces = ceil_div(dim, 8);
+  int lanes = 64;
+  while (pieces > 1 && (dim & 7) && pieces % lanes == 1) --lanes;
+  return lanes;
+}
 
 // what a table's gradient takes of the workspace: sorted ids and tokens, the radix sort's other
 // buffers and counts, the parts of ids that reach over chunks
@@ -470,7 +606,7 @@ static GradSpace grad_space(long long tokens, int dim, bool sorted) {
     at += (bytes + 255) & ~(size_t)255;
     return here;
   };
-  const long long chunks = (tokens + GRAD_CHUNK - 1) / GRAD_CHUNK;
+  const long long chunks = ceil_div(tokens, CHUNK);
   if (sorted) {
     g.keys = take(4 * (size_t)tokens);
     g.order = take(4 * (size_t)tokens);
@@ -488,8 +624,8 @@ static GradSpace grad_space(long long tokens, int dim, bool sorted) {
 static bool grad_shape(long long tokens, long long rows, long long pos_rows, int dim) {
   // launches stay below 2^32 threads
   return tokens >= 0 && tokens < (1LL << 27) && rows >= 0 && rows < (1LL << 29) &&
-         pos_rows >= 0 && pos_rows < (1LL << 29) && dim >= 0 && dim <= 65535 * 512 &&
-         (tokens / GRAD_CHUNK + 1) * ((dim + 511) / 512) < (1LL << 25);
+         pos_rows >= 0 && pos_rows < (1LL << 29) && dim >= 0 && dim <= (1 << 23) &&
+         (tokens / CHUNK + 1) * (dim / 256 + 1) < (1LL << 25);
 }
 
 // One job: its buffers, and how many workgroups it takes.
@@ -508,11 +644,11 @@ static void grad_job(GradJob& j, const GradArgs& a, const void* ids, void* out, 
   j.rows = (int)rows;
   j.scale = scale;
   j.accumulate = accumulate;
-  j.chunks = ceil_div(a.tokens, a.chunk);
+  j.chunks = ceil_div(a.tokens, CHUNK);
   j.reduce_groups = ceil_div((long long)j.chunks * a.ctiles, 4);
   j.fill_groups = accumulate || (!ids && a.tokens > 0 && a.seq >= rows) ? 0
                                                                          : ceil_div(rows, FILL_ROWS);
-  j.spans = j.chunks > 1 && (ids || a.chunk % a.batch != 0);
+  j.spans = a.dim >= 8 && j.chunks > 1 && (ids || CHUNK % a.batch != 0);
 }
 
 }  // namespace dmh
@@ -606,18 +742,21 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   a.batch = a.tokens / a.seq < 1 ? 1 : a.tokens / a.seq;
   a.dim = dim;
   a.dimp = (dim + 7) / 8 * 8;
-  a.ctiles = ceil_div(dim, 512);
-  a.chunk = GRAD_CHUNK;
+  a.lanes = grad_lanes(dim);
+  a.ctiles = ceil_div(dim, 8 * a.lanes);
+  
   a.rng = make_rng(seed, offset, rng_state, cut);
   if (tok)
-    grad_job(a.job[0], a, ids, out, rows, padding_idx, scale, accumulate != 0, (char*)ws, ts);
+    grad_job(a.job[0], a, ids, out, rows, padding_idx, scale * a.rng.scale, accumulate != 0,
+             (char*)ws, ts);
   if (pos)
-    grad_job(a.job[1], a, positions, pos_out, pos_rows, -1, 1.f, pos_accumulate != 0,
+    grad_job(a.job[1], a, positions, pos_out, pos_rows, -1, a.rng.scale, pos_accumulate != 0,
              (char*)ws + ts.bytes, ps);
-  if (tokens > 0 && (a.job[0].ids || a.job[1].ids)) {
+  const int sorts = (a.job[0].ids != nullptr) + (a.job[1].ids != nullptr);
+  if (tokens > 0 && sorts) {
     if (tokens <= RANK_MAX) {
-      hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), 2), dim3(RANK_THREADS), 0,
-                         stream, a);
+      hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), sorts),
+                         dim3(RANK_THREADS), 0, stream, a);
       DMH_CHECK_LAUNCH("embed_rank");
     } else {
       const long long most = rows > pos_rows ? rows : pos_rows;   // the largest key
@@ -625,11 +764,11 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
       while (most >> (8 * passes)) ++passes;
       const int runs = tokens > (long long)RADIX_RUNS * RADIX_ROUND
                            ? RADIX_RUNS : ceil_div(tokens, RADIX_ROUND);
+      const dim3 grid(runs, sorts), block(256);
       for (int p = 0; p < passes; ++p) {
-        // an odd number of passes starts from the other buffers, so that all end in the first
         const int parity = (passes - p) & 1;
-        hipLaunchKernelGGL(radix_count, dim3(runs, 2), dim3(256), 0, stream, a, p, runs, parity);
-        hipLaunchKernelGGL(radix_move, dim3(runs, 2), dim3(256), 0, stream, a, p, runs, parity);
+        hipLaunchKernelGGL(radix_count, grid, block, 0, stream, a, p, runs, parity);
+        hipLaunchKernelGGL(radix_move, grid, block, 0, stream, a, p, runs, parity);
         DMH_CHECK_LAUNCH("radix sort");
       }
     }
@@ -637,8 +776,8 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   DMH_FOR_TYPE(dtype, TG, DMH_FOR_TYPE(out_dtype, TO, (launch_grad<TG, TO>(stream, a))))
   DMH_CHECK_LAUNCH("embed_grad");
   if (a.job[0].spans || a.job[1].spans) {
-    const int chunks = ceil_div(tokens, a.chunk);
-    DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), dim3(chunks - 1, a.ctiles, 2),
+    const int chunks = ceil_div(tokens, CHUNK);
+    DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), dim3(chunks - 1, a.ctiles, a.job[0].spans + a.job[1].spans),
                                                    dim3(64 * JOIN_WAVES), 0, stream, a))
     DMH_CHECK_LAUNCH("embed_join");
   }

@@ -21,19 +21,30 @@ struct Piece {
   typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// eight consecutive elements as fp32
+// eight consecutive elements, as they are in memory
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  constexpr int N = Piece<T>::N;
+struct Raw8 {
+  typename Piece<T>::type p[8 / Piece<T>::N];
+  __device__ __forceinline__ void load(const T* at) {
 #pragma unroll
-  for (int k = 0; k < 8 / N; ++k) {
-    const typename Piece<T>::type x = *(const typename Piece<T>::type*)(p + k * N);
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[k * N + j] = (float)x[j];
+    for (int k = 0; k < 8 / Piece<T>::N; ++k)
+      p[k] = *(const typename Piece<T>::type*)(at + k * Piece<T>::N);
   }
+  __device__ __forceinline__ float operator[](int j) const {
+    return (float)p[j / Piece<T>::N][j % Piece<T>::N];
+  }
+};
+
+// ... and as fp32
+template <class T>
+__device__ __forceinline__ void load8(const T* at, float (&v)[8]) {
+  Raw8<T> x;
+  x.load(at);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = x[j];
 }
 
-// ... and back, each rounded to nearest even
+// back, each rounded to nearest even
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   constexpr int N = Piece<T>::N;
@@ -110,9 +121,10 @@ __device__ __forceinline__ void philox(const RngKey& key, unsigned long long blo
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u;
     const unsigned long long b = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    // (x ^ y ^ z in one instruction)
+    c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), c1, k0, 0x96);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), c3, k1, 0x96);
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -123,41 +135,45 @@ __device__ __forceinline__ void philox(const RngKey& key, unsigned long long blo
   w[3] = c3;
 }
 
-// dropout of the eight elements of one block: what is dropped is replaced, not multiplied, so
-// an infinity or NaN there leaves nothing behind
-__device__ __forceinline__ void drop_block(const Rng& r, const RngKey& key,
-                                           unsigned long long block, float (&v)[8]) {
-  uint32_t w[4];
+// The kept elements of a block as bits: element j has bit (j >> 1) + 16 (j & 1), that is, its
+// word's number in the half that its draw comes from: two packed 16-bit instructions a word
+// and three to join them, where a comparison for each draw takes twice as many.  cut >= 1.
+__device__ __forceinline__ uint32_t keep_bits(const Rng& r, const RngKey& key,
+                                              unsigned long long block) {
+  uint32_t w[4], m = 0;
   philox(key, block, w);
+  const uint32_t least = (r.cut - 1) * 0x10001u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t draw = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-    v[j] = draw >= r.cut ? v[j] * r.scale : 0.f;
+  for (int k = 0; k < 4; ++k) {
+    // draw - (cut - 1), not below zero, is positive where the element is kept
+    uint32_t t;
+    asm("v_pk_sub_u16 %0, %1, %2 clamp" : "=v"(t) : "v"(w[k]), "s"(least));
+    asm("v_pk_min_u16 %0, %1, %2" : "=v"(t) : "v"(t), "s"(0x10001u));
+    m |= t << k;
   }
+  return m;
 }
 
-// ... of eight elements from flat index e on, which two blocks may hold
-__device__ __forceinline__ void drop_at(const Rng& r, const RngKey& key, unsigned long long e,
-                                        float (&v)[8]) {
-  const int skip = (int)(e & 7);
-  if (skip == 0) {
-    drop_block(r, key, e >> 3, v);
-    return;
+// ... of the eight elements from flat index e on.  SPLIT: e may lie inside a block, and the next
+// one has the rest.
+template <bool SPLIT>
+__device__ __forceinline__ uint32_t keep_bits_at(const Rng& r, const RngKey& key,
+                                                 unsigned long long e) {
+  uint32_t m = keep_bits(r, key, e >> 3);
+  if (SPLIT) {
+    m |= keep_bits(r, key, (e >> 3) + 1) << 4;   // the halves' bits of 16 elements
+    const int t = (int)(e & 7) >> 1;
+    const uint32_t even = m >> t, odd = (m >> 16 >> t & 15) | (m >> (t + 1) & 15) << 16;
+    m = e & 1 ? odd : even & 0x000F000Fu;
   }
-  uint32_t keep = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t w[4];
-    philox(key, (e >> 3) + h, w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t draw = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-      keep |= (draw >= r.cut ? 1u : 0u) << (8 * h + j);
-    }
-  }
-  keep >>= skip;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (keep >> j & 1) ? v[j] * r.scale : 0.f;
+  return m;
+}
+
+// x where element j is kept, else zero: what is dropped is replaced, not multiplied, so an
+// infinity or NaN there leaves nothing behind
+__device__ __forceinline__ float kept(uint32_t bits, int j, float x) {
+  const int all = (int)(bits << (31 - (j >> 1) - 16 * (j & 1))) >> 31;
+  return __builtin_bit_cast(float, all & __builtin_bit_cast(int, x));
 }
 
 }  // namespace dmh

@@ -359,6 +359,16 @@ def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, keep_lse=
     return loss, count, lse
 
 
+def _like_rows(logits):
+    """A tensor for the gradient of logits: with the rows of a padded view as far apart as the
+    view's, which keeps their alignment for this and the next product; else contiguous."""
+    t, n, classes, stride = _rows(logits)
+    if t is logits and classes < stride <= classes + 256:
+        buf = torch.empty(n * stride, dtype=logits.dtype, device=logits.device)
+        return buf.as_strided(logits.shape, logits.stride())
+    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+
+
 class _CrossEntropy(Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
@@ -373,13 +383,13 @@ class _CrossEntropy(Function):
     def backward(ctx, grad):
         logits, targets, count, lse = ctx.saved_tensors
         ignore_index, smoothing, z_loss, reduction = ctx.args
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dz = _like_rows(logits)
         if dz.numel():
             z, n, classes, stride = _rows(logits)
             _native.cross_entropy_grad(z, (n, classes, stride), targets.contiguous(),
                                        ignore_index, smoothing, z_loss, lse, count,
                                        grad.float().contiguous(), reduction == "none", dz,
-                                       classes)
+                                       _rows(dz)[3])
         return dz, *[None] * 5
 
 
@@ -419,7 +429,7 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
                               "to write a gradient to")
         dlogits = logits
     else:
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dlogits = _like_rows(logits)
     loss, _, _ = _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction,
                        dlogits=dlogits, grad_scale=grad_scale)
     return loss, dlogits

@@ -282,22 +282,23 @@ def test_position_gradient(T, batch, seq, rows, dim, dtype, out, p):
     close(dq, want, grad_bound(want, size, n, out))
 
 
-@pytest.mark.parametrize("out", [F32, BF16])
-def test_gradients_are_added(T, out):
+@pytest.mark.parametrize("dim", [1, 5, 13, 72, 515, 519, 1031])
+@pytest.mark.parametrize("out,p", [(F32, 0.0), (BF16, 0.0), (F32, 0.2)])
+def test_gradients_are_added(T, dim, out, p):
     ids = ids_of((4, 500), 300)
-    g = normal(4, 500, 72)
-    w0, p0 = normal(300, 72, dtype=out, seed=5), normal(512, 72, dtype=out, seed=6)
-    w, p = w0.to(DEV), p0.to(DEV)
+    g = normal(4, 500, dim)
+    w0, p0 = normal(300, dim, dtype=out, seed=5), normal(512, dim, dtype=out, seed=6)
+    w, pg = w0.to(DEV), p0.to(DEV)
     dw, dp = T.embedding_backward(g.to(DEV), ids.to(DEV), 300, pos_rows=512, scale=2.0,
-                                  weight_grad=w, pos_grad=p)
-    assert dw is w and dp is p
-    want, size, n = R.table_grad(g, ids, 300, 2.0)
+                                  weight_grad=w, pos_grad=pg, dropout_p=p, rng=RNG)
+    assert dw is w and dp is pg
+    want, size, n = R.table_grad(g, ids, 300, 2.0, p, RNG)
     close(w, want + w0.double(), grad_bound(want + w0.double(), size + w0.abs(), n, out))
     untouched = n[:, 0] == 0
     assert untouched.any() and torch.equal(w.cpu()[untouched], w0[untouched])
-    want, size, n = R.table_grad(g, torch.arange(500).expand(4, 500), 512)
-    close(p, want + p0.double(), grad_bound(want + p0.double(), size + p0.abs(), n, out))
-    assert torch.equal(p.cpu()[500:], p0[500:])
+    want, size, n = R.table_grad(g, torch.arange(500).expand(4, 500), 512, 1.0, p, RNG)
+    close(pg, want + p0.double(), grad_bound(want + p0.double(), size + p0.abs(), n, out))
+    assert torch.equal(pg.cpu()[500:], p0[500:])
 
 
 def test_gradient_of_strided_output(T):
