@@ -257,7 +257,7 @@ int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long to
  * positions NULL: pos_i = i % seq (tokens a multiple of seq).  Every row of an output is
  * written, those that no token names with zero; with `accumulate` the sums are added to what
  * it holds and other rows stay untouched.  padding_idx (-1: none) and ids outside a table
- * take no gradient.  tokens < 2^27, rows < 2^29.
+ * take no gradient.  tokens, rows < 2^27.
  * The workspace depends on how many of the outputs are wanted through ids or positions
  * (`sorts`, 0 .. 2; implicit positions need no sort). */
 int dmh_embedding_grad_workspace_size(long long tokens, int dim, int sorts, size_t* bytes);

@@ -106,6 +106,7 @@ struct GradArgs {
   const void* g;
   long long gstride;
   int is64, tokens, seq, batch, dim, dimp, ctiles, lanes;   // a wave: `lanes` x 8 columns
+  int small;           // embed_grad_small's
   Rng rng;
 };
 
@@ -459,6 +460,76 @@ __global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
     store8(part + (began_here ? a.dimp : 0), sum);
 }
 
+// A handful of tokens and a small table: one launch, whose workgroups each sort the tokens in LDS
+// and then take SMALL_ROWS rows of a table, a wave a row, to clear or to add up.  256 tokens
+// against the three launches, dim 768: 15.2 / 20.1 us for 2000 rows, 18.2 / 20.1 for 8000,
+// 21.0 / 21.6 for 16000, 37.2 / 32.0 for 50257, where every workgroup's own sort is in the way of
+// the clearing; dim 1280: 18.6 / 19.9 for 2000, 20.2 / 19.8 for 4000, 24.1 / 21.6 for 8000.
+constexpr int SMALL_TOKENS = 256, SMALL_ROWS = 16, SMALL_AHEAD = 8;
+constexpr long long SMALL_TABLE = 6 << 20;   // elements
+
+template <class TG, class TO, bool DROP>
+__global__ __launch_bounds__(256) void embed_grad_small(GradArgs a) {
+  __shared__ int raw[SMALL_TOKENS], keys[SMALL_TOKENS], order[SMALL_TOKENS];
+  __shared__ int first[SMALL_ROWS + 1];
+  const int groups = (a.job[0].rows + SMALL_ROWS - 1) / SMALL_ROWS;
+  const int jn = (int)blockIdx.x >= groups;
+  const GradJob& j = a.job[jn];
+  const int v0 = ((int)blockIdx.x - jn * groups) * SMALL_ROWS, n = a.tokens, t = threadIdx.x;
+  if (j.ids) {
+    const int mine = t < n ? sort_key(j, load_index(j.ids, a.is64, t)) : 0;
+    raw[t] = mine;
+    __syncthreads();
+    int at = 0;
+    for (int i = 0; i < n; ++i) at += raw[i] < mine + (i < t);
+    if (t < n) {
+      keys[at] = mine;
+      order[at] = t;
+    }
+    __syncthreads();
+    if (t <= SMALL_ROWS) first[t] = first_at(keys, 0, n, v0 + t);
+  } else if (t <= SMALL_ROWS) {
+    first[t] = (v0 + t < a.seq ? v0 + t : a.seq) * (n ? a.batch : 0);
+  }
+  __syncthreads();
+  const RngKey rk = DROP ? rng_key(a.rng) : RngKey{};
+  const int lane = t & 63;
+  for (int r = t >> 6; r < SMALL_ROWS; r += 4) {
+    const int v = v0 + r;
+    if (v >= j.rows) return;
+    const int s0 = __builtin_amdgcn_readfirstlane(first[r]);
+    const int s1 = __builtin_amdgcn_readfirstlane(first[r + 1]);
+    if (s0 == s1 && j.accumulate) continue;
+    for (int c = lane * 8; c < a.dim && lane < a.lanes; c += 8 * a.lanes) {
+      if (c + 8 > a.dim) c = a.dim - 8;   // overlaps its neighbour's, as in embed_grad
+      float sum[8] = {};
+      for (int s = s0; s < s1; s += SMALL_AHEAD) {
+        Raw8<TG> x[SMALL_AHEAD];
+#pragma unroll
+        for (int q = 0; q < SMALL_AHEAD; ++q) {
+          const int e = s + q < s1 ? s + q : s1 - 1;
+          const int i = j.ids ? order[e] : (e % a.batch) * a.seq + e / a.batch;
+          x[q].load((const TG*)a.g + (long long)i * a.gstride + c);
+        }
+#pragma unroll
+        for (int q = 0; q < SMALL_AHEAD; ++q) {
+          if (s + q >= s1) break;
+          uint32_t bits = ~0u;
+          if (DROP) {
+            const int e = s + q;
+            const int i = j.ids ? order[e] : (e % a.batch) * a.seq + e / a.batch;
+            const unsigned long long f = (unsigned long long)i * a.dim + c;
+            bits = a.dim & 7 ? keep_bits_at<true>(a.rng, rk, f) : keep_bits_at<false>(a.rng, rk, f);
+          }
+#pragma unroll
+          for (int z = 0; z < 8; ++z) sum[z] += DROP ? kept(bits, z, x[q][z]) : x[q][z];
+        }
+      }
+      put_row<TO>(a, j, v, c, sum);
+    }
+  }
+}
+
 // Tables narrower than eight columns: a thread has one element of the table and walks through
 // its tokens.
 template <class TG, class TO, bool DROP>
@@ -571,6 +642,11 @@ static void launch_grad(hipStream_t stream, const GradArgs& a) {
                            stream, a, jn);
     return;
   }
+  if (a.small) {
+    const int groups = ceil_div(a.job[0].rows, SMALL_ROWS) + ceil_div(a.job[1].rows, SMALL_ROWS);
+    hipLaunchKernelGGL((embed_grad_small<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
+    return;
+  }
   const int groups = a.job[0].reduce_groups + a.job[1].reduce_groups + a.job[0].fill_groups +
                      a.job[1].fill_groups;
   if (groups == 0) return;   // no tokens to add
@@ -623,8 +699,8 @@ static GradSpace grad_space(long long tokens, int dim, bool sorted) {
 
 static bool grad_shape(long long tokens, long long rows, long long pos_rows, int dim) {
   // launches stay below 2^32 threads
-  return tokens >= 0 && tokens < (1LL << 27) && rows >= 0 && rows < (1LL << 29) &&
-         pos_rows >= 0 && pos_rows < (1LL << 29) && dim >= 0 && dim <= (1 << 23) &&
+  return tokens >= 0 && tokens < (1LL << 27) && rows >= 0 && rows < (1LL << 27) &&
+         pos_rows >= 0 && pos_rows < (1LL << 27) && dim >= 0 && dim <= (1 << 23) &&
          (tokens / CHUNK + 1) * (dim / 256 + 1) < (1LL << 25);
 }
 
@@ -753,7 +829,9 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
     grad_job(a.job[1], a, positions, pos_out, pos_rows, -1, a.rng.scale, pos_accumulate != 0,
              (char*)ws + ts.bytes, ps);
   const int sorts = (a.job[0].ids != nullptr) + (a.job[1].ids != nullptr);
-  if (tokens > 0 && sorts) {
+  a.small = dim >= 8 && tokens <= SMALL_TOKENS &&
+            ((tok ? rows : 0) + (pos ? pos_rows : 0)) * dim <= SMALL_TABLE;
+  if (tokens > 0 && sorts && !a.small) {
     if (tokens <= RANK_MAX) {
       hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), sorts),
                          dim3(RANK_THREADS), 0, stream, a);
@@ -775,7 +853,7 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   }
   DMH_FOR_TYPE(dtype, TG, DMH_FOR_TYPE(out_dtype, TO, (launch_grad<TG, TO>(stream, a))))
   DMH_CHECK_LAUNCH("embed_grad");
-  if (a.job[0].spans || a.job[1].spans) {
+  if (!a.small && (a.job[0].spans || a.job[1].spans)) {
     const int chunks = ceil_div(tokens, CHUNK);
     DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), dim3(chunks - 1, a.ctiles, a.job[0].spans + a.job[1].spans),
                                                    dim3(64 * JOIN_WAVES), 0, stream, a))

@@ -453,12 +453,17 @@ def adamw_step(tab, w1, w2, eps, decay, alpha):
 # element types of the training operators and their codes (include/defmuon_hip.h)
 FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+# the current stream's handle by device index: torch.cuda.current_stream builds a Stream object
+# for it, 2 us of the 11 that a small call takes
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def dropout(x, residual, out, cut, rng, rows):
     """out = dropout(x) [+ residual]; rows: (rows, cols, x's row stride, the residual's)."""
     n, cols, xs, rs = rows
     seed, offset, state = rng
-    _check(load().dmh_dropout(_stream(x.device), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
+    _check(load().dmh_dropout(_raw_stream(x.device.index), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
                               0 if residual is None else residual.data_ptr(), rs,
                               out.data_ptr(), FLOATS[out.dtype], cut, seed, offset, state),
            "dmh_dropout")
@@ -471,7 +476,7 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     seq = ids.shape[-1] if ids.ndim else 1
     pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr(), pos_weight.shape[0],
                                                 pos_weight.stride(0))
-    _check(load().dmh_embedding(_stream(weight.device), ids.data_ptr(),
+    _check(load().dmh_embedding(_raw_stream(weight.device.index), ids.data_ptr(),
                                 ids.dtype == torch.int64, ids.numel(), seq, weight.data_ptr(),
                                 FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
                                 0 if positions is None else positions.data_ptr(), scale, cut,
@@ -497,7 +502,7 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
     ws = _workspace(nbytes, some.device)
     rows = (0, 0) if out is None else (out.data_ptr(), out.shape[0])
     prows = (0, 0) if pos_out is None else (pos_out.data_ptr(), pos_out.shape[0])
-    _check(load().dmh_embedding_grad(_stream(some.device), ids.data_ptr(),
+    _check(load().dmh_embedding_grad(_raw_stream(some.device.index), ids.data_ptr(),
                                      0 if positions is None else positions.data_ptr(),
                                      ids.dtype == torch.int64, tokens, seq, grad.data_ptr(),
                                      FLOATS[grad.dtype], gstride, dim, padding_idx, scale, cut,
@@ -509,16 +514,17 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
                   count, lse, dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
-    stride) of the logits."""
+    stride) of the logits.  A mean's count of rows is kept in `count` if that is wanted."""
     n, classes, zs = rows
     lib = load()
-    nbytes = 4 * n
-    ws = _workspace(nbytes, logits.device) if reduction else None
-    _check(lib.dmh_cross_entropy(_stream(logits.device), logits.data_ptr(),
+    nbytes = 4 * n   # dmh_cross_entropy_workspace_size, and a place for the count
+    ws = torch.empty(n + 1, dtype=torch.float32, device=logits.device) if reduction else None
+    _check(lib.dmh_cross_entropy(_raw_stream(logits.device.index), logits.data_ptr(),
                                  FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
                                  targets.dtype == torch.int64, ignore, smoothing, z_loss,
                                  reduction, grad_scale, loss.data_ptr(),
-                                 0 if count is None else count.data_ptr(),
+                                 count.data_ptr() if count is not None else
+                                 ws.data_ptr() + nbytes if reduction else 0,
                                  0 if lse is None else lse.data_ptr(),
                                  0 if dlogits is None else dlogits.data_ptr(), dstride,
                                  0 if ws is None else ws.data_ptr(), nbytes),
@@ -529,7 +535,7 @@ def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, lse, co
                        per_row, dlogits, dstride):
     """The gradient of the logits from a forward pass's lse, times grad_out."""
     n, classes, zs = rows
-    _check(load().dmh_cross_entropy_grad(_stream(logits.device), logits.data_ptr(),
+    _check(load().dmh_cross_entropy_grad(_raw_stream(logits.device.index), logits.data_ptr(),
                                          FLOATS[logits.dtype], n, classes, zs,
                                          targets.data_ptr(), targets.dtype == torch.int64,
                                          ignore, smoothing, z_loss, lse.data_ptr(),

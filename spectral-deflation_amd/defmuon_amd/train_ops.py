@@ -108,7 +108,9 @@ def draw_rng():
 # ---- dropout --------------------------------------------------------------------------------
 
 def _dropout(x, residual, cut, rng, dtype):
-    out = torch.empty(x.shape, dtype=dtype, device=x.device)
+    out = x.new_empty(x.shape) if dtype == x.dtype else (
+        torch.empty(x.shape, dtype=dtype, device=x.device) if residual is None
+        else residual.new_empty(x.shape))
     if out.numel():
         x, rows, cols, stride = _rows(x)
         rstride = 0
@@ -195,7 +197,9 @@ def _positions(positions, ids, what):
 
 
 def _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype):
-    out = torch.empty((*ids.shape, weight.shape[1]), dtype=dtype, device=weight.device)
+    shape = (*ids.shape, weight.shape[1])
+    out = weight.new_empty(shape) if dtype == weight.dtype else torch.empty(
+        shape, dtype=dtype, device=weight.device)
     if out.numel():
         _native.embedding(ids.contiguous(), _table(weight),
                           None if pos_weight is None else _table(pos_weight), positions, scale,
@@ -350,7 +354,7 @@ def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, keep_lse=
     z, n, classes, stride = _rows(logits)
     red = _REDUCTIONS[reduction]
     loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
-    count = torch.empty((), dtype=torch.float32, device=dev) if red == 1 else None
+    count = torch.empty((), dtype=torch.float32, device=dev) if keep_lse and red == 1 else None
     lse = torch.empty((n,), dtype=torch.float32, device=dev) if keep_lse else None
     if n or red:
         _native.cross_entropy(z, (n, classes, stride), targets.contiguous(), ignore_index,
@@ -366,7 +370,7 @@ def _like_rows(logits):
     if t is logits and classes < stride <= classes + 256:
         buf = torch.empty(n * stride, dtype=logits.dtype, device=logits.device)
         return buf.as_strided(logits.shape, logits.stride())
-    return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return logits.new_empty(logits.shape)
 
 
 class _CrossEntropy(Function):

@@ -242,6 +242,7 @@ def grad_bound(want, size, n, dtype):
 
 @pytest.mark.parametrize("tokens,vocab,dim,kind", [
     (1, 5, 1, "flat"), (2, 1, 8, "flat"), (63, 7, 24, "flat"), (64, 1000, 33, "flat"),
+    (256, 40, 136, "same"), (255, 90, 1036, "zipf"),
     (257, 300, 771, "zipf"), (1000, 100, 64, "same"), (2049, 50257, 192, "zipf"),
     (5000, 70000, 40, "zipf"), (8192, 50257, 64, "zipf"), (8193, 1009, 96, "zipf"),
     (20001, 131072, 72, "zipf"), (40000, 17, 136, "flat"), (66000, 70001, 16, "same"),
@@ -282,11 +283,13 @@ def test_position_gradient(T, batch, seq, rows, dim, dtype, out, p):
     close(dq, want, grad_bound(want, size, n, out))
 
 
+@pytest.mark.parametrize("batch", [1, 9])
 @pytest.mark.parametrize("dim", [1, 5, 13, 72, 515, 519, 1031])
 @pytest.mark.parametrize("out,p", [(F32, 0.0), (BF16, 0.0), (F32, 0.2)])
-def test_gradients_are_added(T, dim, out, p):
-    ids = ids_of((4, 500), 300)
-    g = normal(4, 500, dim)
+def test_gradients_are_added(T, batch, dim, out, p):
+    seq = 250
+    ids = ids_of((batch, seq), 300)
+    g = normal(batch, seq, dim)
     w0, p0 = normal(300, dim, dtype=out, seed=5), normal(512, dim, dtype=out, seed=6)
     w, pg = w0.to(DEV), p0.to(DEV)
     dw, dp = T.embedding_backward(g.to(DEV), ids.to(DEV), 300, pos_rows=512, scale=2.0,
@@ -296,9 +299,9 @@ def test_gradients_are_added(T, dim, out, p):
     close(w, want + w0.double(), grad_bound(want + w0.double(), size + w0.abs(), n, out))
     untouched = n[:, 0] == 0
     assert untouched.any() and torch.equal(w.cpu()[untouched], w0[untouched])
-    want, size, n = R.table_grad(g, torch.arange(500).expand(4, 500), 512, 1.0, p, RNG)
+    want, size, n = R.table_grad(g, torch.arange(seq).expand(batch, seq), 512, 1.0, p, RNG)
     close(pg, want + p0.double(), grad_bound(want + p0.double(), size + p0.abs(), n, out))
-    assert torch.equal(pg.cpu()[500:], p0[500:])
+    assert torch.equal(pg.cpu()[seq:], p0[seq:])
 
 
 def test_gradient_of_strided_output(T):

@@ -75,9 +75,9 @@ def test_entry_points_refuse_without_launching(lib):
                                       a["out"], a["rows"], 0, a["pout"], a["prows"], 0, a["ot"],
                                       a["ws"], a["nb"])
     for bad in (dict(g=None), dict(ids=None), dict(tokens=-1), dict(tokens=1 << 27),
-                dict(rows=-1), dict(rows=1 << 29), dict(dim=-1), dict(dim=1 << 30), dict(dt=9),
+                dict(rows=-1), dict(rows=1 << 27), dict(dim=-1), dict(dim=1 << 30), dict(dt=9),
                 dict(ot=9), dict(gs=-1), dict(cut=-2), dict(pout=one, prows=2, seq=0),
-                dict(pout=one, prows=2, seq=3), dict(pout=one, prows=1 << 29)):
+                dict(pout=one, prows=2, seq=3), dict(pout=one, prows=1 << 27)):
         assert grad(**bad) == 1, bad
         assert b"dmh_embedding_grad" in lib.dmh_last_error()
     assert grad(nb=3) == 2 and grad(ws=None) == 2
