@@ -172,13 +172,26 @@ def plain_step(arm, stacks, pgroups, ns_steps, events=None):
     return outs
 
 
-def _gpt2(vocab, ctx, d, layers, heads):
+def _gpt2(vocab, ctx, d, layers, heads, ops="torch", dropout=0.0):
     """GPT-2 with nn.Linear weights named as the reference's model names them
     (attn.c_attn, attn.c_proj, mlp.c_fc, mlp.c_proj; wte, wpe, tied lm_head), so
-    Muon routes and splits them the same way; bf16 autocast in the forward."""
+    Muon routes and splits them the same way; bf16 autocast in the forward.
+
+    model.train_step(idx, targets) computes the loss and every gradient.  ops: "torch" takes
+    the embedding, dropout (after the embedding and in front of the residual additions) and
+    the loss from torch, "hip" from defmuon_amd.train_ops."""
     import torch
     import torch.nn as nn
     import torch.nn.functional as F
+    from defmuon_amd import train_ops
+
+    def add(x, y):
+        """x + dropout(y)"""
+        if not dropout:
+            return x + y
+        if ops == "hip":
+            return train_ops.dropout(y, dropout, train_ops.draw_rng(), residual=x)
+        return x + F.dropout(y, dropout)
 
     class Attn(nn.Module):
         def __init__(self):
@@ -206,8 +219,8 @@ def _gpt2(vocab, ctx, d, layers, heads):
             self.ln_1, self.attn, self.ln_2, self.mlp = nn.LayerNorm(d), Attn(), nn.LayerNorm(d), Mlp()
 
         def forward(self, x):
-            x = x + self.attn(self.ln_1(x))
-            return x + self.mlp(self.ln_2(x))
+            x = add(x, self.attn(self.ln_1(x)))
+            return add(x, self.mlp(self.ln_2(x)))
 
     class GPT(nn.Module):
         def __init__(self):
@@ -218,12 +231,28 @@ def _gpt2(vocab, ctx, d, layers, heads):
             self.lm_head = nn.Linear(d, vocab, bias=False)
             self.lm_head.weight = self.wte.weight
 
-        def forward(self, idx, targets):
-            x = self.wte(idx) + self.wpe(torch.arange(idx.shape[1], device=idx.device))
+        def logits(self, idx):
+            if ops == "hip":
+                x = train_ops.embedding(idx, self.wte.weight, self.wpe.weight, dropout_p=dropout,
+                                        rng=train_ops.draw_rng() if dropout else None)
+            else:
+                x = self.wte(idx) + self.wpe(torch.arange(idx.shape[1], device=idx.device))
+                x = F.dropout(x, dropout) if dropout else x
             for blk in self.h:
                 x = blk(x)
-            logits = self.lm_head(self.ln_f(x))
-            return F.cross_entropy(logits.float().view(-1, vocab), targets.reshape(-1))
+            return self.lm_head(self.ln_f(x))
+
+        def train_step(self, idx, targets, autocast=True):
+            with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+                z = self.logits(idx)
+                if ops == "torch":
+                    loss = F.cross_entropy(z.float().view(-1, vocab), targets.reshape(-1))
+            if ops == "torch":
+                loss.backward()
+            else:   # the gradient takes the logits' memory
+                loss, dz = train_ops.cross_entropy_step(z, targets, inplace=True)
+                z.backward(dz)
+            return loss.detach()
 
     return GPT()
 
@@ -234,13 +263,14 @@ def train_step_report(args, dev):
     split), AdamW on embeddings, norms and biases.  Reports the step time, its
     forward+backward and optimizer parts, the polar path inside the optimizer step
     (events around the groups' clips + iterations) and its share, and the optimizer
-    step with the reference's torch glue instead of the fused glue."""
+    step with the reference's torch glue instead of the fused glue.  --ops and --dropout
+    choose where the model's embedding, dropout and loss come from."""
     import torch
     from defmuon_amd.optim import deflation_cutoff
     from defmuon_amd.optim.muon import Muon
     deflation_cutoff.install()
     torch.manual_seed(0)
-    model = _gpt2(50257, 1024, 1280, 36, 20).to(dev)
+    model = _gpt2(50257, 1024, 1280, 36, 20, args.ops, args.dropout).to(dev)
     g = torch.Generator(device=dev)
     g.manual_seed(1)
     tok = torch.randint(0, 50257, (8, 1025), device=dev, generator=g)
@@ -263,9 +293,7 @@ def train_step_report(args, dev):
     def one(evs):
         e = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
         e[0].record()
-        with torch.autocast("cuda", dtype=torch.bfloat16):
-            loss = model(x, y)
-        loss.backward()
+        model.train_step(x, y)
         e[1].record()
         opt.step()
         opt.zero_grad(set_to_none=True)
@@ -301,7 +329,7 @@ def train_step_report(args, dev):
             "data": "random init, random token ids uniform over 50257, batch 8 x 1024",
             "config": {"workload": "gpt2-large train step: d=1280, 36 layers, 20 heads, MLP "
                                    "5120; Muon deflated_ns_cut on 144 hidden matrices, AdamW "
-                                   "on the rest"}}
+                                   "on the rest", "ops": args.ops, "dropout": args.dropout}}
 
 
 def cpu_baseline(groups, arm, min_s=12.0, max_reps=20):
@@ -708,6 +736,12 @@ def main():
                          "kernel trace (see --summarize-trace); horner-f32: the fp32 "
                          "iteration (the convergence study's path) over the workload's "
                          "shape groups")
+    ap.add_argument("--ops", default="torch", choices=["torch", "hip"],
+                    help="--mode train: the model's embedding, dropout and loss from torch, or "
+                         "from defmuon_amd.train_ops")
+    ap.add_argument("--dropout", type=float, default=0.0, metavar="P",
+                    help="--mode train: dropout after the embedding and in front of the "
+                         "residual additions")
     ap.add_argument("--summarize-pmc", nargs="+", metavar="COUNTER_CSV",
                     help="print per-kernel counter sums per polar step of rocprofv3 --pmc "
                          "counter_collection.csv files taken over this bench with the same "

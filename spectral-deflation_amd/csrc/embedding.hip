@@ -20,55 +20,70 @@ struct EmbedArgs {
   void* out;
   long long tokens, vocab, wstride, prows, pstride;
   int is64, seq, dim;
+  int lanes, log_lanes;   // of a token
   float scale;
   Rng rng;
 };
 
-// Eight columns of one token a thread.  The last eight of a row overlap those before them where
-// the width is no multiple of eight (SPLIT), and are written twice with the same values; rows
-// narrower than eight go column by column (NARROW).
+// A token is `lanes` (a power of two up to a wave) neighbouring lanes' work, which take eight of
+// its columns each, `lanes` pieces apart: as many as leave the fewest idle at the row's end, so
+// that ids, positions and row addresses are found once for several pieces and without divisions.
+// The last eight columns of a row overlap those before them where the width is no multiple of
+// eight (SPLIT), and are written twice with the same values; rows narrower than eight go column
+// by column (NARROW).
 template <class TW, class TO, bool POS, bool DROP, bool SPLIT, bool NARROW>
 __global__ __launch_bounds__(256) void embed_rows(EmbedArgs a) {
-  constexpr int W = NARROW ? 1 : 8;
-  const int pieces = (a.dim + W - 1) / W;
-  const long long items = a.tokens * pieces, step = (long long)gridDim.x * 256;
+  constexpr int W = NARROW ? 1 : 8, AHEAD = 2;
+  const int lane = threadIdx.x & (a.lanes - 1);
+  const long long step = (long long)gridDim.x * (256 >> a.log_lanes);
   const RngKey key = DROP ? rng_key(a.rng) : RngKey{};
-  for (long long it = (long long)blockIdx.x * 256 + threadIdx.x; it < items; it += step) {
-    const bool small = items < (1LL << 32);   // cheaper divisions
-    const long long i = small ? (long long)((unsigned)it / (unsigned)pieces) : it / pieces;
-    int c = (int)(it - i * pieces) * W;
-    if (SPLIT && !NARROW) c = c + 8 > a.dim ? a.dim - 8 : c;
+  for (long long i = (long long)blockIdx.x * (256 >> a.log_lanes) + (threadIdx.x >> a.log_lanes);
+       i < a.tokens; i += step) {
     const long long id = load_index(a.ids, a.is64, i);
-    const long long t = !POS ? 0 : a.pos   ? load_index(a.pos, a.is64, i)
-                                : small ? (unsigned)i % (unsigned)a.seq
-                                        : i % a.seq;
-    const unsigned long long e = (unsigned long long)i * a.dim + c;
+    const long long t = !POS    ? 0
+                        : a.pos ? load_index(a.pos, a.is64, i)
+                        : a.tokens < (1LL << 32) ? (unsigned)i % (unsigned)a.seq
+                                                 : i % a.seq;
     const bool ok = (unsigned long long)id < (unsigned long long)a.vocab &&
                     (!POS || (unsigned long long)t < (unsigned long long)a.prows);
-    TO* o = (TO*)a.out + e;
-    const TW* w = (const TW*)a.w + (ok ? id : 0) * a.wstride + c;
-    const TW* p = (const TW*)a.p + (ok ? t : 0) * a.pstride + c;
-    if (NARROW) {
-      float v = __builtin_nanf("");
-      if (ok) {
-        v = POS ? fmaf((float)*w, a.scale, (float)*p) : (float)*w * a.scale;
-        if (DROP) v = kept(keep_bits_at<true>(a.rng, key, e), 0, v * a.rng.scale);
+    const unsigned long long row = (unsigned long long)i * a.dim;
+    TO* out = (TO*)a.out + row;
+    const TW* w = (const TW*)a.w + (ok ? id : 0) * a.wstride;
+    const TW* p = (const TW*)a.p + (ok ? t : 0) * a.pstride;
+    if (!ok) {
+      for (int c = lane; c < a.dim; c += a.lanes) out[c] = (TO)__builtin_nanf("");
+    } else if (NARROW) {
+      for (int c = lane; c < a.dim; c += a.lanes) {
+        float v = POS ? fmaf((float)w[c], a.scale, (float)p[c]) : (float)w[c] * a.scale;
+        if (DROP) v = kept(keep_bits_at<true>(a.rng, key, row + c), 0, v * a.rng.scale);
+        out[c] = (TO)v;
       }
-      *o = (TO)v;
     } else {
-      float v[8], q[8] = {};
-      if (ok) {
-        load8(w, v);
-        if (POS) load8(p, q);
-      }
-      const uint32_t bits = DROP ? keep_bits_at<SPLIT>(a.rng, key, e) : 0;
+      for (int c0 = lane * W; c0 < a.dim; c0 += AHEAD * W * a.lanes) {
+        Raw8<TW> x[AHEAD], q[AHEAD];
+        int c[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = POS ? fmaf(v[j], a.scale, q[j]) : v[j] * a.scale;
-        if (DROP) v[j] = kept(bits, j, v[j] * a.rng.scale);
-        if (!ok) v[j] = __builtin_nanf("");
+        for (int k = 0; k < AHEAD; ++k) {
+          c[k] = c0 + k * W * a.lanes;
+          // beyond the row: the piece before again
+          c[k] = c[k] >= a.dim ? c0 : c[k];
+          c[k] = SPLIT && c[k] + 8 > a.dim ? a.dim - 8 : c[k];
+          x[k].load(w + c[k]);
+          if (POS) q[k].load(p + c[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          if (k && c0 + k * W * a.lanes >= a.dim) break;
+          const uint32_t bits = DROP ? keep_bits_at<SPLIT>(a.rng, key, row + c[k]) : 0;
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = POS ? fmaf(x[k][j], a.scale, q[k][j]) : x[k][j] * a.scale;
+            if (DROP) v[j] = kept(bits, j, v[j] * a.rng.scale);
+          }
+          store8(out + c[k], v);
+        }
       }
-      store8(o, v);
     }
   }
 }
@@ -466,7 +481,8 @@ __global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
 // 21.0 / 21.6 for 16000, 37.2 / 32.0 for 50257, where every workgroup's own sort is in the way of
 // the clearing; dim 1280: 18.6 / 19.9 for 2000, 20.2 / 19.8 for 4000, 24.1 / 21.6 for 8000.
 constexpr int SMALL_TOKENS = 256, SMALL_ROWS = 16, SMALL_AHEAD = 8;
-constexpr long long SMALL_TABLE = 6 << 20;   // elements
+// 16 tokens, dim 768: 14.6 / 17.4 for 8000, 14.7 / 17.1 for 16000, 19.9 / 18.7 for 32000.
+constexpr long long SMALL_TABLE = 6 << 20, SMALL_TABLE_FEW = 16 << 20;   // elements
 
 template <class TG, class TO, bool DROP>
 __global__ __launch_bounds__(256) void embed_grad_small(GradArgs a) {
@@ -610,8 +626,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join(GradArgs a) {
 
 template <class TW, class TO, bool POS, bool DROP>
 static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
-  const int w = a.dim < 8 ? 1 : 8;
-  const long long groups = (a.tokens * ((a.dim + w - 1) / w) + 255) / 256;
+  const long long groups = (a.tokens + (256 >> a.log_lanes) - 1) / (256 >> a.log_lanes);
   const dim3 grid((unsigned)(groups < (1 << 22) ? groups : (1 << 22))), block(256);
   if (a.dim < 8)
     hipLaunchKernelGGL((embed_rows<TW, TO, POS, DROP, true, true>), grid, block, 0, stream, a);
@@ -765,6 +780,18 @@ int dmh_embedding(hipStream_t stream, const void* ids, int ids_64, long long tok
   a.is64 = ids_64 != 0;
   a.seq = seq;
   a.dim = dim;
+  // the most lanes of those that leave the fewest idle in a row's last round
+  const int pieces = dim < 8 ? dim : ceil_div(dim, 8);
+  int best = 1 << 30;
+  for (int l = 6; l >= 0; --l) {
+    const int rounds = ceil_div(pieces, 1 << l);
+    if (rounds > 8 && l < 6) break;
+    if (rounds << l < best) {
+      best = rounds << l;
+      a.log_lanes = l;
+      a.lanes = 1 << l;
+    }
+  }
   a.scale = scale;
   a.rng = make_rng(seed, offset, rng_state, cut);
   DMH_FOR_TYPE(dtype, TW, DMH_FOR_TYPE(out_dtype, TO, (launch_rows<TW, TO>(stream, a))))
@@ -830,7 +857,8 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
              (char*)ws + ts.bytes, ps);
   const int sorts = (a.job[0].ids != nullptr) + (a.job[1].ids != nullptr);
   a.small = dim >= 8 && tokens <= SMALL_TOKENS &&
-            ((tok ? rows : 0) + (pos ? pos_rows : 0)) * dim <= SMALL_TABLE;
+            ((tok ? rows : 0) + (pos ? pos_rows : 0)) * dim <=
+                (tokens <= CHUNK ? SMALL_TABLE_FEW : SMALL_TABLE);
   if (tokens > 0 && sorts && !a.small) {
     if (tokens <= RANK_MAX) {
       hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), sorts),

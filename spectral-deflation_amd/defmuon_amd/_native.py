@@ -512,34 +512,35 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
 
 
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
-                  count, lse, dlogits, dstride):
+                  dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
-    stride) of the logits.  A mean's count of rows is kept in `count` if that is wanted."""
+    stride) of the logits.  Returns what the backward pass needs: fp32, each row's lse and then
+    the number of rows with a target (for a mean)."""
     n, classes, zs = rows
     lib = load()
-    nbytes = 4 * n   # dmh_cross_entropy_workspace_size, and a place for the count
-    ws = torch.empty(n + 1, dtype=torch.float32, device=logits.device) if reduction else None
+    nbytes = 4 * n   # dmh_cross_entropy_workspace_size
+    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=logits.device)
+    at = stats.data_ptr()
     _check(lib.dmh_cross_entropy(_raw_stream(logits.device.index), logits.data_ptr(),
                                  FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
                                  targets.dtype == torch.int64, ignore, smoothing, z_loss,
-                                 reduction, grad_scale, loss.data_ptr(),
-                                 count.data_ptr() if count is not None else
-                                 ws.data_ptr() + nbytes if reduction else 0,
-                                 0 if lse is None else lse.data_ptr(),
+                                 reduction, grad_scale, loss.data_ptr(), at + nbytes, at,
                                  0 if dlogits is None else dlogits.data_ptr(), dstride,
-                                 0 if ws is None else ws.data_ptr(), nbytes),
+                                 at + nbytes + 4, nbytes),
            "dmh_cross_entropy")
+    return stats
 
 
-def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, lse, count, grad_out,
-                       per_row, dlogits, dstride):
-    """The gradient of the logits from a forward pass's lse, times grad_out."""
+def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reduction, stats,
+                       grad_out, dlogits, dstride):
+    """The gradient of the logits from cross_entropy's statistics, times grad_out."""
     n, classes, zs = rows
+    at = stats.data_ptr()
     _check(load().dmh_cross_entropy_grad(_raw_stream(logits.device.index), logits.data_ptr(),
                                          FLOATS[logits.dtype], n, classes, zs,
                                          targets.data_ptr(), targets.dtype == torch.int64,
-                                         ignore, smoothing, z_loss, lse.data_ptr(),
-                                         0 if count is None else count.data_ptr(),
-                                         grad_out.data_ptr(), per_row, dlogits.data_ptr(),
-                                         dstride),
+                                         ignore, smoothing, z_loss, at,
+                                         at + 4 * n if reduction == 1 else 0,
+                                         grad_out.data_ptr(), reduction == 0,
+                                         dlogits.data_ptr(), dstride),
            "dmh_cross_entropy_grad")

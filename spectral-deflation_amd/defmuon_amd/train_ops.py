@@ -347,20 +347,19 @@ def _xent_args(logits, targets, label_smoothing, z_loss, reduction, what):
         raise NativeError(f"{what}: reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
 
 
-def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, keep_lse=False,
-          dlogits=None, grad_scale=1.0):
-    """(loss, count, lse) and, in place, dlogits."""
-    dev = logits.device
+def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, dlogits=None,
+          grad_scale=1.0):
+    """(loss, statistics for the backward pass) and, in place, dlogits."""
     z, n, classes, stride = _rows(logits)
     red = _REDUCTIONS[reduction]
-    loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32, device=dev)
-    count = torch.empty((), dtype=torch.float32, device=dev) if keep_lse and red == 1 else None
-    lse = torch.empty((n,), dtype=torch.float32, device=dev) if keep_lse else None
+    loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32,
+                       device=logits.device)
+    stats = None
     if n or red:
-        _native.cross_entropy(z, (n, classes, stride), targets.contiguous(), ignore_index,
-                              smoothing, z_loss, red, grad_scale, loss, count, lse, dlogits,
-                              0 if dlogits is None else _rows(dlogits)[3])
-    return loss, count, lse
+        stats = _native.cross_entropy(z, (n, classes, stride), targets.contiguous(),
+                                      ignore_index, smoothing, z_loss, red, grad_scale, loss,
+                                      dlogits, 0 if dlogits is None else _rows(dlogits)[3])
+    return loss, stats
 
 
 def _like_rows(logits):
@@ -376,24 +375,20 @@ def _like_rows(logits):
 class _CrossEntropy(Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
-        loss, count, lse = _xent(logits, targets, ignore_index, smoothing, z_loss, reduction,
-                                 keep_lse=True)
-        ctx.save_for_backward(logits, targets, count, lse)
-        ctx.args = ignore_index, smoothing, z_loss, reduction
+        loss, stats = _xent(logits, targets, ignore_index, smoothing, z_loss, reduction)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.args = ignore_index, smoothing, z_loss, _REDUCTIONS[reduction]
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        logits, targets, count, lse = ctx.saved_tensors
-        ignore_index, smoothing, z_loss, reduction = ctx.args
+        logits, targets, stats = ctx.saved_tensors
         dz = _like_rows(logits)
         if dz.numel():
-            z, n, classes, stride = _rows(logits)
-            _native.cross_entropy_grad(z, (n, classes, stride), targets.contiguous(),
-                                       ignore_index, smoothing, z_loss, lse, count,
-                                       grad.float().contiguous(), reduction == "none", dz,
-                                       _rows(dz)[3])
+            z, *rows = _rows(logits)
+            _native.cross_entropy_grad(z, rows, targets.contiguous(), *ctx.args, stats,
+                                       grad.float().contiguous(), dz, _rows(dz)[3])
         return dz, *[None] * 5
 
 
@@ -434,6 +429,6 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
         dlogits = logits
     else:
         dlogits = _like_rows(logits)
-    loss, _, _ = _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction,
+    loss, _ = _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction,
                        dlogits=dlogits, grad_scale=grad_scale)
     return loss, dlogits

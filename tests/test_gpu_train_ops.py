@@ -709,3 +709,34 @@ def test_in_a_captured_graph(T):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), k
+
+
+def test_model_step_matches_torch():
+    """The GPT-2 training step of the benchmark with these operators and with torch's, in fp32:
+    the same loss and gradients.  Each gradient differs by the rounding of sums of some thousand
+    fp32 terms (2^-24 each, relative to its norm) at each of a dozen products on its way."""
+    import bench
+    tok = ids_of((3, 41), 517, kind="flat").to(DEV)
+    got = {}
+    for ops in ("torch", "hip"):
+        torch.manual_seed(0)
+        m = bench._gpt2(517, 64, 64, 2, 4, ops).to(DEV)
+        loss = m.train_step(tok[:, :-1], tok[:, 1:], autocast=False)
+        got[ops] = float(loss), {n: p.grad for n, p in m.named_parameters()}
+    (a, ga), (b, gb) = got["torch"], got["hip"]
+    assert abs(a - b) <= 1e-5 * a
+    assert ga.keys() == gb.keys()
+    for n in ga:
+        assert float((ga[n] - gb[n]).norm()) <= 12 * 2000 * E32 * float(ga[n].norm()), n
+
+
+def test_model_step_with_dropout_follows_the_seed():
+    import bench
+    tok = ids_of((3, 41), 517, kind="flat").to(DEV)
+    m = bench._gpt2(517, 64, 64, 2, 4, "hip", 0.3).to(DEV)
+    losses = []
+    for seed in (1, 2, 1):
+        torch.manual_seed(seed)
+        losses.append(float(m.train_step(tok[:, :-1], tok[:, 1:])))
+    assert losses[0] == losses[2] != losses[1]
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())
