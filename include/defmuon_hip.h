@@ -280,7 +280,7 @@ int dmh_embedding_grad(dmh_stream_t stream, const void* ids, const void* positio
  *              logits' type; may be the logits themselves; NULL for the loss alone
  * dmh_cross_entropy_grad: the gradient from a forward call's lse (and count, for a mean; NULL
  * otherwise), times *grad_out, or grad_out[row] if grad_out_rows.
- * 1 <= classes <= 2^27, rows < 2^23. */
+ * 1 <= classes <= 2^27, rows < 2^22. */
 int dmh_cross_entropy_workspace_size(long long rows, long long classes, size_t* bytes);
 int dmh_cross_entropy(dmh_stream_t stream, const void* logits, int dtype, long long rows,
                       long long classes, long long z_rstride, const void* targets,

@@ -448,7 +448,7 @@ static bool row_in_registers(int dtype, long long classes) {
 }
 
 static bool xent_shape(long long rows, long long classes) {
-  return rows >= 0 && rows < (1LL << 23) && classes >= 1 && classes <= (1LL << 27);
+  return rows >= 0 && rows < (1LL << 22) && classes >= 1 && classes <= (1LL << 27);
 }
 
 }  // namespace dmh

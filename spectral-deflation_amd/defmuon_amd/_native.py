@@ -459,16 +459,31 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _on_device(call):
+    """`call` with the device of its first tensor current: a default stream's handle, null,
+    means the current device's."""
+    @functools.wraps(call)
+    def on_device(first, *args):
+        index = first.device.index
+        if index == torch.cuda.current_device():
+            return call(first, *args)
+        with torch.cuda.device(index):
+            return call(first, *args)
+    return on_device
+
+
+@_on_device
 def dropout(x, residual, out, cut, rng, rows):
     """out = dropout(x) [+ residual]; rows: (rows, cols, x's row stride, the residual's)."""
     n, cols, xs, rs = rows
     seed, offset, state = rng
-    _check(load().dmh_dropout(_raw_stream(x.device.index), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
-                              0 if residual is None else residual.data_ptr(), rs,
+    _check(load().dmh_dropout(_raw_stream(x.device.index), x.data_ptr(), FLOATS[x.dtype], n,
+                              cols, xs, 0 if residual is None else residual.data_ptr(), rs,
                               out.data_ptr(), FLOATS[out.dtype], cut, seed, offset, state),
            "dmh_dropout")
 
 
+@_on_device
 def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     """Token rows times scale plus position rows through dropout into out (tokens, dim)."""
     seed, offset, state = rng
@@ -493,6 +508,7 @@ def embedding_grad_workspace_bytes(tokens, dim, sorts):
     return nbytes.value
 
 
+@_on_device
 def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx, scale, cut, rng,
                    out, add, pos_out, pos_add):
     """The gradients of the token table (out) and the position table (pos_out), either None."""
@@ -511,6 +527,7 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
            "dmh_embedding_grad")
 
 
+@_on_device
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
                   dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
@@ -531,6 +548,7 @@ def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, g
     return stats
 
 
+@_on_device
 def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reduction, stats,
                        grad_out, dlogits, dstride):
     """The gradient of the logits from cross_entropy's statistics, times grad_out."""

@@ -414,8 +414,8 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     autograd: each is read once and its gradient written once.
 
     dlogits is the gradient of grad_scale * loss (1 / micro-batches, a loss scale) in the
-    logits' type; with inplace it takes the logits' own memory.  logits.backward(dlogits)
-    goes on from there."""
+    logits' type; with inplace it takes the logits' own memory (what lies beside the rows of a
+    padded view stays).  logits.backward(dlogits) goes on from there."""
     what = "cross_entropy_step"
     logits = logits.detach()
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)

@@ -49,7 +49,7 @@ def drop_bound(x, r, want, dtype):
 
 
 @pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
-@pytest.mark.parametrize("shape", [(1,), (7,), (1, 8), (3, 8), (5, 771), (64, 768),
+@pytest.mark.parametrize("shape", [(), (1,), (7,), (1, 8), (3, 8), (5, 771), (64, 768),
                                    (2, 3, 5, 33), (257, 2050)])
 @pytest.mark.parametrize("dtype,res", [(F32, None), (BF16, None), (F16, None), (BF16, F32),
                                        (F16, F16), (F32, BF16)])

@@ -99,7 +99,7 @@ def test_entry_points_refuse_without_launching(lib):
                                      -100, 0.0, 0.0, a["red"], 1.0, a["loss"], a["count"], None,
                                      None, a["ds"], a["ws"], a["nb"])
     for bad in (dict(z=None), dict(y=None), dict(loss=None), dict(count=None), dict(dt=3),
-                dict(rows=-1), dict(rows=1 << 23), dict(v=0), dict(v=1 << 31), dict(zs=-1),
+                dict(rows=-1), dict(rows=1 << 22), dict(v=0), dict(v=1 << 31), dict(zs=-1),
                 dict(ds=-1), dict(red=3), dict(red=-1)):
         assert xent(**bad) == 1, bad
         assert b"dmh_cross_entropy" in lib.dmh_last_error()
@@ -113,7 +113,7 @@ def test_entry_points_refuse_without_launching(lib):
                                           a["y"], 1, -100, 0.0, 0.0, a["lse"], None, a["go"], 0,
                                           a["dz"], a["ds"])
     for bad in (dict(z=None), dict(y=None), dict(lse=None), dict(go=None), dict(dz=None),
-                dict(dt=5), dict(rows=1 << 23), dict(v=0), dict(zs=-2), dict(ds=-2)):
+                dict(dt=5), dict(rows=1 << 22), dict(v=0), dict(zs=-2), dict(ds=-2)):
         assert xgrad(**bad) == 1, bad
         assert b"dmh_cross_entropy_grad" in lib.dmh_last_error()
     assert xgrad(rows=0) == 0
