@@ -38,13 +38,14 @@ __device__ __forceinline__ float exp_diff(float x, float m) {
   return __builtin_amdgcn_exp2f((x - m) * LOG2E);
 }
 
-// The sum of one value a thread over THREADS threads: a wave, or a workgroup of as many.
+// The sum of one value a thread over THREADS threads: part of a wave, a wave, or a workgroup of as
+// many.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* lds) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1) v += __shfl_xor(v, d);
   constexpr int W = THREADS / 64;
-  if (W == 1) return v;
+  if (W <= 1) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -68,9 +69,10 @@ __device__ __forceinline__ Part join(Part a, Part b) {
 template <int THREADS>
 __device__ __forceinline__ Part block_join(Part p, Part* lds) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
+    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
   constexpr int W = THREADS / 64;
-  if (W == 1) return p;
+  if (W <= 1) return p;
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
   __syncthreads();
   // every wave joins the waves' parts in the same way
@@ -80,20 +82,27 @@ __device__ __forceinline__ Part block_join(Part p, Part* lds) {
   return {__shfl(p.m, 0), __shfl(p.s, 0)};
 }
 
-// The number of rows that have a target, in every thread of the workgroup.
-template <int THREADS>
+// The number of rows that have a target, in every thread of the workgroup.  One workgroup goes
+// through all rows, so it has AHEAD loads a thread on their way.
+template <int THREADS, int AHEAD>
 __device__ __forceinline__ float count_targets(const XentArgs& a, float* lds) {
   int n = 0;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < (int)a.rows; i += THREADS)
-    n += load_index(a.targets, a.t64, i) != a.ignore;
-  // exact below 2^24 rows
-  return block_sum<THREADS>((float)n, lds);
+  const int rows = (int)a.rows;
+  auto count = [&](auto* targets) {
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * THREADS < rows; i += AHEAD * THREADS) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) n += targets[i + k * THREADS] != a.ignore;
+    }
+    for (; i < rows; i += THREADS) n += targets[i] != a.ignore;
+  };
+  if (a.t64) count((const long long*)a.targets); else count((const int*)a.targets);
+  return block_sum<THREADS>((float)n, lds);   // exact: below 2^24 rows
 }
 
 __global__ __launch_bounds__(1024) void xent_count(XentArgs a, float* count) {
   __shared__ float lds[16];
-  const float n = count_targets<1024>(a, lds);
+  const float n = count_targets<1024, 8>(a, lds);
   if (threadIdx.x == 0) *count = n;
 }
 
@@ -102,11 +111,20 @@ __global__ __launch_bounds__(1024) void xent_count(XentArgs a, float* count) {
 template <bool COUNT>
 __global__ __launch_bounds__(1024) void xent_reduce(XentArgs a, float* count, float* loss) {
   __shared__ float lds[16];
+  constexpr int AHEAD = 16;
+  const int rows = (int)a.rows;
   float s = 0.f;
-#pragma unroll 8
-  for (long long i = threadIdx.x; i < a.rows; i += 1024) s += a.row_loss[i];
+  int i = threadIdx.x;
+  for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
+    float v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = a.row_loss[i + k * 1024];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) s += v[k];
+  }
+  for (; i < rows; i += 1024) s += a.row_loss[i];
   s = block_sum<1024>(s, lds);
-  const float n = COUNT ? count_targets<1024>(a, lds) : count ? *count : 1.f;
+  const float n = COUNT ? count_targets<1024, 8>(a, lds) : count ? *count : 1.f;
   if (threadIdx.x == 0) {
     if (COUNT) *count = n;
     *loss = s / n;
@@ -171,13 +189,14 @@ __device__ __forceinline__ void repack(i32x4 (&x)[HELD]) {
 }
 
 template <class T, int THREADS, int HELD, bool GRAD, bool COUNT>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, HELD > 8 ? 4 : THREADS == 64 ? 7 : 8) void xent_row(XentArgs a) {
+__global__ __launch_bounds__(THREADS < 128 ? 256 : THREADS,
+                             HELD > 16 ? 2 : HELD > 8 ? 4 : THREADS < 128 ? 7 : 8) void xent_row(XentArgs a) {
   __shared__ Part parts[16];
   __shared__ float lds[16];
-  constexpr int N = Piece<T>::N, GROUP = THREADS < 256 ? 256 : THREADS;
+  constexpr int N = Piece<T>::N, GROUP = THREADS < 128 ? 256 : THREADS;
   float count = 1.f;
   if (COUNT)
-    count = count_targets<GROUP>(a, lds);
+    count = count_targets<GROUP, 2>(a, lds);
   else if (a.count)
     count = *a.count;
   const long long row = THREADS == GROUP
@@ -408,17 +427,25 @@ __global__ __launch_bounds__(256) void xent_grad(XentArgs a) {
 template <class T, bool GRAD, bool COUNT>
 static void launch_rows(hipStream_t stream, const XentArgs& a) {
   const int pieces = a.classes / Piece<T>::N, rows = (int)a.rows;   // at most
-  if (pieces <= 64 * 8)
-    hipLaunchKernelGGL((xent_row<T, 64, 8, GRAD, COUNT>), dim3(ceil_div(rows, 4)), dim3(256), 0,
-                       stream, a);
-  else if (pieces <= 256 * 8)
-    hipLaunchKernelGGL((xent_row<T, 256, 8, GRAD, COUNT>), dim3(rows), dim3(256), 0, stream, a);
-  else if (pieces <= 1024 * 8)
-    hipLaunchKernelGGL((xent_row<T, 1024, 8, GRAD, COUNT>), dim3(rows), dim3(1024), 0, stream, a);
-  else if (pieces <= 1024 * 16)
-    hipLaunchKernelGGL((xent_row<T, 1024, 16, GRAD, COUNT>), dim3(rows), dim3(1024), 0, stream, a);
-  else
-    hipLaunchKernelGGL((xent_stream<T, GRAD>), dim3(rows), dim3(1024), 0, stream, a);
+#define DMH_ROWS(THREADS, HELD)                                                           \
+  if (pieces <= THREADS * HELD) {                                                         \
+    constexpr int PER = THREADS < 128 ? 256 / THREADS : 1;                                \
+    hipLaunchKernelGGL((xent_row<T, THREADS, HELD, GRAD, COUNT>), dim3(ceil_div(rows, PER)), \
+                       dim3(PER * THREADS), 0, stream, a);                                \
+    return;                                                                               \
+  }
+  DMH_ROWS(16, 8)
+  DMH_ROWS(64, 8)
+  DMH_ROWS(128, 8)
+  DMH_ROWS(256, 8)
+  DMH_ROWS(512, 8)
+  DMH_ROWS(1024, 8)
+  if constexpr (GRAD) {
+    DMH_ROWS(1024, 16)
+    DMH_ROWS(512, 48)
+  }
+#undef DMH_ROWS
+  hipLaunchKernelGGL((xent_stream<T, GRAD>), dim3(rows), dim3(1024), 0, stream, a);
 }
 template <class T>
 static void launch_xent(hipStream_t stream, const XentArgs& a) {
@@ -444,7 +471,7 @@ constexpr long long COUNT_ROWS = 2048;
 
 // what launch_rows asks of xent_row
 static bool row_in_registers(int dtype, long long classes) {
-  return classes / (dtype == DMH_F32 ? 4 : 8) <= 1024 * 16;
+  return classes / (dtype == DMH_F32 ? 4 : 8) <= 512 * 48;
 }
 
 static bool xent_shape(long long rows, long long classes) {
