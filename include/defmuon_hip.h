@@ -258,9 +258,10 @@ int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long to
  * written, those that no token names with zero; with `accumulate` the sums are added to what
  * it holds and other rows stay untouched.  padding_idx (-1: none) and ids outside a table
  * take no gradient.  tokens, rows < 2^27.
- * The workspace depends on how many of the outputs are wanted through ids or positions
- * (`sorts`, 0 .. 2; implicit positions need no sort). */
-int dmh_embedding_grad_workspace_size(long long tokens, int dim, int sorts, size_t* bytes);
+ * Workspace: for the rows of the outputs that are wanted (0: not wanted); positions: nonzero if
+ * positions are given. */
+int dmh_embedding_grad_workspace_size(long long tokens, long long rows, long long pos_rows,
+                                      int dim, int positions, size_t* bytes);
 int dmh_embedding_grad(dmh_stream_t stream, const void* ids, const void* positions, int ids_64,
                        long long tokens, int seq, const void* grad, int dtype,
                        long long g_rstride, int dim, long long padding_idx, float scale,

@@ -734,6 +734,12 @@ static GradSpace grad_space(long long tokens, int dim, bool sorted) {
   return g;
 }
 
+// Whether the gradients take one launch (embed_grad_small), and no workspace.
+static bool small_grad(long long tokens, long long rows, int dim) {
+  return dim >= 8 && tokens <= SMALL_TOKENS &&
+         rows * dim <= (tokens <= CHUNK ? SMALL_TABLE_FEW : SMALL_TABLE);
+}
+
 static bool grad_shape(long long tokens, long long rows, long long pos_rows, int dim) {
   // launches stay below 2^32 threads
   return tokens >= 0 && tokens < (1LL << 27) && rows >= 0 && rows < (1LL << 27) &&
@@ -821,13 +827,17 @@ int dmh_embedding(hipStream_t stream, const void* ids, int ids_64, long long tok
   return DMH_OK;
 }
 
-int dmh_embedding_grad_workspace_size(long long tokens, int dim, int sorts, size_t* bytes) {
-  if (!bytes || !grad_shape(tokens, 0, 0, dim) || sorts < 0 || sorts > 2) {
-    set_error("dmh_embedding_grad_workspace_size: bad arguments (tokens=%lld dim=%d sorts=%d)",
-              tokens, dim, sorts);
+int dmh_embedding_grad_workspace_size(long long tokens, long long rows, long long pos_rows,
+                                      int dim, int positions, size_t* bytes) {
+  if (!bytes || !grad_shape(tokens, rows, pos_rows, dim)) {
+    set_error("dmh_embedding_grad_workspace_size: bad arguments (tokens=%lld rows=%lld,%lld "
+              "dim=%d)", tokens, rows, pos_rows, dim);
     return DMH_EINVAL;
   }
-  *bytes = grad_space(tokens, dim, sorts > 0).bytes + grad_space(tokens, dim, sorts > 1).bytes;
+  *bytes = small_grad(tokens, rows + pos_rows, dim)
+               ? 0
+               : (rows ? grad_space(tokens, dim, true).bytes : 0) +
+                     (pos_rows ? grad_space(tokens, dim, positions != 0).bytes : 0);
   return DMH_OK;
 }
 
@@ -853,7 +863,9 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   }
   const GradSpace ts = tok ? grad_space(tokens, dim, true) : GradSpace{};
   const GradSpace ps = pos ? grad_space(tokens, dim, positions != nullptr) : GradSpace{};
-  const size_t need = ts.bytes + ps.bytes;
+  size_t need;
+  dmh_embedding_grad_workspace_size(tokens, tok ? rows : 0, pos ? pos_rows : 0, dim,
+                                    positions != nullptr, &need);
   if (need > 0 && (!ws || ws_bytes < need)) {
     set_error("dmh_embedding_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
     return DMH_EWORKSPACE;
@@ -877,9 +889,7 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
     grad_job(a.job[1], a, positions, pos_out, pos_rows, -1, a.rng.scale, pos_accumulate != 0,
              (char*)ws + ts.bytes, ps);
   const int sorts = (a.job[0].ids != nullptr) + (a.job[1].ids != nullptr);
-  a.small = dim >= 8 && tokens <= SMALL_TOKENS &&
-            ((tok ? rows : 0) + (pos ? pos_rows : 0)) * dim <=
-                (tokens <= CHUNK ? SMALL_TABLE_FEW : SMALL_TABLE);
+  a.small = small_grad(tokens, (tok ? rows : 0) + (pos ? pos_rows : 0), dim);
   if (tokens > 0 && sorts && !a.small) {
     if (tokens <= RANK_MAX) {
       hipLaunchKernelGGL(embed_rank, dim3(ceil_div(tokens, RANK_TOKENS), sorts),

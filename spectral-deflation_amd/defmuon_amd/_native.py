@@ -72,7 +72,8 @@ _SIGS = {
     "dmh_embedding": (c_int, [c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll, c_int, c_ll,
                               c_vp, c_ll, c_ll, c_vp, c_float, c_int, c_ull, c_ull, c_vp, c_vp,
                               c_int]),
-    "dmh_embedding_grad_workspace_size": (c_int, [c_ll, c_int, c_int, ctypes.POINTER(c_sz)]),
+    "dmh_embedding_grad_workspace_size": (c_int, [c_ll, c_ll, c_ll, c_int, c_int,
+                                                  ctypes.POINTER(c_sz)]),
     "dmh_embedding_grad": (c_int, [c_vp, c_vp, c_vp, c_int, c_ll, c_int, c_vp, c_int, c_ll,
                                    c_int, c_ll, c_float, c_int, c_ull, c_ull, c_vp, c_vp, c_ll,
                                    c_int, c_vp, c_ll, c_int, c_int, c_vp, c_sz]),
@@ -458,6 +459,8 @@ FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
 
 def _on_device(call):
     """`call` with the device of its first tensor current: a default stream's handle, null,
@@ -465,7 +468,7 @@ def _on_device(call):
     @functools.wraps(call)
     def on_device(first, *args):
         index = first.device.index
-        if index == torch.cuda.current_device():
+        if index == _current_device():
             return call(first, *args)
         with torch.cuda.device(index):
             return call(first, *args)
@@ -500,10 +503,11 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
 
 
 @functools.lru_cache(maxsize=1024)
-def embedding_grad_workspace_bytes(tokens, dim, sorts):
-    """Workspace of embedding_grad with `sorts` tables whose rows ids or positions name."""
+def embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions):
+    """Workspace of embedding_grad (0 rows: that table's gradient is not wanted)."""
     nbytes = c_sz()
-    _check(load().dmh_embedding_grad_workspace_size(tokens, dim, sorts, ctypes.byref(nbytes)),
+    _check(load().dmh_embedding_grad_workspace_size(tokens, rows, pos_rows, dim, positions,
+                                                    ctypes.byref(nbytes)),
            "dmh_embedding_grad_workspace_size")
     return nbytes.value
 
@@ -513,17 +517,18 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
                    out, add, pos_out, pos_add):
     """The gradients of the token table (out) and the position table (pos_out), either None."""
     seed, offset, state = rng
-    some = pos_out if out is None else out
-    nbytes = embedding_grad_workspace_bytes(tokens, dim, 2)
-    ws = _workspace(nbytes, some.device)
-    rows = (0, 0) if out is None else (out.data_ptr(), out.shape[0])
-    prows = (0, 0) if pos_out is None else (pos_out.data_ptr(), pos_out.shape[0])
-    _check(load().dmh_embedding_grad(_raw_stream(some.device.index), ids.data_ptr(),
+    rows = 0 if out is None else out.shape[0]
+    pos_rows = 0 if pos_out is None else pos_out.shape[0]
+    nbytes = embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions is not None)
+    ws = _workspace(nbytes, ids.device) if nbytes else None
+    _check(load().dmh_embedding_grad(_raw_stream(ids.device.index), ids.data_ptr(),
                                      0 if positions is None else positions.data_ptr(),
                                      ids.dtype == torch.int64, tokens, seq, grad.data_ptr(),
                                      FLOATS[grad.dtype], gstride, dim, padding_idx, scale, cut,
-                                     seed, offset, state, *rows, add, *prows, pos_add,
-                                     FLOATS[some.dtype], ws.data_ptr(), nbytes),
+                                     seed, offset, state, out.data_ptr() if rows else 0, rows,
+                                     add, pos_out.data_ptr() if pos_rows else 0, pos_rows,
+                                     pos_add, FLOATS[(out if rows else pos_out).dtype],
+                                     ws.data_ptr() if nbytes else 0, nbytes),
            "dmh_embedding_grad")
 
 

@@ -271,14 +271,15 @@ def _padding(padding_idx, rows, what):
         raise NativeError(f"{what}: padding_idx {padding_idx} is not one of {rows} rows")
 
 
-def _table_grad(given, rows, dim, dtype, device, what, name):
+def _table_grad(given, rows, dtype, grad, what, name):
     """(tensor, add to it) for the gradient of a table."""
+    dim = grad.shape[-1]
     if given is None:
-        return torch.empty((rows, dim), dtype=dtype, device=device), False
+        return grad.new_empty((rows, dim), dtype=dtype), False
     _float(given, what, name)
-    if given.shape != (rows, dim) or given.device != device or not given.is_contiguous():
-        raise NativeError(f"{what}: {name} must be contiguous ({rows}, {dim}) on {device}, got "
-                          f"{tuple(given.shape)} on {given.device}")
+    if given.shape != (rows, dim) or given.device != grad.device or not given.is_contiguous():
+        raise NativeError(f"{what}: {name} must be contiguous ({rows}, {dim}) on {grad.device}, "
+                          f"got {tuple(given.shape)} on {given.device}")
     return given, True
 
 
@@ -312,9 +313,9 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     dw = dp = None
     add = pos_add = False
     if rows:
-        dw, add = _table_grad(weight_grad, rows, dim, dtype, grad.device, what, "weight_grad")
+        dw, add = _table_grad(weight_grad, rows, dtype, grad, what, "weight_grad")
     if pos_rows:
-        dp, pos_add = _table_grad(pos_grad, pos_rows, dim, dtype, grad.device, what, "pos_grad")
+        dp, pos_add = _table_grad(pos_grad, pos_rows, dtype, grad, what, "pos_grad")
     padding_idx = -1 if padding_idx is None else padding_idx
     if dw is not None and dp is not None and dw.dtype != dp.dtype:
         # one launch writes one type
@@ -347,10 +348,10 @@ def _xent_args(logits, targets, label_smoothing, z_loss, reduction, what):
         raise NativeError(f"{what}: reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
 
 
-def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, dlogits=None,
-          grad_scale=1.0):
-    """(loss, statistics for the backward pass) and, in place, dlogits."""
-    z, n, classes, stride = _rows(logits)
+def _xent(logits, rows, targets, ignore_index, smoothing, z_loss, reduction, dlogits=None,
+          dstride=0, grad_scale=1.0):
+    """(loss, statistics for the backward pass) and, in place, dlogits; rows: _rows(logits)."""
+    z, n, classes, stride = rows
     red = _REDUCTIONS[reduction]
     loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32,
                        device=logits.device)
@@ -358,24 +359,25 @@ def _xent(logits, targets, ignore_index, smoothing, z_loss, reduction, dlogits=N
     if n or red:
         stats = _native.cross_entropy(z, (n, classes, stride), targets.contiguous(),
                                       ignore_index, smoothing, z_loss, red, grad_scale, loss,
-                                      dlogits, 0 if dlogits is None else _rows(dlogits)[3])
+                                      dlogits, dstride)
     return loss, stats
 
 
-def _like_rows(logits):
-    """A tensor for the gradient of logits: with the rows of a padded view as far apart as the
-    view's, which keeps their alignment for this and the next product; else contiguous."""
-    t, n, classes, stride = _rows(logits)
-    if t is logits and classes < stride <= classes + 256:
-        buf = torch.empty(n * stride, dtype=logits.dtype, device=logits.device)
-        return buf.as_strided(logits.shape, logits.stride())
-    return logits.new_empty(logits.shape)
+def _like_rows(logits, rows):
+    """(tensor, row stride) for the gradient of logits: the rows of a padded view as far apart as
+    the view's, which keeps their alignment for this and the next product; else contiguous."""
+    z, _, classes, stride = rows
+    if z is logits and classes < stride <= classes + 256:
+        return torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype,
+                                   device=logits.device), stride
+    return logits.new_empty(logits.shape), classes
 
 
 class _CrossEntropy(Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
-        loss, stats = _xent(logits, targets, ignore_index, smoothing, z_loss, reduction)
+        loss, stats = _xent(logits, _rows(logits), targets, ignore_index, smoothing, z_loss,
+                            reduction)
         ctx.save_for_backward(logits, targets, stats)
         ctx.args = ignore_index, smoothing, z_loss, _REDUCTIONS[reduction]
         return loss
@@ -384,11 +386,11 @@ class _CrossEntropy(Function):
     @once_differentiable
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors
-        dz = _like_rows(logits)
+        z, *rows = _rows(logits)
+        dz, stride = _like_rows(logits, (z, *rows))
         if dz.numel():
-            z, *rows = _rows(logits)
             _native.cross_entropy_grad(z, rows, targets.contiguous(), *ctx.args, stats,
-                                       grad.float().contiguous(), dz, _rows(dz)[3])
+                                       grad.float().contiguous(), dz, stride)
         return dz, *[None] * 5
 
 
@@ -405,7 +407,8 @@ def cross_entropy(logits, targets, ignore_index=-100, label_smoothing=0.0, z_los
     if torch.is_grad_enabled() and logits.requires_grad:
         return _CrossEntropy.apply(logits, targets, ignore_index, label_smoothing, z_loss,
                                    reduction)
-    return _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction)[0]
+    return _xent(logits, _rows(logits), targets, ignore_index, label_smoothing, z_loss,
+                 reduction)[0]
 
 
 def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, z_loss=0.0,
@@ -421,14 +424,15 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)
     if reduction == "none":
         raise NativeError(f"{what}: the loss must be a mean or a sum")
-    if inplace:
-        if _rows(logits)[0] is not logits or (logits.numel() > logits.shape[-1]
-                                              and _rows(logits)[3] < logits.shape[-1]):
-            raise NativeError(f"{what}: logits of strides {tuple(logits.stride())} have no rows "
-                              "to write a gradient to")
-        dlogits = logits
+    rows = _rows(logits)
+    z, n, classes, stride = rows
+    if not inplace:
+        dlogits, dstride = _like_rows(logits, rows)
+    elif z is logits and (n <= 1 or stride >= classes):
+        dlogits, dstride = logits, stride
     else:
-        dlogits = _like_rows(logits)
-    loss, _ = _xent(logits, targets, ignore_index, label_smoothing, z_loss, reduction,
-                       dlogits=dlogits, grad_scale=grad_scale)
+        raise NativeError(f"{what}: logits of strides {tuple(logits.stride())} have no rows to "
+                          "write a gradient to")
+    loss, _ = _xent(logits, rows, targets, ignore_index, label_smoothing, z_loss, reduction,
+                    dlogits, dstride, grad_scale)
     return loss, dlogits

@@ -264,6 +264,21 @@ def test_embedding_gradient(T, tokens, vocab, dim, kind, dtype, out, p):
     close(dw, want, grad_bound(want, size, n, out))
 
 
+def test_gradient_of_a_table_of_many_rows(T):
+    """Ids of 25 bits: four passes of the sort."""
+    rows, tokens, dim = (1 << 24) + 9, 9001, 8
+    ids = ids_of((tokens,), rows, kind="flat")
+    ids[::7], ids[5], ids[11] = ids[0], rows - 1, rows
+    g = normal(tokens, dim)
+    dw, _ = T.embedding_backward(g.to(DEV), ids.to(DEV), rows)
+    named, place = torch.unique(ids, return_inverse=True)
+    want, size, n = R.table_grad(g, place, len(named))
+    inside = named < rows
+    named, want, bound = named[inside], want[inside], grad_bound(want, size, n, F32)[inside]
+    close(dw[named.to(DEV)], want, bound)
+    assert int(dw.ne(0).any(1).sum()) == len(named)
+
+
 @pytest.mark.parametrize("batch,seq,rows,dim", [(1, 1, 1, 8), (1, 9, 16, 24), (8, 128, 128, 96),
                                                 (300, 3, 5, 40), (2000, 1, 1, 520),
                                                 (33, 70, 200, 17)])

@@ -67,7 +67,7 @@ def test_entry_points_refuse_without_launching(lib):
     assert embed(tokens=0, ids=None) == 0 and embed(dim=0, w=None) == 0
 
     def grad(**kw):
-        a = dict(ids=one, pos=None, tokens=4, seq=2, g=one, dt=0, gs=8, rows=9, dim=8, cut=0,
+        a = dict(ids=one, pos=None, tokens=400, seq=2, g=one, dt=0, gs=8, rows=9, dim=8, cut=0,
                  out=one, pout=None, prows=0, ot=0, ws=one, nb=1 << 20)
         a.update(kw)
         return lib.dmh_embedding_grad(None, a["ids"], a["pos"], 1, a["tokens"], a["seq"], a["g"],
@@ -85,11 +85,14 @@ def test_entry_points_refuse_without_launching(lib):
     assert grad(out=None) == 0 and grad(rows=0) == 0 and grad(dim=0) == 0
 
     nb = ctypes.c_size_t()
-    assert lib.dmh_embedding_grad_workspace_size(-1, 8, 1, ctypes.byref(nb)) == 1
-    assert lib.dmh_embedding_grad_workspace_size(5, 8, 1, None) == 1
-    assert lib.dmh_embedding_grad_workspace_size(5, 8, 3, ctypes.byref(nb)) == 1
-    assert lib.dmh_embedding_grad_workspace_size(0, 8, 2, ctypes.byref(nb)) == 0
-    assert nb.value == 0
+    size = lib.dmh_embedding_grad_workspace_size
+    assert size(-1, 5, 5, 8, 0, ctypes.byref(nb)) == 1 and size(5, 5, 5, 8, 0, None) == 1
+    assert size(5, 1 << 27, 5, 8, 0, ctypes.byref(nb)) == 1
+    assert size(1000, 0, 0, 8, 1, ctypes.byref(nb)) == 0 and nb.value == 0
+    # sorted tokens and parts of 32 chunks; implicit positions have parts alone
+    assert size(1000, 50, 0, 64, 0, ctypes.byref(nb)) == 0
+    assert nb.value == 2 * 4096 + 32 * 2 * 64 * 4
+    assert size(1000, 0, 50, 64, 0, ctypes.byref(nb)) == 0 and nb.value == 32 * 2 * 64 * 4
 
     def xent(**kw):
         a = dict(z=one, dt=0, rows=2, v=5, zs=5, y=one, red=1, loss=one, count=one, ds=5, ws=one,
