@@ -567,8 +567,8 @@ __global__ __launch_bounds__(256) void embed_grad_small(GradArgs a) {
   }
 }
 
-// Tables narrower than eight columns: a thread has one element of the table and walks through
-// its tokens.
+// Tables narrower than eight columns, which no piece of a row fits: a thread has one element of the
+// table and walks through its tokens.  Right for any such table, and made for none to be fast.
 template <class TG, class TO, bool DROP>
 __global__ __launch_bounds__(256) void embed_grad_narrow(GradArgs a, int jn) {
   const GradJob& j = a.job[jn];

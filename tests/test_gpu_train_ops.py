@@ -468,7 +468,7 @@ class Xent:
 
 
 SHAPES = [(1, 1), (1, 2), (3, 7), (5, 255), (70, 65), (4, 1000), (9, 4096), (7, 4097), (6, 8009),
-          (3, 16385), (33, 50257), (2, 65537), (2, 131077), (1, 300001)]
+          (3, 16385), (33, 50257), (2, 65537), (3, 70001), (2, 131077), (3, 150001), (1, 300001)]
 
 
 def xent_case(n, v, dtype, seed=0, std=2.0, ignored=True):
@@ -547,7 +547,7 @@ def test_cross_entropy_of_strided_logits(T, layout, dtype):
         assert torch.equal(work.cpu()[left], base[left])   # nothing beside the rows is written
 
 
-@pytest.mark.parametrize("v", [40, 5000, 50257, 140001])
+@pytest.mark.parametrize("v", [40, 600, 5000, 50257, 70001, 140001])
 def test_masked_and_non_finite_logits(T, v):
     inf, nan = float("inf"), float("nan")
     z, y = xent_case(12, v, F32, ignored=False)
