@@ -459,42 +459,37 @@ FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
+# a default stream's handle, null, means the current device's: each call below goes again with its
+# tensors' device current if another one is
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on_device(call):
-    """`call` with the device of its first tensor current: a default stream's handle, null,
-    means the current device's."""
-    @functools.wraps(call)
-    def on_device(first, *args):
-        index = first.device.index
-        if index == _current_device():
-            return call(first, *args)
-        with torch.cuda.device(index):
-            return call(first, *args)
-    return on_device
-
-
-@_on_device
 def dropout(x, residual, out, cut, rng, rows):
     """out = dropout(x) [+ residual]; rows: (rows, cols, x's row stride, the residual's)."""
+    index = x.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return dropout(x, residual, out, cut, rng, rows)
     n, cols, xs, rs = rows
     seed, offset, state = rng
-    _check(load().dmh_dropout(_raw_stream(x.device.index), x.data_ptr(), FLOATS[x.dtype], n,
+    _check(load().dmh_dropout(_raw_stream(index), x.data_ptr(), FLOATS[x.dtype], n,
                               cols, xs, 0 if residual is None else residual.data_ptr(), rs,
                               out.data_ptr(), FLOATS[out.dtype], cut, seed, offset, state),
            "dmh_dropout")
 
 
-@_on_device
 def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     """Token rows times scale plus position rows through dropout into out (tokens, dim)."""
+    index = ids.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return embedding(ids, weight, pos_weight, positions, scale, cut, rng, out)
     seed, offset, state = rng
     vocab, dim = weight.shape
     seq = ids.shape[-1] if ids.ndim else 1
     pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr(), pos_weight.shape[0],
                                                 pos_weight.stride(0))
-    _check(load().dmh_embedding(_raw_stream(weight.device.index), ids.data_ptr(),
+    _check(load().dmh_embedding(_raw_stream(index), ids.data_ptr(),
                                 ids.dtype == torch.int64, ids.numel(), seq, weight.data_ptr(),
                                 FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
                                 0 if positions is None else positions.data_ptr(), scale, cut,
@@ -512,16 +507,20 @@ def embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions):
     return nbytes.value
 
 
-@_on_device
 def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx, scale, cut, rng,
                    out, add, pos_out, pos_add):
     """The gradients of the token table (out) and the position table (pos_out), either None."""
+    index = ids.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
+                                  scale, cut, rng, out, add, pos_out, pos_add)
     seed, offset, state = rng
     rows = 0 if out is None else out.shape[0]
     pos_rows = 0 if pos_out is None else pos_out.shape[0]
     nbytes = embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions is not None)
     ws = _workspace(nbytes, ids.device) if nbytes else None
-    _check(load().dmh_embedding_grad(_raw_stream(ids.device.index), ids.data_ptr(),
+    _check(load().dmh_embedding_grad(_raw_stream(index), ids.data_ptr(),
                                      0 if positions is None else positions.data_ptr(),
                                      ids.dtype == torch.int64, tokens, seq, grad.data_ptr(),
                                      FLOATS[grad.dtype], gstride, dim, padding_idx, scale, cut,
@@ -532,18 +531,22 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
            "dmh_embedding_grad")
 
 
-@_on_device
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
                   dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
     stride) of the logits.  Returns what the backward pass needs: fp32, each row's lse and then
     the number of rows with a target (for a mean)."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction,
+                                 grad_scale, loss, dlogits, dstride)
     n, classes, zs = rows
     lib = load()
     nbytes = 4 * n   # dmh_cross_entropy_workspace_size
     stats = torch.empty(2 * n + 1, dtype=torch.float32, device=logits.device)
     at = stats.data_ptr()
-    _check(lib.dmh_cross_entropy(_raw_stream(logits.device.index), logits.data_ptr(),
+    _check(lib.dmh_cross_entropy(_raw_stream(index), logits.data_ptr(),
                                  FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
                                  targets.dtype == torch.int64, ignore, smoothing, z_loss,
                                  reduction, grad_scale, loss.data_ptr(), at + nbytes, at,
@@ -553,13 +556,17 @@ def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, g
     return stats
 
 
-@_on_device
 def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reduction, stats,
                        grad_out, dlogits, dstride):
     """The gradient of the logits from cross_entropy's statistics, times grad_out."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss,
+                                      reduction, stats, grad_out, dlogits, dstride)
     n, classes, zs = rows
     at = stats.data_ptr()
-    _check(load().dmh_cross_entropy_grad(_raw_stream(logits.device.index), logits.data_ptr(),
+    _check(load().dmh_cross_entropy_grad(_raw_stream(index), logits.data_ptr(),
                                          FLOATS[logits.dtype], n, classes, zs,
                                          targets.data_ptr(), targets.dtype == torch.int64,
                                          ignore, smoothing, z_loss, at,

@@ -108,9 +108,15 @@ def draw_rng():
 # ---- dropout --------------------------------------------------------------------------------
 
 def _dropout(x, residual, cut, rng, dtype):
-    out = x.new_empty(x.shape) if dtype == x.dtype else (
-        torch.empty(x.shape, dtype=dtype, device=x.device) if residual is None
-        else residual.new_empty(x.shape))
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        like = x if dtype == x.dtype else residual
+        out = torch.empty_like(like) if like is not None and like.dtype == dtype else (
+            torch.empty_like(x, dtype=dtype))
+        n = x.numel()
+        if n:
+            _native.dropout(x, residual, out, cut, rng, (1, n, n, n))
+        return out
+    out = torch.empty(x.shape, dtype=dtype, device=x.device)
     if out.numel():
         x, rows, cols, stride = _rows(x)
         rstride = 0
@@ -239,26 +245,29 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
     gradient.  An id or position outside its table gives a row of NaN."""
     what = "embedding"
     _float(weight, what, "weight")
-    if weight.ndim != 2:
-        raise NativeError(f"{what}: weight must be (rows, dim), got {tuple(weight.shape)}")
-    _ints(ids, weight.device, what, "ids")
-    positions = _positions(positions, ids, what)
-    if pos_weight is None:
-        if positions is not None:
+    device, dtype, shape = weight.device, weight.dtype, weight.shape
+    if len(shape) != 2:
+        raise NativeError(f"{what}: weight must be (rows, dim), got {tuple(shape)}")
+    _ints(ids, device, what, "ids")
+    if positions is not None:
+        positions = _positions(positions, ids, what)
+        if pos_weight is None:
             raise NativeError(f"{what}: positions without a position table")
-    else:
-        if (pos_weight.ndim != 2 or pos_weight.shape[1] != weight.shape[1]
-                or pos_weight.dtype != weight.dtype or pos_weight.device != weight.device):
-            raise NativeError(f"{what}: the position table {tuple(pos_weight.shape)} "
-                              f"{pos_weight.dtype} does not fit {tuple(weight.shape)} "
-                              f"{weight.dtype}")
-        if positions is None and (ids.ndim < 1 or ids.shape[-1] > pos_weight.shape[0]):
+    if pos_weight is not None:
+        pshape = pos_weight.shape
+        if (len(pshape) != 2 or pshape[1] != shape[1] or pos_weight.dtype != dtype
+                or pos_weight.device != device):
+            raise NativeError(f"{what}: the position table {tuple(pshape)} {pos_weight.dtype} "
+                              f"does not fit {tuple(shape)} {dtype}")
+        if positions is None and (ids.ndim < 1 or ids.shape[-1] > pshape[0]):
             raise NativeError(f"{what}: ids {tuple(ids.shape)} have more positions than the "
-                              f"table's {pos_weight.shape[0]}")
-    _padding(padding_idx, weight.shape[0], what)
-    dtype = out_dtype or weight.dtype
-    _out_type(dtype, what)
-    cut, key = _drop(dropout_p, rng, weight.device, what)
+                              f"table's {pshape[0]}")
+    if padding_idx is not None:
+        _padding(padding_idx, shape[0], what)
+    if out_dtype is not None:
+        dtype = out_dtype
+        _out_type(dtype, what)
+    cut, key = _drop(dropout_p, rng, device, what)
     if torch.is_grad_enabled() and (weight.requires_grad
                                     or pos_weight is not None and pos_weight.requires_grad):
         return _Embedding.apply(weight, pos_weight, ids, positions, scale, padding_idx,
