@@ -25,6 +25,7 @@ element is replaced by zero, also where it is not finite.
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from defmuon_amd import _native
 from defmuon_amd._native import FLOATS, NativeError
@@ -335,6 +336,11 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     elif (rows or pos_rows) and dim:
         _native.embedding_grad(ids, positions, tokens, seq, grad, stride, dim, padding_idx, scale,
                                cut, key, dw, add, dp, pos_add)
+    # autograd does not see a write through a pointer
+    if add:
+        increment_version(dw)
+    if pos_add:
+        increment_version(dp)
     return dw, dp
 
 
@@ -427,7 +433,9 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
 
     dlogits is the gradient of grad_scale * loss (1 / micro-batches, a loss scale) in the
     logits' type; with inplace it takes the logits' own memory (what lies beside the rows of a
-    padded view stays).  logits.backward(dlogits) goes on from there."""
+    padded view stays).  logits.backward(dlogits) goes on from there; after a call in place it
+    raises torch's error where the logits' values are needed for it (a soft-cap's tanh, another
+    loss of the same logits)."""
     what = "cross_entropy_step"
     logits = logits.detach()
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)
@@ -444,4 +452,6 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
                           "write a gradient to")
     loss, _ = _xent(logits, rows, targets, ignore_index, label_smoothing, z_loss, reduction,
                     dlogits, dstride, grad_scale)
+    if inplace:   # autograd does not see a write through a pointer
+        increment_version(logits)
     return loss, dlogits

@@ -755,3 +755,20 @@ def test_model_step_with_dropout_follows_the_seed():
         losses.append(float(m.train_step(tok[:, :-1], tok[:, 1:])))
     assert losses[0] == losses[2] != losses[1]
     assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def test_writes_in_place_are_seen_by_autograd(T):
+    h, y = normal(64, 96).to(DEV).requires_grad_(), ids_of((64,), 300).to(DEV)
+    w = normal(96, 300, seed=1).to(DEV)
+    want = torch.autograd.grad(z := h @ w, h, T.cross_entropy_step(z, y)[1])[0]
+    z = h @ w
+    dz = T.cross_entropy_step(z, y, inplace=True)[1]
+    assert torch.equal(torch.autograd.grad(z, h, dz)[0], want)
+    z = torch.tanh(h @ w)
+    dz = T.cross_entropy_step(z, y, inplace=True)[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward(dz)
+    dw, g = torch.zeros(300, 96, device=DEV), normal(64, 96).to(DEV)
+    before = dw._version
+    T.embedding_backward(g, y, 300, weight_grad=dw)
+    assert dw._version == before + 1

@@ -163,3 +163,68 @@ def test_draws_follow_the_seed():
     a, b = draw_rng(), draw_rng()
     torch.manual_seed(3)
     assert draw_rng() == a != b
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """train_ops on CPU tensors: plain forms in place of the launches."""
+    from defmuon_amd import _native, train_ops as T
+
+    def cross_entropy(z, rows, y, ignore, smoothing, z_loss, reduction, grad_scale, loss, dz,
+                      dstride):
+        zz = z.detach().clone()
+        rows, d, _ = R.xent(zz, y, ignore, smoothing, z_loss)
+        n = 1 if reduction == 2 else int((y != ignore).sum())
+        loss.copy_(rows if reduction == 0 else rows.sum() / n)
+        if dz is not None:   # through its memory, as a kernel writes it
+            dz.numpy()[...] = (d * grad_scale / n).float().numpy()
+        return torch.zeros(1)
+
+    def embedding_grad(ids, positions, tokens, seq, grad, stride, dim, padding, scale, cut, rng,
+                       out, add, pos_out, pos_add):
+        for table in (out, pos_out):
+            if table is not None:
+                table.numpy()[...] += 1.0
+
+    monkeypatch.setattr(T, "_float", lambda *a: None)
+    monkeypatch.setattr(_native, "cross_entropy", cross_entropy)
+    monkeypatch.setattr(_native, "embedding_grad", embedding_grad)
+    return T
+
+
+def test_writes_in_place_are_seen_by_autograd(stand_in):
+    T = stand_in
+    h, y = torch.randn(6, 11, requires_grad=True), torch.arange(6)
+    w = torch.randn(11, 11)
+    want = {}
+    for name, f in (("tanh", torch.tanh), ("product", lambda t: t @ w)):
+        z = f(h)
+        (want[name],) = torch.autograd.grad(z, h, T.cross_entropy_step(z, y)[1])
+        assert z._version == 0
+    z = h @ w   # its backward pass needs no logits
+    loss, dz = T.cross_entropy_step(z, y, inplace=True)
+    assert dz.data_ptr() == z.data_ptr() and z._version == 1
+    assert torch.equal(torch.autograd.grad(z, h, dz)[0], want["product"])
+    for view in (lambda t: t.view(2, 3, 11), lambda t: t[:, :9]):   # ... nor has it as a view
+        z = view(h @ w)
+        t = y.clamp(max=8).view(z.shape[:-1])
+        ref = torch.autograd.grad(z, h, T.cross_entropy_step(z, t)[1], retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(z, h, T.cross_entropy_step(z, t, inplace=True)[1])[0],
+                           ref)
+    z = torch.tanh(h)
+    dz = T.cross_entropy_step(z, y, inplace=True)[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward(dz)
+    z = h @ w   # a loss that has saved the same logits
+    loss = T.cross_entropy(z, y)
+    T.cross_entropy_step(z, y, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        T.cross_entropy_step(h @ w, y, inplace=True)
+    g, ids = torch.randn(2, 3, 8), torch.zeros(2, 3, dtype=torch.int64)
+    dw, dp = torch.zeros(5, 8), torch.zeros(4, 8)
+    T.embedding_backward(g, ids, 5, pos_rows=4, weight_grad=dw)
+    assert (dw._version, dp._version) == (1, 0) and bool((dw == 1).all())
+    T.embedding_backward(g, ids, 5, pos_rows=4, weight_grad=dw, pos_grad=dp)
+    assert (dw._version, dp._version) == (2, 1)
