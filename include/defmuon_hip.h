@@ -276,11 +276,14 @@ int dmh_embedding_grad(dmh_stream_t stream, const void* ids, const void* positio
  * gradient of zero; other targets outside [0, classes) give NaN.
  *   reduction  0 none: loss has `rows` values; 1 mean over the rows that have a target (their
  *              number goes to `count`); 2 sum
- *   lse        (rows), kept for dmh_cross_entropy_grad; may be NULL
+ *   lse        (rows); may be NULL
  *   dlogits    the gradient of grad_scale * loss (of the sum, for reduction 0), in the
  *              logits' type; may be the logits themselves; NULL for the loss alone
- * dmh_cross_entropy_grad: the gradient from a forward call's lse (and count, for a mean; NULL
- * otherwise), times *grad_out, or grad_out[row] if grad_out_rows.
+ * dmh_cross_entropy_stats: the same, which keeps each row's maximum and sum exp(z - maximum)
+ * instead, (rows) each.
+ * dmh_cross_entropy_grad_stats: the gradient from these (and count, for a mean; NULL otherwise),
+ * times *grad_out, or grad_out[row] if grad_out_rows.  dmh_cross_entropy_grad takes lse, whose
+ * rounding leaves each probability off by a relative 2^-24 |lse|.
  * 1 <= classes <= 2^27, rows < 2^22. */
 int dmh_cross_entropy_workspace_size(long long rows, long long classes, size_t* bytes);
 int dmh_cross_entropy(dmh_stream_t stream, const void* logits, int dtype, long long rows,
@@ -288,12 +291,25 @@ int dmh_cross_entropy(dmh_stream_t stream, const void* logits, int dtype, long l
                       int targets_64, long long ignore_index, float smoothing, float z_loss,
                       int reduction, float grad_scale, float* loss, float* count, float* lse,
                       void* dlogits, long long d_rstride, void* ws, size_t ws_bytes);
+int dmh_cross_entropy_stats(dmh_stream_t stream, const void* logits, int dtype, long long rows,
+                            long long classes, long long z_rstride, const void* targets,
+                            int targets_64, long long ignore_index, float smoothing,
+                            float z_loss, int reduction, float grad_scale, float* loss,
+                            float* count, float* row_max, float* row_sum, void* dlogits,
+                            long long d_rstride, void* ws, size_t ws_bytes);
 int dmh_cross_entropy_grad(dmh_stream_t stream, const void* logits, int dtype, long long rows,
                            long long classes, long long z_rstride, const void* targets,
                            int targets_64, long long ignore_index, float smoothing,
                            float z_loss, const float* lse, const float* count,
                            const float* grad_out, int grad_out_rows, void* dlogits,
                            long long d_rstride);
+int dmh_cross_entropy_grad_stats(dmh_stream_t stream, const void* logits, int dtype,
+                                 long long rows, long long classes, long long z_rstride,
+                                 const void* targets, int targets_64, long long ignore_index,
+                                 float smoothing, float z_loss, const float* row_max,
+                                 const float* row_sum, const float* count,
+                                 const float* grad_out, int grad_out_rows, void* dlogits,
+                                 long long d_rstride);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,14 @@
 //   loss = lse - (1 - eps) z_y - eps mean(z) + zeta lse^2
 //   dz   = (p (1 + 2 zeta lse) - (1 - eps) delta_y - eps / V) * g,     p = exp(z - lse)
 //
+// with m = max z and s = sum exp(z - m) computed as
+//
+//   loss = log s + (m - z_y) - eps mean(z - z_y) + zeta (m + log s)^2,     p = exp(z - m) / s
+//
+// so that what all logits of a row have in common cancels before anything is rounded: lse itself
+// in 32 bits is off by half a last place of the logits' size, more than the whole loss of a row
+// that is sure of its target.
+//
 // eps is the label smoothing, zeta the weight of the z-loss; g is grad_scale, divided by the
 // number of rows that have a target for a mean.  A row whose target is ignore_index has loss 0
 // and gradient 0 whatever its logits hold; any other target outside [0, V) makes both NaN.  A
@@ -21,8 +29,9 @@ struct XentArgs {
   const void* targets;
   void* dz;              // or null
   float* row_loss;
-  float* lse;            // per row, written (forward) or read (gradient); may be null in the
-                         // forward pass
+  float* row_max;        // per row, written (forward) or read (gradient): its maximum, and
+  float* row_sum;        // sum exp(z - maximum); lse and 1 if row_sum is null.  Both may be null
+                         // in the forward pass
   const float* count;    // rows that have a target, or null
   int counts;            // the rows' launch counts them itself
   const float* gout;     // gradient of the loss (gradient kernel): one, or one a row
@@ -137,14 +146,33 @@ __global__ __launch_bounds__(1024) void xent_reduce(XentArgs a, float* count, fl
 struct Grad {
   float ps, base, top;
 };
-__device__ __forceinline__ float row_loss(const XentArgs& a, float lse, float zy, float zsum) {
-  float loss = lse - (1.f - a.eps) * zy;
-  if (a.eps != 0.f) loss -= a.eps * (zsum / a.classes);
+// Differences to the target's logit are summed up 2^-28 times their size, which costs nothing in a
+// fused multiply-add: classes at the lowest and the highest values of the type do not overflow.
+constexpr float SMALL = 0x1p-28f, BIG = 0x1p28f;
+__device__ __forceinline__ float small_diff(float z, float zy) {
+  return fmaf(z, SMALL, zy * -SMALL);
+}
+// zsum: the sum of small_diff(z, zy); from 0 in place of a zy that is not finite, whose loss
+// is not either
+__device__ __forceinline__ float row_loss(const XentArgs& a, float m, float log_s, float zy,
+                                          float zsum) {
+  float loss = log_s + (m - zy);
+  if (a.eps != 0.f) loss -= zsum * (a.eps / a.classes) * BIG;
+  const float lse = m + log_s;
   if (a.zeta != 0.f) loss += a.zeta * lse * lse;
   return loss;
 }
-__device__ __forceinline__ Grad row_grad(const XentArgs& a, float g, float lse, float s) {
-  return {g * (1.f + 2.f * a.zeta * lse) / s, -g * (a.eps / a.classes), -g * (1.f - a.eps)};
+// (Each store under a condition of its own: from an if and an else with three stores ROCm 7.2's
+// compiler made one whose address was the wrong array's.)
+__device__ __forceinline__ void put_stats(const XentArgs& a, long long row, float m, float s,
+                                          float log_s) {
+  if (a.row_max) a.row_max[row] = a.row_sum ? m : m + log_s;
+  if (a.row_sum) a.row_sum[row] = s;
+}
+__device__ __forceinline__ Grad row_grad(const XentArgs& a, float g, float m, float s,
+                                         float log_s) {
+  return {g * (1.f + 2.f * a.zeta * (m + log_s)) / s, -g * (a.eps / a.classes),
+          -g * (1.f - a.eps)};
 }
 
 // A row in aligned pieces of 16 bytes, and the classes before the first and behind the last one,
@@ -228,7 +256,7 @@ void xent_row(XentArgs a) {
   if (y == a.ignore) {
     if (t == 0) {
       a.row_loss[row] = 0.f;
-      if (a.lse) a.lse[row] = 0.f;
+      put_stats(a, row, 0.f, 1.f, 0.f);
     }
     if (GRAD) {
       const type zero = {};
@@ -240,14 +268,15 @@ void xent_row(XentArgs a) {
   }
   const bool known = y >= 0 && y < a.classes;
   const float zy = known ? (float)z[y] : __builtin_nanf("");
-  float zsum = ec >= 0 ? ex : 0.f;
+  const float ref = fabsf(zy) < INF ? zy : 0.f;
+  float zsum = ec >= 0 ? small_diff(ex, ref) : 0.f;
   if (a.eps != 0.f) {
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
       if (k * THREADS + t < r.pieces) {
         const type v = __builtin_bit_cast(type, x[k]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) zsum += (float)v[j];
+        for (int j = 0; j < N; ++j) zsum += small_diff((float)v[j], ref);
       }
     }
   }
@@ -275,13 +304,13 @@ void xent_row(XentArgs a) {
   repack(x);
   p = block_join<THREADS>(p, parts);
   if (a.eps != 0.f) zsum = block_sum<THREADS>(zsum, lds);
-  const float lse = p.m + __builtin_amdgcn_logf(p.s) * LN2;
+  const float log_s = __builtin_amdgcn_logf(p.s) * LN2;
   if (t == 0) {
-    a.row_loss[row] = row_loss(a, lse, zy, zsum);
-    if (a.lse) a.lse[row] = lse;
+    a.row_loss[row] = row_loss(a, p.m, log_s, zy, zsum);
+    put_stats(a, row, p.m, p.s, log_s);
   }
   if (!GRAD) return;
-  const Grad g = row_grad(a, known ? a.gscale / count : __builtin_nanf(""), lse, p.s);
+  const Grad g = row_grad(a, known ? a.gscale / count : __builtin_nanf(""), p.m, p.s, log_s);
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int i = k * THREADS + t;
@@ -318,7 +347,7 @@ __global__ __launch_bounds__(1024) void xent_stream(XentArgs a) {
   if (y == a.ignore) {
     if (threadIdx.x == 0) {
       a.row_loss[row] = 0.f;
-      if (a.lse) a.lse[row] = 0.f;
+      put_stats(a, row, 0.f, 1.f, 0.f);
     }
     if (GRAD) {
       for (int i = threadIdx.x; i < r.pieces; i += 1024) *(type*)(dz + r.piece_class(i)) = zero;
@@ -329,7 +358,8 @@ __global__ __launch_bounds__(1024) void xent_stream(XentArgs a) {
   const bool known = y >= 0 && y < a.classes;
   const float zy = known ? (float)z[y] : __builtin_nanf("");
   const float ex = ec >= 0 ? (float)z[ec] : -INF;
-  float zsum = ec >= 0 ? ex : 0.f;
+  const float ref = fabsf(zy) < INF ? zy : 0.f;
+  float zsum = ec >= 0 ? small_diff(ex, ref) : 0.f;
   Part p = {fmaxf(ex, -INF), 0.f};
   p.s = exp_diff(ex, p.m == -INF ? 0.f : p.m);
   for (int i0 = threadIdx.x; i0 < r.pieces; i0 += AHEAD * 1024) {
@@ -354,21 +384,21 @@ __global__ __launch_bounds__(1024) void xent_stream(XentArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         e += exp_diff((float)x[k][j], m0);
-        if (a.eps != 0.f) zsum += in ? (float)x[k][j] : 0.f;
+        if (a.eps != 0.f) zsum += in ? small_diff((float)x[k][j], ref) : 0.f;
       }
       p.s += in ? e : 0.f;
     }
   }
   p = block_join<1024>(p, parts);
   zsum = block_sum<1024>(zsum, lds);   // also: every read of z[y] is before dz, which may be z
-  const float lse = p.m + __builtin_amdgcn_logf(p.s) * LN2;
+  const float log_s = __builtin_amdgcn_logf(p.s) * LN2;
   if (threadIdx.x == 0) {
-    a.row_loss[row] = row_loss(a, lse, zy, zsum);
-    if (a.lse) a.lse[row] = lse;
+    a.row_loss[row] = row_loss(a, p.m, log_s, zy, zsum);
+    put_stats(a, row, p.m, p.s, log_s);
   }
   if (!GRAD) return;
   const float count = a.count ? *a.count : 1.f;
-  const Grad g = row_grad(a, known ? a.gscale / count : __builtin_nanf(""), lse, p.s);
+  const Grad g = row_grad(a, known ? a.gscale / count : __builtin_nanf(""), p.m, p.s, log_s);
   for (int i0 = threadIdx.x; i0 < r.pieces; i0 += AHEAD * 1024) {
     type x[AHEAD];
 #pragma unroll
@@ -390,7 +420,7 @@ __global__ __launch_bounds__(1024) void xent_stream(XentArgs a) {
     dz[y] = (T)(fmaf(exp_diff(zy, p.m), g.ps, g.base) + g.top);
 }
 
-// The gradient from a forward pass's lse, element by element: THREADS threads a row, AHEAD
+// The gradient from a forward pass's statistics, element by element: THREADS threads a row, AHEAD
 // pieces each.  Bound by the memory: 78 us for 2000 fp32 rows of 32003 (512 MB, 6.6 TB/s; the
 // logits are partly in the last-level cache still).
 template <class T, int THREADS>
@@ -414,12 +444,13 @@ __global__ __launch_bounds__(256) void xent_grad(XentArgs a) {
   const float ex = ec >= 0 ? (float)z[ec] : 0.f;
   const long long y = load_index(a.targets, a.t64, row);
   const bool live = y != a.ignore, known = y >= 0 && y < a.classes;
-  const float lse = a.lse[row];
+  const float m = a.row_max[row], s = a.row_sum ? a.row_sum[row] : 1.f;
   float go = a.gout[a.gout_rows ? row : 0];
   if (a.count) go /= *a.count;
-  const Grad g = row_grad(a, known ? go : __builtin_nanf(""), lse, 1.f);
+  const Grad g = row_grad(a, known ? go : __builtin_nanf(""), m, s,
+                          __builtin_amdgcn_logf(s) * LN2);
   auto grad = [&](float v, int c) {
-    float d = fmaf(exp_diff(v, lse), g.ps, g.base);
+    float d = fmaf(exp_diff(v, m), g.ps, g.base);
     if (c == (int)y) d += g.top;
     return (T)(live ? d : 0.f);
   };
@@ -510,11 +541,14 @@ int dmh_cross_entropy_workspace_size(long long rows, long long classes, size_t* 
   return DMH_OK;
 }
 
-int dmh_cross_entropy(hipStream_t stream, const void* logits, int dtype, long long rows,
-                      long long classes, long long z_rstride, const void* targets,
-                      int targets_64, long long ignore_index, float smoothing, float z_loss,
-                      int reduction, float grad_scale, float* loss, float* count, float* lse,
-                      void* dlogits, long long d_rstride, void* ws, size_t ws_bytes) {
+}  // extern "C"
+
+static int xent_forward(hipStream_t stream, const void* logits, int dtype, long long rows,
+                        long long classes, long long z_rstride, const void* targets,
+                        int targets_64, long long ignore_index, float smoothing, float z_loss,
+                        int reduction, float grad_scale, float* loss, float* count, float* row_max,
+                        float* row_sum, void* dlogits, long long d_rstride, void* ws,
+                        size_t ws_bytes) {
   if (!xent_shape(rows, classes) || z_rstride < 0 || d_rstride < 0 || !float_code(dtype) ||
       reduction < RED_NONE || reduction > RED_SUM) {
     set_error("dmh_cross_entropy: bad arguments (rows=%lld classes=%lld dtype=%d reduction=%d)",
@@ -536,7 +570,8 @@ int dmh_cross_entropy(hipStream_t stream, const void* logits, int dtype, long lo
   a.targets = targets;
   a.dz = dlogits;
   a.row_loss = reduction == RED_NONE ? loss : (float*)ws;
-  a.lse = lse;
+  a.row_max = row_max;
+  a.row_sum = row_sum;
   a.count = reduction == RED_MEAN ? count : nullptr;
   a.rows = rows;
   a.zs = z_rstride;
@@ -570,18 +605,19 @@ int dmh_cross_entropy(hipStream_t stream, const void* logits, int dtype, long lo
   return DMH_OK;
 }
 
-int dmh_cross_entropy_grad(hipStream_t stream, const void* logits, int dtype, long long rows,
-                           long long classes, long long z_rstride, const void* targets,
-                           int targets_64, long long ignore_index, float smoothing, float z_loss,
-                           const float* lse, const float* count, const float* grad_out,
-                           int grad_out_rows, void* dlogits, long long d_rstride) {
+static int xent_backward(hipStream_t stream, const void* logits, int dtype, long long rows,
+                         long long classes, long long z_rstride, const void* targets,
+                         int targets_64, long long ignore_index, float smoothing, float z_loss,
+                         const float* row_max, const float* row_sum, const float* count,
+                         const float* grad_out, int grad_out_rows, void* dlogits,
+                         long long d_rstride) {
   if (!xent_shape(rows, classes) || z_rstride < 0 || d_rstride < 0 || !float_code(dtype)) {
     set_error("dmh_cross_entropy_grad: bad arguments (rows=%lld classes=%lld dtype=%d)", rows,
               classes, dtype);
     return DMH_EINVAL;
   }
   if (rows == 0) return DMH_OK;
-  if (!logits || !targets || !lse || !grad_out || !dlogits) {
+  if (!logits || !targets || !row_max || !grad_out || !dlogits) {
     set_error("dmh_cross_entropy_grad: null tensor");
     return DMH_EINVAL;
   }
@@ -589,7 +625,8 @@ int dmh_cross_entropy_grad(hipStream_t stream, const void* logits, int dtype, lo
   a.z = logits;
   a.targets = targets;
   a.dz = dlogits;
-  a.lse = (float*)lse;
+  a.row_max = (float*)row_max;
+  a.row_sum = (float*)row_sum;
   a.count = count;
   a.gout = grad_out;
   a.gout_rows = grad_out_rows != 0;
@@ -604,6 +641,59 @@ int dmh_cross_entropy_grad(hipStream_t stream, const void* logits, int dtype, lo
   DMH_FOR_TYPE(dtype, T, (launch_xent_grad<T>(stream, a)))
   DMH_CHECK_LAUNCH("xent_grad");
   return DMH_OK;
+}
+
+extern "C" {
+
+int dmh_cross_entropy(hipStream_t stream, const void* logits, int dtype, long long rows,
+                      long long classes, long long z_rstride, const void* targets,
+                      int targets_64, long long ignore_index, float smoothing, float z_loss,
+                      int reduction, float grad_scale, float* loss, float* count, float* lse,
+                      void* dlogits, long long d_rstride, void* ws, size_t ws_bytes) {
+  return xent_forward(stream, logits, dtype, rows, classes, z_rstride, targets, targets_64,
+                      ignore_index, smoothing, z_loss, reduction, grad_scale, loss, count, lse,
+                      nullptr, dlogits, d_rstride, ws, ws_bytes);
+}
+
+int dmh_cross_entropy_stats(hipStream_t stream, const void* logits, int dtype, long long rows,
+                            long long classes, long long z_rstride, const void* targets,
+                            int targets_64, long long ignore_index, float smoothing,
+                            float z_loss, int reduction, float grad_scale, float* loss,
+                            float* count, float* row_max, float* row_sum, void* dlogits,
+                            long long d_rstride, void* ws, size_t ws_bytes) {
+  if (rows > 0 && (!row_max || !row_sum)) {
+    set_error("dmh_cross_entropy_stats: null statistics");
+    return DMH_EINVAL;
+  }
+  return xent_forward(stream, logits, dtype, rows, classes, z_rstride, targets, targets_64,
+                      ignore_index, smoothing, z_loss, reduction, grad_scale, loss, count, row_max,
+                      row_sum, dlogits, d_rstride, ws, ws_bytes);
+}
+
+int dmh_cross_entropy_grad(hipStream_t stream, const void* logits, int dtype, long long rows,
+                           long long classes, long long z_rstride, const void* targets,
+                           int targets_64, long long ignore_index, float smoothing, float z_loss,
+                           const float* lse, const float* count, const float* grad_out,
+                           int grad_out_rows, void* dlogits, long long d_rstride) {
+  return xent_backward(stream, logits, dtype, rows, classes, z_rstride, targets, targets_64,
+                       ignore_index, smoothing, z_loss, lse, nullptr, count, grad_out,
+                       grad_out_rows, dlogits, d_rstride);
+}
+
+int dmh_cross_entropy_grad_stats(hipStream_t stream, const void* logits, int dtype,
+                                 long long rows, long long classes, long long z_rstride,
+                                 const void* targets, int targets_64, long long ignore_index,
+                                 float smoothing, float z_loss, const float* row_max,
+                                 const float* row_sum, const float* count,
+                                 const float* grad_out, int grad_out_rows, void* dlogits,
+                                 long long d_rstride) {
+  if (rows > 0 && !row_sum) {
+    set_error("dmh_cross_entropy_grad_stats: null statistics");
+    return DMH_EINVAL;
+  }
+  return xent_backward(stream, logits, dtype, rows, classes, z_rstride, targets, targets_64,
+                       ignore_index, smoothing, z_loss, row_max, row_sum, count, grad_out,
+                       grad_out_rows, dlogits, d_rstride);
 }
 
 }  // extern "C"

@@ -81,8 +81,14 @@ _SIGS = {
     "dmh_cross_entropy": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
                                   c_float, c_float, c_int, c_float, c_vp, c_vp, c_vp, c_vp, c_ll,
                                   c_vp, c_sz]),
+    "dmh_cross_entropy_stats": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
+                                        c_float, c_float, c_int, c_float, c_vp, c_vp, c_vp, c_vp,
+                                        c_vp, c_ll, c_vp, c_sz]),
     "dmh_cross_entropy_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
                                        c_float, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_ll]),
+    "dmh_cross_entropy_grad_stats": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int,
+                                             c_ll, c_float, c_float, c_vp, c_vp, c_vp, c_vp,
+                                             c_int, c_vp, c_ll]),
 }
 
 
@@ -534,8 +540,8 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
                   dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
-    stride) of the logits.  Returns what the backward pass needs: fp32, each row's lse and then
-    the number of rows with a target (for a mean)."""
+    stride) of the logits.  Returns what the backward pass needs: fp32, the rows' maxima, their
+    sums exp(z - maximum), and the number of rows with a target (for a mean)."""
     index = logits.get_device()
     if index != _current_device():
         with torch.cuda.device(index):
@@ -544,15 +550,15 @@ def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, g
     n, classes, zs = rows
     lib = load()
     nbytes = 4 * n   # dmh_cross_entropy_workspace_size
-    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=logits.device)
+    stats = torch.empty(3 * n + 1, dtype=torch.float32, device=logits.device)
     at = stats.data_ptr()
-    _check(lib.dmh_cross_entropy(_raw_stream(index), logits.data_ptr(),
-                                 FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
-                                 targets.dtype == torch.int64, ignore, smoothing, z_loss,
-                                 reduction, grad_scale, loss.data_ptr(), at + nbytes, at,
-                                 0 if dlogits is None else dlogits.data_ptr(), dstride,
-                                 at + nbytes + 4, nbytes),
-           "dmh_cross_entropy")
+    _check(lib.dmh_cross_entropy_stats(_raw_stream(index), logits.data_ptr(),
+                                       FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
+                                       targets.dtype == torch.int64, ignore, smoothing, z_loss,
+                                       reduction, grad_scale, loss.data_ptr(), at + 8 * n, at,
+                                       at + 4 * n, 0 if dlogits is None else dlogits.data_ptr(),
+                                       dstride, at + 8 * n + 4, nbytes),
+           "dmh_cross_entropy_stats")
     return stats
 
 
@@ -566,11 +572,11 @@ def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reducti
                                       reduction, stats, grad_out, dlogits, dstride)
     n, classes, zs = rows
     at = stats.data_ptr()
-    _check(load().dmh_cross_entropy_grad(_raw_stream(index), logits.data_ptr(),
-                                         FLOATS[logits.dtype], n, classes, zs,
-                                         targets.data_ptr(), targets.dtype == torch.int64,
-                                         ignore, smoothing, z_loss, at,
-                                         at + 4 * n if reduction == 1 else 0,
-                                         grad_out.data_ptr(), reduction == 0,
-                                         dlogits.data_ptr(), dstride),
-           "dmh_cross_entropy_grad")
+    _check(load().dmh_cross_entropy_grad_stats(_raw_stream(index), logits.data_ptr(),
+                                               FLOATS[logits.dtype], n, classes, zs,
+                                               targets.data_ptr(), targets.dtype == torch.int64,
+                                               ignore, smoothing, z_loss, at, at + 4 * n,
+                                               at + 8 * n if reduction == 1 else 0,
+                                               grad_out.data_ptr(), reduction == 0,
+                                               dlogits.data_ptr(), dstride),
+           "dmh_cross_entropy_grad_stats")

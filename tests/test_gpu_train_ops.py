@@ -772,3 +772,80 @@ def test_writes_in_place_are_seen_by_autograd(T):
     before = dw._version
     T.embedding_backward(g, y, 300, weight_grad=dw)
     assert dw._version == before + 1
+
+
+@pytest.mark.parametrize("v", [200, 1000, 8009, 32003, 150001])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+@pytest.mark.parametrize("offset", [0.0, 30.0, -1000.0, 1e4])
+def test_what_all_logits_have_in_common_costs_nothing(T, v, eps, offset):
+    """Rows that are sure of their target, far from zero.  The bounds know differences of logits
+    alone: rho is the relative error of a row's sum (Xent), a loss adds the rounding of its
+    three terms and of the logarithm, and the sum of differences that many of the largest."""
+    z = normal(24, v, seed=v)
+    y = ids_of((24,), v, seed=3, kind="flat")
+    z[torch.arange(24), y] += torch.linspace(0.0, 24.0, 24)
+    z += offset
+    c = Xent(z, y, eps)
+    zd = z.double()
+    m = zd.amax(1)
+    depth = m - zd.amin(1)
+    chain = max(64, v // 256) + 32
+    rho = (chain + 4 * depth) * E32
+    gap = m - zd.gather(1, y[:, None])[:, 0]
+    size = torch.log(torch.exp(zd - m[:, None]).sum(1)) + gap + eps * depth
+    loss_err = rho + 6 * E32 * size + eps * chain * E32 * depth
+    p = torch.exp(zd - torch.logsumexp(zd, 1, keepdim=True))
+    q = (c.dz - p).abs()
+    dz_err = p * (rho[:, None] + (4 * (m[:, None] - zd) + 8) * E32) + 6 * E32 * (p + q)
+    zg, yg = z.to(DEV), y.to(DEV)
+    close(T.cross_entropy(zg, yg, label_smoothing=eps, reduction="none"), c.loss, loss_err)
+    loss, dz = T.cross_entropy_step(zg, yg, label_smoothing=eps, reduction="sum")
+    close(loss, c.loss.sum(), loss_err.sum() + 24 * E32 * c.loss.sum())
+    close(dz, c.dz, dz_err)
+    leaf = zg.requires_grad_()
+    for red, g in (("sum", torch.ones(())), ("none", torch.ones(24))):
+        loss = T.cross_entropy(leaf, yg, label_smoothing=eps, reduction=red)
+        close(torch.autograd.grad(loss, leaf, g.to(DEV))[0], c.dz, dz_err)
+
+
+@pytest.mark.parametrize("v", [50, 5000, 150001])
+def test_smoothed_losses_of_lowest_and_highest_values(T, v):
+    """Masks of the type's lowest value count in the mean over the classes, and no sum of them
+    overflows: z times 2^-28 keeps every bit."""
+    low = torch.finfo(F32).min
+    z, y = xent_case(6, v, F32, ignored=False)
+    y[:] = torch.arange(6) + 10
+    z[0, 30:] = low
+    z[1, y[1]] = low                     # the target itself
+    z[2] = low
+    z[3, ::2] = low / 4
+    z[4, 3:8] = -low / 4
+    z[5, 40] = -float("inf")
+    want = R.xent(z, y, eps=0.1)[0]
+    size = torch.where(torch.isfinite(z), z.double().abs(), 0.0).amax(1)
+    got = T.cross_entropy(z.to(DEV), y.to(DEV), label_smoothing=0.1, reduction="none")
+    close(got, want, (max(64, v // 256) + 40) * E32 * (2 * size + 20))
+    assert want[5] == float("inf") and torch.isfinite(want[:5]).all()
+
+
+@pytest.mark.parametrize("n,v", [(5, 40), (33, 5001), (3, 200001)])
+def test_entries_that_keep_lse(n, v):
+    """The C entries whose statistic is lse alone."""
+    from defmuon_amd import _native
+    lib = _native.load()
+    z, y = xent_case(n, v, F32)
+    c = Xent(z, y, 0.1, 1e-3)
+    zg, yg = z.to(DEV), y.to(DEV)
+    loss, lse, ws = (torch.empty(k, device=DEV) for k in (1, n, n))
+    count, go, dz = torch.empty(1, device=DEV), torch.ones(1, device=DEV), torch.empty_like(zg)
+    stream = torch.cuda.current_stream().cuda_stream
+    args = (stream, zg.data_ptr(), 0, n, v, v, yg.data_ptr(), 1, -100, 0.1, 1e-3)
+    assert lib.dmh_cross_entropy(*args, 1, 1.0, loss.data_ptr(), count.data_ptr(), lse.data_ptr(),
+                                 None, v, ws.data_ptr(), 4 * n) == 0
+    assert lib.dmh_cross_entropy_grad(*args, lse.data_ptr(), count.data_ptr(), go.data_ptr(), 0,
+                                      dz.data_ptr(), v) == 0
+    want, err, live = c.mean()
+    close(loss[0], want, err)
+    assert int(count) == live
+    close(lse, torch.where(c.live, torch.logsumexp(z.double(), 1), 0.0), c.lse_err)
+    close(dz, *c.grad_bound(1.0 / live, F32))

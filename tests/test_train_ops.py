@@ -228,3 +228,20 @@ def test_writes_in_place_are_seen_by_autograd(stand_in):
     assert (dw._version, dp._version) == (1, 0) and bool((dw == 1).all())
     T.embedding_backward(g, ids, 5, pos_rows=4, weight_grad=dw, pos_grad=dp)
     assert (dw._version, dp._version) == (2, 1)
+
+
+def test_entries_that_keep_row_statistics_refuse(lib):
+    one = ctypes.c_void_p(256)   # never read
+
+    def fwd(top=one, total=one, rows=2, dt=0, red=1):
+        return lib.dmh_cross_entropy_stats(None, one, dt, rows, 5, 5, one, 1, -100, 0.0, 0.0, red,
+                                           1.0, one, one, top, total, None, 5, one, 1 << 20)
+
+    def bwd(top=one, total=one, rows=2, dt=0):
+        return lib.dmh_cross_entropy_grad_stats(None, one, dt, rows, 5, 5, one, 1, -100, 0.0, 0.0,
+                                                top, total, None, one, 0, one, 5)
+    for call in (fwd, bwd):
+        for bad in (dict(top=None), dict(total=None), dict(rows=1 << 22), dict(dt=3)):
+            assert call(**bad) == 1, bad
+            assert b"dmh_cross_entropy" in lib.dmh_last_error()
+    assert fwd(rows=0, red=0, top=None, total=None) == 0 and bwd(rows=0, total=None) == 0
