@@ -10,7 +10,8 @@ fp32, bf16 and fp16 tensors; everything is computed in fp32 and rounded once.  A
 run through the HIP library on the current stream and synchronise nothing; there is no CPU
 fallback.  embedding, dropout and cross_entropy take part in autograd; the *_backward
 functions and cross_entropy_step are for programs that call the gradients themselves.
-Arguments that do not fit raise NativeError.
+Arguments that do not fit raise NativeError, as do tensors that carry a forward-mode tangent:
+there is no such derivative.
 
 Random numbers: `rng` names the mask of a dropout.  It is a pair of integers (seed, offset), or
 an int64 tensor of the two on the GPU, which is read when a kernel runs: a captured graph
@@ -23,7 +24,7 @@ element is replaced by zero, also where it is not finite.
 """
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -39,7 +40,14 @@ _NO_RNG = (0, 0, 0)
 
 # ---- arguments ------------------------------------------------------------------------------
 
+def _no_tangent(t, what, name):
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NativeError(f"{what}: no forward-mode derivative ({name} has a tangent)")
+
+
 def _float(t, what, name):
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, what, name)
     if not t.is_cuda:
         raise NativeError(f"{what}: the HIP path needs a GPU tensor ({name} is on {t.device})")
     if t.dtype not in FLOATS:
@@ -255,6 +263,8 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
         if pos_weight is None:
             raise NativeError(f"{what}: positions without a position table")
     if pos_weight is not None:
+        if forward_ad._current_level >= 0:
+            _no_tangent(pos_weight, what, "pos_weight")
         pshape = pos_weight.shape
         if (len(pshape) != 2 or pshape[1] != shape[1] or pos_weight.dtype != dtype
                 or pos_weight.device != device):
@@ -400,6 +410,8 @@ class _CrossEntropy(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        if forward_ad._current_level >= 0:
+            _no_tangent(grad, "cross_entropy", "the loss's gradient")
         logits, targets, stats = ctx.saved_tensors
         z, *rows = _rows(logits)
         dz, stride = _like_rows(logits, (z, *rows))
@@ -437,8 +449,8 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     raises torch's error where the logits' values are needed for it (a soft-cap's tanh, another
     loss of the same logits)."""
     what = "cross_entropy_step"
-    logits = logits.detach()
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)
+    logits = logits.detach()
     if reduction == "none":
         raise NativeError(f"{what}: the loss must be a mean or a sum")
     rows = _rows(logits)

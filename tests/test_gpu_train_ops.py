@@ -849,3 +849,17 @@ def test_entries_that_keep_lse(n, v):
     assert int(count) == live
     close(lse, torch.where(c.live, torch.logsumexp(z.double(), 1), 0.0), c.lse_err)
     close(dz, *c.grad_bound(1.0 / live, F32))
+
+
+def test_forward_mode_is_refused(T, Err):
+    import torch.autograd.forward_ad as fwd
+    x, y = normal(4, 8).to(DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: T.dropout(d, 0.1, RNG), lambda: T.dropout(x, 0.1, RNG, residual=d),
+                     lambda: T.embedding(y, d), lambda: T.embedding(y, x, d, positions=y),
+                     lambda: T.embedding_backward(x, y, 4, weight_grad=d),
+                     lambda: T.cross_entropy(d, y), lambda: T.cross_entropy_step(d, y)):
+            with pytest.raises(Err, match="forward-mode"):
+                call()
+        T.dropout(x, 0.1, RNG, residual=x)   # no tangent, no refusal

@@ -245,3 +245,39 @@ def test_entries_that_keep_row_statistics_refuse(lib):
             assert call(**bad) == 1, bad
             assert b"dmh_cross_entropy" in lib.dmh_last_error()
     assert fwd(rows=0, red=0, top=None, total=None) == 0 and bwd(rows=0, total=None) == 0
+
+
+def test_forward_mode_is_refused(monkeypatch):
+    """A tangent is never dropped, whether or not a gradient is wanted too."""
+    import torch.autograd.forward_ad as fwd
+    from defmuon_amd import train_ops as T
+    from defmuon_amd._native import NativeError
+    w, x = torch.randn(4, 8), torch.randn(2, 3, 8)
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    with fwd.dual_level():
+        def dual(t, grad=False):
+            return fwd.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+        for grad in (False, True):
+            for call in (lambda: T.dropout(dual(x, grad), 0.1, (1, 2)),
+                         lambda: T.dropout_backward(dual(x, grad), 0.1, (1, 2)),
+                         lambda: T.embedding(ids, dual(w, grad)),
+                         lambda: T.embedding_backward(dual(x, grad), ids, 4),
+                         lambda: T.cross_entropy(dual(x, grad), ids),
+                         lambda: T.cross_entropy_step(dual(x, grad), ids)):
+                with pytest.raises(NativeError, match="forward-mode"):
+                    call()
+        with pytest.raises(NativeError, match="GPU"):   # without a tangent, the ordinary way
+            T.dropout(x, 0.1, (1, 2))
+        monkeypatch.setattr(T, "_float", lambda *a: None)   # past the first table's check
+        with pytest.raises(NativeError, match="forward-mode"):
+            T.embedding(ids, w, dual(w))
+
+
+def test_a_tangent_of_the_gradient_is_refused(stand_in):
+    import torch.autograd.forward_ad as fwd
+    from defmuon_amd._native import NativeError
+    z = torch.randn(6, 11, requires_grad=True)
+    with fwd.dual_level():
+        loss = stand_in.cross_entropy(z, torch.arange(6))
+        with pytest.raises(NativeError, match="forward-mode"):
+            torch.autograd.grad(loss, z, fwd.make_dual(torch.ones(()), torch.ones(())))
