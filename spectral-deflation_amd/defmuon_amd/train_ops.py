@@ -11,7 +11,9 @@ run through the HIP library on the current stream and synchronise nothing; there
 fallback.  embedding, dropout and cross_entropy take part in autograd; the *_backward
 functions and cross_entropy_step are for programs that call the gradients themselves.
 Arguments that do not fit raise NativeError, as do tensors that carry a forward-mode tangent:
-there is no such derivative.
+there is no such derivative.  So do traces that would record the results' allocation and not the
+launch behind it: make_fx and fake tensors for all functions, torch.jit.trace (which records
+autograd functions) for those outside autograd.
 
 Random numbers: `rng` names the mask of a dropout.  It is a pair of integers (seed, offset), or
 an int64 tensor of the two on the GPU, which is read when a kernel runs: a captured graph
@@ -34,6 +36,10 @@ from defmuon_amd._native import FLOATS, NativeError
 __all__ = ["embedding", "embedding_backward", "dropout", "dropout_backward", "Dropout",
            "draw_rng", "cross_entropy", "cross_entropy_step"]
 
+_is_tracing = torch._C._is_tracing
+_modes = torch._C._len_torch_dispatch_stack
+_early_proxy = torch._ops._mode_stack_state_for_pre_dispatch.get   # make_fx(pre_dispatch=True)
+
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _NO_RNG = (0, 0, 0)
 
@@ -43,6 +49,18 @@ _NO_RNG = (0, 0, 0)
 def _no_tangent(t, what, name):
     if forward_ad.unpack_dual(t).tangent is not None:
         raise NativeError(f"{what}: no forward-mode derivative ({name} has a tangent)")
+
+
+def _eager(what, function=False):
+    """Refuse to be traced (function: torch.jit.trace records an autograd function instead)."""
+    if not function and _is_tracing():
+        raise NativeError(f"{what}: torch.jit.trace cannot record a launch")
+    traced = _early_proxy(0) is not None
+    if _modes():
+        key, mode = torch._C._TorchDispatchModeKey, torch._C._get_dispatch_mode
+        traced |= mode(key.PROXY) is not None or mode(key.FAKE) is not None
+    if traced:
+        raise NativeError(f"{what}: a trace of torch calls cannot record a launch")
 
 
 def _float(t, what, name):
@@ -69,8 +87,8 @@ def _out_type(dtype, what):
 def _rows(t):
     """(tensor, rows, columns, row stride) of a tensor taken as rows of its last dimension; a
     copy where its rows are not contiguous or not evenly spaced."""
-    cols = t.shape[-1] if t.ndim else 1
-    rows = t.numel() // cols if cols else 0
+    cols = int(t.shape[-1]) if t.ndim else 1   # (a trace's sizes are tensors)
+    rows = int(t.numel()) // cols if cols else 0
     if t.is_contiguous():
         return t, rows, cols, cols
     if t.stride(-1) == 1 or cols == 1:
@@ -153,6 +171,7 @@ class _Dropout(Function):
 
 def dropout(x, p, rng, residual=None):
     """Dropout of x, plus `residual` (same shape; the result then has its type)."""
+    _eager("dropout", function=True)
     _float(x, "dropout", "x")
     if residual is not None:
         _float(residual, "dropout", "residual")
@@ -160,8 +179,8 @@ def dropout(x, p, rng, residual=None):
             raise NativeError(f"dropout: residual is {tuple(residual.shape)} on "
                               f"{residual.device}, x {tuple(x.shape)} on {x.device}")
     cut, key = _drop(p, rng, x.device, "dropout")
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or residual is not None and residual.requires_grad):
+    if _is_tracing() or torch.is_grad_enabled() and (
+            x.requires_grad or residual is not None and residual.requires_grad):
         return _Dropout.apply(x, residual, p, rng)
     return _dropout(x, residual, cut, key, x.dtype if residual is None else residual.dtype)
 
@@ -169,6 +188,7 @@ def dropout(x, p, rng, residual=None):
 def dropout_backward(grad, p, rng, dtype=None):
     """The gradient of dropout's x (in `dtype`, the gradient's own by default); that of its
     residual is `grad` itself."""
+    _eager("dropout_backward")
     _float(grad, "dropout_backward", "grad")
     dtype = dtype or grad.dtype
     _out_type(dtype, "dropout_backward")
@@ -253,6 +273,7 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
     dimension.  The tables have one type; out_dtype is theirs by default.  padding_idx takes no
     gradient.  An id or position outside its table gives a row of NaN."""
     what = "embedding"
+    _eager(what, function=True)
     _float(weight, what, "weight")
     device, dtype, shape = weight.device, weight.dtype, weight.shape
     if len(shape) != 2:
@@ -279,8 +300,8 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
         dtype = out_dtype
         _out_type(dtype, what)
     cut, key = _drop(dropout_p, rng, device, what)
-    if torch.is_grad_enabled() and (weight.requires_grad
-                                    or pos_weight is not None and pos_weight.requires_grad):
+    if _is_tracing() or torch.is_grad_enabled() and (
+            weight.requires_grad or pos_weight is not None and pos_weight.requires_grad):
         return _Embedding.apply(weight, pos_weight, ids, positions, scale, padding_idx,
                                 dropout_p, rng, dtype)
     return _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype)
@@ -313,6 +334,7 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     gradient of a tied head, or that of the micro-batches before).  The sums are fp32, in an
     order that the ids decide: the same inputs give the same bits."""
     what = "embedding_backward"
+    _eager(what)
     _float(grad, what, "grad")
     _ints(ids, grad.device, what, "ids")
     if grad.ndim != ids.ndim + 1 or grad.shape[:-1] != ids.shape:
@@ -430,8 +452,9 @@ def cross_entropy(logits, targets, ignore_index=-100, label_smoothing=0.0, z_los
     with s the label smoothing; summed, averaged over the rows that have a target, or (for
     "none") one a row.  Rows whose target is ignore_index count for nothing; another target
     outside the classes gives NaN, as does a row of logits that are all -inf."""
+    _eager("cross_entropy", function=True)
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, "cross_entropy")
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
         return _CrossEntropy.apply(logits, targets, ignore_index, label_smoothing, z_loss,
                                    reduction)
     return _xent(logits, _rows(logits), targets, ignore_index, label_smoothing, z_loss,
@@ -449,6 +472,7 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     raises torch's error where the logits' values are needed for it (a soft-cap's tanh, another
     loss of the same logits)."""
     what = "cross_entropy_step"
+    _eager(what)
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)
     logits = logits.detach()
     if reduction == "none":

@@ -851,6 +851,7 @@ def test_entries_that_keep_lse(n, v):
     close(dz, *c.grad_bound(1.0 / live, F32))
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_forward_mode_is_refused(T, Err):
     import torch.autograd.forward_ad as fwd
     x, y = normal(4, 8).to(DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
@@ -863,3 +864,21 @@ def test_forward_mode_is_refused(T, Err):
             with pytest.raises(Err, match="forward-mode"):
                 call()
         T.dropout(x, 0.1, RNG, residual=x)   # no tangent, no refusal
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traces(T, Err):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    w, w2 = normal(50, 24).to(DEV), normal(50, 24, seed=1).to(DEV)
+    ids, y = ids_of((9,), 50).to(DEV), ids_of((9,), 24).to(DEV)
+
+    def step(t):
+        x = T.embedding(ids, t, dropout_p=0.1, rng=RNG)
+        return T.cross_entropy(T.dropout(x, 0.2, RNG, residual=x), y)
+    for grad in (False, True):
+        traced = torch.jit.trace(step, w.clone().requires_grad_(grad))
+        assert torch.equal(traced(w2), step(w2))
+    for call in (step, lambda t: T.dropout_backward(t, 0.1, RNG),
+                 lambda t: T.cross_entropy_step(t[:9], y)[1]):
+        with pytest.raises(Err, match="trace"):
+            make_fx(call)(w)

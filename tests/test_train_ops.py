@@ -172,6 +172,7 @@ def stand_in(monkeypatch):
 
     def cross_entropy(z, rows, y, ignore, smoothing, z_loss, reduction, grad_scale, loss, dz,
                       dstride):
+        assert all(type(n) is int for n in rows)
         zz = z.detach().clone()
         rows, d, _ = R.xent(zz, y, ignore, smoothing, z_loss)
         n = 1 if reduction == 2 else int((y != ignore).sum())
@@ -247,6 +248,7 @@ def test_entries_that_keep_row_statistics_refuse(lib):
     assert fwd(rows=0, red=0, top=None, total=None) == 0 and bwd(rows=0, total=None) == 0
 
 
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
 def test_forward_mode_is_refused(monkeypatch):
     """A tangent is never dropped, whether or not a gradient is wanted too."""
     import torch.autograd.forward_ad as fwd
@@ -281,3 +283,42 @@ def test_a_tangent_of_the_gradient_is_refused(stand_in):
         loss = stand_in.cross_entropy(z, torch.arange(6))
         with pytest.raises(NativeError, match="forward-mode"):
             torch.autograd.grad(loss, z, fwd.make_dual(torch.ones(()), torch.ones(())))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_traces_record_the_call_or_refuse(stand_in, monkeypatch):
+    """torch.jit.trace records autograd functions; every other trace would hold the allocation
+    of the results alone."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    from defmuon_amd import _native
+    T = stand_in
+
+    def dropout(x, residual, out, cut, rng, rows):
+        out.detach().numpy()[...] = 2 * x.detach().numpy()
+
+    def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
+        out.detach().numpy()[...] = weight.detach().numpy()[ids.numpy()]
+    monkeypatch.setattr(_native, "dropout", dropout)
+    monkeypatch.setattr(_native, "embedding", embedding)
+    x, z, y = torch.randn(3, 5), torch.randn(3, 5), torch.arange(3)
+    ops = (lambda t: T.dropout(t + 1, 0.1, (1, 2)) * 3, lambda t: T.embedding(y, t),
+           lambda t: T.cross_entropy(t, y, reduction="none"))
+    steps = (lambda t: T.dropout_backward(t, 0.1, (1, 2)),
+             lambda t: T.embedding_backward(t, y, 4)[0], lambda t: T.cross_entropy_step(t, y)[1])
+    for grad in (False, True):
+        for op in ops:
+            traced = torch.jit.trace(op, x.clone().requires_grad_(grad))
+            assert torch.equal(traced(z), op(z))
+    for op in ops + steps:
+        for kw in ({}, dict(tracing_mode="symbolic"), dict(pre_dispatch=True)):
+            with pytest.raises(_native.NativeError, match="trace"):
+                make_fx(op, **kw)(x)
+        with FakeTensorMode() as mode, pytest.raises(_native.NativeError, match="trace"):
+            op(mode.from_tensor(x))
+        with FlopCounterMode(display=False):   # a mode that records nothing
+            op(x)
+    for op in steps:
+        with pytest.raises(_native.NativeError, match="trace"):
+            torch.jit.trace(op, x)
