@@ -127,7 +127,7 @@ struct GradArgs {
   GradJob job[2];      // the token table's and the position table's
   const void* g;
   long long gstride;
-  int is64, tokens, seq, batch, dim, dimp, ctiles, lanes;   // a wave: `lanes` x 8 columns
+  int is64, tokens, seq, batch, dim, dimp, ctiles;   // a wave: 512 columns
   int small;           // embed_grad_small's
   Rng rng;
 };
@@ -350,7 +350,10 @@ __device__ __forceinline__ int wave_first_at(const int* keys, int hi, int v) {
   return lo;
 }
 
-// the scaled sum of one id into eight columns of its row
+// The scaled sum of one id into eight columns of its row.  The last eight columns of a width that is
+// no multiple of eight begin inside the piece before them (c & 7), and both lanes write what they
+// share with the same values; where sums are added, the later lane leaves it to the other, so
+// that no element is written by one lane while another has yet to read it.
 template <class TO>
 __device__ __forceinline__ void put_row(const GradArgs& a, const GradJob& j, int row, int c,
                                         const float (&sum)[8]) {
@@ -359,7 +362,13 @@ __device__ __forceinline__ void put_row(const GradArgs& a, const GradJob& j, int
   if (j.accumulate) load8(o, v);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(sum[k], j.scale, v[k]);
-  store8(o, v);
+  if (j.accumulate && (c & 7)) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k >= 8 - (c & 7)) o[k] = (TO)v[k];
+  } else {
+    store8(o, v);
+  }
 }
 
 // Sorted tokens a chunk: 16 leave twice the parts to join (32768 tokens 115 us instead of 101),
@@ -415,8 +424,7 @@ __device__ void clear_rows(const GradArgs& a, const GradJob& j, int group) {
 // bf16 ones (431 MB, 6.3 TB/s).
 //
 // A lane has eight columns.  Where the width is no multiple of eight, the last lane of a row takes
-// its last eight columns, some of them its neighbour's too: both write the same values, and lie in
-// one wave (grad_lanes), so that both read before either writes where sums are added.
+// its last eight columns, some of them its neighbour's too.
 template <class TG, class TO, bool DROP>
 __global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
   // the sums first: their latency is under the writes of the rows cleared behind them
@@ -435,8 +443,8 @@ __global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(b * 4 + (int)(threadIdx.x >> 6));
   const int chunk = w / a.ctiles;
   if (chunk >= j.chunks) return;
-  int c = ((w - chunk * a.ctiles) * a.lanes + lane) * 8;
-  const bool mine = lane < a.lanes && c < a.dim;
+  int c = ((w - chunk * a.ctiles) * 64 + lane) * 8;
+  const bool mine = c < a.dim;
   c = mine && c + 8 <= a.dim ? c : a.dim - 8;   // lanes without columns read, and write nothing
   const int s0 = chunk * CHUNK, count = a.tokens - s0 < CHUNK ? a.tokens - s0 : CHUNK;
   // lane l has the chunk's entry l; behind the last one, that one again
@@ -537,7 +545,7 @@ __global__ __launch_bounds__(256) void embed_grad_small(GradArgs a) {
     const int s0 = __builtin_amdgcn_readfirstlane(first[r]);
     const int s1 = __builtin_amdgcn_readfirstlane(first[r + 1]);
     if (s0 == s1 && j.accumulate) continue;
-    for (int c = lane * 8; c < a.dim && lane < a.lanes; c += 8 * a.lanes) {
+    for (int c = lane * 8; c < a.dim; c += 8 * 64) {
       if (c + 8 > a.dim) c = a.dim - 8;   // overlaps its neighbour's, as in embed_grad
       float sum[8] = {};
       for (int s = s0; s < s1; s += SMALL_AHEAD) {
@@ -613,8 +621,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join(GradArgs a) {
   if (id >= j.rows || key_at(a, j, end) != id) return;
   if (chunk && key_at(a, j, chunk * CHUNK - 1) == id) return;   // began before
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int c = (blockIdx.y * a.lanes + lane) * 8;
-  const bool mine = lane < a.lanes && c < a.dim;
+  int c = (blockIdx.y * 64 + lane) * 8;
+  const bool mine = c < a.dim;
   c = mine && c + 8 <= a.dim ? c : a.dim - 8;
   // the id has a part in every chunk from here on whose first id it is; the sorted list says at
   // once of 64 chunks whether they are
@@ -695,15 +703,6 @@ static void launch_grad(hipStream_t stream, const GradArgs& a) {
     launch_grad<TG, TO, true>(stream, a);
   else
     launch_grad<TG, TO, false>(stream, a);
-}
-
-// Lanes of a wave that take columns: such that the last wave of a row has two at least where the
-// last lane's columns overlap its neighbour's.
-static int grad_lanes(int dim) {
-  const int pieces = ceil_div(dim, 8);
-  int lanes = 64;
-  while (pieces > 1 && (dim & 7) && pieces % lanes == 1) --lanes;
-  return lanes;
 }
 
 // what a table's gradient takes of the workspace: sorted ids and tokens, the radix sort's other
@@ -879,8 +878,7 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   a.batch = a.tokens / a.seq < 1 ? 1 : a.tokens / a.seq;
   a.dim = dim;
   a.dimp = (dim + 7) / 8 * 8;
-  a.lanes = grad_lanes(dim);
-  a.ctiles = ceil_div(dim, 8 * a.lanes);
+  a.ctiles = ceil_div(dim, 8 * 64);
   a.rng = make_rng(seed, offset, rng_state, cut);
   if (tok)
     grad_job(a.job[0], a, ids, out, rows, padding_idx, scale * a.rng.scale, accumulate != 0,

@@ -882,3 +882,24 @@ def test_traces(T, Err):
                  lambda t: T.cross_entropy_step(t[:9], y)[1]):
         with pytest.raises(Err, match="trace"):
             make_fx(call)(w)
+
+
+@pytest.mark.parametrize("dim", [9, 15, 500, 513, 519, 1025, 1027, 2049])
+@pytest.mark.parametrize("tokens,rows", [(200, 300), (3000, 40), (9000, 700)])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_overlapping_columns_are_added_once(T, dim, tokens, rows, out):
+    """Widths whose last eight columns share some with the piece before, in the same wave and
+    (8 x 64 n + 1 .. 7) in another: each sum is added once, in one launch, chunk by chunk and
+    joined, for the sums of either table."""
+    ids, t = ids_of((tokens,), rows), ids_of((tokens,), 64, seed=1)
+    g = normal(tokens, dim)
+    w0, p0 = normal(rows, dim, dtype=out, seed=5), normal(64, dim, dtype=out, seed=6)
+    w, pg = w0.to(DEV), p0.to(DEV)
+    for _ in range(2):
+        T.embedding_backward(g.to(DEV), ids.to(DEV), rows, pos_rows=64, positions=t.to(DEV),
+                             weight_grad=w, pos_grad=pg)
+        for got, first, idx in ((w, w0, ids), (pg, p0, t)):
+            want, size, n = R.table_grad(g, idx, first.shape[0])
+            want = want + first.double()
+            close(got, want, grad_bound(want, size + first.double().abs(), n, out))
+        w0, p0 = w.cpu(), pg.cpu()
