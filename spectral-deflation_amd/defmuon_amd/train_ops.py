@@ -222,13 +222,16 @@ def _table(t):
 
 
 def _positions(positions, ids, what):
+    """(ids, positions) as the kernels take them, both of the wider type of the two."""
     if positions is None:
-        return None
+        return ids, None
     _ints(positions, ids.device, what, "positions")
     if positions.shape != ids.shape:
         raise NativeError(f"{what}: positions are {tuple(positions.shape)}, ids "
                           f"{tuple(ids.shape)}")
-    return positions.to(ids.dtype).contiguous()
+    if positions.dtype != ids.dtype:
+        ids, positions = ids.long(), positions.long()
+    return ids, positions.contiguous()
 
 
 def _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype):
@@ -280,7 +283,7 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
         raise NativeError(f"{what}: weight must be (rows, dim), got {tuple(shape)}")
     _ints(ids, device, what, "ids")
     if positions is not None:
-        positions = _positions(positions, ids, what)
+        ids, positions = _positions(positions, ids, what)
         if pos_weight is None:
             raise NativeError(f"{what}: positions without a position table")
     if pos_weight is not None:
@@ -344,7 +347,7 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     if rows < 0 or pos_rows < 0:
         raise NativeError(f"{what}: {rows} and {pos_rows} rows")
     _padding(padding_idx, rows, what)
-    positions = _positions(positions, ids, what)
+    ids, positions = _positions(positions, ids, what)
     if pos_rows and positions is None and (ids.ndim < 1 or ids.shape[-1] > pos_rows):
         raise NativeError(f"{what}: ids {tuple(ids.shape)} have more positions than {pos_rows}")
     cut, key = _drop(dropout_p, rng, grad.device, what)

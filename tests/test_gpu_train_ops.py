@@ -903,3 +903,17 @@ def test_overlapping_columns_are_added_once(T, dim, tokens, rows, out):
             want = want + first.double()
             close(got, want, grad_bound(want, size + first.double().abs(), n, out))
         w0, p0 = w.cpu(), pg.cpu()
+
+
+def test_positions_of_another_type_outside_the_table(T):
+    w, pos = normal(10, 24).to(DEV), normal(4, 24, seed=1).to(DEV)
+    ids, t = torch.tensor([3, 1, 4, 9, 2]), torch.tensor([1, 2 ** 32 + 1, -2 ** 32, 2 ** 31, 3])
+    g = normal(5, 24)
+    for i, p in ((ids.int(), t), (t, ids.int() % 4)):
+        y = T.embedding(i.to(DEV), w, pos, positions=p.to(DEV)).cpu()
+        ok = (i >= 0) & (i < 10) & (p >= 0) & (p < 4)
+        assert torch.equal(torch.isnan(y).all(1), ~ok) and not torch.isnan(y[ok]).any()
+        dw, dp = T.embedding_backward(g.to(DEV), i.to(DEV), 10, pos_rows=4, positions=p.to(DEV))
+        for got, idx, rows in ((dw, i, 10), (dp, p, 4)):
+            want, size, n = R.table_grad(g, idx, rows)
+            close(got, want, grad_bound(want, size, n, F32))

@@ -322,3 +322,14 @@ def test_traces_record_the_call_or_refuse(stand_in, monkeypatch):
     for op in steps:
         with pytest.raises(_native.NativeError, match="trace"):
             torch.jit.trace(op, x)
+
+
+def test_positions_and_ids_keep_their_values():
+    from defmuon_amd.train_ops import _positions
+    a, b = torch.tensor([3, -1], dtype=torch.int32), torch.tensor([2 ** 32 + 1, -2 ** 32])
+    for ids, positions, dtype in ((a, b, torch.int64), (b, a, torch.int64),
+                                  (a, a.flip(0), torch.int32), (b, b.flip(0), torch.int64)):
+        i, p = _positions(positions, ids, "embedding")
+        assert i.dtype == p.dtype == dtype
+        assert i.tolist() == ids.tolist() and p.tolist() == positions.tolist()
+    assert _positions(None, a, "embedding")[0] is a
