@@ -493,8 +493,10 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     seed, offset, state = rng
     vocab, dim = weight.shape
     seq = ids.shape[-1] if ids.ndim else 1
-    pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr(), pos_weight.shape[0],
-                                                pos_weight.stride(0))
+    # a table without rows has no address, and must not pass for no table: any address will do,
+    # nothing of it is read
+    pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr() or out.data_ptr(),
+                                                pos_weight.shape[0], pos_weight.stride(0))
     _check(load().dmh_embedding(_raw_stream(index), ids.data_ptr(),
                                 ids.dtype == torch.int64, ids.numel(), seq, weight.data_ptr(),
                                 FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,

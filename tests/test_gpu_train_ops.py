@@ -917,3 +917,20 @@ def test_positions_of_another_type_outside_the_table(T):
         for got, idx, rows in ((dw, i, 10), (dp, p, 4)):
             want, size, n = R.table_grad(g, idx, rows)
             close(got, want, grad_bound(want, size, n, F32))
+
+
+def test_a_position_table_without_rows(T):
+    """Every position is outside it."""
+    w, none = normal(10, 24).to(DEV).requires_grad_(), torch.empty(0, 24, device=DEV)
+    ids = torch.tensor([3, 1, 4]).to(DEV)
+    y = T.embedding(ids, w, none, positions=torch.zeros_like(ids))
+    assert torch.isnan(y).all()
+    g = normal(3, 24)
+    (dw,) = torch.autograd.grad(y, w, g.to(DEV))
+    want, size, n = R.table_grad(g, ids.cpu(), 10)
+    close(dw, want, grad_bound(want, size, n, F32))
+    assert torch.isnan(T.embedding(ids, none, none, positions=ids)).all()
+    assert torch.isnan(T.embedding(ids, none)).all()
+    assert T.embedding(ids[:0], w, none).shape == (0, 24)
+    # no rows, no gradient of them
+    assert T.embedding_backward(g.to(DEV), ids, 10, pos_rows=0, positions=ids)[1] is None
