@@ -408,6 +408,13 @@ __device__ void clear_rows(const GradArgs& a, const GradJob& j, int group) {
   }
   __syncthreads();
   const unsigned long long m = named;
+  if (a.dim < 8) {   // rows shorter than a piece: all of them together
+    const int count = (j.rows - v0 < FILL_ROWS ? j.rows - v0 : FILL_ROWS) * a.dim;
+    TO* o = (TO*)j.out + (long long)v0 * a.dim;
+    for (int e = threadIdx.x; e < count; e += 256)
+      if (!(m >> (e / a.dim) & 1)) o[e] = (TO)0.f;
+    return;
+  }
   constexpr int N = Piece<TO>::N;
   const typename Piece<TO>::type zero = {};
   const int whole = a.dim / N;
@@ -575,36 +582,72 @@ __global__ __launch_bounds__(256) void embed_grad_small(GradArgs a) {
   }
 }
 
-// Tables narrower than eight columns, which no piece of a row fits: a thread has one element of the
-// table and walks through its tokens.  Right for any such table, and made for none to be fast.
+// Tables narrower than eight columns, which no piece of a row fits: the same chunks and parts, by
+// eight lanes a chunk, one a column.  Right for any such table, and made for none to be fast; but
+// a thread has no more than one chunk's tokens to walk through, however often an id occurs:
+// 200000 tokens of four columns take 50 us if all have one id and 69 with 50257 of them, where a
+// thread for each element of the table took 33000 and 56 (and stopped adding at 2^24 ones).
+constexpr int NARROW_CHUNKS = 32;   // a workgroup
+
 template <class TG, class TO, bool DROP>
-__global__ __launch_bounds__(256) void embed_grad_narrow(GradArgs a, int jn) {
+__global__ __launch_bounds__(256) void embed_grad_narrow(GradArgs a) {
+  const int sums = a.job[0].reduce_groups + a.job[1].reduce_groups;
+  int b = blockIdx.x;
+  if (b >= sums) {
+    b -= sums;
+    const int second = b >= a.job[0].fill_groups;
+    clear_rows<TO>(a, a.job[second], second ? b - a.job[0].fill_groups : b);
+    return;
+  }
+  const int jn = b >= a.job[0].reduce_groups;
   const GradJob& j = a.job[jn];
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (long long)j.rows * a.dim) return;
-  const int v = (int)(at / a.dim), c = (int)(at - (long long)v * a.dim);
-  int s0, s1;
-  if (j.ids) {
-    s0 = first_at(j.keys, 0, a.tokens, v);
-    s1 = first_at(j.keys, s0, a.tokens, v + 1);
-  } else {
-    s0 = v < a.seq ? v * a.batch : 0;
-    s1 = v < a.seq && a.tokens ? s0 + a.batch : s0;
-  }
+  if (jn) b -= a.job[0].reduce_groups;
+  const int c = threadIdx.x & 7, chunk = b * NARROW_CHUNKS + (int)(threadIdx.x >> 3);
+  if (chunk >= j.chunks || c >= a.dim) return;
+  const int s0 = chunk * CHUNK, s1 = a.tokens - s0 < CHUNK ? a.tokens : s0 + CHUNK;
+  const int before = s0 ? key_at(a, j, s0 - 1) : -1;
+  const int after = s1 < a.tokens ? key_at(a, j, s1) : -1;
   const RngKey rk = DROP ? rng_key(a.rng) : RngKey{};
+  float* part = j.part + (long long)chunk * 2 * a.dimp + c;
+  auto put = [&](int row, float sum) {
+    TO* o = (TO*)j.out + (long long)row * a.dim + c;
+    *o = (TO)fmaf(sum, j.scale, j.accumulate ? (float)*o : 0.f);
+  };
   float sum = 0.f;
-  for (int s = s0; s < s1; ++s) {
-    const long long i = token_at(a, j, s);
-    float x = (float)((const TG*)a.g)[i * a.gstride + c];
-    if (DROP) x = kept(keep_bits_at<true>(a.rng, rk, (unsigned long long)(i * a.dim + c)), 0, x);
-    sum += x;
+  int cur = key_at(a, j, s0);
+  bool began_here = cur != before;
+  constexpr int AHEAD = 8;
+  for (int e = s0; e < s1; e += AHEAD) {
+    int key[AHEAD];
+    long long tok[AHEAD];
+    float x[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      const int s = e + q < s1 ? e + q : s1 - 1;
+      key[q] = key_at(a, j, s);
+      tok[q] = token_at(a, j, s);
+    }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) x[q] = (float)((const TG*)a.g)[tok[q] * a.gstride + c];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      if (e + q >= s1) break;
+      if (key[q] != cur) {
+        if (began_here) put(cur, sum); else *part = sum;
+        cur = key[q];
+        began_here = true;
+        sum = 0.f;
+      }
+      if (cur >= j.rows) return;   // the rest takes no gradient
+      const unsigned long long f = (unsigned long long)(tok[q] * a.dim + c);
+      sum += DROP ? kept(keep_bits(a.rng, rk, f >> 3), (int)(f & 7), x[q]) : x[q];
+    }
   }
-  TO* o = (TO*)j.out + at;
-  if (j.accumulate) {
-    if (s1 > s0) *o = (TO)fmaf(sum, j.scale, (float)*o);
-  } else {
-    *o = (TO)(sum * j.scale);
-  }
+  if (cur >= j.rows) return;
+  if (began_here && after != cur)
+    put(cur, sum);
+  else
+    part[began_here ? a.dimp : 0] = sum;
 }
 
 // The ids that reach over a chunk's end: the part in the chunk where an id begins and those of
@@ -654,6 +697,33 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join(GradArgs a) {
   put_row<TO>(a, j, id, c, sum);
 }
 
+// ... of the narrow tables: 32 parts at a time, one column a lane
+template <class TO>
+__global__ __launch_bounds__(256) void embed_join_narrow(GradArgs a) {
+  constexpr int PARTS = 256 / 8;
+  __shared__ float lds[PARTS][8];
+  const GradJob& j = a.job[blockIdx.z + !a.job[0].spans];
+  const int chunk = blockIdx.x;
+  const int end = (chunk + 1) * CHUNK, id = key_at(a, j, end - 1);
+  if (id >= j.rows || key_at(a, j, end) != id) return;
+  if (chunk && key_at(a, j, chunk * CHUNK - 1) == id) return;   // began before
+  // the chunk with the id's last token
+  const int last = ((j.ids ? first_at(j.keys, end, a.tokens, id + 1) : (id + 1) * a.batch) - 1) /
+                   CHUNK;
+  const int c = threadIdx.x & 7, p = threadIdx.x >> 3;
+  const float* part = j.part + c;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int q = chunk + 1 + p; q <= last; q += PARTS) sum += part[(long long)q * 2 * a.dimp];
+  lds[p][c] = sum;
+  __syncthreads();
+  if (p || c >= a.dim) return;
+  sum = part[((long long)chunk * 2 + 1) * a.dimp];
+  for (int q = 0; q < PARTS; ++q) sum += lds[q][c];
+  TO* o = (TO*)j.out + (long long)id * a.dim + c;
+  *o = (TO)fmaf(sum, j.scale, j.accumulate ? (float)*o : 0.f);
+}
+
 template <class TW, class TO, bool POS, bool DROP>
 static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
   const long long groups = (a.tokens + (256 >> a.log_lanes) - 1) / (256 >> a.log_lanes);
@@ -679,14 +749,6 @@ static void launch_rows(hipStream_t stream, const EmbedArgs& a) {
 
 template <class TG, class TO, bool DROP>
 static void launch_grad(hipStream_t stream, const GradArgs& a) {
-  if (a.dim < 8) {
-    for (int jn = 0; jn < 2; ++jn)
-      if (a.job[jn].rows)
-        hipLaunchKernelGGL((embed_grad_narrow<TG, TO, DROP>),
-                           dim3(ceil_div((long long)a.job[jn].rows * a.dim, 256)), dim3(256), 0,
-                           stream, a, jn);
-    return;
-  }
   if (a.small) {
     const int groups = ceil_div(a.job[0].rows, SMALL_ROWS) + ceil_div(a.job[1].rows, SMALL_ROWS);
     hipLaunchKernelGGL((embed_grad_small<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
@@ -695,7 +757,10 @@ static void launch_grad(hipStream_t stream, const GradArgs& a) {
   const int groups = a.job[0].reduce_groups + a.job[1].reduce_groups + a.job[0].fill_groups +
                      a.job[1].fill_groups;
   if (groups == 0) return;   // no tokens to add
-  hipLaunchKernelGGL((embed_grad<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
+  if (a.dim < 8)
+    hipLaunchKernelGGL((embed_grad_narrow<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((embed_grad<TG, TO, DROP>), dim3(groups), dim3(256), 0, stream, a);
 }
 template <class TG, class TO>
 static void launch_grad(hipStream_t stream, const GradArgs& a) {
@@ -763,10 +828,11 @@ static void grad_job(GradJob& j, const GradArgs& a, const void* ids, void* out, 
   j.scale = scale;
   j.accumulate = accumulate;
   j.chunks = ceil_div(a.tokens, CHUNK);
-  j.reduce_groups = ceil_div((long long)j.chunks * a.ctiles, 4);
+  j.reduce_groups = a.dim < 8 ? ceil_div(j.chunks, NARROW_CHUNKS)
+                              : ceil_div((long long)j.chunks * a.ctiles, 4);
   const bool all_named = !ids && a.tokens > 0 && a.seq >= rows;
   j.fill_groups = accumulate || all_named ? 0 : ceil_div(rows, FILL_ROWS);
-  j.spans = a.dim >= 8 && j.chunks > 1 && (ids || CHUNK % a.batch != 0);
+  j.spans = j.chunks > 1 && (ids || CHUNK % a.batch != 0);
 }
 
 }  // namespace dmh
@@ -913,8 +979,13 @@ int dmh_embedding_grad(hipStream_t stream, const void* ids, const void* position
   if (!a.small && (a.job[0].spans || a.job[1].spans)) {
     const int chunks = ceil_div(tokens, CHUNK);
     const dim3 grid(chunks - 1, a.ctiles, a.job[0].spans + a.job[1].spans);
-    DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), grid, dim3(64 * JOIN_WAVES),
-                                                   0, stream, a))
+    if (dim < 8) {
+      DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join_narrow<TO>), grid, dim3(256), 0,
+                                                     stream, a))
+    } else {
+      DMH_FOR_TYPE(out_dtype, TO, hipLaunchKernelGGL((embed_join<TO>), grid,
+                                                     dim3(64 * JOIN_WAVES), 0, stream, a))
+    }
     DMH_CHECK_LAUNCH("embed_join");
   }
   return DMH_OK;

@@ -934,3 +934,44 @@ def test_a_position_table_without_rows(T):
     assert T.embedding(ids[:0], w, none).shape == (0, 24)
     # no rows, no gradient of them
     assert T.embedding_backward(g.to(DEV), ids, 10, pos_rows=0, positions=ids)[1] is None
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("kind", ["same", "zipf"])
+@pytest.mark.parametrize("dtype,out,p", [(F32, F32, 0.0), (BF16, BF16, 0.2)])
+def test_narrow_tables_of_many_tokens(T, dim, kind, dtype, out, p):
+    """Terms of one sign, one id for most of 200000 tokens.  No sum adds more in sequence than a
+    chunk's 32, one in 32 of the chunks, 32 of those and the first chunk's, and two roundings
+    each of the scales and the sum."""
+    n, rows = 200000, 50
+    ids = ids_of((n,), rows, kind=kind)
+    g = (normal(n, dim).abs() * 0.01 + 0.1).to(dtype)
+    kw = dict(scale=1.5, dropout_p=p, rng=RNG)
+    dw, dp = T.embedding_backward(g.view(2000, 100, dim).to(DEV), ids.view(2000, 100).to(DEV),
+                                  rows, pos_rows=120, dtype=out, **kw)
+    chain = 32 + n / 32 / 32 + 32 + 1 + 4
+    want, size, _ = R.table_grad(g, ids, rows, 1.5, p, RNG)
+    close(dw, want, chain * E32 * size + 1.01 * U[out] * want + TINY[out])
+    t = torch.arange(100).repeat(2000)
+    want, size, _ = R.table_grad(g, t, 120, 1.0, p, RNG)
+    close(dp, want, chain * E32 * size + 1.01 * U[out] * want + TINY[out])
+    # added to what a table holds, its other rows untouched
+    w0 = normal(rows + 70, dim, dtype=out)
+    w = w0.to(DEV)
+    T.embedding_backward(g.to(DEV), ids.to(DEV), rows + 70, weight_grad=w, **kw)
+    want, size, terms = R.table_grad(g, ids, rows + 70, 1.5, p, RNG)
+    total = want + w0.double()
+    close(w, total, chain * E32 * size + 1.01 * U[out] * total.abs() + E32 * w0.double().abs()
+          + TINY[out])
+    gone = terms[:, 0] == 0
+    assert gone.any() and torch.equal(w.cpu()[gone], w0[gone])
+
+
+def test_more_tokens_of_one_id_than_fp32_counts(T):
+    """Ones: every sum below 2^24 is exact, and two roundings remain."""
+    n = (1 << 24) + 12345
+    ids = torch.ones(n, dtype=torch.int32, device=DEV)
+    ids[-5:] = 2
+    dw, _ = T.embedding_backward(torch.ones(n, 1, device=DEV), ids, 4)
+    assert dw[0] == 0 and dw[2] == 5 and dw[3] == 0
+    assert abs(float(dw[1]) - (n - 5)) <= 33 * E32 * n
