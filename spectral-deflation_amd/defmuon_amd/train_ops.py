@@ -129,7 +129,7 @@ def _drop(p, rng, device, what):
 def draw_rng():
     """A fresh (seed, offset) from torch's CPU generator: torch.manual_seed fixes it, and
     activation checkpointing draws the same one again when it repeats a forward pass."""
-    return tuple(torch.randint(-1 << 63, (1 << 63) - 1, (2,)).tolist())
+    return tuple(torch.randint(-1 << 63, (1 << 63) - 1, (2,), device="cpu").tolist())
 
 
 # ---- dropout --------------------------------------------------------------------------------

@@ -333,3 +333,12 @@ def test_positions_and_ids_keep_their_values():
         assert i.dtype == p.dtype == dtype
         assert i.tolist() == ids.tolist() and p.tolist() == positions.tolist()
     assert _positions(None, a, "embedding")[0] is a
+
+
+def test_draws_come_from_the_cpu_generator():
+    from defmuon_amd.train_ops import draw_rng
+    torch.manual_seed(3)
+    want = draw_rng()
+    torch.manual_seed(3)
+    with torch.device("meta"):   # a default device for the program's own tensors
+        assert draw_rng() == want
