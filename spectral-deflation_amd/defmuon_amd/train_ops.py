@@ -18,7 +18,10 @@ autograd functions) for those outside autograd.
 Random numbers: `rng` names the mask of a dropout.  It is a pair of integers (seed, offset), or
 an int64 tensor of the two on the GPU, which is read when a kernel runs: a captured graph
 draws a new mask at each replay if the program changes the tensor between its replays (after
-the backward pass, which reads it again).  Two calls with
+the backward pass, which reads it again).  The rows of a (layers, 2) tensor serve a model:
+different offsets, and the seeds set anew by one operation.  A pair of integers would be the
+same at every replay, so draw_rng, and with it Dropout without an rng, raises NativeError while a
+graph is captured.  Two calls with
 the same pair, shape and p drop the same elements, which is how the backward pass has its mask
 without storing it; calls that should differ take different pairs (draw_rng).  p is taken to
 the nearest 1/65536, and kept elements are scaled by the reciprocal of exactly that.  A dropped
@@ -128,7 +131,11 @@ def _drop(p, rng, device, what):
 
 def draw_rng():
     """A fresh (seed, offset) from torch's CPU generator: torch.manual_seed fixes it, and
-    activation checkpointing draws the same one again when it repeats a forward pass."""
+    activation checkpointing draws the same one again when it repeats a forward pass.  Not in a
+    captured graph or a trace, which would repeat it."""
+    if _is_tracing() or torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise NativeError("draw_rng: a captured graph or a trace would repeat one mask; give "
+                          "dropout an rng tensor")
     return tuple(torch.randint(-1 << 63, (1 << 63) - 1, (2,), device="cpu").tolist())
 
 
@@ -196,8 +203,8 @@ def dropout_backward(grad, p, rng, dtype=None):
 
 
 class Dropout(torch.nn.Module):
-    """Dropout and an optional residual's addition; a mask of its own at each call in training,
-    x (+ residual) in evaluation."""
+    """Dropout and an optional residual's addition; in training a mask of its own at each call,
+    or that of `rng` (which a captured graph needs, as a tensor), in evaluation x (+ residual)."""
 
     def __init__(self, p=0.1):
         super().__init__()
@@ -208,11 +215,11 @@ class Dropout(torch.nn.Module):
     def extra_repr(self):
         return f"p={self.p}"
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, rng=None):
         p = self.p if self.training else 0.0
         if p == 0.0 and residual is None:
             return x
-        return dropout(x, p, draw_rng() if p else None, residual)
+        return dropout(x, p, draw_rng() if p and rng is None else rng, residual)
 
 
 # ---- embedding ------------------------------------------------------------------------------

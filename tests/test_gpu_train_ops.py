@@ -975,3 +975,44 @@ def test_more_tokens_of_one_id_than_fp32_counts(T):
     dw, _ = T.embedding_backward(torch.ones(n, 1, device=DEV), ids, 4)
     assert dw[0] == 0 and dw[2] == 5 and dw[3] == 0
     assert abs(float(dw[1]) - (n - 5)) <= 33 * E32 * n
+
+
+def test_dropout_module_in_a_captured_graph(T, Err):
+    """Two layers whose rng are rows of one tensor: the masks differ from each other and from
+    replay to replay, and are those of eager calls, gradients too."""
+    layers = [T.Dropout(0.4), T.Dropout(0.4)]
+    x = normal(64, 96).to(DEV).requires_grad_()
+    state = torch.tensor([[7, 0], [7, 1]], device=DEV)
+
+    def step():
+        h = layers[0](x, rng=state[0])
+        y = layers[1](h, residual=h, rng=state[1])
+        return h, y, torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        refused = 0
+        for call in (T.draw_rng, lambda: layers[0](x)):
+            try:
+                call()
+            except Err:
+                refused += 1
+        outs = step()
+    assert refused == 2
+    before = None
+    for k in range(4):
+        state[:, 0] += 1
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b), k
+        masks = outs[0] != 0, (outs[1] - outs[0]) != 0
+        assert not torch.equal(*masks)
+        assert before is None or not torch.equal(before, masks[0])
+        before = masks[0]

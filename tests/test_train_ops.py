@@ -342,3 +342,22 @@ def test_draws_come_from_the_cpu_generator():
     torch.manual_seed(3)
     with torch.device("meta"):   # a default device for the program's own tensors
         assert draw_rng() == want
+
+
+def test_graphs_and_traces_do_not_repeat_a_mask(monkeypatch):
+    from defmuon_amd import train_ops as T
+    from defmuon_amd._native import NativeError
+    x = torch.randn(4, 8)
+    monkeypatch.setattr(T, "dropout", lambda x, p, rng, residual: rng)
+    m, state = T.Dropout(0.3), torch.zeros(5, 2, dtype=torch.int64)
+    assert m(x) != m(x) and m(x, rng=(1, 2)) == (1, 2) and m(x, rng=state[3]).tolist() == [0, 0]
+    with monkeypatch.context() as c:
+        c.setattr(torch.cuda, "is_initialized", lambda: True)
+        c.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for call in (T.draw_rng, lambda: m(x)):
+            with pytest.raises(NativeError, match="graph"):
+                call()
+        assert m(x, rng=state[1]).tolist() == [0, 0]   # not drawn here
+        assert m.eval()(x) is x and m(x, residual=x) is None
+    with pytest.raises(NativeError, match="trace"), pytest.warns():
+        torch.jit.trace(lambda t: t * T.draw_rng()[0], x)
