@@ -18,7 +18,8 @@ autograd functions) for those outside autograd.
 Random numbers: `rng` names the mask of a dropout.  It is a pair of integers (seed, offset), or
 an int64 tensor of the two on the GPU, which is read when a kernel runs: a captured graph
 draws a new mask at each replay if the program changes the tensor between its replays (after
-the backward pass, which reads it again).  The rows of a (layers, 2) tensor serve a model:
+the backward pass, which reads it again; a change before raises torch's error for saved tensors).
+The rows of a (layers, 2) tensor serve a model:
 different offsets, and the seeds set anew by one operation.  A pair of integers would be the
 same at every replay, so draw_rng, and with it Dropout without an rng, raises NativeError while a
 graph is captured.  Two calls with
@@ -164,6 +165,9 @@ class _Dropout(Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng):
         ctx.p, ctx.rng, ctx.dtype = p, rng, x.dtype
+        if isinstance(rng, torch.Tensor):   # saved: autograd says so if it has changed
+            ctx.save_for_backward(rng)
+            ctx.rng = None
         cut, key = _drop(p, rng, x.device, "dropout")
         return _dropout(x, residual, cut, key, x.dtype if residual is None else residual.dtype)
 
@@ -172,7 +176,8 @@ class _Dropout(Function):
     def backward(ctx, grad):
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = dropout_backward(grad, ctx.p, ctx.rng, ctx.dtype)
+            rng = ctx.saved_tensors[0] if ctx.saved_tensors else ctx.rng
+            dx = dropout_backward(grad, ctx.p, rng, ctx.dtype)
         return dx, grad if ctx.needs_input_grad[1] else None, None, None
 
 
@@ -255,8 +260,9 @@ def _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype):
 class _Embedding(Function):
     @staticmethod
     def forward(ctx, weight, pos_weight, ids, positions, scale, padding_idx, p, rng, dtype):
-        ctx.save_for_backward(ids, positions)
-        ctx.args = scale, padding_idx, p, rng
+        tensor = isinstance(rng, torch.Tensor)   # saved: autograd says so if it has changed
+        ctx.save_for_backward(ids, positions, rng if tensor else None)
+        ctx.args = scale, padding_idx, p, None if tensor else rng
         ctx.weight = weight.shape[0], weight.dtype
         ctx.pos = None if pos_weight is None else (pos_weight.shape[0], pos_weight.dtype)
         cut, key = _drop(p, rng, weight.device, "embedding")
@@ -265,13 +271,13 @@ class _Embedding(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        ids, positions = ctx.saved_tensors
+        ids, positions, state = ctx.saved_tensors
         scale, padding_idx, p, rng = ctx.args
         need_w, need_p = ctx.needs_input_grad[:2]
         dw, dp = embedding_backward(
             grad, ids, ctx.weight[0] if need_w else 0, pos_rows=ctx.pos[0] if need_p else 0,
             positions=positions, scale=scale, padding_idx=padding_idx if need_w else None,
-            dropout_p=p, rng=rng, dtype=ctx.weight[1])
+            dropout_p=p, rng=rng if state is None else state, dtype=ctx.weight[1])
         return dw if need_w else None, dp if need_p else None, *[None] * 7
 
 

@@ -361,3 +361,21 @@ def test_graphs_and_traces_do_not_repeat_a_mask(monkeypatch):
         assert m.eval()(x) is x and m(x, residual=x) is None
     with pytest.raises(NativeError, match="trace"), pytest.warns():
         torch.jit.trace(lambda t: t * T.draw_rng()[0], x)
+
+
+def test_an_rng_tensor_changed_before_the_backward_pass(stand_in, monkeypatch):
+    from defmuon_amd import _native
+    T, seen = stand_in, []
+    monkeypatch.setattr(_native, "dropout", lambda *a: seen.append(a[4]))
+    monkeypatch.setattr(_native, "embedding", lambda *a: None)
+    x = torch.randn(3, 8, requires_grad=True)
+    state, ids = torch.tensor([[1, 2], [1, 3]]), torch.zeros(2, 3, dtype=torch.int64)
+    for op in (lambda rng: T.dropout(x, 0.5, rng), lambda rng: T.dropout(x, 0.5, rng, residual=x),
+               lambda rng: T.embedding(ids, x, dropout_p=0.5, rng=rng)):
+        op(state[1]).sum().backward()
+        op((5, 6)).sum().backward()
+        y = op(state[1])
+        state[:, 0] += 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    assert seen[1] == (0, 0, state[1].data_ptr()) and seen[3] == (5, 6, 0)
