@@ -539,6 +539,14 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
            "dmh_embedding_grad")
 
 
+@functools.lru_cache(maxsize=1024)
+def cross_entropy_workspace_bytes(rows, classes):
+    nbytes = c_sz()
+    _check(load().dmh_cross_entropy_workspace_size(rows, classes, ctypes.byref(nbytes)),
+           "dmh_cross_entropy_workspace_size")
+    return nbytes.value
+
+
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
                   dlogits, dstride):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
@@ -550,16 +558,17 @@ def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, g
             return cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction,
                                  grad_scale, loss, dlogits, dstride)
     n, classes, zs = rows
-    lib = load()
-    nbytes = 4 * n   # dmh_cross_entropy_workspace_size
-    stats = torch.empty(3 * n + 1, dtype=torch.float32, device=logits.device)
+    nbytes = cross_entropy_workspace_bytes(n, classes)
+    # the workspace behind the statistics: one allocation a call
+    stats = torch.empty(2 * n + 1 + (nbytes + 3) // 4, dtype=torch.float32, device=logits.device)
     at = stats.data_ptr()
-    _check(lib.dmh_cross_entropy_stats(_raw_stream(index), logits.data_ptr(),
-                                       FLOATS[logits.dtype], n, classes, zs, targets.data_ptr(),
-                                       targets.dtype == torch.int64, ignore, smoothing, z_loss,
-                                       reduction, grad_scale, loss.data_ptr(), at + 8 * n, at,
-                                       at + 4 * n, 0 if dlogits is None else dlogits.data_ptr(),
-                                       dstride, at + 8 * n + 4, nbytes),
+    _check(load().dmh_cross_entropy_stats(_raw_stream(index), logits.data_ptr(),
+                                          FLOATS[logits.dtype], n, classes, zs,
+                                          targets.data_ptr(), targets.dtype == torch.int64,
+                                          ignore, smoothing, z_loss, reduction, grad_scale,
+                                          loss.data_ptr(), at + 8 * n, at, at + 4 * n,
+                                          0 if dlogits is None else dlogits.data_ptr(), dstride,
+                                          at + 8 * n + 4, nbytes),
            "dmh_cross_entropy_stats")
     return stats
 

@@ -379,3 +379,28 @@ def test_an_rng_tensor_changed_before_the_backward_pass(stand_in, monkeypatch):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
     assert seen[1] == (0, 0, state[1].data_ptr()) and seen[3] == (5, 6, 0)
+
+
+def test_the_workspace_is_the_librarys_size(monkeypatch):
+    """The allocation and the size passed follow dmh_cross_entropy_workspace_size."""
+    from defmuon_amd import _native
+    seen = []
+
+    class Lib:
+        def dmh_cross_entropy_workspace_size(self, rows, classes, out):
+            out._obj.value = 1000 * rows + classes
+            return 0
+
+        def dmh_cross_entropy_stats(self, *a):
+            seen.append(a)
+            return 0
+    _native.cross_entropy_workspace_bytes.cache_clear()
+    monkeypatch.setattr(_native, "_lib", Lib())
+    monkeypatch.setattr(_native, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(_native, "_current_device", lambda: -1)
+    z, y = torch.randn(3, 5), torch.arange(3)
+    stats = _native.cross_entropy(z, (3, 5, 5), y, -100, 0.0, 0.0, 1, 1.0, torch.empty(()), None, 0)
+    _native.cross_entropy_workspace_bytes.cache_clear()
+    at, nbytes = seen[0][-2:]
+    assert nbytes == 3005
+    assert stats.data_ptr() + 4 * stats.numel() >= at + nbytes
