@@ -243,7 +243,8 @@ int dmh_dropout(dmh_stream_t stream, const void* x, int x_dtype, long long rows,
 /* out[i, :] = dropout(scale * weight[ids[i], :] + pos_weight[pos_i, :]) over `tokens` rows of
  * `dim`; pos_i = positions[i], or i % seq where positions is NULL; pos_weight NULL for none.
  * ids and positions are int64 (ids_64) or int32.  Both tables have `dtype`.  An id or position
- * outside its table gives a row of NaN.  out is contiguous. */
+ * outside its table gives a row of NaN.  out is contiguous.  tokens, vocab <= 2^40,
+ * dim <= 2^30. */
 int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long tokens, int seq,
                   const void* weight, int dtype, long long vocab, int dim, long long w_rstride,
                   const void* pos_weight, long long pos_rows, long long p_rstride,
@@ -257,7 +258,7 @@ int dmh_embedding(dmh_stream_t stream, const void* ids, int ids_64, long long to
  * positions NULL: pos_i = i % seq (tokens a multiple of seq).  Every row of an output is
  * written, those that no token names with zero; with `accumulate` the sums are added to what
  * it holds and other rows stay untouched.  padding_idx (-1: none) and ids outside a table
- * take no gradient.  tokens, rows < 2^27.
+ * take no gradient.  tokens, rows < 2^27, dim <= 2^23.
  * Workspace: for the rows of the outputs that are wanted (0: not wanted); positions: nonzero if
  * positions are given. */
 int dmh_embedding_grad_workspace_size(long long tokens, long long rows, long long pos_rows,

@@ -848,7 +848,7 @@ int dmh_embedding(hipStream_t stream, const void* ids, int ids_64, long long tok
                   unsigned long long offset, const void* rng_state, void* out, int out_dtype) {
   if (tokens < 0 || vocab < 0 || dim < 0 || w_rstride < 0 || pos_rows < 0 || p_rstride < 0 ||
       !float_code(dtype) || !float_code(out_dtype) || cut < 0 || cut > 65536 ||
-      tokens > (1LL << 40) || vocab > (1LL << 40) ||
+      tokens > (1LL << 40) || vocab > (1LL << 40) || dim > (1 << 30) ||   // columns are ints
       (tokens > 0 && pos_weight && !positions && seq < 1)) {
     set_error("dmh_embedding: bad arguments (tokens=%lld seq=%d vocab=%lld dim=%d dtypes=%d,%d "
               "cut=%d)", tokens, seq, vocab, dim, dtype, out_dtype, cut);

@@ -294,6 +294,8 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
     device, dtype, shape = weight.device, weight.dtype, weight.shape
     if len(shape) != 2:
         raise NativeError(f"{what}: weight must be (rows, dim), got {tuple(shape)}")
+    if shape[1] > 1 << 30 or pos_weight is not None and ids.ndim and ids.shape[-1] >= 1 << 31:
+        raise NativeError(f"{what}: ids {tuple(ids.shape)} and rows of {shape[1]} are too long")
     _ints(ids, device, what, "ids")
     if positions is not None:
         ids, positions = _positions(positions, ids, what)
@@ -357,6 +359,8 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
         raise NativeError(f"{what}: grad {tuple(grad.shape)} does not fit ids "
                           f"{tuple(ids.shape)}")
     _out_type(dtype, what)
+    if grad.shape[-1] > 1 << 23:
+        raise NativeError(f"{what}: rows of {grad.shape[-1]} are too long")
     if rows < 0 or pos_rows < 0:
         raise NativeError(f"{what}: {rows} and {pos_rows} rows")
     _padding(padding_idx, rows, what)

@@ -404,3 +404,22 @@ def test_the_workspace_is_the_librarys_size(monkeypatch):
     at, nbytes = seen[0][-2:]
     assert nbytes == 3005
     assert stats.data_ptr() + 4 * stats.numel() >= at + nbytes
+
+
+def test_rows_of_more_columns_than_an_int_counts(lib, monkeypatch):
+    """A C int would keep the low 32 bits of the width."""
+    from defmuon_amd import _native, train_ops as T
+    one = ctypes.c_void_p(256)   # never read
+    assert lib.dmh_embedding(None, one, 1, 1, 1, one, 0, 2, (1 << 30) + 1, 8, None, 0, 0, None, 1.0,
+                             0, 0, 0, None, one, 0) == 1
+    monkeypatch.setattr(T, "_float", lambda *a: None)
+    for name in ("embedding", "embedding_grad"):
+        monkeypatch.setattr(_native, name, lambda *a: pytest.fail("launched"))
+    x, ids = torch.zeros(()), torch.zeros(1, dtype=torch.int64)
+    for wide in ((1 << 30) + 1, (1 << 32) + 8):
+        with pytest.raises(_native.NativeError, match="too long"):
+            T.embedding(ids, x.expand(2, wide))
+        with pytest.raises(_native.NativeError, match="too long"):
+            T.embedding_backward(x.expand(1, wide), ids, 2)
+    with pytest.raises(_native.NativeError, match="too long"):
+        T.embedding(ids.expand((1 << 32) + 1), x.expand(2, 8), x.expand(1 << 33, 8))
