@@ -478,10 +478,12 @@ def dropout(x, residual, out, cut, rng, rows):
             return dropout(x, residual, out, cut, rng, rows)
     n, cols, xs, rs = rows
     seed, offset, state = rng
-    _check(load().dmh_dropout(_raw_stream(index), x.data_ptr(), FLOATS[x.dtype], n,
-                              cols, xs, 0 if residual is None else residual.data_ptr(), rs,
-                              out.data_ptr(), FLOATS[out.dtype], cut, seed, offset, state),
-           "dmh_dropout")
+    rc = (_lib or load()).dmh_dropout(
+        _raw_stream(index), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
+        0 if residual is None else residual.data_ptr(), rs, out.data_ptr(), FLOATS[out.dtype],
+        cut, seed, offset, state)
+    if rc:
+        _check(rc, "dmh_dropout")
 
 
 def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
@@ -497,12 +499,13 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     # nothing of it is read
     pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr() or out.data_ptr(),
                                                 pos_weight.shape[0], pos_weight.stride(0))
-    _check(load().dmh_embedding(_raw_stream(index), ids.data_ptr(),
-                                ids.dtype == torch.int64, ids.numel(), seq, weight.data_ptr(),
-                                FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
-                                0 if positions is None else positions.data_ptr(), scale, cut,
-                                seed, offset, state, out.data_ptr(), FLOATS[out.dtype]),
-           "dmh_embedding")
+    rc = (_lib or load()).dmh_embedding(
+        _raw_stream(index), ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), seq,
+        weight.data_ptr(), FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
+        0 if positions is None else positions.data_ptr(), scale, cut, seed, offset, state,
+        out.data_ptr(), FLOATS[out.dtype])
+    if rc:
+        _check(rc, "dmh_embedding")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -528,15 +531,14 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
     pos_rows = 0 if pos_out is None else pos_out.shape[0]
     nbytes = embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions is not None)
     ws = _workspace(nbytes, ids.device) if nbytes else None
-    _check(load().dmh_embedding_grad(_raw_stream(index), ids.data_ptr(),
-                                     0 if positions is None else positions.data_ptr(),
-                                     ids.dtype == torch.int64, tokens, seq, grad.data_ptr(),
-                                     FLOATS[grad.dtype], gstride, dim, padding_idx, scale, cut,
-                                     seed, offset, state, out.data_ptr() if rows else 0, rows,
-                                     add, pos_out.data_ptr() if pos_rows else 0, pos_rows,
-                                     pos_add, FLOATS[(out if rows else pos_out).dtype],
-                                     ws.data_ptr() if nbytes else 0, nbytes),
-           "dmh_embedding_grad")
+    rc = (_lib or load()).dmh_embedding_grad(
+        _raw_stream(index), ids.data_ptr(), 0 if positions is None else positions.data_ptr(),
+        ids.dtype == torch.int64, tokens, seq, grad.data_ptr(), FLOATS[grad.dtype], gstride, dim,
+        padding_idx, scale, cut, seed, offset, state, out.data_ptr() if rows else 0, rows, add,
+        pos_out.data_ptr() if pos_rows else 0, pos_rows, pos_add,
+        FLOATS[(out if rows else pos_out).dtype], ws.data_ptr() if nbytes else 0, nbytes)
+    if rc:
+        _check(rc, "dmh_embedding_grad")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -548,28 +550,37 @@ def cross_entropy_workspace_bytes(rows, classes):
 
 
 def cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction, grad_scale, loss,
-                  dlogits, dstride):
+                  dlogits, dstride, keep=True):
     """Losses (and the gradient of grad_scale * loss into dlogits); rows: (rows, classes, row
-    stride) of the logits.  Returns what the backward pass needs: fp32, the rows' maxima, their
-    sums exp(z - maximum), and the number of rows with a target (for a mean)."""
+    stride) of the logits.  Returns what the backward pass needs (keep): fp32, the rows' maxima,
+    their sums exp(z - maximum), and the number of rows with a target (for a mean)."""
     index = logits.get_device()
     if index != _current_device():
         with torch.cuda.device(index):
             return cross_entropy(logits, rows, targets, ignore, smoothing, z_loss, reduction,
-                                 grad_scale, loss, dlogits, dstride)
+                                 grad_scale, loss, dlogits, dstride, keep)
     n, classes, zs = rows
-    nbytes = cross_entropy_workspace_bytes(n, classes)
-    # the workspace behind the statistics: one allocation a call
-    stats = torch.empty(2 * n + 1 + (nbytes + 3) // 4, dtype=torch.float32, device=logits.device)
-    at = stats.data_ptr()
-    _check(load().dmh_cross_entropy_stats(_raw_stream(index), logits.data_ptr(),
-                                          FLOATS[logits.dtype], n, classes, zs,
-                                          targets.data_ptr(), targets.dtype == torch.int64,
-                                          ignore, smoothing, z_loss, reduction, grad_scale,
-                                          loss.data_ptr(), at + 8 * n, at, at + 4 * n,
-                                          0 if dlogits is None else dlogits.data_ptr(), dstride,
-                                          at + 8 * n + 4, nbytes),
-           "dmh_cross_entropy_stats")
+    lib = _lib or load()
+    # statistics, count and workspace: one allocation a call, none for the losses alone
+    kept = 2 * n if keep else 0
+    nbytes = cross_entropy_workspace_bytes(n, classes) if reduction else 0
+    stats, at = None, 0
+    if keep or reduction:
+        stats = torch.empty(kept + 1 + (nbytes + 3) // 4, dtype=torch.float32,
+                            device=logits.device)
+        at = stats.data_ptr()
+    count = at + 4 * kept
+    args = (_raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+            targets.data_ptr(), targets.dtype == torch.int64, ignore, smoothing, z_loss,
+            reduction, grad_scale, loss.data_ptr(), count)
+    tail = (0 if dlogits is None else dlogits.data_ptr(), dstride, count + 4 if nbytes else 0,
+            nbytes)
+    if keep:
+        rc = lib.dmh_cross_entropy_stats(*args, at, at + 4 * n, *tail)
+    else:
+        rc = lib.dmh_cross_entropy(*args, 0, *tail)
+    if rc:
+        _check(rc, "dmh_cross_entropy")
     return stats
 
 
@@ -583,11 +594,10 @@ def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reducti
                                       reduction, stats, grad_out, dlogits, dstride)
     n, classes, zs = rows
     at = stats.data_ptr()
-    _check(load().dmh_cross_entropy_grad_stats(_raw_stream(index), logits.data_ptr(),
-                                               FLOATS[logits.dtype], n, classes, zs,
-                                               targets.data_ptr(), targets.dtype == torch.int64,
-                                               ignore, smoothing, z_loss, at, at + 4 * n,
-                                               at + 8 * n if reduction == 1 else 0,
-                                               grad_out.data_ptr(), reduction == 0,
-                                               dlogits.data_ptr(), dstride),
-           "dmh_cross_entropy_grad_stats")
+    rc = (_lib or load()).dmh_cross_entropy_grad_stats(
+        _raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+        targets.data_ptr(), targets.dtype == torch.int64, ignore, smoothing, z_loss, at,
+        at + 4 * n, at + 8 * n if reduction == 1 else 0, grad_out.data_ptr(), reduction == 0,
+        dlogits.data_ptr(), dstride)
+    if rc:
+        _check(rc, "dmh_cross_entropy_grad_stats")

@@ -42,7 +42,9 @@ __all__ = ["embedding", "embedding_backward", "dropout", "dropout_backward", "Dr
 
 _is_tracing = torch._C._is_tracing
 _modes = torch._C._len_torch_dispatch_stack
-_early_proxy = torch._ops._mode_stack_state_for_pre_dispatch.get   # make_fx(pre_dispatch=True)
+# the tracing mode of make_fx(pre_dispatch=True) is the first of a list of torch's own
+_early_modes = vars(torch._ops._mode_stack_state_for_pre_dispatch).get(
+    "_ModeStackStateForPreDispatch__infra_modes", [None])
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 _NO_RNG = (0, 0, 0)
@@ -59,7 +61,7 @@ def _eager(what, function=False):
     """Refuse to be traced (function: torch.jit.trace records an autograd function instead)."""
     if not function and _is_tracing():
         raise NativeError(f"{what}: torch.jit.trace cannot record a launch")
-    traced = _early_proxy(0) is not None
+    traced = _early_modes[0] is not None
     if _modes():
         key, mode = torch._C._TorchDispatchModeKey, torch._C._get_dispatch_mode
         traced |= mode(key.PROXY) is not None or mode(key.FAKE) is not None
@@ -111,17 +113,17 @@ def _rows(t):
     return t.contiguous(), rows, cols, cols
 
 
-def _drop(p, rng, device, what):
-    """(cut, (seed, offset, state address)) of a dropout."""
+def _drop(p, rng, like, what):
+    """(cut, (seed, offset, state address)) of a dropout on `like`'s device."""
     if not 0.0 <= p <= 1.0:
         raise NativeError(f"{what}: p must be between 0 and 1, not {p}")
     cut = int(round(p * 65536))
     if cut == 0:
         return 0, _NO_RNG
     if isinstance(rng, torch.Tensor):
-        if (rng.device != device or rng.dtype != torch.int64 or rng.shape != (2,)
+        if (rng.device != like.device or rng.dtype != torch.int64 or rng.shape != (2,)
                 or not rng.is_contiguous()):
-            raise NativeError(f"{what}: rng must be two int64 on {device}")
+            raise NativeError(f"{what}: rng must be two int64 on {like.device}")
         return cut, (0, 0, rng.data_ptr())
     try:
         seed, offset = rng
@@ -168,7 +170,7 @@ class _Dropout(Function):
         if isinstance(rng, torch.Tensor):   # saved: autograd says so if it has changed
             ctx.save_for_backward(rng)
             ctx.rng = None
-        cut, key = _drop(p, rng, x.device, "dropout")
+        cut, key = _drop(p, rng, x, "dropout")
         return _dropout(x, residual, cut, key, x.dtype if residual is None else residual.dtype)
 
     @staticmethod
@@ -190,7 +192,7 @@ def dropout(x, p, rng, residual=None):
         if residual.shape != x.shape or residual.device != x.device:
             raise NativeError(f"dropout: residual is {tuple(residual.shape)} on "
                               f"{residual.device}, x {tuple(x.shape)} on {x.device}")
-    cut, key = _drop(p, rng, x.device, "dropout")
+    cut, key = _drop(p, rng, x, "dropout")
     if _is_tracing() or torch.is_grad_enabled() and (
             x.requires_grad or residual is not None and residual.requires_grad):
         return _Dropout.apply(x, residual, p, rng)
@@ -204,7 +206,7 @@ def dropout_backward(grad, p, rng, dtype=None):
     _float(grad, "dropout_backward", "grad")
     dtype = dtype or grad.dtype
     _out_type(dtype, "dropout_backward")
-    return _dropout(grad, None, *_drop(p, rng, grad.device, "dropout_backward"), dtype)
+    return _dropout(grad, None, *_drop(p, rng, grad, "dropout_backward"), dtype)
 
 
 class Dropout(torch.nn.Module):
@@ -265,7 +267,7 @@ class _Embedding(Function):
         ctx.args = scale, padding_idx, p, None if tensor else rng
         ctx.weight = weight.shape[0], weight.dtype
         ctx.pos = None if pos_weight is None else (pos_weight.shape[0], pos_weight.dtype)
-        cut, key = _drop(p, rng, weight.device, "embedding")
+        cut, key = _drop(p, rng, weight, "embedding")
         return _embed(ids, weight, pos_weight, positions, scale, cut, key, dtype)
 
     @staticmethod
@@ -317,7 +319,7 @@ def embedding(ids, weight, pos_weight=None, positions=None, scale=1.0, padding_i
     if out_dtype is not None:
         dtype = out_dtype
         _out_type(dtype, what)
-    cut, key = _drop(dropout_p, rng, device, what)
+    cut, key = _drop(dropout_p, rng, weight, what)
     if _is_tracing() or torch.is_grad_enabled() and (
             weight.requires_grad or pos_weight is not None and pos_weight.requires_grad):
         return _Embedding.apply(weight, pos_weight, ids, positions, scale, padding_idx,
@@ -367,7 +369,7 @@ def embedding_backward(grad, ids, rows, pos_rows=0, positions=None, scale=1.0, p
     ids, positions = _positions(positions, ids, what)
     if pos_rows and positions is None and (ids.ndim < 1 or ids.shape[-1] > pos_rows):
         raise NativeError(f"{what}: ids {tuple(ids.shape)} have more positions than {pos_rows}")
-    cut, key = _drop(dropout_p, rng, grad.device, what)
+    cut, key = _drop(dropout_p, rng, grad, what)
     dim, tokens = grad.shape[-1], ids.numel()
     seq = ids.shape[-1] if ids.ndim else 1
     ids = ids.contiguous()
@@ -416,8 +418,9 @@ def _xent_args(logits, targets, label_smoothing, z_loss, reduction, what):
 
 
 def _xent(logits, rows, targets, ignore_index, smoothing, z_loss, reduction, dlogits=None,
-          dstride=0, grad_scale=1.0):
-    """(loss, statistics for the backward pass) and, in place, dlogits; rows: _rows(logits)."""
+          dstride=0, grad_scale=1.0, keep=False):
+    """(loss, statistics for the backward pass if `keep`) and, in place, dlogits; rows:
+    _rows(logits)."""
     z, n, classes, stride = rows
     red = _REDUCTIONS[reduction]
     loss = torch.empty(targets.shape if red == 0 else (), dtype=torch.float32,
@@ -426,7 +429,7 @@ def _xent(logits, rows, targets, ignore_index, smoothing, z_loss, reduction, dlo
     if n or red:
         stats = _native.cross_entropy(z, (n, classes, stride), targets.contiguous(),
                                       ignore_index, smoothing, z_loss, red, grad_scale, loss,
-                                      dlogits, dstride)
+                                      dlogits, dstride, keep)
     return loss, stats
 
 
@@ -444,7 +447,7 @@ class _CrossEntropy(Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
         loss, stats = _xent(logits, _rows(logits), targets, ignore_index, smoothing, z_loss,
-                            reduction)
+                            reduction, keep=True)
         ctx.save_for_backward(logits, targets, stats)
         ctx.args = ignore_index, smoothing, z_loss, _REDUCTIONS[reduction]
         return loss

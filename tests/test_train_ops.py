@@ -171,7 +171,7 @@ def stand_in(monkeypatch):
     from defmuon_amd import _native, train_ops as T
 
     def cross_entropy(z, rows, y, ignore, smoothing, z_loss, reduction, grad_scale, loss, dz,
-                      dstride):
+                      dstride, keep):
         assert all(type(n) is int for n in rows)
         zz = z.detach().clone()
         rows, d, _ = R.xent(zz, y, ignore, smoothing, z_loss)
