@@ -1016,3 +1016,26 @@ def test_dropout_module_in_a_captured_graph(T, Err):
         assert not torch.equal(*masks)
         assert before is None or not torch.equal(before, masks[0])
         before = masks[0]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+def test_compiled_programs_run_the_calls(T, grad):
+    """Outside the compiled graphs, as they are: masks drawn at each call among them."""
+    w, w2 = normal(50, 24).to(DEV).requires_grad_(grad), normal(24, 24, seed=1).to(DEV)
+    ids, y = ids_of((9,), 50).to(DEV), ids_of((9,), 24).to(DEV)
+    drop = T.Dropout(0.5)
+
+    def step(t):
+        x = T.embedding(ids, t, dropout_p=0.1, rng=RNG) @ w2
+        return T.cross_entropy(drop(x * 2, residual=x), y, reduction="none")
+    compiled = torch.compile(step, backend="aot_eager")
+    runs = []
+    for f in (step, compiled, compiled):
+        torch.manual_seed(len(runs) // 2)   # the same, the same, another
+        loss = f(w)
+        runs.append((loss, torch.autograd.grad(loss.sum(), w)[0] if grad else loss))
+    for a, b in zip(runs[0], runs[1]):
+        assert torch.equal(a, b)
+    assert not torch.equal(runs[1][0], runs[2][0])
+    torch._dynamo.reset()
