@@ -470,6 +470,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _address(t, what):
+    """The address of an optional tensor, whose null would pass for its absence: a subclass that
+    wraps other tensors has none."""
+    at = t.data_ptr()
+    if not at:
+        raise NativeError(f"{what}: a {type(t).__name__} has no memory of its own")
+    return at
+
+
 def dropout(x, residual, out, cut, rng, rows):
     """out = dropout(x) [+ residual]; rows: (rows, cols, x's row stride, the residual's)."""
     index = x.get_device()
@@ -480,8 +489,8 @@ def dropout(x, residual, out, cut, rng, rows):
     seed, offset, state = rng
     rc = (_lib or load()).dmh_dropout(
         _raw_stream(index), x.data_ptr(), FLOATS[x.dtype], n, cols, xs,
-        0 if residual is None else residual.data_ptr(), rs, out.data_ptr(), FLOATS[out.dtype],
-        cut, seed, offset, state)
+        0 if residual is None else _address(residual, "dropout"), rs, out.data_ptr(),
+        FLOATS[out.dtype], cut, seed, offset, state)
     if rc:
         _check(rc, "dmh_dropout")
 
@@ -495,15 +504,17 @@ def embedding(ids, weight, pos_weight, positions, scale, cut, rng, out):
     seed, offset, state = rng
     vocab, dim = weight.shape
     seq = ids.shape[-1] if ids.ndim else 1
-    # a table without rows has no address, and must not pass for no table: any address will do,
-    # nothing of it is read
-    pos = (0, 0, 0) if pos_weight is None else (pos_weight.data_ptr() or out.data_ptr(),
-                                                pos_weight.shape[0], pos_weight.stride(0))
+    pos = (0, 0, 0)
+    if pos_weight is not None:
+        # a table without rows has no address, and must not pass for no table: any address will
+        # do, nothing of it is read
+        pos = (_address(pos_weight if pos_weight.shape[0] else out, "embedding"),
+               pos_weight.shape[0], pos_weight.stride(0))
     rc = (_lib or load()).dmh_embedding(
         _raw_stream(index), ids.data_ptr(), ids.dtype == torch.int64, ids.numel(), seq,
         weight.data_ptr(), FLOATS[weight.dtype], vocab, dim, weight.stride(0), *pos,
-        0 if positions is None else positions.data_ptr(), scale, cut, seed, offset, state,
-        out.data_ptr(), FLOATS[out.dtype])
+        0 if positions is None else _address(positions, "embedding"), scale, cut, seed, offset,
+        state, out.data_ptr(), FLOATS[out.dtype])
     if rc:
         _check(rc, "dmh_embedding")
 
@@ -531,11 +542,13 @@ def embedding_grad(ids, positions, tokens, seq, grad, gstride, dim, padding_idx,
     pos_rows = 0 if pos_out is None else pos_out.shape[0]
     nbytes = embedding_grad_workspace_bytes(tokens, rows, pos_rows, dim, positions is not None)
     ws = _workspace(nbytes, ids.device) if nbytes else None
+    what = "embedding_backward"
     rc = (_lib or load()).dmh_embedding_grad(
-        _raw_stream(index), ids.data_ptr(), 0 if positions is None else positions.data_ptr(),
+        _raw_stream(index), ids.data_ptr(),
+        _address(positions, what) if positions is not None and tokens else 0,
         ids.dtype == torch.int64, tokens, seq, grad.data_ptr(), FLOATS[grad.dtype], gstride, dim,
-        padding_idx, scale, cut, seed, offset, state, out.data_ptr() if rows else 0, rows, add,
-        pos_out.data_ptr() if pos_rows else 0, pos_rows, pos_add,
+        padding_idx, scale, cut, seed, offset, state, _address(out, what) if rows else 0, rows, add,
+        _address(pos_out, what) if pos_rows else 0, pos_rows, pos_add,
         FLOATS[(out if rows else pos_out).dtype], ws.data_ptr() if nbytes else 0, nbytes)
     if rc:
         _check(rc, "dmh_embedding_grad")

@@ -423,3 +423,36 @@ def test_rows_of_more_columns_than_an_int_counts(lib, monkeypatch):
             T.embedding_backward(x.expand(1, wide), ids, 2)
     with pytest.raises(_native.NativeError, match="too long"):
         T.embedding(ids.expand((1 << 32) + 1), x.expand(2, 8), x.expand(1 << 33, 8))
+
+
+def test_tensors_without_memory_do_not_pass_for_absent_ones(monkeypatch):
+    from defmuon_amd import _native as N
+
+    class Wrapper(torch.Tensor):
+        """As a distributed tensor: no storage of its own."""
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype,
+                                                       device=t.device, strides=t.stride())
+
+        __torch_dispatch__ = classmethod(lambda *a, **kw: pytest.fail("dispatched"))
+    monkeypatch.setattr(N, "_lib", type("Lib", (), {"__getattr__": lambda *a: lambda *b: 0})())
+    monkeypatch.setattr(N, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(N, "_current_device", lambda: -1)
+    x, ids, rng = torch.randn(3, 8), torch.zeros(3, dtype=torch.int64), (0, 0, 0)
+
+    def grad(positions, out, pos_out):
+        N.embedding_grad(ids, positions, 3, 3, x, 8, 8, -1, 1.0, 0, rng, out, True, pos_out, True)
+
+    def embed(pos, positions):
+        N.embedding(ids, x, pos, positions, 1.0, 0, rng, torch.empty(3, 8))
+    N.dropout(x, x, x, 0, rng, (3, 8, 8, 8))   # the stand-in takes ordinary tensors
+    embed(x, ids), grad(ids, x, x)
+    embed(torch.empty(0, 8), ids)
+    w = Wrapper(x)
+    for call in (lambda: N.dropout(x, w, x, 0, rng, (3, 8, 8, 8)), lambda: embed(w, None),
+                 lambda: embed(x, Wrapper(ids)), lambda: grad(Wrapper(ids), x, x),
+                 lambda: grad(None, w, None), lambda: grad(None, None, w)):
+        with pytest.raises(N.NativeError, match="no memory"):
+            call()
+    N.embedding_grad_workspace_bytes.cache_clear()
