@@ -22,7 +22,8 @@ struct DropArgs {
 //
 // One block of eight flat elements a thread: one evaluation of the generator.  FLAT: x and the
 // residual are contiguous; otherwise a block finds its row by a division and takes its elements
-// one by one where a row ends inside it.
+// one by one where a row ends inside it: 11.5 us for 8192 rows of 1280 bf16 columns out of 2560,
+// 12.7 for 1281 out of 1283, where contiguous rows take 10.4.
 template <class TX, class TO, bool RES, bool FLAT>
 __global__ __launch_bounds__(256) void dropout(DropArgs a) {
   const TX* x = (const TX*)a.x;

@@ -26,7 +26,8 @@ struct EmbedArgs {
 };
 
 // Bound by the rows it reads and writes: 8192 tokens of 1280 fp32 columns with positions and
-// dropout take 14.1 us, 65 MB at 4.6 TB/s.
+// dropout take 14.1 us, 65 MB at 4.6 TB/s, where the tables' rows are in the last-level cache from
+// the call before.  In a training step they come from HBM, and it takes 25.3.
 //
 // A token is `lanes` (a power of two up to a wave) neighbouring lanes' work, which take eight of
 // its columns each, `lanes` pieces apart: as many as leave the fewest idle at the row's end, so
