@@ -493,7 +493,8 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     logits' type; with inplace it takes the logits' own memory (what lies beside the rows of a
     padded view stays).  logits.backward(dlogits) goes on from there; after a call in place it
     raises torch's error where the logits' values are needed for it (a soft-cap's tanh, another
-    loss of the same logits)."""
+    loss of the same logits), and should start at the tensor that the product returned: as for
+    any view written in place, autograd copies a view's gradient."""
     what = "cross_entropy_step"
     _eager(what)
     _xent_args(logits, targets, label_smoothing, z_loss, reduction, what)

@@ -1039,3 +1039,18 @@ def test_compiled_programs_run_the_calls(T, grad):
         assert torch.equal(a, b)
     assert not torch.equal(runs[1][0], runs[2][0])
     torch._dynamo.reset()
+
+
+def test_in_place_gradients_of_views(T):
+    """From the view, and from the product's own output: the same gradient."""
+    h, y = normal(6, 10, 96).to(DEV).requires_grad_(), ids_of((60,), 304, kind="flat").to(DEV)
+    w = normal(96, 304, seed=1).to(DEV)
+    want = torch.autograd.grad(z := h @ w, h, T.cross_entropy_step(z.view(-1, 304), y)[1]
+                               .view_as(z))[0]
+    z = h @ w
+    dz = T.cross_entropy_step(z.view(-1, 304), y, inplace=True)[1]
+    assert dz.data_ptr() == z.data_ptr()
+    assert torch.equal(torch.autograd.grad(z, h, dz.view_as(z))[0], want)
+    view = (h @ w).view(-1, 304)
+    dz = T.cross_entropy_step(view, y, inplace=True)[1]
+    assert torch.equal(torch.autograd.grad(view, h, dz)[0], want)
