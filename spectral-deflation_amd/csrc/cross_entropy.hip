@@ -16,11 +16,9 @@
 // number of rows that have a target for a mean.  A row whose target is ignore_index has loss 0
 // and gradient 0 whatever its logits hold; any other target outside [0, V) makes both NaN.  A
 // row of -inf alone has no softmax: its loss and gradient are NaN.
-#include "train_ops.h"
+#include "rows.h"
 
 namespace dmh {
-
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 enum { RED_NONE = 0, RED_MEAN = 1, RED_SUM = 2 };
 
@@ -39,57 +37,6 @@ struct XentArgs {
   int classes, t64, gout_rows;
   float eps, zeta, gscale;
 };
-
-constexpr float INF = __builtin_inff();
-
-// exp(x - m) by the hardware's 2^x (results below 2^-126 are zero)
-__device__ __forceinline__ float exp_diff(float x, float m) {
-  return __builtin_amdgcn_exp2f((x - m) * LOG2E);
-}
-
-// The sum of one value a thread over THREADS threads: part of a wave, a wave, or a workgroup of as
-// many.
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-#pragma unroll
-  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1) v += __shfl_xor(v, d);
-  constexpr int W = THREADS / 64;
-  if (W <= 1) return v;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = lds[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) s += lds[w];
-  return s;
-}
-
-// Parts of a row: m their maximum, s = sum exp(z - m); (-inf, 0) for none, and for values of
-// -inf alone.  A NaN ends in s.
-struct Part {
-  float m, s;
-};
-__device__ __forceinline__ Part join(Part a, Part b) {
-  const float m = fmaxf(a.m, b.m);
-  // nothing to scale where the maximum stays; both -inf must not give inf - inf
-  const float fa = a.m == m ? 1.f : exp_diff(a.m, m), fb = b.m == m ? 1.f : exp_diff(b.m, m);
-  return {m, a.s * fa + b.s * fb};
-}
-template <int THREADS>
-__device__ __forceinline__ Part block_join(Part p, Part* lds) {
-#pragma unroll
-  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
-    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
-  constexpr int W = THREADS / 64;
-  if (W <= 1) return p;
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
-  __syncthreads();
-  // every wave joins the waves' parts in the same way
-  p = (threadIdx.x & 63) < W ? lds[threadIdx.x & 63] : Part{-INF, 0.f};
-#pragma unroll
-  for (int d = W / 2; d; d >>= 1) p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
-  return {__shfl(p.m, 0), __shfl(p.s, 0)};
-}
 
 // The number of rows that have a target, in every thread of the workgroup.  One workgroup goes
 // through all rows, so it has AHEAD loads a thread on their way.
@@ -177,34 +124,6 @@ __device__ __forceinline__ Grad row_grad(const XentArgs& a, float g, float m, fl
           -g * (1.f - a.eps)};
 }
 
-// A row in aligned pieces of 16 bytes, and the classes before the first and behind the last one,
-// up to seven on each side, which the first sixteen threads of a row take one by one.  Rows of an
-// odd number of classes start anywhere; with pieces from the row's start instead the loads
-// and stores of bf16 rows of 50257 took 13% longer.
-template <class T>
-struct Row {
-  static constexpr int N = Piece<T>::N;
-  typedef typename Piece<T>::type type;
-  int head, pieces, classes;
-  __device__ __forceinline__ Row(const T* z, int v) : classes(v) {
-    head = (int)(-((uintptr_t)z / sizeof(T)) & (N - 1));
-    head = head < v ? head : v;
-    pieces = (v - head) / N;
-  }
-  __device__ __forceinline__ int piece_class(int i) const { return head + i * N; }
-  // the single class of thread t, or -1
-  __device__ __forceinline__ int edge(int t) const {
-    const int c = t < 8 ? (t < head ? t : -1) : piece_class(pieces) + t - 8;
-    return c < classes && t < 16 ? c : -1;
-  }
-  // the thread that writes class c
-  template <int THREADS>
-  __device__ __forceinline__ int owner(int c) const {
-    const int i = (c - head) / N;
-    return c < head ? c : i < pieces ? i % THREADS : 8 + c - piece_class(pieces);
-  }
-};
-
 // Bound by the memory, and close to it by arithmetic: 8192 bf16 rows of 50257 with gradient take
 // 296 us (1647 MB, 5.6 TB/s), the vector units busy 85% of the time; the loss alone 141 us for half
 // the bytes.  A sweep of its own each for the maximum, the sum and the gradient took 1270 us.
@@ -216,13 +135,6 @@ struct Row {
 // workgroups of 1024 fit a compute unit up to 65536 16-bit classes and one's loads run under
 // the other's arithmetic: with the unpacked values kept, 8192 bf16 rows of 50257 took 381
 // instead of 332 us.
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-template <int HELD>
-__device__ __forceinline__ void repack(i32x4 (&x)[HELD]) {
-#pragma unroll
-  for (int k = 0; k < HELD; ++k) asm volatile("" : "+v"(x[k]));
-}
-
 template <class T, int THREADS, int HELD, bool GRAD, bool COUNT>
 __global__ __launch_bounds__(THREADS < 128 ? 256 : THREADS, HELD > 16      ? 2
                                                             : HELD > 8      ? 4

@@ -1,0 +1,554 @@
+// Distillation: the divergence of rows of logits from a teacher's lists of classes, with its
+// gradient.
+//
+//   x = z / tau,  p = softmax(x),  lists of classes i_j with log probabilities t_j
+//   q = softmax(t)                     loss = tau^2 sum_j q_j (log q_j - log p_{i_j})
+//                                      dz   = tau (p - sum over j with i_j = v of q_j)
+//
+// or with the classes outside the list (the rest, R) as one more,
+//
+//   q = exp(t), r = max(0, 1 - sum q)  loss = tau^2 (sum_j q_j (log q_j - log p_{i_j})
+//                                                    + r (log r - log p_R)),  p_R = sum_R p
+//                                      dz   = tau (w p - q),  w = sum q + r, on the list
+//                                             tau (w p - r p / p_R)          off it
+//
+// The rest has a maximum and a sum of its own, m_R and s_R: p / p_R = exp(x - m_R) / s_R and
+// log p_R = m_R + log s_R - lse, where 1 - sum p would have lost all digits for a student that is
+// sure of the list.  Off the list, dz is one exponential times one factor of the row.
+//
+// An entry whose class is `ignore` is left out; a row whose first entry is has no teacher, loss 0
+// and gradient 0.  A class outside [0, V) makes its row NaN, as does a row without a softmax.  What
+// has q_j = 0 (or r = 0) adds nothing, whatever p is.  A class that is listed twice has two terms.
+#include "rows.h"
+
+namespace dmh {
+
+enum { RED_NONE = 0, RED_MEAN = 1, RED_SUM = 2 };
+
+constexpr int LIST_MAX = 1024;
+
+struct DistillArgs {
+  const void* z;
+  const void* ids;       // (rows, k)
+  const void* teacher;   // (rows, k)
+  void* dz;              // or null
+  float* row_loss;
+  float* stats;          // (6, rows), written (forward; may be null) or read (gradient)
+  const float* count;    // rows that have a teacher, or null
+  const float* gout;     // gradient of the loss (gradient kernel): one, or one a row
+  long long rows, zs, ds, ignore;
+  int classes, k, i64, ttype, gout_rows;
+  float itau, c2;        // 1 / tau; log2(e) / tau
+  float lscale, gscale;  // tau^2; tau times the gradient's scale
+};
+
+__device__ __forceinline__ float load_float(const void* p, int type, long long i) {
+  return type == DMH_F32    ? ((const float*)p)[i]
+         : type == DMH_BF16 ? (float)((const bf16*)p)[i]
+                            : (float)((const fp16*)p)[i];
+}
+
+// The number of rows that have a teacher: their first entries by one workgroup.
+__device__ __forceinline__ float count_rows(const DistillArgs& a, float* lds) {
+  constexpr int AHEAD = 8;
+  int n = 0;
+  const int rows = (int)a.rows;
+  auto count = [&](auto* ids) {
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) n += ids[(long long)(i + k * 1024) * a.k] != a.ignore;
+    }
+    for (; i < rows; i += 1024) n += ids[(long long)i * a.k] != a.ignore;
+  };
+  if (a.i64) count((const long long*)a.ids); else count((const int*)a.ids);
+  return block_sum<1024>((float)n, lds);   // exact: below 2^24 rows
+}
+
+__global__ __launch_bounds__(1024) void distill_count(DistillArgs a, float* count) {
+  __shared__ float lds[16];
+  const float n = count_rows(a, lds);
+  if (threadIdx.x == 0) *count = n;
+}
+
+// The sum of the rows' losses, divided by the number of rows with a teacher for a mean, which it
+// counts if no launch before has (COUNT).
+template <bool COUNT>
+__global__ __launch_bounds__(1024) void distill_reduce(DistillArgs a, float* count, float* loss) {
+  __shared__ float lds[16];
+  constexpr int AHEAD = 16;
+  const int rows = (int)a.rows;
+  float s = 0.f;
+  int i = threadIdx.x;
+  for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
+    float v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = a.row_loss[i + k * 1024];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) s += v[k];
+  }
+  for (; i < rows; i += 1024) s += a.row_loss[i];
+  s = block_sum<1024>(s, lds);
+  const float n = COUNT ? count_rows(a, lds) : count ? *count : 1.f;
+  if (threadIdx.x == 0) {
+    if (COUNT) *count = n;
+    *loss = s / n;
+  }
+}
+
+// What a row's gradient needs: off the list 2^((z - ref) c2) coef, on it
+// 2^((z - m) c2) ws - q, q = 2^((t - tm) log2 e) qs, all times tau and the loss's gradient.
+struct RowStats {
+  float ref, coef, m, ws, tm, qs;
+};
+
+__device__ __forceinline__ float natural_exp(float x) {
+  return __builtin_amdgcn_exp2f(x * LOG2E);
+}
+__device__ __forceinline__ float natural_log(float x) { return __builtin_amdgcn_logf(x) * LN2; }
+
+template <int THREADS>
+__device__ __forceinline__ float block_max(float v, float* lds) {
+#pragma unroll
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  constexpr int W = THREADS / 64;
+  if (W <= 1) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = lds[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) s = fmaxf(s, lds[w]);
+  return s;
+}
+
+// A row by a workgroup that reads it for the sums and, with a gradient, again.
+template <class T, int THREADS, bool REST, bool GRAD>
+__global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
+  constexpr int N = Piece<T>::N, AHEAD = 4, SPAN = THREADS == 1024 ? 32768 : 2048;
+  __shared__ Part parts[16], list_parts[16];
+  __shared__ float lds[16];
+  __shared__ int ids[LIST_MAX];
+  __shared__ float zs[LIST_MAX], ts[LIST_MAX];   // the list's logits; log probabilities, then q
+  __shared__ uint32_t marks[SPAN / 4];           // of SPAN pieces
+  __shared__ uint32_t edge_marks;
+  __shared__ int twice, bad;
+  typedef typename Row<T>::type type;
+  const long long row = blockIdx.x;
+  const int t = threadIdx.x, K = a.k;
+  const T* z = (const T*)a.z + row * a.zs;
+  T* dz = GRAD ? (T*)a.dz + row * a.ds : nullptr;
+  const Row<T> r(z, a.classes);
+  const int ec = r.edge(t);
+  if (load_index(a.ids, a.i64, row * K) == a.ignore) {
+    if (t == 0) a.row_loss[row] = 0.f;
+    if (t < 6 && a.stats) a.stats[t * a.rows + row] = 0.f;
+    if (GRAD) {
+      const type zero = {};
+      for (int i = t; i < r.pieces; i += THREADS) *(type*)(dz + r.piece_class(i)) = zero;
+      if (ec >= 0) dz[ec] = (T)0.f;
+    }
+    return;
+  }
+  if (t == 0) {
+    edge_marks = 0;
+    twice = bad = 0;
+  }
+  __syncthreads();
+  // the list: its entries that are left out have q = 0
+  float tm = -INF;
+  for (int j = t; j < K; j += THREADS) {
+    const long long c = load_index(a.ids, a.i64, row * K + j);
+    const bool in = c >= 0 && c < a.classes;
+    if (!in && c != a.ignore) bad = 1;
+    ids[j] = in ? (int)c : -1;
+    zs[j] = in ? (float)z[c] : 0.f;
+    const float q = in ? load_float(a.teacher, a.ttype, row * K + j) : -INF;
+    ts[j] = q;
+    tm = fmaxf(tm, q);
+  }
+  tm = REST ? 0.f : block_max<THREADS>(tm, lds);
+  float qsum = 0.f;
+  for (int j = t; j < K; j += THREADS)
+    qsum += ids[j] >= 0 ? natural_exp(ts[j] - tm) : 0.f;
+  qsum = block_sum<THREADS>(qsum, lds);
+  // the row
+  const float ex = ec >= 0 ? (float)z[ec] : -INF;
+  Part p = {-INF, 0.f};
+  uint32_t firsts = 0;
+  for (int first = 0; first == 0 || first < r.pieces; first += SPAN) {
+    const int last = first + SPAN < r.pieces ? first + SPAN : r.pieces;
+    __syncthreads();
+    for (int i = t; i < (last - first + 3) / 4; i += THREADS) marks[i] = 0;
+    __syncthreads();
+    int it = 0;
+    for (int j = t; j < K; j += THREADS, ++it) {
+      uint32_t *word, bit;
+      if (ids[j] >= 0 &&
+          find_mark(r, ids[j], first, SPAN, first == 0, marks, &edge_marks, word, bit)) {
+        if (atomicOr(word, bit) & bit) twice = 1;
+        else firsts |= 1u << it;
+      }
+    }
+    __syncthreads();
+    if (first == 0 && ec >= 0 && !(REST && edge_marks >> t & 1)) {
+      p.m = fmaxf(ex, -INF);
+      p.s = __builtin_amdgcn_exp2f((ex - (p.m == -INF ? 0.f : p.m)) * a.c2);
+    }
+    for (int i0 = first + t; i0 < last; i0 += AHEAD * THREADS) {
+      type x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * THREADS;
+        x[k] = *(const type*)(z + r.piece_class(i < last ? i : i0));
+      }
+      float m = p.m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * THREADS < last ? i0 + k * THREADS : i0;
+        if (REST) {
+          const uint32_t listed = ((const uint8_t*)marks)[i - first];
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (listed >> j & 1) x[k][j] = (T)-INF;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, (float)x[k][j]);
+      }
+      rescale(p, m, a.c2);
+      const float m0 = m == -INF ? 0.f : m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * THREADS < last) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            p.s += __builtin_amdgcn_exp2f(((float)x[k][j] - m0) * a.c2);
+        }
+    }
+  }
+  p = block_join<THREADS>(p, a.c2, parts);
+  Part all = p;
+  if (REST) {
+    Part l = {-INF, 0.f};
+    int it = 0;
+    for (int j = t; j < K; j += THREADS, ++it) {
+      const float v = zs[j];
+      if (firsts >> it & 1)
+        l = join(l, {fmaxf(v, -INF), v == -INF ? 0.f : v - v + 1.f}, a.c2);
+    }
+    all = join(p, block_join<THREADS>(l, a.c2, list_parts), a.c2);
+  }
+  // coefficients
+  const float log_s = natural_log(all.s);
+  const float left = REST ? fmaxf(1.f - qsum, 0.f) : 0.f;
+  float w = REST ? (qsum <= 1.f ? 1.f : qsum) : qsum / qsum;
+  if (bad || !(all.s >= 0.5f)) w = __builtin_nanf("");
+  RowStats st;
+  st.m = all.m;
+  st.ws = w / all.s;
+  st.tm = tm;
+  st.qs = REST ? 1.f : 1.f / qsum;
+  st.ref = p.m == -INF ? 0.f : p.m;
+  st.coef = st.ws;
+  if (REST) {
+    st.coef = st.ws * (p.m == -INF ? 0.f : __builtin_amdgcn_exp2f((p.m - all.m) * a.c2));
+    if (left > 0.f && p.s > 0.f) st.coef -= left / p.s;
+  }
+  float loss = 0.f;
+  const float log_q = REST ? 0.f : natural_log(qsum);
+  for (int j = t; j < K; j += THREADS) {
+    const float q = ids[j] >= 0 ? natural_exp(ts[j] - tm) * st.qs : 0.f;
+    // not below: a NaN goes on
+    if (!(q <= 0.f)) loss += q * ((ts[j] - tm - log_q) - ((zs[j] - all.m) * a.itau - log_s));
+    ts[j] = q;
+  }
+  loss = block_sum<THREADS>(loss, lds);
+  if (t == 0) {
+    if (REST && left > 0.f)
+      loss += left * (natural_log(left) - ((p.m - all.m) * a.itau + natural_log(p.s) - log_s));
+    a.row_loss[row] = w == w ? loss * a.lscale : w;
+    if (a.stats) a.stats[row] = st.ref;
+    if (a.stats) a.stats[a.rows + row] = st.coef;
+    if (a.stats) a.stats[2 * a.rows + row] = st.m;
+    if (a.stats) a.stats[3 * a.rows + row] = st.ws;
+    if (a.stats) a.stats[4 * a.rows + row] = st.tm;
+    if (a.stats) a.stats[5 * a.rows + row] = st.qs;
+  }
+  if (!GRAD) return;
+  const float g = a.gscale / (a.count ? *a.count : 1.f);
+  const float coef = st.coef * g;
+  for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
+    type x[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * THREADS;
+      x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * THREADS;
+      type d;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        d[j] = (T)(__builtin_amdgcn_exp2f(((float)x[k][j] - st.ref) * a.c2) * coef);
+      if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+    }
+  }
+  if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
+  __syncthreads();
+  // the listed classes again, each by one thread
+  int it = 0;
+  for (int j = t; j < K; j += THREADS, ++it) {
+    if (firsts >> it & 1) {
+      const int c = ids[j];
+      float q = ts[j];
+      if (twice) {   // a class listed more than once: its terms in their order
+        q = 0.f;
+        for (int i = 0; i < K; ++i) q += ids[i] == c ? ts[i] : 0.f;
+      }
+      dz[c] = (T)((__builtin_amdgcn_exp2f((zs[j] - st.m) * a.c2) * st.ws - q) * g);
+    }
+  }
+}
+
+template <class T, bool REST, bool GRAD>
+static void launch_rows(hipStream_t stream, const DistillArgs& a) {
+  const dim3 rows((unsigned)a.rows);
+  if (a.classes <= 8192)
+    hipLaunchKernelGGL((distill_row<T, 256, REST, GRAD>), rows, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((distill_row<T, 1024, REST, GRAD>), rows, dim3(1024), 0, stream, a);
+}
+template <class T>
+static void launch_distill(hipStream_t stream, const DistillArgs& a, bool rest) {
+  if (rest)
+    a.dz ? launch_rows<T, true, true>(stream, a) : launch_rows<T, true, false>(stream, a);
+  else
+    a.dz ? launch_rows<T, false, true>(stream, a) : launch_rows<T, false, false>(stream, a);
+}
+
+// The gradient from a forward pass's statistics, element by element, 256 threads for four pieces
+// each of a row; the listed classes are written again behind a barrier.
+template <class T>
+__global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
+  constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;
+  __shared__ int ids[LIST_MAX];
+  __shared__ float qs[LIST_MAX];
+  __shared__ uint32_t marks[THREADS];
+  __shared__ uint32_t edge_marks;
+  __shared__ int twice;
+  typedef typename Row<T>::type type;
+  const long long row = blockIdx.x;
+  const int t = threadIdx.x, K = a.k;
+  const T* z = (const T*)a.z + row * a.zs;
+  T* dz = (T*)a.dz + row * a.ds;
+  const Row<T> r(z, a.classes);
+  const int first = blockIdx.y * THREADS * AHEAD, i0 = first + t;
+  const int ec = blockIdx.y == 0 ? r.edge(t) : -1;
+  if (load_index(a.ids, a.i64, row * K) == a.ignore) {
+    const type zero = {};
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i0 + k * THREADS < r.pieces) *(type*)(dz + r.piece_class(i0 + k * THREADS)) = zero;
+    if (ec >= 0) dz[ec] = (T)0.f;
+    return;
+  }
+  type x[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = i0 + k * THREADS;
+    if (r.pieces) x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : 0));
+  }
+  const float ex = ec >= 0 ? (float)z[ec] : 0.f;
+  RowStats st;
+  st.ref = a.stats[row];
+  st.coef = a.stats[a.rows + row];
+  st.m = a.stats[2 * a.rows + row];
+  st.ws = a.stats[3 * a.rows + row];
+  st.tm = a.stats[4 * a.rows + row];
+  st.qs = a.stats[5 * a.rows + row];
+  float g = a.gout[a.gout_rows ? row : 0] * a.gscale;
+  if (a.count) g /= *a.count;
+  marks[t] = 0;
+  if (t == 0) {
+    edge_marks = 0;
+    twice = 0;
+  }
+  for (int j = t; j < K; j += THREADS) {
+    const long long c = load_index(a.ids, a.i64, row * K + j);
+    const bool in = c >= 0 && c < a.classes;
+    ids[j] = in ? (int)c : -1;
+    qs[j] = in ? natural_exp(load_float(a.teacher, a.ttype, row * K + j) - st.tm) * st.qs : 0.f;
+  }
+  const float coef = st.coef * g;
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = i0 + k * THREADS;
+    type d;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      d[j] = (T)(__builtin_amdgcn_exp2f(((float)x[k][j] - st.ref) * a.c2) * coef);
+    if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+  }
+  if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
+  __syncthreads();   // also: the list is written
+  uint32_t firsts = 0;
+  int it = 0;
+  for (int j = t; j < K; j += THREADS, ++it) {
+    uint32_t *word, bit;
+    if (ids[j] >= 0 && find_mark(r, ids[j], first, THREADS * AHEAD, blockIdx.y == 0, marks,
+                                 &edge_marks, word, bit)) {
+      if (atomicOr(word, bit) & bit) twice = 1;
+      else firsts |= 1u << it;
+    }
+  }
+  __syncthreads();
+  it = 0;
+  for (int j = t; j < K; j += THREADS, ++it) {
+    if (firsts >> it & 1) {
+      const int c = ids[j];
+      float q = qs[j];
+      if (twice) {
+        q = 0.f;
+        for (int i = 0; i < K; ++i) q += ids[i] == c ? qs[i] : 0.f;
+      }
+      dz[c] = (T)((__builtin_amdgcn_exp2f(((float)z[c] - st.m) * a.c2) * st.ws - q) * g);
+    }
+  }
+}
+
+template <class T>
+static void launch_distill_grad(hipStream_t stream, const DistillArgs& a) {
+  const int whole = a.classes / Piece<T>::N;
+  hipLaunchKernelGGL((distill_grad<T>),
+                     dim3((unsigned)a.rows, (unsigned)(whole ? ceil_div(whole, 1024) : 1)),
+                     dim3(256), 0, stream, a);
+}
+
+static bool distill_shape(long long rows, long long classes, long long k) {
+  return rows >= 0 && rows < (1LL << 22) && classes >= 1 && classes <= (1LL << 27) && k >= 1 &&
+         k <= LIST_MAX;
+}
+
+static DistillArgs distill_args(const void* logits, long long rows, long long classes,
+                                long long z_rstride, const void* ids, int ids_64, int k,
+                                const void* teacher, int teacher_dtype, long long ignore_index,
+                                float temperature, float* stats, const float* count,
+                                void* dlogits, long long d_rstride) {
+  DistillArgs a{};
+  a.z = logits;
+  a.ids = ids;
+  a.teacher = teacher;
+  a.dz = dlogits;
+  a.stats = stats;
+  a.count = count;
+  a.rows = rows;
+  a.zs = z_rstride;
+  a.ds = d_rstride;
+  a.ignore = ignore_index;
+  a.classes = (int)classes;
+  a.k = k;
+  a.i64 = ids_64 != 0;
+  a.ttype = teacher_dtype;
+  a.itau = (float)(1.0 / temperature);
+  a.c2 = (float)(1.4426950408889634 / temperature);
+  a.lscale = temperature * temperature;
+  a.gscale = temperature;
+  return a;
+}
+
+}  // namespace dmh
+
+using namespace dmh;
+
+extern "C" {
+
+int dmh_distill_workspace_size(long long rows, size_t* bytes) {
+  if (!bytes || !distill_shape(rows, 1, 1)) {
+    set_error("dmh_distill_workspace_size: bad arguments (rows=%lld)", rows);
+    return DMH_EINVAL;
+  }
+  *bytes = 4 * (size_t)rows;
+  return DMH_OK;
+}
+
+int dmh_distill(hipStream_t stream, const void* logits, int dtype, long long rows,
+                long long classes, long long z_rstride, const void* ids, int ids_64, int k,
+                const void* teacher, int teacher_dtype, long long ignore_index, float temperature,
+                int rest, int reduction, float grad_scale, float* loss, float* count,
+                float* stats, void* dlogits, long long d_rstride, void* ws, size_t ws_bytes) {
+  if (!distill_shape(rows, classes, k) || z_rstride < 0 || d_rstride < 0 || !float_code(dtype) ||
+      !float_code(teacher_dtype) || !(temperature >= 1e-6f && temperature <= 1e6f) ||
+      reduction < RED_NONE || reduction > RED_SUM) {
+    set_error("dmh_distill: bad arguments (rows=%lld classes=%lld dtype=%d k=%d teacher_dtype=%d "
+              "temperature=%g reduction=%d)", rows, classes, dtype, k, teacher_dtype,
+              (double)temperature, reduction);
+    return DMH_EINVAL;
+  }
+  if (!loss || (reduction == RED_MEAN && !count) ||
+      (rows > 0 && (!logits || !ids || !teacher))) {
+    set_error("dmh_distill: null tensor");
+    return DMH_EINVAL;
+  }
+  size_t need;
+  dmh_distill_workspace_size(rows, &need);
+  if (reduction != RED_NONE && need > 0 && (!ws || ws_bytes < need)) {
+    set_error("dmh_distill: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    return DMH_EWORKSPACE;
+  }
+  const bool mean = reduction == RED_MEAN;
+  DistillArgs a = distill_args(logits, rows, classes, z_rstride, ids, ids_64, k, teacher,
+                               teacher_dtype, ignore_index, temperature, stats,
+                               mean ? count : nullptr, dlogits, d_rstride);
+  a.row_loss = reduction == RED_NONE ? loss : (float*)ws;
+  a.gscale *= grad_scale;
+  // a mean's gradient needs the count at the start, its loss in the end
+  const bool before = mean && dlogits && rows > 0;
+  if (before) {
+    hipLaunchKernelGGL(distill_count, dim3(1), dim3(1024), 0, stream, a, count);
+    DMH_CHECK_LAUNCH("distill_count");
+  }
+  if (rows > 0) {
+    DMH_FOR_TYPE(dtype, T, (launch_distill<T>(stream, a, rest != 0)))
+    DMH_CHECK_LAUNCH("distill_row");
+  }
+  if (reduction != RED_NONE) {
+    if (mean && !before)
+      hipLaunchKernelGGL(distill_reduce<true>, dim3(1), dim3(1024), 0, stream, a, count, loss);
+    else
+      hipLaunchKernelGGL(distill_reduce<false>, dim3(1), dim3(1024), 0, stream, a,
+                         mean ? count : nullptr, loss);
+    DMH_CHECK_LAUNCH("distill_reduce");
+  }
+  return DMH_OK;
+}
+
+int dmh_distill_grad(hipStream_t stream, const void* logits, int dtype, long long rows,
+                     long long classes, long long z_rstride, const void* ids, int ids_64, int k,
+                     const void* teacher, int teacher_dtype, long long ignore_index,
+                     float temperature, const float* stats, const float* count,
+                     const float* grad_out, int grad_out_rows, void* dlogits,
+                     long long d_rstride) {
+  if (!distill_shape(rows, classes, k) || z_rstride < 0 || d_rstride < 0 || !float_code(dtype) ||
+      !float_code(teacher_dtype) || !(temperature >= 1e-6f && temperature <= 1e6f)) {
+    set_error("dmh_distill_grad: bad arguments (rows=%lld classes=%lld dtype=%d k=%d "
+              "teacher_dtype=%d temperature=%g)", rows, classes, dtype, k, teacher_dtype,
+              (double)temperature);
+    return DMH_EINVAL;
+  }
+  if (rows == 0) return DMH_OK;
+  if (!logits || !ids || !teacher || !stats || !grad_out || !dlogits) {
+    set_error("dmh_distill_grad: null tensor");
+    return DMH_EINVAL;
+  }
+  DistillArgs a = distill_args(logits, rows, classes, z_rstride, ids, ids_64, k, teacher,
+                               teacher_dtype, ignore_index, temperature, (float*)stats, count,
+                               dlogits, d_rstride);
+  a.gout = grad_out;
+  a.gout_rows = grad_out_rows != 0;
+  DMH_FOR_TYPE(dtype, T, (launch_distill_grad<T>(stream, a)))
+  DMH_CHECK_LAUNCH("distill_grad");
+  return DMH_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,146 @@
+// Rows of logits: the reductions, the exponentials and the pieces that the operators over the classes
+// of a vocabulary share.
+#pragma once
+
+#include "train_ops.h"
+
+namespace dmh {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+constexpr float INF = __builtin_inff();
+
+// exp(x - m) by the hardware's 2^x (results below 2^-126 are zero)
+__device__ __forceinline__ float exp_diff(float x, float m) {
+  return __builtin_amdgcn_exp2f((x - m) * LOG2E);
+}
+
+// The sum of one value a thread over THREADS threads: part of a wave, a wave, or a workgroup of as
+// many.
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+#pragma unroll
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1) v += __shfl_xor(v, d);
+  constexpr int W = THREADS / 64;
+  if (W <= 1) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = lds[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) s += lds[w];
+  return s;
+}
+
+// Parts of a row: m their maximum, s = sum exp(z - m); (-inf, 0) for none, and for values of
+// -inf alone.  A NaN ends in s.
+struct Part {
+  float m, s;
+};
+__device__ __forceinline__ Part join(Part a, Part b) {
+  const float m = fmaxf(a.m, b.m);
+  // nothing to scale where the maximum stays; both -inf must not give inf - inf
+  const float fa = a.m == m ? 1.f : exp_diff(a.m, m), fb = b.m == m ? 1.f : exp_diff(b.m, m);
+  return {m, a.s * fa + b.s * fb};
+}
+template <int THREADS>
+__device__ __forceinline__ Part block_join(Part p, Part* lds) {
+#pragma unroll
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
+    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
+  constexpr int W = THREADS / 64;
+  if (W <= 1) return p;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
+  __syncthreads();
+  // every wave joins the waves' parts in the same way
+  p = (threadIdx.x & 63) < W ? lds[threadIdx.x & 63] : Part{-INF, 0.f};
+#pragma unroll
+  for (int d = W / 2; d; d >>= 1) p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)});
+  return {__shfl(p.m, 0), __shfl(p.s, 0)};
+}
+
+// The same in units of 2: s = sum 2^((z - m) c2), c2 = log2(e) / temperature.
+__device__ __forceinline__ void rescale(Part& p, float m, float c2) {
+  if (p.m != m) {   // never for two of -inf
+    p.s *= __builtin_amdgcn_exp2f((p.m - m) * c2);
+    p.m = m;
+  }
+}
+__device__ __forceinline__ Part join(Part a, Part b, float c2) {
+  const float m = fmaxf(a.m, b.m);
+  rescale(a, m, c2);
+  rescale(b, m, c2);
+  return {m, a.s + b.s};
+}
+template <int THREADS>
+__device__ __forceinline__ Part block_join(Part p, float c2, Part* lds) {
+#pragma unroll
+  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
+    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
+  constexpr int W = THREADS / 64;
+  if (W <= 1) return p;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
+  __syncthreads();
+  p = (threadIdx.x & 63) < W ? lds[threadIdx.x & 63] : Part{-INF, 0.f};
+#pragma unroll
+  for (int d = W / 2; d; d >>= 1) p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
+  return {__shfl(p.m, 0), __shfl(p.s, 0)};
+}
+
+// A row in aligned pieces of 16 bytes, and the classes before the first and behind the last one,
+// up to seven on each side, which the first sixteen threads of a row take one by one.  Rows of an
+// odd number of classes start anywhere; with pieces from the row's start instead the loads
+// and stores of bf16 rows of 50257 took 13% longer.
+template <class T>
+struct Row {
+  static constexpr int N = Piece<T>::N;
+  typedef typename Piece<T>::type type;
+  int head, pieces, classes;
+  __device__ __forceinline__ Row(const T* z, int v) : classes(v) {
+    head = (int)(-((uintptr_t)z / sizeof(T)) & (N - 1));
+    head = head < v ? head : v;
+    pieces = (v - head) / N;
+  }
+  __device__ __forceinline__ int piece_class(int i) const { return head + i * N; }
+  // the single class of thread t, or -1
+  __device__ __forceinline__ int edge(int t) const {
+    const int c = t < 8 ? (t < head ? t : -1) : piece_class(pieces) + t - 8;
+    return c < classes && t < 16 ? c : -1;
+  }
+  // the thread that writes class c
+  template <int THREADS>
+  __device__ __forceinline__ int owner(int c) const {
+    const int i = (c - head) / N;
+    return c < head ? c : i < pieces ? i % THREADS : 8 + c - piece_class(pieces);
+  }
+};
+
+// Marks of listed classes in LDS: a byte for each of `count` pieces from `first` on, a bit for each
+// class of a piece, and (edges) a word for the classes before and behind the pieces, bit t that of
+// the class of thread t.  False where class c has no mark here.
+template <class T>
+__device__ __forceinline__ bool find_mark(const Row<T>& r, int c, int first, int count, bool edges,
+                                          uint32_t* marks, uint32_t* edge, uint32_t*& word,
+                                          uint32_t& bit) {
+  const int i = (c - r.head) / Row<T>::N;
+  if (c < r.head || i >= r.pieces) {
+    word = edge;
+    bit = 1u << (c < r.head ? c : 8 + c - r.piece_class(r.pieces));
+    return edges;
+  }
+  const int q = i - first;
+  word = marks + (q >> 2);
+  bit = 1u << ((q & 3) * 8 + (c - r.head) % Row<T>::N);
+  return q >= 0 && q < count;
+}
+
+// A row that stays packed in registers between the steps: what one has unpacked may not stay there
+// for the next.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <int HELD>
+__device__ __forceinline__ void repack(i32x4 (&x)[HELD]) {
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) asm volatile("" : "+v"(x[k]));
+}
+
+}  // namespace dmh

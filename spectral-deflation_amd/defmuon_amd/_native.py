@@ -89,6 +89,16 @@ _SIGS = {
     "dmh_cross_entropy_grad_stats": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int,
                                              c_ll, c_float, c_float, c_vp, c_vp, c_vp, c_vp,
                                              c_int, c_vp, c_ll]),
+    "dmh_log_probs": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll, c_float,
+                              c_int, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "dmh_log_probs_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_ll,
+                                   c_float, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_ll]),
+    "dmh_distill_workspace_size": (c_int, [c_ll, ctypes.POINTER(c_sz)]),
+    "dmh_distill": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_int, c_vp, c_int,
+                            c_ll, c_float, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_vp, c_ll,
+                            c_vp, c_sz]),
+    "dmh_distill_grad": (c_int, [c_vp, c_vp, c_int, c_ll, c_ll, c_ll, c_vp, c_int, c_int, c_vp,
+                                 c_int, c_ll, c_float, c_vp, c_vp, c_vp, c_int, c_vp, c_ll]),
 }
 
 
@@ -614,3 +624,104 @@ def cross_entropy_grad(logits, rows, targets, ignore, smoothing, z_loss, reducti
         dlogits.data_ptr(), dstride)
     if rc:
         _check(rc, "dmh_cross_entropy_grad_stats")
+
+
+def log_probs(logits, rows, tokens, ignore, temperature, top, out, entropy, top_out, top_ids,
+              stats):
+    """Log probabilities of tokens, entropies and top classes of the logits' rows (rows, classes,
+    row stride); tokens with out, top_out with top_ids, and stats (3, rows) may be None."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return log_probs(logits, rows, tokens, ignore, temperature, top, out, entropy, top_out,
+                             top_ids, stats)
+    n, classes, zs = rows
+    scored = tokens is not None
+    rc = (_lib or load()).dmh_log_probs(
+        _raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+        _address(tokens, "token_log_probs") if scored else 0,
+        scored and tokens.dtype == torch.int64, ignore, temperature, top,
+        out.data_ptr() if scored else 0, entropy.data_ptr(), top_out.data_ptr() if top else 0,
+        top_ids.data_ptr() if top else 0, 0 if stats is None else stats.data_ptr())
+    if rc:
+        _check(rc, "dmh_log_probs")
+
+
+def log_probs_grad(logits, rows, tokens, ignore, temperature, top_ids, stats, grads, dlogits,
+                   dstride):
+    """The gradient of the logits from log_probs' statistics; grads: those of its log
+    probabilities, entropies and top classes' log probabilities, each fp32 or None."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return log_probs_grad(logits, rows, tokens, ignore, temperature, top_ids, stats, grads,
+                                  dlogits, dstride)
+    n, classes, zs = rows
+    what = "token_log_probs"
+    rc = (_lib or load()).dmh_log_probs_grad(
+        _raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+        0 if tokens is None else _address(tokens, what),
+        tokens is not None and tokens.dtype == torch.int64, ignore, temperature,
+        0 if top_ids is None else top_ids.shape[-1],
+        0 if top_ids is None else _address(top_ids, what), stats.data_ptr(),
+        *(0 if g is None else _address(g, what) for g in grads), dlogits.data_ptr(), dstride)
+    if rc:
+        _check(rc, "dmh_log_probs_grad")
+
+
+@functools.lru_cache(maxsize=1024)
+def distill_workspace_bytes(rows):
+    nbytes = c_sz()
+    _check(load().dmh_distill_workspace_size(rows, ctypes.byref(nbytes)),
+           "dmh_distill_workspace_size")
+    return nbytes.value
+
+
+def distill(logits, rows, ids, teacher, ignore, temperature, rest, reduction, grad_scale, loss,
+            dlogits, dstride, keep):
+    """Divergences from the teacher's lists (and the gradient of grad_scale * loss into dlogits);
+    rows: (rows, classes, row stride) of the logits.  Returns what the backward pass needs (keep):
+    fp32, six statistics of the rows and the number of rows with a teacher (for a mean)."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return distill(logits, rows, ids, teacher, ignore, temperature, rest, reduction,
+                           grad_scale, loss, dlogits, dstride, keep)
+    n, classes, zs = rows
+    # statistics, count and workspace: one allocation a call, none for the losses alone
+    kept = 6 * n if keep else 0
+    nbytes = distill_workspace_bytes(n) if reduction else 0
+    stats, at = None, 0
+    if keep or reduction:
+        stats = torch.empty(kept + 1 + (nbytes + 3) // 4, dtype=torch.float32,
+                            device=logits.device)
+        at = stats.data_ptr()
+    count = at + 4 * kept
+    rc = (_lib or load()).dmh_distill(
+        _raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+        ids.data_ptr(), ids.dtype == torch.int64, ids.shape[-1], teacher.data_ptr(),
+        FLOATS[teacher.dtype], ignore, temperature, rest, reduction, grad_scale, loss.data_ptr(),
+        count, at if keep else 0, 0 if dlogits is None else dlogits.data_ptr(), dstride,
+        count + 4 if nbytes else 0, nbytes)
+    if rc:
+        _check(rc, "dmh_distill")
+    return stats
+
+
+def distill_grad(logits, rows, ids, teacher, ignore, temperature, reduction, stats, grad_out,
+                 dlogits, dstride):
+    """The gradient of the logits from distill's statistics, times grad_out."""
+    index = logits.get_device()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return distill_grad(logits, rows, ids, teacher, ignore, temperature, reduction, stats,
+                                grad_out, dlogits, dstride)
+    n, classes, zs = rows
+    at = stats.data_ptr()
+    rc = (_lib or load()).dmh_distill_grad(
+        _raw_stream(index), logits.data_ptr(), FLOATS[logits.dtype], n, classes, zs,
+        ids.data_ptr(), ids.dtype == torch.int64, ids.shape[-1], teacher.data_ptr(),
+        FLOATS[teacher.dtype], ignore, temperature, at, at + 24 * n if reduction == 1 else 0,
+        grad_out.data_ptr(), reduction == 0, dlogits.data_ptr(), dstride)
+    if rc:
+        _check(rc, "dmh_distill_grad")

@@ -29,6 +29,8 @@ the nearest 1/65536, and kept elements are scaled by the reciprocal of exactly t
 element is replaced by zero, also where it is not finite.
 """
 
+import collections
+
 import torch
 from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
@@ -38,7 +40,8 @@ from defmuon_amd import _native
 from defmuon_amd._native import FLOATS, NativeError
 
 __all__ = ["embedding", "embedding_backward", "dropout", "dropout_backward", "Dropout",
-           "draw_rng", "cross_entropy", "cross_entropy_step"]
+           "draw_rng", "cross_entropy", "cross_entropy_step", "token_log_probs", "TokenLogProbs",
+           "distillation", "distillation_step"]
 
 _is_tracing = torch._C._is_tracing
 _modes = torch._C._len_torch_dispatch_stack
@@ -443,6 +446,17 @@ def _like_rows(logits, rows):
     return logits.new_empty(logits.shape), classes
 
 
+def _step_grad(logits, rows, inplace, what):
+    """(tensor, row stride) for the gradient of a step: the logits themselves with inplace."""
+    z, n, classes, stride = rows
+    if not inplace:
+        return _like_rows(logits, rows)
+    if z is logits and (n <= 1 or stride >= classes):
+        return logits, stride
+    raise NativeError(f"{what}: logits of strides {tuple(logits.stride())} have no rows to "
+                      "write a gradient to")
+
+
 class _CrossEntropy(Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index, smoothing, z_loss, reduction):
@@ -502,16 +516,212 @@ def cross_entropy_step(logits, targets, ignore_index=-100, label_smoothing=0.0, 
     if reduction == "none":
         raise NativeError(f"{what}: the loss must be a mean or a sum")
     rows = _rows(logits)
-    z, n, classes, stride = rows
-    if not inplace:
-        dlogits, dstride = _like_rows(logits, rows)
-    elif z is logits and (n <= 1 or stride >= classes):
-        dlogits, dstride = logits, stride
-    else:
-        raise NativeError(f"{what}: logits of strides {tuple(logits.stride())} have no rows to "
-                          "write a gradient to")
+    dlogits, dstride = _step_grad(logits, rows, inplace, what)
     loss, _ = _xent(logits, rows, targets, ignore_index, label_smoothing, z_loss, reduction,
                     dlogits, dstride, grad_scale)
+    if inplace:   # autograd does not see a write through a pointer
+        increment_version(logits)
+    return loss, dlogits
+
+
+# ---- log probabilities ----------------------------------------------------------------------
+
+TokenLogProbs = collections.namedtuple("TokenLogProbs",
+                                       "log_probs entropy top_log_probs top_ids")
+
+_MAX_TOP, _MAX_LIST = 256, 1024
+
+
+def _temperature(tau, what):
+    if not 1e-6 <= tau <= 1e6:
+        raise NativeError(f"{what}: temperature must be between 1e-6 and 1e6, not {tau}")
+
+
+def _log_probs(logits, rows, tokens, top, tau, ignore_index, keep=False):
+    """(TokenLogProbs, statistics for the backward pass if `keep`); rows: _rows(logits)."""
+    z, n, classes, stride = rows
+    shape, device = logits.shape[:-1], logits.device
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    lp = top_lp = ids = stats = None
+    if tokens is not None:
+        lp = torch.empty(shape, dtype=torch.float32, device=device)
+        tokens = tokens.contiguous()
+    if top:
+        top_lp = torch.empty((*shape, top), dtype=torch.float32, device=device)
+        ids = torch.empty((*shape, top), dtype=torch.int64, device=device)
+    if keep:
+        stats = torch.empty(3 * n, dtype=torch.float32, device=device)
+    if n:
+        _native.log_probs(z, (n, classes, stride), tokens, ignore_index, tau, top, lp, entropy,
+                          top_lp, ids, stats)
+    return TokenLogProbs(lp, entropy, top_lp, ids), stats
+
+
+class _TokenLogProbs(Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, tau, ignore_index):
+        out, stats = _log_probs(logits, _rows(logits), tokens, top, tau, ignore_index, keep=True)
+        ctx.save_for_backward(logits, tokens, out.top_ids, stats)
+        ctx.args = tau, ignore_index
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(out.top_ids)
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        logits, tokens, ids, stats = ctx.saved_tensors
+        tau, ignore_index = ctx.args
+        grads = grads[:3]
+        if forward_ad._current_level >= 0:
+            for g in grads:
+                if g is not None:
+                    _no_tangent(g, "token_log_probs", "an output's gradient")
+        z, *rows = _rows(logits)
+        dz, stride = _like_rows(logits, (z, *rows))
+        if dz.numel():
+            _native.log_probs_grad(
+                z, rows, None if tokens is None else tokens.contiguous(), ignore_index, tau, ids,
+                stats, [None if g is None else g.float().contiguous() for g in grads], dz, stride)
+        return dz, None, None, None, None
+
+
+def token_log_probs(logits, tokens=None, top=0, temperature=1.0, ignore_index=-100):
+    """What logits (..., classes) say, by softmax(logits / temperature), in fp32:
+
+        log_probs      (...)       log probability of each row's token (None without tokens)
+        entropy        (...)       of each row
+        top_log_probs  (..., top)  the largest log probabilities, falling (None for top 0)
+        top_ids        (..., top)  their classes (int64); of equal logits the lower class first
+
+    tokens: int64 or int32 (...); top up to 256.  The three log probabilities and entropies take
+    part in autograd.  A row whose token is ignore_index gives zeros, and ignore_index for its
+    classes, which distillation skips in turn; another token outside the classes gives NaN for its
+    log probability (and for its row's gradient).  A row without a softmax (a NaN, an infinity,
+    -inf alone) gives NaN, and the classes 0, 1, ... for its top."""
+    what = "token_log_probs"
+    _eager(what, function=True)
+    _float(logits, what, "logits")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise NativeError(f"{what}: logits must be (..., classes), got {tuple(logits.shape)}")
+    if tokens is not None:
+        _ints(tokens, logits.device, what, "tokens")
+        if tokens.shape != logits.shape[:-1]:
+            raise NativeError(f"{what}: tokens {tuple(tokens.shape)} do not fit logits "
+                              f"{tuple(logits.shape)}")
+    if not 0 <= top <= min(_MAX_TOP, logits.shape[-1]):
+        raise NativeError(f"{what}: top must be between 0 and {_MAX_TOP} and no more than the "
+                          f"{logits.shape[-1]} classes, not {top}")
+    _temperature(temperature, what)
+    if _is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogProbs(*_TokenLogProbs.apply(logits, tokens, top, temperature,
+                                                   ignore_index))
+    return _log_probs(logits, _rows(logits), tokens, top, temperature, ignore_index)[0]
+
+
+# ---- distillation ---------------------------------------------------------------------------
+
+def _distill_args(logits, ids, teacher, tau, reduction, what):
+    _float(logits, what, "logits")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise NativeError(f"{what}: logits must be (..., classes), got {tuple(logits.shape)}")
+    _ints(ids, logits.device, what, "ids")
+    _float(teacher, what, "teacher")
+    if (ids.ndim != logits.ndim or ids.shape[:-1] != logits.shape[:-1]
+            or teacher.shape != ids.shape or teacher.device != logits.device):
+        raise NativeError(f"{what}: ids {tuple(ids.shape)} and teacher {tuple(teacher.shape)} on "
+                          f"{teacher.device} do not fit logits {tuple(logits.shape)} on "
+                          f"{logits.device}")
+    if not 1 <= ids.shape[-1] <= _MAX_LIST:
+        raise NativeError(f"{what}: lists must have 1 to {_MAX_LIST} classes, not "
+                          f"{ids.shape[-1]}")
+    if torch.is_grad_enabled() and teacher.requires_grad:
+        raise NativeError(f"{what}: the teacher takes no gradient; give teacher.detach()")
+    _temperature(tau, what)
+    if reduction not in _REDUCTIONS:
+        raise NativeError(f"{what}: reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
+
+
+def _distill(logits, rows, ids, teacher, tau, rest, ignore_index, reduction, dlogits=None,
+             dstride=0, grad_scale=1.0, keep=False):
+    """(loss, statistics for the backward pass if `keep`) and, in place, dlogits; rows:
+    _rows(logits)."""
+    z, n, classes, stride = rows
+    red = _REDUCTIONS[reduction]
+    loss = torch.empty(logits.shape[:-1] if red == 0 else (), dtype=torch.float32,
+                       device=logits.device)
+    stats = None
+    if n or red:
+        stats = _native.distill(z, (n, classes, stride), ids.contiguous(), teacher.contiguous(),
+                                ignore_index, tau, rest, red, grad_scale, loss, dlogits, dstride,
+                                keep)
+    return loss, stats
+
+
+class _Distillation(Function):
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, tau, rest, ignore_index, reduction):
+        loss, stats = _distill(logits, _rows(logits), ids, teacher, tau, rest, ignore_index,
+                               reduction, keep=True)
+        ctx.save_for_backward(logits, ids, teacher, stats)
+        ctx.args = ignore_index, tau, _REDUCTIONS[reduction]
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        if forward_ad._current_level >= 0:
+            _no_tangent(grad, "distillation", "the loss's gradient")
+        logits, ids, teacher, stats = ctx.saved_tensors
+        z, *rows = _rows(logits)
+        dz, stride = _like_rows(logits, (z, *rows))
+        if dz.numel():
+            _native.distill_grad(z, rows, ids.contiguous(), teacher.contiguous(), *ctx.args, stats,
+                                 grad.float().contiguous(), dz, stride)
+        return dz, *[None] * 6
+
+
+def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index=-100,
+                 reduction="mean"):
+    """How far softmax(logits / temperature) is from a teacher's, of which each row has a list of
+    classes ids (..., k) with their log probabilities teacher (..., k), in fp32:
+
+        temperature^2 sum over the list of q (log q - log p),    q = softmax(teacher)
+
+    or, with `rest`, q = exp(teacher) and the classes outside the list as one more, whose q is
+    what the list's leave of 1 (nothing, if they sum to more) and whose p is the sum of theirs.
+    Reductions as in cross_entropy, a mean over the rows that have a teacher.
+
+    token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is
+    taken as it is, at the temperature already (raw logits go in divided by it, without `rest`).
+    k up to 1024.  An entry whose class is ignore_index is left out, and a row whose first entry
+    is counts for nothing; another class outside the logits' makes its row NaN, as does a row
+    without a softmax.  An entry of -inf adds nothing, whatever the logits say; a row of
+    those alone is NaN, with `rest` it leaves all to the others.  The teacher takes no gradient."""
+    _eager("distillation", function=True)
+    _distill_args(logits, ids, teacher, temperature, reduction, "distillation")
+    if _is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
+        return _Distillation.apply(logits, ids, teacher, temperature, bool(rest), ignore_index,
+                                   reduction)
+    return _distill(logits, _rows(logits), ids, teacher, temperature, bool(rest), ignore_index,
+                    reduction)[0]
+
+
+def distillation_step(logits, ids, teacher, temperature=1.0, rest=False, ignore_index=-100,
+                      reduction="mean", grad_scale=1.0, inplace=False):
+    """(loss, dlogits) of distillation ("mean" or "sum") outside autograd, the logits read once
+    where a workgroup's registers hold a row; grad_scale and inplace as in cross_entropy_step."""
+    what = "distillation_step"
+    _eager(what)
+    _distill_args(logits, ids, teacher, temperature, reduction, what)
+    logits = logits.detach()
+    if reduction == "none":
+        raise NativeError(f"{what}: the loss must be a mean or a sum")
+    rows = _rows(logits)
+    dlogits, dstride = _step_grad(logits, rows, inplace, what)
+    loss, _ = _distill(logits, rows, ids, teacher, temperature, bool(rest), ignore_index,
+                       reduction, dlogits, dstride, grad_scale)
     if inplace:   # autograd does not see a write through a pointer
         increment_version(logits)
     return loss, dlogits
