@@ -107,27 +107,34 @@ __device__ __forceinline__ float natural_exp(float x) {
 }
 __device__ __forceinline__ float natural_log(float x) { return __builtin_amdgcn_logf(x) * LN2; }
 
-template <int THREADS>
-__device__ __forceinline__ float block_max(float v, float* lds) {
+// Parts of a row in lanes 0, 16 and 32 from the waves' own: the row's, the list's, the teacher's
+// (that one with 2^((t - m) log2 e)).
+constexpr int ROW_PART = 0, LIST_PART = 16, TEACHER_PART = 32;
+__device__ __forceinline__ Part wave_join(Part p, float c2, int from) {
 #pragma unroll
-  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  constexpr int W = THREADS / 64;
-  if (W <= 1) return v;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = lds[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) s = fmaxf(s, lds[w]);
-  return s;
+  for (int d = from / 2; d; d >>= 1)
+    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
+  return p;
+}
+__device__ __forceinline__ Part part_of(Part p, int lane) {
+  return {__shfl(p.m, lane), __shfl(p.s, lane)};
 }
 
-// A row by a workgroup that reads it for the sums and, with a gradient, again.
-template <class T, int THREADS, bool REST, bool GRAD>
-__global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
-  constexpr int N = Piece<T>::N, AHEAD = 4, SPAN = THREADS == 1024 ? 32768 : 2048;
-  __shared__ Part parts[16], list_parts[16];
-  __shared__ float lds[16];
+// One row by THREADS threads that hold it in registers, HELD pieces each, packed between the
+// steps: it is read once, and its gradient written once.  With HELD = 0 a workgroup streams its row,
+// twice with a gradient.
+//
+// Thread j deals with entries j, j + THREADS, ... of the list, while the row is on its way.  A bitmap
+// of the classes says which entry of a class is its first (the others add nothing to the list's
+// sum, and the first writes the gradient), and with REST which logits are not the rest's: they
+// become -inf before the row is summed.
+template <class T, int THREADS, int HELD, bool REST, bool GRAD>
+__global__ __launch_bounds__(THREADS, HELD > 16 ? 2 : HELD > 8 ? 4 : 8)
+void distill_row(DistillArgs a) {
+  constexpr int N = Piece<T>::N, AHEAD = 4, W = THREADS / 64;
+  constexpr int SPAN = HELD ? HELD * THREADS : 32768;
+  __shared__ Part parts[48];
+  __shared__ float sums[16];
   __shared__ int ids[LIST_MAX];
   __shared__ float zs[LIST_MAX], ts[LIST_MAX];   // the list's logits; log probabilities, then q
   __shared__ uint32_t marks[SPAN / 4];           // of SPAN pieces
@@ -140,7 +147,22 @@ __global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
   T* dz = GRAD ? (T*)a.dz + row * a.ds : nullptr;
   const Row<T> r(z, a.classes);
   const int ec = r.edge(t);
-  if (load_index(a.ids, a.i64, row * K) == a.ignore) {
+  const long long named = load_index(a.ids, a.i64, row * K);
+  // the thread's first entry is on its way before the row, which the list's logits follow
+  long long c0 = a.ignore;
+  float q0 = 0.f, z0 = 0.f;
+  if (t < K) {
+    c0 = load_index(a.ids, a.i64, row * K + t);
+    q0 = load_float(a.teacher, a.ttype, row * K + t);
+  }
+  i32x4 x[HELD ? HELD : 1] = {};
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = k * THREADS + t;
+    if (i < r.pieces) x[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i)));
+  }
+  const float ex = ec >= 0 ? (float)z[ec] : -INF;
+  if (named == a.ignore) {
     if (t == 0) a.row_loss[row] = 0.f;
     if (t < 6 && a.stats) a.stats[t * a.rows + row] = 0.f;
     if (GRAD) {
@@ -154,33 +176,30 @@ __global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
     edge_marks = 0;
     twice = bad = 0;
   }
+  for (int i = t; i < SPAN / 4 && 4 * i < r.pieces; i += THREADS) marks[i] = 0;
+  if (t < 48) parts[t] = {-INF, 0.f};
   __syncthreads();
-  // the list: its entries that are left out have q = 0
-  float tm = -INF;
-  for (int j = t; j < K; j += THREADS) {
-    const long long c = load_index(a.ids, a.i64, row * K + j);
+  // the list; entries that are left out have no class
+  Part tp = {-INF, 0.f};
+  auto entry = [&](int j, long long c, float q) {
     const bool in = c >= 0 && c < a.classes;
     if (!in && c != a.ignore) bad = 1;
     ids[j] = in ? (int)c : -1;
-    zs[j] = in ? (float)z[c] : 0.f;
-    const float q = in ? load_float(a.teacher, a.ttype, row * K + j) : -INF;
-    ts[j] = q;
-    tm = fmaxf(tm, q);
+    ts[j] = in ? q : -INF;
+    if (in) {   // a NaN ends in the sum
+      if (REST) tp = {0.f, tp.s + natural_exp(q)};
+      else tp = join(tp, {fmaxf(q, -INF), q == -INF ? 0.f : q - q + 1.f}, LOG2E);
+    }
+    return in;
+  };
+  if (t < K && entry(t, c0, q0)) z0 = (float)z[c0];
+  for (int j = t + THREADS; j < K; j += THREADS) {
+    const long long c = load_index(a.ids, a.i64, row * K + j);
+    if (entry(j, c, load_float(a.teacher, a.ttype, row * K + j))) zs[j] = (float)z[c];
   }
-  tm = REST ? 0.f : block_max<THREADS>(tm, lds);
-  float qsum = 0.f;
-  for (int j = t; j < K; j += THREADS)
-    qsum += ids[j] >= 0 ? natural_exp(ts[j] - tm) : 0.f;
-  qsum = block_sum<THREADS>(qsum, lds);
-  // the row
-  const float ex = ec >= 0 ? (float)z[ec] : -INF;
-  Part p = {-INF, 0.f};
+  // the first entry of each class among SPAN pieces from `first` on
   uint32_t firsts = 0;
-  for (int first = 0; first == 0 || first < r.pieces; first += SPAN) {
-    const int last = first + SPAN < r.pieces ? first + SPAN : r.pieces;
-    __syncthreads();
-    for (int i = t; i < (last - first + 3) / 4; i += THREADS) marks[i] = 0;
-    __syncthreads();
+  auto mark_list = [&](int first) {
     int it = 0;
     for (int j = t; j < K; j += THREADS, ++it) {
       uint32_t *word, bit;
@@ -191,53 +210,122 @@ __global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
       }
     }
     __syncthreads();
-    if (first == 0 && ec >= 0 && !(REST && edge_marks >> t & 1)) {
-      p.m = fmaxf(ex, -INF);
-      p.s = __builtin_amdgcn_exp2f((ex - (p.m == -INF ? 0.f : p.m)) * a.c2);
-    }
-    for (int i0 = first + t; i0 < last; i0 += AHEAD * THREADS) {
-      type x[AHEAD];
+  };
+  const uint8_t* byte_marks = (const uint8_t*)marks;
+  Part p = {-INF, 0.f};
+  mark_list(0);
+  const bool edge_in = ec >= 0 && !(REST && edge_marks >> t & 1);
+  if (edge_in) p.m = fmaxf(ex, -INF);
+  if constexpr (HELD > 0) {
+    if constexpr (REST) {
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int i = i0 + k * THREADS;
-        x[k] = *(const type*)(z + r.piece_class(i < last ? i : i0));
-      }
-      float m = p.m;
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int i = i0 + k * THREADS < last ? i0 + k * THREADS : i0;
-        if (REST) {
-          const uint32_t listed = ((const uint8_t*)marks)[i - first];
+      for (int k = 0; k < HELD; ++k) {
+        const int i = k * THREADS + t;
+        const uint32_t listed = i < r.pieces ? byte_marks[i] : 0;
+        if (listed) {
+          type v = __builtin_bit_cast(type, x[k]);
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            if (listed >> j & 1) x[k][j] = (T)-INF;
+            if (listed >> j & 1) v[j] = (T)-INF;
+          x[k] = __builtin_bit_cast(i32x4, v);
         }
-#pragma unroll
-        for (int j = 0; j < N; ++j) m = fmaxf(m, (float)x[k][j]);
       }
-      rescale(p, m, a.c2);
-      const float m0 = m == -INF ? 0.f : m;
+      repack(x);
+    }
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (i0 + k * THREADS < last) {
+    for (int k = 0; k < HELD; ++k) {
+      if (k * THREADS + t < r.pieces) {
+        const type v = __builtin_bit_cast(type, x[k]);
 #pragma unroll
-          for (int j = 0; j < N; ++j)
-            p.s += __builtin_amdgcn_exp2f(((float)x[k][j] - m0) * a.c2);
+        for (int j = 0; j < N; ++j) p.m = fmaxf(p.m, (float)v[j]);
+      }
+    }
+    repack(x);
+    const float m0 = p.m == -INF ? 0.f : p.m;
+    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - m0) * a.c2);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      if (k * THREADS + t < r.pieces) {
+        const type v = __builtin_bit_cast(type, x[k]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) p.s += __builtin_amdgcn_exp2f(((float)v[j] - m0) * a.c2);
+      }
+    }
+    repack(x);
+  } else {
+    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - (p.m == -INF ? 0.f : p.m)) * a.c2);
+    for (int first = 0; first < r.pieces; first += SPAN) {
+      const int last = first + SPAN < r.pieces ? first + SPAN : r.pieces;
+      if (first > 0) {
+        __syncthreads();
+        for (int i = t; i < (last - first + 3) / 4; i += THREADS) marks[i] = 0;
+        __syncthreads();
+        mark_list(first);
+      }
+      for (int i0 = first + t; i0 < last; i0 += AHEAD * THREADS) {
+        type v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          v[k] = *(const type*)(z + r.piece_class(i < last ? i : i0));
         }
+        float m = p.m;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS < last ? i0 + k * THREADS : i0;
+          if (REST) {
+            const uint32_t listed = byte_marks[i - first];
+            if (listed) {
+#pragma unroll
+              for (int j = 0; j < N; ++j)
+                if (listed >> j & 1) v[k][j] = (T)-INF;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
+        }
+        rescale(p, m, a.c2);
+        const float m0 = m == -INF ? 0.f : m;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (i0 + k * THREADS < last) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              p.s += __builtin_amdgcn_exp2f(((float)v[k][j] - m0) * a.c2);
+          }
+      }
     }
   }
-  p = block_join<THREADS>(p, a.c2, parts);
-  Part all = p;
-  if (REST) {
-    Part l = {-INF, 0.f};
-    int it = 0;
-    for (int j = t; j < K; j += THREADS, ++it) {
-      const float v = zs[j];
-      if (firsts >> it & 1)
-        l = join(l, {fmaxf(v, -INF), v == -INF ? 0.f : v - v + 1.f}, a.c2);
+  // every wave joins the waves' parts in the same way
+  p = wave_join(p, a.c2, 64);
+  const int wave = t >> 6, lane = t & 63;
+  if (lane == 0) parts[ROW_PART + wave] = p;
+  if ((t & ~63) < K) {   // waves with a part of the list
+    if (t < K) zs[t] = z0;
+    Part lp = {-INF, 0.f};
+    if (REST) {
+      int it = 0;
+      for (int j = t; j < K; j += THREADS, ++it) {
+        const float v = zs[j];
+        if (firsts >> it & 1)
+          lp = join(lp, {fmaxf(v, -INF), v == -INF ? 0.f : v - v + 1.f}, a.c2);
+      }
+      lp = wave_join(lp, a.c2, 64);
     }
-    all = join(p, block_join<THREADS>(l, a.c2, list_parts), a.c2);
+    tp = wave_join(tp, LOG2E, 64);
+    if (lane == 0) {
+      parts[LIST_PART + wave] = lp;
+      parts[TEACHER_PART + wave] = tp;
+    }
   }
+  __syncthreads();
+  Part all = wave_join(lane < 48 ? parts[lane] : Part{-INF, 0.f},
+                       lane < TEACHER_PART ? a.c2 : LOG2E, 16);
+  p = part_of(all, ROW_PART);
+  const Part lp = part_of(all, LIST_PART);
+  tp = part_of(all, TEACHER_PART);
+  all = REST ? join(p, lp, a.c2) : p;
+  const float tm = REST ? 0.f : tp.m, qsum = tp.s;
   // coefficients
   const float log_s = natural_log(all.s);
   const float left = REST ? fmaxf(1.f - qsum, 0.f) : 0.f;
@@ -254,16 +342,74 @@ __global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
     st.coef = st.ws * (p.m == -INF ? 0.f : __builtin_amdgcn_exp2f((p.m - all.m) * a.c2));
     if (left > 0.f && p.s > 0.f) st.coef -= left / p.s;
   }
-  float loss = 0.f;
-  const float log_q = REST ? 0.f : natural_log(qsum);
-  for (int j = t; j < K; j += THREADS) {
-    const float q = ids[j] >= 0 ? natural_exp(ts[j] - tm) * st.qs : 0.f;
-    // not below: a NaN goes on
-    if (!(q <= 0.f)) loss += q * ((ts[j] - tm - log_q) - ((zs[j] - all.m) * a.itau - log_s));
-    ts[j] = q;
+  if ((t & ~63) < K) {
+    float loss = 0.f;
+    const float log_q = REST ? 0.f : natural_log(qsum);
+    for (int j = t; j < K; j += THREADS) {
+      const float q = ids[j] >= 0 ? natural_exp(ts[j] - tm) * st.qs : 0.f;
+      // not below: a NaN goes on
+      if (!(q <= 0.f)) loss += q * ((ts[j] - tm - log_q) - ((zs[j] - all.m) * a.itau - log_s));
+      ts[j] = q;
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) loss += __shfl_xor(loss, d);
+    if (lane == 0) sums[wave] = loss;
   }
-  loss = block_sum<THREADS>(loss, lds);
+  if (GRAD) {
+    const float g = a.gscale / (a.count ? *a.count : 1.f);
+    const float coef = st.coef * g;
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const int i = k * THREADS + t;
+        if (i < r.pieces) {
+          const type v = __builtin_bit_cast(type, x[k]);
+          type d;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            d[j] = (T)(__builtin_amdgcn_exp2f(((float)v[j] - st.ref) * a.c2) * coef);
+          *(type*)(dz + r.piece_class(i)) = d;
+        }
+      }
+    } else {
+      for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
+        type v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          type d;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            d[j] = (T)(__builtin_amdgcn_exp2f(((float)v[k][j] - st.ref) * a.c2) * coef);
+          if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+        }
+      }
+    }
+    if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
+    __syncthreads();   // the sums; and the listed classes again, each by one thread
+    int it = 0;
+    for (int j = t; j < K; j += THREADS, ++it) {
+      if (firsts >> it & 1) {
+        const int c = ids[j];
+        float q = ts[j];
+        if (twice) {   // a class listed more than once: its terms in their order
+          q = 0.f;
+          for (int i = 0; i < K; ++i) q += ids[i] == c ? ts[i] : 0.f;
+        }
+        dz[c] = (T)((__builtin_amdgcn_exp2f((zs[j] - st.m) * a.c2) * st.ws - q) * g);
+      }
+    }
+  } else {
+    __syncthreads();
+  }
   if (t == 0) {
+    float loss = sums[0];
+    for (int i = 1; i < W && i * 64 < K; ++i) loss += sums[i];
     if (REST && left > 0.f)
       loss += left * (natural_log(left) - ((p.m - all.m) * a.itau + natural_log(p.s) - log_s));
     a.row_loss[row] = w == w ? loss * a.lscale : w;
@@ -274,50 +420,28 @@ __global__ __launch_bounds__(THREADS) void distill_row(DistillArgs a) {
     if (a.stats) a.stats[4 * a.rows + row] = st.tm;
     if (a.stats) a.stats[5 * a.rows + row] = st.qs;
   }
-  if (!GRAD) return;
-  const float g = a.gscale / (a.count ? *a.count : 1.f);
-  const float coef = st.coef * g;
-  for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
-    type x[AHEAD];
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int i = i0 + k * THREADS;
-      x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
-    }
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int i = i0 + k * THREADS;
-      type d;
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        d[j] = (T)(__builtin_amdgcn_exp2f(((float)x[k][j] - st.ref) * a.c2) * coef);
-      if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
-    }
-  }
-  if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
-  __syncthreads();
-  // the listed classes again, each by one thread
-  int it = 0;
-  for (int j = t; j < K; j += THREADS, ++it) {
-    if (firsts >> it & 1) {
-      const int c = ids[j];
-      float q = ts[j];
-      if (twice) {   // a class listed more than once: its terms in their order
-        q = 0.f;
-        for (int i = 0; i < K; ++i) q += ids[i] == c ? ts[i] : 0.f;
-      }
-      dz[c] = (T)((__builtin_amdgcn_exp2f((zs[j] - st.m) * a.c2) * st.ws - q) * g);
-    }
-  }
 }
 
+// The fewest threads that hold a row; longer rows are held for the gradient as far as registers
+// go, and streamed for the loss alone.
 template <class T, bool REST, bool GRAD>
 static void launch_rows(hipStream_t stream, const DistillArgs& a) {
+  const int pieces = a.classes / Piece<T>::N;   // at most
   const dim3 rows((unsigned)a.rows);
-  if (a.classes <= 8192)
-    hipLaunchKernelGGL((distill_row<T, 256, REST, GRAD>), rows, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((distill_row<T, 1024, REST, GRAD>), rows, dim3(1024), 0, stream, a);
+#define DMH_ROWS(THREADS, HELD)                                                             \
+  if (pieces <= THREADS * HELD) {                                                           \
+    hipLaunchKernelGGL((distill_row<T, THREADS, HELD, REST, GRAD>), rows, dim3(THREADS), 0, \
+                       stream, a);                                                          \
+    return;                                                                                 \
+  }
+  DMH_ROWS(256, 8)
+  DMH_ROWS(1024, 8)
+  if constexpr (GRAD) {
+    DMH_ROWS(1024, 16)
+    DMH_ROWS(512, 48)
+  }
+#undef DMH_ROWS
+  hipLaunchKernelGGL((distill_row<T, 1024, 0, REST, GRAD>), rows, dim3(1024), 0, stream, a);
 }
 template <class T>
 static void launch_distill(hipStream_t stream, const DistillArgs& a, bool rest) {

@@ -86,46 +86,85 @@ __device__ __forceinline__ u64 rank_key(float x, int c) {
   return (u64)order_key(x) << 32 | (uint32_t)~c;
 }
 
+constexpr int CANDS = 1024;   // what is sorted out in the end, K <= TOP_MAX of them kept
+
 struct TopLds {
-  u64 cand[1024];
-  int slots[96];   // a counter for each step of a search
+  uint32_t keys[1024];   // of groups of threads
+  u64 cand[CANDS];
+  uint32_t cut, most;
+  int slots[64];         // a counter for each step of the search over all classes
   int n;
 };
-constexpr int CANDS = 1024;
 
-// The number over the whole workgroup, through counter `slot` (zero before).
-__device__ __forceinline__ int block_count(int n, int* slot) {
+// A lower bound of the K-th largest of a row, by the first wave: the K-th largest of the maxima of
+// `groups` groups of threads, since K groups have a class that large.  A bit at a time, and no
+// further than to a few groups more than K.  The other waves go on with the row's sum.
+template <int PER>
+__device__ __forceinline__ void group_cut(int K, TopLds& l) {
+  uint32_t k[PER], most = 0;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-  if ((threadIdx.x & 63) == 0 && n) atomicAdd(slot, n);
-  __syncthreads();
-  return *slot;
-}
-
-// The K largest classes of a row by one workgroup; each(f) calls f(value, class) for every class of
-// the thread, `largest` is their maximum (-inf for none).
-template <int THREADS, class Each>
-__device__ __forceinline__ void select_top(int K, float largest, const Each& each, TopLds& l) {
-  for (int i = threadIdx.x; i < 96; i += THREADS) l.slots[i] = 0;
-  if (threadIdx.x == 0) l.n = 0;
-  __syncthreads();
-  // K threads have a class that is at least the K-th largest of the threads' maxima, so K
-  // classes are: a bit at a time, until few more threads are left
-  const uint32_t mine = order_key(largest);
-  uint32_t cut = 0;
-  int step = 0;
+  for (int i = 0; i < PER; ++i) {
+    k[i] = l.keys[i * 64 + (threadIdx.x & 63)];
+    most = k[i] > most ? k[i] : most;
+  }
   const int enough = K + K / 4 + 4;
+  uint32_t cut = 0;
   for (int b = 31; b >= 0; --b) {
     const uint32_t c = cut | 1u << b;
-    const int n = block_count(mine >= c, &l.slots[step++]);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(k[i] >= c));
     if (n >= K) {
       cut = c;
       if (n <= enough) break;
     }
   }
-  u64 from = (u64)cut << 32;
-  auto gather = [&]() {
-    each([&](float v, int c) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const uint32_t o = __shfl_xor(most, d);
+    most = o > most ? o : most;
+  }
+  if (threadIdx.x == 0) {
+    l.cut = cut;
+    l.most = most;
+  }
+}
+
+// The threads' maxima by groups: as many groups as hold four times K apart, up to one a thread.
+template <int THREADS>
+__device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
+  uint32_t k = order_key(largest), o;
+  int t = threadIdx.x;
+  if (THREADS == 1024 && K <= 128) {
+    o = __shfl_xor(k, 1);
+    k = o > k ? o : k;
+    t >>= 1;
+    if (K <= 64) {
+      o = __shfl_xor(k, 2);
+      k = o > k ? o : k;
+      t >>= 1;
+    }
+  }
+  l.keys[t] = k;   // the same from all threads of a group
+  if (threadIdx.x == 0) l.n = 0;
+  if (threadIdx.x < 64) l.slots[threadIdx.x] = 0;
+}
+template <int THREADS>
+__device__ __forceinline__ void find_cut(int K, TopLds& l) {
+  if (THREADS == 256 || K <= 64) group_cut<4>(K, l);
+  else if (K <= 128) group_cut<THREADS == 1024 ? 8 : 4>(K, l);
+  else group_cut<THREADS / 64>(K, l);
+}
+
+// The candidates, CANDS at most and the K largest among them, behind a barrier that follows
+// find_cut.  each(cut, f) calls f(value, class) for all classes of the thread whose order_key is at
+// least cut, and may for others; each_once is the same for one call.
+template <int THREADS, class Each, class Again>
+__device__ __forceinline__ void gather_top(int K, int classes, const Each& each_once,
+                                           const Again& each, TopLds& l) {
+  u64 from = (u64)l.cut << 32;
+  auto gather = [&](const auto& each) {
+    each((uint32_t)(from >> 32), [&](float v, int c) {
       const u64 k = rank_key(v, c);
       if (k >= from) {
         const int at = atomicAdd(&l.n, 1);
@@ -134,31 +173,62 @@ __device__ __forceinline__ void select_top(int K, float largest, const Each& eac
     });
     __syncthreads();
   };
-  gather();
+  gather(each_once);
   if (l.n > CANDS) {
-    // few threads with many large classes, or many equal ones: the same over all classes
-    step = 32;
-    from = 0;
-    for (int b = 63; b >= 0; --b) {
-      const u64 t = from | 1ull << b;
+    // Many large classes in few groups, or many equal ones: a bit at a time over all classes.
+    // The K-th largest is between cut and the largest: the bits that these two share need no
+    // step, nor do a class's bits above those of the last one.
+    const uint32_t cut = l.cut, most = l.most;
+    const int high = cut == most ? -1 : 31 - __clz(cut ^ most);
+    const int low = 32 - __clz(classes);   // classes < 2^low
+    from = (u64)(high < 0 ? most : most & ~((2u << high) - 1u)) << 32;
+    if (high < 0) from |= ~((1u << low) - 1u);
+    int step = 0;
+    for (int b = high < 0 ? low - 1 : 32 + high; b >= 0; --b) {
+      if (b == 31) {   // all classes share these
+        from |= ~((1u << low) - 1u);
+        b = low - 1;
+      }
+      const u64 c = from | 1ull << b;
       int n = 0;
-      each([&](float v, int c) { n += rank_key(v, c) >= t; });
-      n = block_count(n, &l.slots[step++]);
+      each((uint32_t)(c >> 32), [&](float v, int i) { n += rank_key(v, i) >= c; });
+#pragma unroll
+      for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+      if ((threadIdx.x & 63) == 0 && n) atomicAdd(&l.slots[step], n);
+      __syncthreads();
+      n = l.slots[step++];
       if (n >= K) {
-        from = t;
+        from = c;
         if (n <= CANDS) break;
       }
     }
-    __syncthreads();
     if (threadIdx.x == 0) l.n = 0;
     __syncthreads();
-    gather();
+    gather(each);
   }
 }
 
-// Rows of any length: a workgroup reads its row for the sums, and again for its largest classes.
-template <class T, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS) void log_prob_row(LogProbArgs a) {
+// The K largest candidates in their order: put(place, value, class).  A candidate's place is the
+// number of larger ones, which as many threads as there are for each count together.
+template <int THREADS, class Put>
+__device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) {
+  const int n = l.n;
+  int share = 1;
+  while (share < 64 && 2 * share * n <= THREADS) share *= 2;
+  const int part = threadIdx.x & (share - 1);
+  for (int i = threadIdx.x / share; i < n; i += THREADS / share) {
+    const u64 k = l.cand[i];
+    int before = 0;
+    for (int j = part; j < n; j += share) before += l.cand[j] > k;
+    for (int d = share >> 1; d; d >>= 1) before += __shfl_xor(before, d);
+    if (part == 0 && before < K) put(before, key_value((uint32_t)(k >> 32)), (int)~(uint32_t)k);
+  }
+}
+
+// One row by THREADS threads that hold it in registers, HELD pieces each (packed between the
+// steps), or for HELD = 0 a workgroup that streams it.
+template <class T, int THREADS, int HELD, bool TOP>
+__global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
   __shared__ Part3 parts[16];
   __shared__ typename std::conditional<TOP, TopLds, char>::type top;
   constexpr int N = Piece<T>::N, AHEAD = 4;
@@ -168,6 +238,14 @@ __global__ __launch_bounds__(THREADS) void log_prob_row(LogProbArgs a) {
   const T* z = (const T*)a.z + row * a.zs;
   const Row<T> r(z, a.classes);
   const long long y = a.tokens ? load_index(a.tokens, a.t64, row) : 0;
+  i32x4 x[HELD ? HELD : 1] = {};
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = k * THREADS + t;
+    if (i < r.pieces) x[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i)));
+  }
+  const int ec = r.edge(t);
+  const float ex = ec >= 0 ? (float)z[ec] : -INF;
   if (a.tokens && y == a.ignore) {
     if (t == 0) {
       a.lp[row] = 0.f;
@@ -180,93 +258,154 @@ __global__ __launch_bounds__(THREADS) void log_prob_row(LogProbArgs a) {
     }
     return;
   }
-  const int ec = r.edge(t);
-  const float ex = ec >= 0 ? (float)z[ec] : -INF;
+  const bool known = a.tokens && y >= 0 && y < a.classes;
+  const float zy = known ? (float)z[y] : __builtin_nanf("");
   Part3 p = {fmaxf(ex, -INF), 0.f, 0.f};
   auto add = [&](float v, float m0) {
     const float d = (v - m0) * a.c2, e = __builtin_amdgcn_exp2f(d);
     p.s += e;
     p.t = fmaf(e, fmaxf(d, LOWEST), p.t);
   };
-  if (ec >= 0) add(ex, p.m == -INF ? 0.f : p.m);
-  for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
-    type x[AHEAD];
+  if constexpr (HELD > 0) {
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int i = i0 + k * THREADS;
-      x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
-    }
-    float m = p.m;
+    for (int k = 0; k < HELD; ++k) {
+      if (k * THREADS + t < r.pieces) {
+        const type v = __builtin_bit_cast(type, x[k]);
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-#pragma unroll
-      for (int j = 0; j < N; ++j) m = fmaxf(m, (float)x[k][j]);
-    rescale(p, m, a.c2);
-    const float m0 = m == -INF ? 0.f : m;
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (i0 + k * THREADS < r.pieces) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) add((float)x[k][j], m0);
+        for (int j = 0; j < N; ++j) p.m = fmaxf(p.m, (float)v[j]);
       }
+    }
+    repack(x);
+    if constexpr (TOP) {
+      put_group<THREADS>(K, p.m, top);
+      __syncthreads();
+      if (t < 64) find_cut<THREADS>(K, top);
+    }
+    const float m0 = p.m == -INF ? 0.f : p.m;
+    if (ec >= 0) add(ex, m0);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      if (k * THREADS + t < r.pieces) {
+        const type v = __builtin_bit_cast(type, x[k]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) add((float)v[j], m0);
+      }
+    }
+    repack(x);
+  } else {
+    if (ec >= 0) add(ex, p.m == -INF ? 0.f : p.m);
+    for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
+      type v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * THREADS;
+        v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+      }
+      float m = p.m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
+      rescale(p, m, a.c2);
+      const float m0 = m == -INF ? 0.f : m;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * THREADS < r.pieces) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) add((float)v[k][j], m0);
+        }
+    }
+    if constexpr (TOP) {
+      put_group<THREADS>(K, p.m, top);
+      __syncthreads();
+      if (t < 64) find_cut<THREADS>(K, top);
+    }
   }
   const float largest = p.m;
   p = block_join<THREADS>(p, a.c2, parts);
   const float log_s = __builtin_amdgcn_logf(p.s) * LN2;
-  const bool good = p.s >= 0.5f;   // the maximum alone gives 1
   if (t == 0) {
     const float ent = log_s - LN2 * (p.t / p.s);
     if (a.ent) a.ent[row] = ent;
     if (a.stats) a.stats[row] = p.m;
     if (a.stats) a.stats[a.rows + row] = p.s;
     if (a.stats) a.stats[2 * a.rows + row] = ent;
-    if (a.tokens)
-      a.lp[row] = y >= 0 && y < a.classes ? ((float)z[y] - p.m) * a.itau - log_s
-                                          : __builtin_nanf("");
+    if (a.tokens) a.lp[row] = (zy - p.m) * a.itau - log_s;
   }
   if constexpr (TOP) {
-    if (!good) {
+    if (!(p.s >= 0.5f)) {   // no softmax: the maximum alone gives 1
       for (int i = t; i < K; i += THREADS) {
         a.top_lp[row * K + i] = __builtin_nanf("");
         a.top_ids[row * K + i] = i;
       }
       return;
     }
-    auto each = [&](auto f) {
+    auto reread = [&](uint32_t cut, auto f) {
+      if (order_key(largest) < cut) return;
       if (ec >= 0) f(ex, ec);
-      for (int i = t; i < r.pieces; i += THREADS) {
-        const type x = *(const type*)(z + r.piece_class(i));
+      for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
+        type v[AHEAD];
 #pragma unroll
-        for (int j = 0; j < N; ++j) f((float)x[j], r.piece_class(i) + j);
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          float m = (float)v[k][0];
+#pragma unroll
+          for (int j = 1; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
+          if (i < r.pieces && order_key(m) >= cut) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) f((float)v[k][j], r.piece_class(i) + j);
+          }
+        }
       }
     };
-    select_top<THREADS>(K, largest, each, top);
-    const int n = top.n;
-    for (int i = t; i < n; i += THREADS) {
-      const u64 k = top.cand[i];
-      int before = 0;
-      for (int j = 0; j < n; ++j) before += top.cand[j] > k;
-      if (before < K) {
-        a.top_lp[row * K + before] = (key_value((uint32_t)(k >> 32)) - p.m) * a.itau - log_s;
-        a.top_ids[row * K + before] = (uint32_t)~k;
+    auto held = [&](uint32_t cut, auto f) {
+      if (order_key(largest) < cut) return;
+      if (ec >= 0) f(ex, ec);
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const int i = k * THREADS + t;
+        int c = r.piece_class(i);
+        asm volatile("" : "+v"(x[k]), "+v"(c));   // nothing unpacked waits in registers
+        const type v = __builtin_bit_cast(type, x[k]);
+        float m = (float)v[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) m = fmaxf(m, (float)v[j]);
+        if (i < r.pieces && order_key(m) >= cut) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) f((float)v[j], c + j);
+        }
       }
-    }
+    };
+    if constexpr (HELD > 0)
+      gather_top<THREADS>(K, a.classes, held, reread, top);
+    else
+      gather_top<THREADS>(K, a.classes, reread, reread, top);
+    put_top<THREADS>(K, [&](int place, float v, int c) {
+      a.top_lp[row * K + place] = (v - p.m) * a.itau - log_s;
+      a.top_ids[row * K + place] = c;
+    }, top);
   }
 }
 
+template <class T, bool TOP>
+static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
+  const int pieces = a.classes / Piece<T>::N;   // at most
+  const dim3 rows((unsigned)a.rows);
+  if (pieces <= 256 * 8 && a.top <= 128)
+    hipLaunchKernelGGL((log_prob_row<T, 256, 8, TOP>), rows, dim3(256), 0, stream, a);
+  else if (pieces <= 1024 * 8)
+    hipLaunchKernelGGL((log_prob_row<T, 1024, 8, TOP>), rows, dim3(1024), 0, stream, a);
+  else
+    hipLaunchKernelGGL((log_prob_row<T, 1024, 0, TOP>), rows, dim3(1024), 0, stream, a);
+}
 template <class T>
 static void launch_log_probs(hipStream_t stream, const LogProbArgs& a) {
-  const dim3 rows((unsigned)a.rows);
-  if (a.classes <= 8192) {
-    if (a.top)
-      hipLaunchKernelGGL((log_prob_row<T, 256, true>), rows, dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((log_prob_row<T, 256, false>), rows, dim3(256), 0, stream, a);
-  } else if (a.top) {
-    hipLaunchKernelGGL((log_prob_row<T, 1024, true>), rows, dim3(1024), 0, stream, a);
-  } else {
-    hipLaunchKernelGGL((log_prob_row<T, 1024, false>), rows, dim3(1024), 0, stream, a);
-  }
+  a.top ? launch_rows<T, true>(stream, a) : launch_rows<T, false>(stream, a);
 }
 
 // ---- gradient -----------------------------------------------------------------------------------
