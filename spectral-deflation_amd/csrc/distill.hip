@@ -107,19 +107,6 @@ __device__ __forceinline__ float natural_exp(float x) {
 }
 __device__ __forceinline__ float natural_log(float x) { return __builtin_amdgcn_logf(x) * LN2; }
 
-// Parts of a row in lanes 0, 16 and 32 from the waves' own: the row's, the list's, the teacher's
-// (that one with 2^((t - m) log2 e)).
-constexpr int ROW_PART = 0, LIST_PART = 16, TEACHER_PART = 32;
-__device__ __forceinline__ Part wave_join(Part p, float c2, int from) {
-#pragma unroll
-  for (int d = from / 2; d; d >>= 1)
-    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
-  return p;
-}
-__device__ __forceinline__ Part part_of(Part p, int lane) {
-  return {__shfl(p.m, lane), __shfl(p.s, lane)};
-}
-
 // One row by THREADS threads that hold it in registers, HELD pieces each, packed between the
 // steps: it is read once, and its gradient written once.  With HELD = 0 a workgroup streams its row,
 // twice with a gradient.
@@ -133,8 +120,9 @@ __global__ __launch_bounds__(THREADS, HELD > 16 ? 2 : HELD > 8 ? 4 : 8)
 void distill_row(DistillArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, W = THREADS / 64;
   constexpr int SPAN = HELD ? HELD * THREADS : 32768;
-  __shared__ Part parts[48];
-  __shared__ float sums[16];
+  // the waves' maxima and sums: of the row, the list, the teacher; their losses
+  __shared__ float row_max[16], list_max[16], teacher_max[16];
+  __shared__ float row_sum[16], list_sum[16], teacher_sum[16], losses[16];
   __shared__ int ids[LIST_MAX];
   __shared__ float zs[LIST_MAX], ts[LIST_MAX];   // the list's logits; log probabilities, then q
   __shared__ uint32_t marks[SPAN / 4];           // of SPAN pieces
@@ -142,7 +130,8 @@ void distill_row(DistillArgs a) {
   __shared__ int twice, bad;
   typedef typename Row<T>::type type;
   const long long row = blockIdx.x;
-  const int t = threadIdx.x, K = a.k;
+  const int t = threadIdx.x, wave = t >> 6, K = a.k;
+  const int list_waves = K < THREADS ? (K + 63) >> 6 : W;   // the waves with a part of the list
   const T* z = (const T*)a.z + row * a.zs;
   T* dz = GRAD ? (T*)a.dz + row * a.ds : nullptr;
   const Row<T> r(z, a.classes);
@@ -177,19 +166,15 @@ void distill_row(DistillArgs a) {
     twice = bad = 0;
   }
   for (int i = t; i < SPAN / 4 && 4 * i < r.pieces; i += THREADS) marks[i] = 0;
-  if (t < 48) parts[t] = {-INF, 0.f};
   __syncthreads();
   // the list; entries that are left out have no class
-  Part tp = {-INF, 0.f};
+  float most_t = -INF;
   auto entry = [&](int j, long long c, float q) {
     const bool in = c >= 0 && c < a.classes;
     if (!in && c != a.ignore) bad = 1;
     ids[j] = in ? (int)c : -1;
     ts[j] = in ? q : -INF;
-    if (in) {   // a NaN ends in the sum
-      if (REST) tp = {0.f, tp.s + natural_exp(q)};
-      else tp = join(tp, {fmaxf(q, -INF), q == -INF ? 0.f : q - q + 1.f}, LOG2E);
-    }
+    if (!REST && in) most_t = maximum(most_t, q);
     return in;
   };
   if (t < K && entry(t, c0, q0)) z0 = (float)z[c0];
@@ -209,48 +194,35 @@ void distill_row(DistillArgs a) {
         else firsts |= 1u << it;
       }
     }
-    __syncthreads();
   };
   const uint8_t* byte_marks = (const uint8_t*)marks;
-  Part p = {-INF, 0.f};
-  mark_list(0);
-  const bool edge_in = ec >= 0 && !(REST && edge_marks >> t & 1);
-  if (edge_in) p.m = fmaxf(ex, -INF);
+  auto without_listed = [&](i32x4 v, uint32_t listed) {
+    type e = __builtin_bit_cast(type, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (listed >> j & 1) e[j] = (T)-INF;
+    return __builtin_bit_cast(i32x4, e);
+  };
+  bool edge_in = ec >= 0;
+  if (REST || !HELD) {
+    mark_list(0);
+    __syncthreads();
+    if (REST) edge_in = ec >= 0 && !(edge_marks >> t & 1);
+  }
+  Part p = {edge_in ? ex : -INF, 0.f};
   if constexpr (HELD > 0) {
     if constexpr (REST) {
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
         const int i = k * THREADS + t;
         const uint32_t listed = i < r.pieces ? byte_marks[i] : 0;
-        if (listed) {
-          type v = __builtin_bit_cast(type, x[k]);
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (listed >> j & 1) v[j] = (T)-INF;
-          x[k] = __builtin_bit_cast(i32x4, v);
-        }
+        if (listed) x[k] = without_listed(x[k], listed);
       }
       repack(x);
     }
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      if (k * THREADS + t < r.pieces) {
-        const type v = __builtin_bit_cast(type, x[k]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) p.m = fmaxf(p.m, (float)v[j]);
-      }
-    }
-    repack(x);
-    const float m0 = p.m == -INF ? 0.f : p.m;
-    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - m0) * a.c2);
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      if (k * THREADS + t < r.pieces) {
-        const type v = __builtin_bit_cast(type, x[k]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) p.s += __builtin_amdgcn_exp2f(((float)v[j] - m0) * a.c2);
-      }
-    }
+    for (int k = 0; k < HELD; ++k)
+      if (k * THREADS + t < r.pieces) p.m = maximum(p.m, piece_max<T>(x[k]));
     repack(x);
   } else {
     if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - (p.m == -INF ? 0.f : p.m)) * a.c2);
@@ -261,13 +233,14 @@ void distill_row(DistillArgs a) {
         for (int i = t; i < (last - first + 3) / 4; i += THREADS) marks[i] = 0;
         __syncthreads();
         mark_list(first);
+        __syncthreads();
       }
       for (int i0 = first + t; i0 < last; i0 += AHEAD * THREADS) {
-        type v[AHEAD];
+        i32x4 v[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          v[k] = *(const type*)(z + r.piece_class(i < last ? i : i0));
+          v[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i < last ? i : i0)));
         }
         float m = p.m;
 #pragma unroll
@@ -275,14 +248,9 @@ void distill_row(DistillArgs a) {
           const int i = i0 + k * THREADS < last ? i0 + k * THREADS : i0;
           if (REST) {
             const uint32_t listed = byte_marks[i - first];
-            if (listed) {
-#pragma unroll
-              for (int j = 0; j < N; ++j)
-                if (listed >> j & 1) v[k][j] = (T)-INF;
-            }
+            if (listed) v[k] = without_listed(v[k], listed);
           }
-#pragma unroll
-          for (int j = 0; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
+          m = maximum(m, piece_max<T>(v[k]));
         }
         rescale(p, m, a.c2);
         const float m0 = m == -INF ? 0.f : m;
@@ -291,41 +259,70 @@ void distill_row(DistillArgs a) {
           if (i0 + k * THREADS < last) {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-              p.s += __builtin_amdgcn_exp2f(((float)v[k][j] - m0) * a.c2);
+              p.s += __builtin_amdgcn_exp2f((element<T>(v[k], j) - m0) * a.c2);
           }
       }
     }
   }
-  // every wave joins the waves' parts in the same way
-  p = wave_join(p, a.c2, 64);
-  const int wave = t >> 6, lane = t & 63;
-  if (lane == 0) parts[ROW_PART + wave] = p;
-  if ((t & ~63) < K) {   // waves with a part of the list
+  const float wave_m = wave_max(p.m);
+  if ((t & 63) == 0) row_max[wave] = wave_m;
+  if (wave < list_waves) {
     if (t < K) zs[t] = z0;
-    Part lp = {-INF, 0.f};
+    float most_l = -INF;
     if (REST) {
       int it = 0;
-      for (int j = t; j < K; j += THREADS, ++it) {
-        const float v = zs[j];
-        if (firsts >> it & 1)
-          lp = join(lp, {fmaxf(v, -INF), v == -INF ? 0.f : v - v + 1.f}, a.c2);
-      }
-      lp = wave_join(lp, a.c2, 64);
+      for (int j = t; j < K; j += THREADS, ++it)
+        if (firsts >> it & 1) most_l = maximum(most_l, zs[j]);
+      most_l = wave_max(most_l);
+    } else {
+      most_t = wave_max(most_t);
     }
-    tp = wave_join(tp, LOG2E, 64);
-    if (lane == 0) {
-      parts[LIST_PART + wave] = lp;
-      parts[TEACHER_PART + wave] = tp;
-    }
+    if ((t & 63) == 0) (REST ? list_max : teacher_max)[wave] = REST ? most_l : most_t;
   }
   __syncthreads();
-  Part all = wave_join(lane < 48 ? parts[lane] : Part{-INF, 0.f},
-                       lane < TEACHER_PART ? a.c2 : LOG2E, 16);
-  p = part_of(all, ROW_PART);
-  const Part lp = part_of(all, LIST_PART);
-  tp = part_of(all, TEACHER_PART);
-  all = REST ? join(p, lp, a.c2) : p;
-  const float tm = REST ? 0.f : tp.m, qsum = tp.s;
+  const float m = waves_max(row_max, W), m0 = m == -INF ? 0.f : m;
+  const float ml = REST ? waves_max(list_max, list_waves) : -INF;
+  const float tm = REST ? 0.f : waves_max(teacher_max, list_waves);
+  if constexpr (HELD > 0) {
+    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - m0) * a.c2);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      if (k * THREADS + t < r.pieces) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          p.s += __builtin_amdgcn_exp2f((element<T>(x[k], j) - m0) * a.c2);
+      }
+    }
+    repack(x);
+  } else {
+    rescale(p, m, a.c2);
+  }
+  const float wave_s = wave_sum(p.s);
+  if ((t & 63) == 0) row_sum[wave] = wave_s;
+  if (wave < list_waves) {
+    if (!REST && HELD && GRAD) mark_list(0);
+    float sl = 0.f, st = 0.f;
+    int it = 0;
+    for (int j = t; j < K; j += THREADS, ++it) {
+      if (REST && firsts >> it & 1)
+        sl += ml == -INF ? 0.f : __builtin_amdgcn_exp2f((zs[j] - ml) * a.c2);
+      if (ids[j] >= 0) st += natural_exp(ts[j] - tm);
+    }
+    st = wave_sum(st);
+    if (REST) sl = wave_sum(sl);
+    if ((t & 63) == 0) teacher_sum[wave] = st;
+    if ((t & 63) == 0) list_sum[wave] = sl;
+  }
+  __syncthreads();
+  p = {m, waves_sum(row_sum, W)};
+  const float qsum = waves_sum(teacher_sum, list_waves);
+  Part all = p;
+  if (REST) {
+    all.m = maximum(m, ml);
+    const float sl = waves_sum(list_sum, list_waves);
+    all.s = (m == -INF ? 0.f : p.s * __builtin_amdgcn_exp2f((m - all.m) * a.c2)) +
+            (ml == -INF ? 0.f : sl * __builtin_amdgcn_exp2f((ml - all.m) * a.c2));
+  }
   // coefficients
   const float log_s = natural_log(all.s);
   const float left = REST ? fmaxf(1.f - qsum, 0.f) : 0.f;
@@ -336,13 +333,13 @@ void distill_row(DistillArgs a) {
   st.ws = w / all.s;
   st.tm = tm;
   st.qs = REST ? 1.f : 1.f / qsum;
-  st.ref = p.m == -INF ? 0.f : p.m;
+  st.ref = m0;
   st.coef = st.ws;
   if (REST) {
-    st.coef = st.ws * (p.m == -INF ? 0.f : __builtin_amdgcn_exp2f((p.m - all.m) * a.c2));
+    st.coef = st.ws * (m == -INF ? 0.f : __builtin_amdgcn_exp2f((m - all.m) * a.c2));
     if (left > 0.f && p.s > 0.f) st.coef -= left / p.s;
   }
-  if ((t & ~63) < K) {
+  if (wave < list_waves) {
     float loss = 0.f;
     const float log_q = REST ? 0.f : natural_log(qsum);
     for (int j = t; j < K; j += THREADS) {
@@ -351,9 +348,8 @@ void distill_row(DistillArgs a) {
       if (!(q <= 0.f)) loss += q * ((ts[j] - tm - log_q) - ((zs[j] - all.m) * a.itau - log_s));
       ts[j] = q;
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) loss += __shfl_xor(loss, d);
-    if (lane == 0) sums[wave] = loss;
+    loss = wave_sum(loss);
+    if ((t & 63) == 0) losses[wave] = loss;
   }
   if (GRAD) {
     const float g = a.gscale / (a.count ? *a.count : 1.f);
@@ -363,11 +359,10 @@ void distill_row(DistillArgs a) {
       for (int k = 0; k < HELD; ++k) {
         const int i = k * THREADS + t;
         if (i < r.pieces) {
-          const type v = __builtin_bit_cast(type, x[k]);
           type d;
 #pragma unroll
           for (int j = 0; j < N; ++j)
-            d[j] = (T)(__builtin_amdgcn_exp2f(((float)v[j] - st.ref) * a.c2) * coef);
+            d[j] = (T)(__builtin_amdgcn_exp2f((element<T>(x[k], j) - st.ref) * a.c2) * coef);
           *(type*)(dz + r.piece_class(i)) = d;
         }
       }
@@ -408,10 +403,10 @@ void distill_row(DistillArgs a) {
     __syncthreads();
   }
   if (t == 0) {
-    float loss = sums[0];
-    for (int i = 1; i < W && i * 64 < K; ++i) loss += sums[i];
+    float loss = losses[0];
+    for (int i = 1; i < list_waves; ++i) loss += losses[i];
     if (REST && left > 0.f)
-      loss += left * (natural_log(left) - ((p.m - all.m) * a.itau + natural_log(p.s) - log_s));
+      loss += left * (natural_log(left) - ((m - all.m) * a.itau + natural_log(p.s) - log_s));
     a.row_loss[row] = w == w ? loss * a.lscale : w;
     if (a.stats) a.stats[row] = st.ref;
     if (a.stats) a.stats[a.rows + row] = st.coef;

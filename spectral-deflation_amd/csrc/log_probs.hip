@@ -13,8 +13,6 @@
 // The largest classes go by the logits themselves, ties by the lower class; -0 and 0 are equal.
 // A row whose token is `ignore` gives 0 everywhere and `ignore` for its classes.  A row without a
 // softmax (a NaN, an infinity, -inf alone) gives NaN and the classes 0 to K - 1.
-#include <type_traits>
-
 #include "rows.h"
 
 namespace dmh {
@@ -48,28 +46,6 @@ __device__ __forceinline__ void rescale(Part3& p, float m, float c2) {
     p.m = m;
   }
 }
-__device__ __forceinline__ Part3 join(Part3 a, Part3 b, float c2) {
-  const float m = fmaxf(a.m, b.m);
-  rescale(a, m, c2);
-  rescale(b, m, c2);
-  return {m, a.s + b.s, a.t + b.t};
-}
-template <int THREADS>
-__device__ __forceinline__ Part3 block_join(Part3 p, float c2, Part3* lds) {
-#pragma unroll
-  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
-    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d), __shfl_xor(p.t, d)}, c2);
-  constexpr int W = THREADS / 64;
-  if (W <= 1) return p;
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
-  __syncthreads();
-  p = (threadIdx.x & 63) < W ? lds[threadIdx.x & 63] : Part3{-INF, 0.f, 0.f};
-#pragma unroll
-  for (int d = W / 2; d; d >>= 1)
-    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d), __shfl_xor(p.t, d)}, c2);
-  return {__shfl(p.m, 0), __shfl(p.s, 0), __shfl(p.t, 0)};
-}
-
 // ---- the largest classes ----------------------------------------------------------------------
 typedef unsigned long long u64;
 
@@ -86,10 +62,37 @@ __device__ __forceinline__ u64 rank_key(float x, int c) {
   return (u64)order_key(x) << 32 | (uint32_t)~c;
 }
 
+// The largest of each of HELD pieces, for later: two 16-bit values a register, while fp32 ones are found again from
+// the piece, in three instructions.
+template <class T, int HELD>
+struct PieceMaxima {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  int m[HELD ? HELD / 2 : 1];
+  __device__ __forceinline__ void put(int k, float even, float odd) {   // of pieces k and k + 1
+    if constexpr (std::is_same<T, bf16>::value)
+      m[k / 2] = (int)__builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, odd),
+                                            __builtin_bit_cast(uint32_t, even), 0x07060302u);
+    else
+      m[k / 2] = __builtin_bit_cast(int, pair{(T)even, (T)odd});
+  }
+  __device__ __forceinline__ float get(int k, i32x4) const {
+    return element<T>(i32x4{m[k / 2], 0, 0, 0}, k & 1);
+  }
+};
+template <int HELD>
+struct PieceMaxima<float, HELD> {
+  __device__ __forceinline__ void put(int, float, float) {}
+  __device__ __forceinline__ float get(int, i32x4 x) const { return piece_max<float>(x); }
+};
+// What a value with an order_key of at least cut is at least.
+__device__ __forceinline__ float cut_value(uint32_t cut) {
+  return cut < 0x007FFFFFu ? -INF : key_value(cut);
+}
+
 constexpr int CANDS = 1024;   // what is sorted out in the end, K <= TOP_MAX of them kept
 
 struct TopLds {
-  uint32_t keys[1024];   // of groups of threads
+  uint32_t keys[512];   // of groups of threads
   u64 cand[CANDS];
   uint32_t cut, most;
   int slots[64];         // a counter for each step of the search over all classes
@@ -109,6 +112,7 @@ __device__ __forceinline__ void group_cut(int K, TopLds& l) {
   }
   const int enough = K + K / 4 + 4;
   uint32_t cut = 0;
+  __builtin_amdgcn_s_setprio(3);   // the others wait for this one in the end
   for (int b = 31; b >= 0; --b) {
     const uint32_t c = cut | 1u << b;
     int n = 0;
@@ -130,17 +134,18 @@ __device__ __forceinline__ void group_cut(int K, TopLds& l) {
   }
 }
 
-// The threads' maxima by groups: as many groups as hold four times K apart, up to one a thread.
+// The threads' maxima by groups: 256, or 512 for more than 64 classes.  (Of 256 and K = 64, about
+// 74 classes are as large as the 64th group's; of 512 and K = 256, about 355.)
 template <int THREADS>
 __device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
   uint32_t k = order_key(largest), o;
   int t = threadIdx.x;
-  if (THREADS == 1024 && K <= 128) {
-    o = __shfl_xor(k, 1);
+  if (THREADS == 1024) {
+    o = __builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true);   // lane ^ 1
     k = o > k ? o : k;
     t >>= 1;
     if (K <= 64) {
-      o = __shfl_xor(k, 2);
+      o = __builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true);   // lane ^ 2
       k = o > k ? o : k;
       t >>= 1;
     }
@@ -152,60 +157,81 @@ __device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
 template <int THREADS>
 __device__ __forceinline__ void find_cut(int K, TopLds& l) {
   if (THREADS == 256 || K <= 64) group_cut<4>(K, l);
-  else if (K <= 128) group_cut<THREADS == 1024 ? 8 : 4>(K, l);
-  else group_cut<THREADS / 64>(K, l);
+  else group_cut<8>(K, l);
 }
 
-// The candidates, CANDS at most and the K largest among them, behind a barrier that follows
-// find_cut.  each(cut, f) calls f(value, class) for all classes of the thread whose order_key is at
-// least cut, and may for others; each_once is the same for one call.
-template <int THREADS, class Each, class Again>
-__device__ __forceinline__ void gather_top(int K, int classes, const Each& each_once,
-                                           const Again& each, TopLds& l) {
-  u64 from = (u64)l.cut << 32;
-  auto gather = [&](const auto& each) {
-    each((uint32_t)(from >> 32), [&](float v, int c) {
-      const u64 k = rank_key(v, c);
-      if (k >= from) {
-        const int at = atomicAdd(&l.n, 1);
-        if (at < CANDS) l.cand[at] = k;
-      }
-    });
-    __syncthreads();
-  };
-  gather(each_once);
-  if (l.n > CANDS) {
-    // Many large classes in few groups, or many equal ones: a bit at a time over all classes.
-    // The K-th largest is between cut and the largest: the bits that these two share need no
-    // step, nor do a class's bits above those of the last one.
-    const uint32_t cut = l.cut, most = l.most;
-    const int high = cut == most ? -1 : 31 - __clz(cut ^ most);
-    const int low = 32 - __clz(classes);   // classes < 2^low
-    from = (u64)(high < 0 ? most : most & ~((2u << high) - 1u)) << 32;
-    if (high < 0) from |= ~((1u << low) - 1u);
-    int step = 0;
-    for (int b = high < 0 ? low - 1 : 32 + high; b >= 0; --b) {
-      if (b == 31) {   // all classes share these
-        from |= ~((1u << low) - 1u);
-        b = low - 1;
-      }
-      const u64 c = from | 1ull << b;
-      int n = 0;
-      each((uint32_t)(c >> 32), [&](float v, int i) { n += rank_key(v, i) >= c; });
-#pragma unroll
-      for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-      if ((threadIdx.x & 63) == 0 && n) atomicAdd(&l.slots[step], n);
-      __syncthreads();
-      n = l.slots[step++];
-      if (n >= K) {
-        from = c;
-        if (n <= CANDS) break;
-      }
-    }
-    if (threadIdx.x == 0) l.n = 0;
-    __syncthreads();
-    gather(each);
+// A candidate from each lane that has one; all lanes of the wave come here.
+__device__ __forceinline__ void put_candidate(bool has, u64 key, TopLds& l) {
+  const u64 who = __ballot(has);
+  if (who == 0) return;
+  int at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(&l.n, __popcll(who));
+  at = __builtin_amdgcn_readfirstlane(at) +
+       __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                 __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+  if (has && at < CANDS) l.cand[at] = key;
+}
+
+// Pieces with a class that is large enough, gathered by a wave, 64 at most: their elements side by side in the
+// lanes, 64 at a time.
+struct PieceList {
+  i32x4 data[64];
+  int first[64];   // class of a piece's first element
+};
+template <class T>
+__device__ __forceinline__ void put_pieces(int count, u64 from, const PieceList& p, TopLds& l) {
+  constexpr int N = Piece<T>::N;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int e = threadIdx.x & 63; (e & ~63) < count * N; e += 64) {
+    const bool in = e < count * N;
+    const int q = in ? e : 0;
+    const u64 k = rank_key((float)((const T*)p.data)[q], p.first[q / N] + q % N);
+    put_candidate(in && k >= from, k, l);
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Where more than CANDS classes are above the cut (many large ones in few groups, or many equal
+// ones): the candidates by a bit at a time over all classes.  The K-th largest is between cut and
+// the largest: the bits that these two share need no step, nor do a class's bits above those of the
+// last one.  each(cut, f) calls f(value, class) for all classes of the thread whose order_key is
+// at least cut, and may for others.
+template <int THREADS, class Each>
+__device__ __forceinline__ void search_top(int K, int classes, const Each& each, TopLds& l) {
+  const uint32_t cut = l.cut, most = l.most;
+  const int high = cut == most ? -1 : 31 - __clz(cut ^ most);
+  const int low = 32 - __clz(classes);   // classes < 2^low
+  const uint32_t shared = ~((1u << low) - 1u);
+  u64 from = (u64)(high < 0 ? most : most & ~((2u << high) - 1u)) << 32;
+  if (high < 0) from |= shared;
+  int step = 0;
+  for (int b = high < 0 ? low - 1 : 32 + high; b >= 0; --b) {
+    if (b == 31) {
+      from |= shared;
+      b = low - 1;
+    }
+    const u64 c = from | 1ull << b;
+    int n = 0;
+    each((uint32_t)(c >> 32), [&](float v, int i) { n += rank_key(v, i) >= c; });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
+    if ((threadIdx.x & 63) == 0 && n) atomicAdd(&l.slots[step], n);
+    __syncthreads();
+    n = l.slots[step++];
+    if (n >= K) {
+      from = c;
+      if (n <= CANDS) break;
+    }
+  }
+  if (threadIdx.x == 0) l.n = 0;
+  __syncthreads();
+  each((uint32_t)(from >> 32), [&](float v, int c) {
+    const u64 k = rank_key(v, c);
+    if (k >= from) l.cand[atomicAdd(&l.n, 1)] = k;
+  });
+  __syncthreads();
 }
 
 // The K largest candidates in their order: put(place, value, class).  A candidate's place is the
@@ -219,6 +245,7 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
   for (int i = threadIdx.x / share; i < n; i += THREADS / share) {
     const u64 k = l.cand[i];
     int before = 0;
+#pragma unroll 4
     for (int j = part; j < n; j += share) before += l.cand[j] > k;
     for (int d = share >> 1; d; d >>= 1) before += __shfl_xor(before, d);
     if (part == 0 && before < K) put(before, key_value((uint32_t)(k >> 32)), (int)~(uint32_t)k);
@@ -228,9 +255,11 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
 // One row by THREADS threads that hold it in registers, HELD pieces each (packed between the
 // steps), or for HELD = 0 a workgroup that streams it.
 template <class T, int THREADS, int HELD, bool TOP>
-__global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
-  __shared__ Part3 parts[16];
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(LogProbArgs a) {
+  __shared__ float maxes[16], sums[16], weights[16];   // of the waves
   __shared__ typename std::conditional<TOP, TopLds, char>::type top;
+  __shared__ typename std::conditional<(TOP && HELD > 0), PieceList, char>::type
+      lists[TOP && HELD ? THREADS / 64 : 1];
   constexpr int N = Piece<T>::N, AHEAD = 4;
   typedef typename Row<T>::type type;
   const long long row = blockIdx.x;
@@ -260,28 +289,36 @@ __global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
   }
   const bool known = a.tokens && y >= 0 && y < a.classes;
   const float zy = known ? (float)z[y] : __builtin_nanf("");
-  Part3 p = {fmaxf(ex, -INF), 0.f, 0.f};
+  Part3 p = {ex, 0.f, 0.f};
+  // (a logit of -inf gives 0 * -inf in t, a NaN, which the end mends)
   auto add = [&](float v, float m0) {
     const float d = (v - m0) * a.c2, e = __builtin_amdgcn_exp2f(d);
     p.s += e;
-    p.t = fmaf(e, fmaxf(d, LOWEST), p.t);
+    p.t = fmaf(e, d, p.t);
+  };
+  PieceMaxima<T, HELD> maxima;
+  float m = 0.f, largest = 0.f;   // of the row and of the thread
+  auto join_max = [&]() {
+    largest = p.m;
+    const float w = wave_max(p.m);
+    if ((t & 63) == 0) maxes[t >> 6] = w;
+    if constexpr (TOP) put_group<THREADS>(K, p.m, top);
+    __syncthreads();
+    if constexpr (TOP)
+      if (t < 64) find_cut<THREADS>(K, top);
+    m = waves_max(maxes, THREADS / 64);
   };
   if constexpr (HELD > 0) {
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      if (k * THREADS + t < r.pieces) {
-        const type v = __builtin_bit_cast(type, x[k]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) p.m = fmaxf(p.m, (float)v[j]);
-      }
+    for (int k = 0; k < HELD; k += 2) {
+      const float m0 = k * THREADS + t < r.pieces ? piece_max<T>(x[k]) : -INF;
+      const float m1 = (k + 1) * THREADS + t < r.pieces ? piece_max<T>(x[k + 1]) : -INF;
+      p.m = maximum(p.m, maximum(m0, m1));
+      if constexpr (TOP) maxima.put(k, m0, m1);
     }
     repack(x);
-    if constexpr (TOP) {
-      put_group<THREADS>(K, p.m, top);
-      __syncthreads();
-      if (t < 64) find_cut<THREADS>(K, top);
-    }
-    const float m0 = p.m == -INF ? 0.f : p.m;
+    join_max();
+    const float m0 = m == -INF ? 0.f : m;
     if (ec >= 0) add(ex, m0);
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
@@ -301,13 +338,12 @@ __global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
         const int i = i0 + k * THREADS;
         v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
       }
-      float m = p.m;
+      float most = p.m;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
-#pragma unroll
-        for (int j = 0; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
-      rescale(p, m, a.c2);
-      const float m0 = m == -INF ? 0.f : m;
+        most = maximum(most, piece_max<T>(__builtin_bit_cast(i32x4, v[k])));
+      rescale(p, most, a.c2);
+      const float m0 = most == -INF ? 0.f : most;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
         if (i0 + k * THREADS < r.pieces) {
@@ -315,14 +351,32 @@ __global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
           for (int j = 0; j < N; ++j) add((float)v[k][j], m0);
         }
     }
-    if constexpr (TOP) {
-      put_group<THREADS>(K, p.m, top);
-      __syncthreads();
-      if (t < 64) find_cut<THREADS>(K, top);
+    join_max();
+    rescale(p, m, a.c2);
+  }
+  if (!(p.t == p.t)) {   // the thread's sums again, its logits of -inf apart
+    p.s = p.t = 0.f;
+    const float m0 = m == -INF ? 0.f : m;
+    auto again = [&](float v) {
+      const float d = (v - m0) * a.c2, e = __builtin_amdgcn_exp2f(d);
+      p.s += e;
+      p.t = fmaf(e, fmaxf(d, LOWEST), p.t);
+    };
+    if (r.edge(t) >= 0) again((float)z[r.edge(t)]);
+    for (int i = t; i < r.pieces; i += THREADS) {
+      const type v = *(const type*)(z + r.piece_class(i));
+#pragma unroll
+      for (int j = 0; j < N; ++j) again((float)v[j]);
     }
   }
-  const float largest = p.m;
-  p = block_join<THREADS>(p, a.c2, parts);
+  const float ws = wave_sum(p.s), wt = wave_sum(p.t);
+  if ((t & 63) == 0) {
+    sums[t >> 6] = ws;
+    weights[t >> 6] = wt;
+  }
+  if (TOP && t < 64) __builtin_amdgcn_s_setprio(0);
+  __syncthreads();
+  p = {m, waves_sum(sums, THREADS / 64), waves_sum(weights, THREADS / 64)};
   const float log_s = __builtin_amdgcn_logf(p.s) * LN2;
   if (t == 0) {
     const float ent = log_s - LN2 * (p.t / p.s);
@@ -340,9 +394,10 @@ __global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
       }
       return;
     }
-    auto reread = [&](uint32_t cut, auto f) {
+    // (by value: what a lambda refers to may end in memory)
+    auto each = [=](uint32_t cut, auto f) {
       if (order_key(largest) < cut) return;
-      if (ec >= 0) f(ex, ec);
+      if (r.edge(t) >= 0) f((float)z[r.edge(t)], r.edge(t));
       for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
         type v[AHEAD];
 #pragma unroll
@@ -353,38 +408,53 @@ __global__ __launch_bounds__(THREADS, 8) void log_prob_row(LogProbArgs a) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          float m = (float)v[k][0];
-#pragma unroll
-          for (int j = 1; j < N; ++j) m = fmaxf(m, (float)v[k][j]);
-          if (i < r.pieces && order_key(m) >= cut) {
+          if (i < r.pieces && piece_max<T>(__builtin_bit_cast(i32x4, v[k])) >= cut_value(cut)) {
 #pragma unroll
             for (int j = 0; j < N; ++j) f((float)v[k][j], r.piece_class(i) + j);
           }
         }
       }
     };
-    auto held = [&](uint32_t cut, auto f) {
-      if (order_key(largest) < cut) return;
-      if (ec >= 0) f(ex, ec);
+    const uint32_t cut = top.cut;
+    const u64 from = (u64)cut << 32;
+    if constexpr (HELD > 0) {
+      PieceList& list = lists[t >> 6];
+      const float least = cut_value(cut);
+      if (t < 64) {   // (read again: it would wait in a register all the time)
+        const int c = r.edge(t);
+        const u64 key = c >= 0 ? rank_key((float)z[c], c) : 0;
+        put_candidate(key != 0 && key >= from, key, top);
+      }
+      int count = 0;
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
-        const int i = k * THREADS + t;
-        int c = r.piece_class(i);
-        asm volatile("" : "+v"(x[k]), "+v"(c));   // nothing unpacked waits in registers
-        const type v = __builtin_bit_cast(type, x[k]);
-        float m = (float)v[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) m = fmaxf(m, (float)v[j]);
-        if (i < r.pieces && order_key(m) >= cut) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) f((float)v[j], c + j);
+        const bool has = k * THREADS + t < r.pieces && maxima.get(k, x[k]) >= least;
+        const u64 who = __ballot(has);
+        if (who) {
+          const int at = count + __builtin_amdgcn_mbcnt_hi(
+              (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+          if (has && at < 64) {
+            list.data[at] = x[k];
+            list.first[at] = r.piece_class(k * THREADS + t);
+          }
+          count += __popcll(who);
         }
       }
-    };
-    if constexpr (HELD > 0)
-      gather_top<THREADS>(K, a.classes, held, reread, top);
-    else
-      gather_top<THREADS>(K, a.classes, reread, reread, top);
+      if (count <= 64)
+        put_pieces<T>(count, from, list, top);
+      else if ((t & 63) == 0)
+        atomicAdd(&top.n, CANDS + 1);   // more than this wave's list holds: search_top
+    } else {
+      each(cut, [&](float v, int c) {
+        const u64 k = rank_key(v, c);
+        if (k >= from) {
+          const int at = atomicAdd(&top.n, 1);
+          if (at < CANDS) top.cand[at] = k;
+        }
+      });
+    }
+    __syncthreads();
+    if (top.n > CANDS) search_top<THREADS>(K, a.classes, each, top);
     put_top<THREADS>(K, [&](int place, float v, int c) {
       a.top_lp[row * K + place] = (v - p.m) * a.itau - log_s;
       a.top_ids[row * K + place] = c;

@@ -2,6 +2,8 @@
 // of a vocabulary share.
 #pragma once
 
+#include <type_traits>
+
 #include "train_ops.h"
 
 namespace dmh {
@@ -9,6 +11,8 @@ namespace dmh {
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 constexpr float INF = __builtin_inff();
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // exp(x - m) by the hardware's 2^x (results below 2^-126 are zero)
 __device__ __forceinline__ float exp_diff(float x, float m) {
@@ -66,25 +70,51 @@ __device__ __forceinline__ void rescale(Part& p, float m, float c2) {
     p.m = m;
   }
 }
-__device__ __forceinline__ Part join(Part a, Part b, float c2) {
-  const float m = fmaxf(a.m, b.m);
-  rescale(a, m, c2);
-  rescale(b, m, c2);
-  return {m, a.s + b.s};
+
+// ---- reductions by lane shifts: in the last lane of a row of 16, then of the wave -----------------
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ float shifted(float v, float none) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                         CTRL, ROWS, 0xF, false));
 }
-template <int THREADS>
-__device__ __forceinline__ Part block_join(Part p, float c2, Part* lds) {
-#pragma unroll
-  for (int d = (THREADS < 64 ? THREADS : 64) / 2; d; d >>= 1)
-    p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
-  constexpr int W = THREADS / 64;
-  if (W <= 1) return p;
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = p;
-  __syncthreads();
-  p = (threadIdx.x & 63) < W ? lds[threadIdx.x & 63] : Part{-INF, 0.f};
-#pragma unroll
-  for (int d = W / 2; d; d >>= 1) p = join(p, {__shfl_xor(p.m, d), __shfl_xor(p.s, d)}, c2);
-  return {__shfl(p.m, 0), __shfl(p.s, 0)};
+__device__ __forceinline__ float lane(float v, int i) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
+}
+// (a NaN goes on)
+__device__ __forceinline__ float maximum(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+__device__ __forceinline__ float row16_max(float v) {
+  v = maximum(v, shifted<0x111>(v, -INF));
+  v = maximum(v, shifted<0x112>(v, -INF));
+  v = maximum(v, shifted<0x114>(v, -INF));
+  return maximum(v, shifted<0x118>(v, -INF));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v += shifted<0x111>(v, 0.f);
+  v += shifted<0x112>(v, 0.f);
+  v += shifted<0x114>(v, 0.f);
+  return v + shifted<0x118>(v, 0.f);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = row16_max(v);
+  v = maximum(v, shifted<0x142, 0xA>(v, -INF));
+  return lane(maximum(v, shifted<0x143, 0xC>(v, -INF)), 63);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = row16_sum(v);
+  v += shifted<0x142, 0xA>(v, 0.f);
+  return lane(v + shifted<0x143, 0xC>(v, 0.f), 63);
+}
+// Of the first `waves` waves' values in LDS, behind a barrier, by every wave alike.
+__device__ __forceinline__ float waves_max(const float* lds, int waves) {
+  const int i = threadIdx.x & 15;
+  return lane(row16_max(i < waves ? lds[i] : -INF), 15);
+}
+__device__ __forceinline__ float waves_sum(const float* lds, int waves) {
+  const int i = threadIdx.x & 15;
+  return lane(row16_sum(i < waves ? lds[i] : 0.f), 15);
 }
 
 // A row in aligned pieces of 16 bytes, and the classes before the first and behind the last one,
@@ -115,6 +145,25 @@ struct Row {
   }
 };
 
+// Element j of a piece.  bf16 by its bits: from converted values the compiler makes 16-bit maxima,
+// which it then has to convert back and forth.
+template <class T>
+__device__ __forceinline__ float element(i32x4 x, int j) {
+  if constexpr (std::is_same<T, bf16>::value)
+    return __builtin_bit_cast(float, j & 1 ? x[j / 2] & (int)0xFFFF0000u : x[j / 2] << 16);
+  else
+    return (float)__builtin_bit_cast(typename Piece<T>::type, x)[j];
+}
+// The largest of a piece, or a NaN.  (Packed 16-bit integers would take one and a half instructions
+// for two elements in place of three, and took 4% longer for the whole row.)
+template <class T>
+__device__ __forceinline__ float piece_max(i32x4 x) {
+  float m = element<T>(x, 0);
+#pragma unroll
+  for (int j = 1; j < Piece<T>::N; ++j) m = maximum(m, element<T>(x, j));
+  return m;
+}
+
 // Marks of listed classes in LDS: a byte for each of `count` pieces from `first` on, a bit for each
 // class of a piece, and (edges) a word for the classes before and behind the pieces, bit t that of
 // the class of thread t.  False where class c has no mark here.
@@ -136,7 +185,6 @@ __device__ __forceinline__ bool find_mark(const Row<T>& r, int c, int first, int
 
 // A row that stays packed in registers between the steps: what one has unpacked may not stay there
 // for the next.
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <int HELD>
 __device__ __forceinline__ void repack(i32x4 (&x)[HELD]) {
 #pragma unroll
