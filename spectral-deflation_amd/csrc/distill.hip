@@ -33,65 +33,85 @@ struct DistillArgs {
   const void* teacher;   // (rows, k)
   void* dz;              // or null
   float* row_loss;
+  float* row_has;        // 1 for a row with a teacher, 0 without; or null
   float* stats;          // (6, rows), written (forward; may be null) or read (gradient)
-  const float* count;    // rows that have a teacher, or null
+  const float* counts;   // COUNTS parts of the number of rows that have a teacher, or null
+  int self_count;        // the rows' launch counts them itself
+  const float* count;    // ... their sum (gradient kernel), or null
   const float* gout;     // gradient of the loss (gradient kernel): one, or one a row
   long long rows, zs, ds, ignore;
-  int classes, k, i64, ttype, gout_rows;
+  int classes, k, i64 /* 0 or 1 */, ttype, gout_rows;
   float itau, c2;        // 1 / tau; log2(e) / tau
   float lscale, gscale;  // tau^2; tau times the gradient's scale
 };
 
-__device__ __forceinline__ float load_float(const void* p, int type, long long i) {
-  return type == DMH_F32    ? ((const float*)p)[i]
-         : type == DMH_BF16 ? (float)((const bf16*)p)[i]
-                            : (float)((const fp16*)p)[i];
-}
+// An entry of a list as it is in memory, of any of the types: loaded without a branch, which would
+// wait for the value before the row behind it is on its way.
+struct RawEntry {
+  int lo, hi;             // of the class
+  unsigned short a, b;    // the upper and the lower half of an fp32 value; a 16-bit one, twice
+  __device__ __forceinline__ void load(const DistillArgs& d, long long i) {
+    const int* id = (const int*)d.ids + (i << d.i64);
+    lo = id[0];
+    hi = id[d.i64];
+    const int wide = d.ttype == DMH_F32;
+    const unsigned short* t = (const unsigned short*)d.teacher + (i << wide);
+    a = t[wide];
+    b = t[0];
+  }
+  __device__ __forceinline__ long long id(const DistillArgs& d) const {
+    return (long long)((unsigned long long)(uint32_t)(d.i64 ? hi : lo >> 31) << 32 | (uint32_t)lo);
+  }
+  __device__ __forceinline__ float value(const DistillArgs& d) const {
+    const float f = __builtin_bit_cast(
+        float, (uint32_t)a << 16 | (d.ttype == DMH_F32 ? (uint32_t)b : 0u));
+    return d.ttype == DMH_F16 ? (float)__builtin_bit_cast(fp16, a) : f;
+  }
+};
 
-// The number of rows that have a teacher: their first entries by one workgroup.
-__device__ __forceinline__ float count_rows(const DistillArgs& a, float* lds) {
-  constexpr int AHEAD = 8;
+// A mean's gradient needs the number of rows that have a teacher at the start.  Up to SELF_ROWS
+// every workgroup of the rows' launch counts them itself; else a launch does, by the rows' first
+// entries, which lie k apart: in COUNTS parts, of one workgroup each (8192 rows, k = 64: 16 us by
+// one workgroup alone, 3 by these).
+constexpr int COUNTS = 64, SELF_ROWS = 256;
+
+__device__ __forceinline__ bool has_teacher(const DistillArgs& a, long long row) {
+  RawEntry e;
+  e.load(a, row * a.k);
+  return e.id(a) != a.ignore;
+}
+__global__ __launch_bounds__(256) void distill_count(DistillArgs a, float* counts) {
+  __shared__ float lds[4];
   int n = 0;
-  const int rows = (int)a.rows;
-  auto count = [&](auto* ids) {
-    int i = threadIdx.x;
-    for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) n += ids[(long long)(i + k * 1024) * a.k] != a.ignore;
-    }
-    for (; i < rows; i += 1024) n += ids[(long long)i * a.k] != a.ignore;
-  };
-  if (a.i64) count((const long long*)a.ids); else count((const int*)a.ids);
-  return block_sum<1024>((float)n, lds);   // exact: below 2^24 rows
+  for (long long i = blockIdx.x * 256 + threadIdx.x; i < a.rows; i += COUNTS * 256)
+    n += has_teacher(a, i);
+  const float s = wave_sum((float)n);   // exact: below 2^24 rows
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
 }
 
-__global__ __launch_bounds__(1024) void distill_count(DistillArgs a, float* count) {
-  __shared__ float lds[16];
-  const float n = count_rows(a, lds);
-  if (threadIdx.x == 0) *count = n;
-}
-
-// The sum of the rows' losses, divided by the number of rows with a teacher for a mean, which it
-// counts if no launch before has (COUNT).
-template <bool COUNT>
-__global__ __launch_bounds__(1024) void distill_reduce(DistillArgs a, float* count, float* loss) {
+// The sum of the rows' losses, for a mean divided by the number of rows with a teacher.
+__global__ __launch_bounds__(1024) void distill_reduce(DistillArgs a, float* loss, float* count) {
   __shared__ float lds[16];
   constexpr int AHEAD = 16;
   const int rows = (int)a.rows;
-  float s = 0.f;
-  int i = threadIdx.x;
-  for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
-    float v[AHEAD];
+  auto total = [&](const float* v) {
+    float s = 0.f;
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * 1024 < rows; i += AHEAD * 1024) {
+      float x[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) v[k] = a.row_loss[i + k * 1024];
+      for (int k = 0; k < AHEAD; ++k) x[k] = v[i + k * 1024];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) s += v[k];
-  }
-  for (; i < rows; i += 1024) s += a.row_loss[i];
-  s = block_sum<1024>(s, lds);
-  const float n = COUNT ? count_rows(a, lds) : count ? *count : 1.f;
+      for (int k = 0; k < AHEAD; ++k) s += x[k];
+    }
+    for (; i < rows; i += 1024) s += v[i];
+    return block_sum<1024>(s, lds);
+  };
+  const float s = total(a.row_loss), n = a.row_has ? total(a.row_has) : 1.f;
   if (threadIdx.x == 0) {
-    if (COUNT) *count = n;
+    if (count) *count = n;
     *loss = s / n;
   }
 }
@@ -115,19 +135,21 @@ __device__ __forceinline__ float natural_log(float x) { return __builtin_amdgcn_
 // of the classes says which entry of a class is its first (the others add nothing to the list's
 // sum, and the first writes the gradient), and with REST which logits are not the rest's: they
 // become -inf before the row is summed.
-template <class T, int THREADS, int HELD, bool REST, bool GRAD>
+template <class T, int THREADS, int HELD, bool REST, bool GRAD, bool PAST>
 __global__ __launch_bounds__(THREADS, HELD > 16 ? 2 : HELD > 8 ? 4 : 8)
 void distill_row(DistillArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, W = THREADS / 64;
   constexpr int SPAN = HELD ? HELD * THREADS : 32768;
   // the waves' maxima and sums: of the row, the list, the teacher; their losses
   __shared__ float row_max[16], list_max[16], teacher_max[16];
-  __shared__ float row_sum[16], list_sum[16], teacher_sum[16], losses[16];
+  __shared__ float row_sum[16], list_sum[16], teacher_sum[16], losses[16], counted[16];
   __shared__ int ids[LIST_MAX];
-  __shared__ float zs[LIST_MAX], ts[LIST_MAX];   // the list's logits; log probabilities, then q
-  __shared__ uint32_t marks[SPAN / 4];           // of SPAN pieces
+  // the list's logits; log probabilities, then q
+  __shared__ float zs[LIST_MAX], ts[LIST_MAX];
+  __shared__ __attribute__((aligned(16))) uint32_t marks[SPAN / 4];   // of SPAN pieces
+  __shared__ float edge_logits[16];
   __shared__ uint32_t edge_marks;
-  __shared__ int twice, bad;
+  __shared__ int twice;
   typedef typename Row<T>::type type;
   const long long row = blockIdx.x;
   const int t = threadIdx.x, wave = t >> 6, K = a.k;
@@ -135,52 +157,56 @@ void distill_row(DistillArgs a) {
   const T* z = (const T*)a.z + row * a.zs;
   T* dz = GRAD ? (T*)a.dz + row * a.ds : nullptr;
   const Row<T> r(z, a.classes);
-  const int ec = r.edge(t);
-  const long long named = load_index(a.ids, a.i64, row * K);
+  const int edge = r.edge(t);
+  RawEntry named;
+  named.load(a, row * K);
   // the thread's first entry is on its way before the row, which the list's logits follow
-  long long c0 = a.ignore;
-  float q0 = 0.f, z0 = 0.f;
-  if (t < K) {
-    c0 = load_index(a.ids, a.i64, row * K + t);
-    q0 = load_float(a.teacher, a.ttype, row * K + t);
-  }
+  RawEntry first_entry;
+  first_entry.load(a, row * K + (t < K ? t : 0));
+  float z0 = 0.f;
   i32x4 x[HELD ? HELD : 1] = {};
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int i = k * THREADS + t;
-    if (i < r.pieces) x[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i)));
+    if (i < r.pieces) x[k] = load_piece<T, PAST>(z + r.piece_class(i));
   }
-  const float ex = ec >= 0 ? (float)z[ec] : -INF;
-  if (named == a.ignore) {
+  if (edge >= 0) edge_logits[t] = (float)z[edge];   // (registers are few)
+  if (named.id(a) == a.ignore) {
     if (t == 0) a.row_loss[row] = 0.f;
+    if (t == 0 && a.row_has) a.row_has[row] = 0.f;
     if (t < 6 && a.stats) a.stats[t * a.rows + row] = 0.f;
     if (GRAD) {
       const type zero = {};
       for (int i = t; i < r.pieces; i += THREADS) *(type*)(dz + r.piece_class(i)) = zero;
-      if (ec >= 0) dz[ec] = (T)0.f;
+      if (edge >= 0) dz[edge] = (T)0.f;
     }
     return;
   }
+  // One wave of entries clears the marks that it sets itself, without a barrier.
   if (t == 0) {
     edge_marks = 0;
-    twice = bad = 0;
+    twice = 0;
   }
-  for (int i = t; i < SPAN / 4 && 4 * i < r.pieces; i += THREADS) marks[i] = 0;
-  __syncthreads();
+  const int marking = K <= 64 ? 64 : THREADS;
+  const int words = ((r.pieces < SPAN ? r.pieces : SPAN) + 15) / 16;
+  if (t < marking)
+    for (int i = t; i < words; i += marking) ((i32x4*)marks)[i] = i32x4{0, 0, 0, 0};
+  if ((REST || !HELD) && marking > 64) __syncthreads();
   // the list; entries that are left out have no class
-  float most_t = -INF;
+  float most_t = -INF, bad = 0.f;   // a NaN where a class is outside
   auto entry = [&](int j, long long c, float q) {
     const bool in = c >= 0 && c < a.classes;
-    if (!in && c != a.ignore) bad = 1;
+    if (!in && c != a.ignore) bad = __builtin_nanf("");
     ids[j] = in ? (int)c : -1;
     ts[j] = in ? q : -INF;
     if (!REST && in) most_t = maximum(most_t, q);
     return in;
   };
-  if (t < K && entry(t, c0, q0)) z0 = (float)z[c0];
+  if (t < K && entry(t, first_entry.id(a), first_entry.value(a))) z0 = (float)z[ids[t]];
   for (int j = t + THREADS; j < K; j += THREADS) {
-    const long long c = load_index(a.ids, a.i64, row * K + j);
-    if (entry(j, c, load_float(a.teacher, a.ttype, row * K + j))) zs[j] = (float)z[c];
+    RawEntry e;
+    e.load(a, row * K + j);
+    if (entry(j, e.id(a), e.value(a))) zs[j] = (float)z[ids[j]];
   }
   // the first entry of each class among SPAN pieces from `first` on
   uint32_t firsts = 0;
@@ -203,13 +229,16 @@ void distill_row(DistillArgs a) {
       if (listed >> j & 1) e[j] = (T)-INF;
     return __builtin_bit_cast(i32x4, e);
   };
-  bool edge_in = ec >= 0;
   if (REST || !HELD) {
     mark_list(0);
     __syncthreads();
-    if (REST) edge_in = ec >= 0 && !(edge_marks >> t & 1);
   }
-  Part p = {edge_in ? ex : -INF, 0.f};
+  if (t < K) zs[t] = z0;
+  // the thread's class beside the pieces, if it is the row's
+  auto edge_logit = [&]() {
+    return r.edge(t) < 0 || (REST && edge_marks >> t & 1) ? -INF : edge_logits[t];
+  };
+  Part p = {edge_logit(), 0.f};
   if constexpr (HELD > 0) {
     if constexpr (REST) {
 #pragma unroll
@@ -225,7 +254,7 @@ void distill_row(DistillArgs a) {
       if (k * THREADS + t < r.pieces) p.m = maximum(p.m, piece_max<T>(x[k]));
     repack(x);
   } else {
-    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - (p.m == -INF ? 0.f : p.m)) * a.c2);
+    p.s = __builtin_amdgcn_exp2f((p.m - (p.m == -INF ? 0.f : p.m)) * a.c2);
     for (int first = 0; first < r.pieces; first += SPAN) {
       const int last = first + SPAN < r.pieces ? first + SPAN : r.pieces;
       if (first > 0) {
@@ -240,7 +269,7 @@ void distill_row(DistillArgs a) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          v[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i < last ? i : i0)));
+          v[k] = load_piece<T, PAST>(z + r.piece_class(i < last ? i : i0));
         }
         float m = p.m;
 #pragma unroll
@@ -267,7 +296,6 @@ void distill_row(DistillArgs a) {
   const float wave_m = wave_max(p.m);
   if ((t & 63) == 0) row_max[wave] = wave_m;
   if (wave < list_waves) {
-    if (t < K) zs[t] = z0;
     float most_l = -INF;
     if (REST) {
       int it = 0;
@@ -284,7 +312,7 @@ void distill_row(DistillArgs a) {
   const float ml = REST ? waves_max(list_max, list_waves) : -INF;
   const float tm = REST ? 0.f : waves_max(teacher_max, list_waves);
   if constexpr (HELD > 0) {
-    if (edge_in) p.s = __builtin_amdgcn_exp2f((ex - m0) * a.c2);
+    p.s = __builtin_amdgcn_exp2f((edge_logit() - m0) * a.c2);
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
       if (k * THREADS + t < r.pieces) {
@@ -297,11 +325,17 @@ void distill_row(DistillArgs a) {
   } else {
     rescale(p, m, a.c2);
   }
+  float count = 1.f;
+  if (GRAD && a.counts) count = a.counts[t & 63];
+  if (GRAD && a.self_count) {
+    const float n = wave_sum(t < a.rows && has_teacher(a, t) ? 1.f : 0.f);
+    if ((t & 63) == 0) counted[wave] = n;
+  }
   const float wave_s = wave_sum(p.s);
   if ((t & 63) == 0) row_sum[wave] = wave_s;
   if (wave < list_waves) {
     if (!REST && HELD && GRAD) mark_list(0);
-    float sl = 0.f, st = 0.f;
+    float sl = 0.f, st = bad;
     int it = 0;
     for (int j = t; j < K; j += THREADS, ++it) {
       if (REST && firsts >> it & 1)
@@ -327,7 +361,7 @@ void distill_row(DistillArgs a) {
   const float log_s = natural_log(all.s);
   const float left = REST ? fmaxf(1.f - qsum, 0.f) : 0.f;
   float w = REST ? (qsum <= 1.f ? 1.f : qsum) : qsum / qsum;
-  if (bad || !(all.s >= 0.5f)) w = __builtin_nanf("");
+  if (!(all.s >= 0.5f)) w = __builtin_nanf("");
   RowStats st;
   st.m = all.m;
   st.ws = w / all.s;
@@ -351,52 +385,51 @@ void distill_row(DistillArgs a) {
     loss = wave_sum(loss);
     if ((t & 63) == 0) losses[wave] = loss;
   }
-  if (GRAD) {
-    const float g = a.gscale / (a.count ? *a.count : 1.f);
+  if constexpr (GRAD) {
+    if (a.counts) count = wave_sum(count);
+    if (a.self_count) count = waves_sum(counted, W);
+    const float g = a.gscale / count;
     const float coef = st.coef * g;
+    auto gradient = [&](i32x4 v) {
+      type d;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        d[j] = (T)(__builtin_amdgcn_exp2f((element<T>(v, j) - st.ref) * a.c2) * coef);
+      return __builtin_bit_cast(i32x4, d);
+    };
     if constexpr (HELD > 0) {
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
         const int i = k * THREADS + t;
-        if (i < r.pieces) {
-          type d;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            d[j] = (T)(__builtin_amdgcn_exp2f((element<T>(x[k], j) - st.ref) * a.c2) * coef);
-          *(type*)(dz + r.piece_class(i)) = d;
-        }
+        if (i < r.pieces) store_piece<T, PAST>(dz + r.piece_class(i), gradient(x[k]));
       }
     } else {
       for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
-        type v[AHEAD];
+        i32x4 v[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+          v[k] = load_piece<T, PAST>(z + r.piece_class(i < r.pieces ? i : i0));
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          type d;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            d[j] = (T)(__builtin_amdgcn_exp2f(((float)v[k][j] - st.ref) * a.c2) * coef);
-          if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+          if (i < r.pieces) store_piece<T, PAST>(dz + r.piece_class(i), gradient(v[k]));
         }
       }
     }
-    if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
-    __syncthreads();   // the sums; and the listed classes again, each by one thread
+    if (r.edge(t) >= 0)
+      dz[r.edge(t)] = (T)(__builtin_amdgcn_exp2f((edge_logits[t] - st.ref) * a.c2) * coef);
+    __syncthreads();   // the losses; and the listed classes again, by the first entry of each
     int it = 0;
     for (int j = t; j < K; j += THREADS, ++it) {
       if (firsts >> it & 1) {
-        const int c = ids[j];
         float q = ts[j];
         if (twice) {   // a class listed more than once: its terms in their order
           q = 0.f;
-          for (int i = 0; i < K; ++i) q += ids[i] == c ? ts[i] : 0.f;
+          for (int i = 0; i < K; ++i) q += ids[i] == ids[j] ? ts[i] : 0.f;
         }
-        dz[c] = (T)((__builtin_amdgcn_exp2f((zs[j] - st.m) * a.c2) * st.ws - q) * g);
+        dz[ids[j]] = (T)((__builtin_amdgcn_exp2f((zs[j] - st.m) * a.c2) * st.ws - q) * g);
       }
     }
   } else {
@@ -408,6 +441,7 @@ void distill_row(DistillArgs a) {
     if (REST && left > 0.f)
       loss += left * (natural_log(left) - ((m - all.m) * a.itau + natural_log(p.s) - log_s));
     a.row_loss[row] = w == w ? loss * a.lscale : w;
+    if (a.row_has) a.row_has[row] = 1.f;
     if (a.stats) a.stats[row] = st.ref;
     if (a.stats) a.stats[a.rows + row] = st.coef;
     if (a.stats) a.stats[2 * a.rows + row] = st.m;
@@ -419,15 +453,15 @@ void distill_row(DistillArgs a) {
 
 // The fewest threads that hold a row; longer rows are held for the gradient as far as registers
 // go, and streamed for the loss alone.
-template <class T, bool REST, bool GRAD>
+template <class T, bool REST, bool GRAD, bool PAST>
 static void launch_rows(hipStream_t stream, const DistillArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
   const dim3 rows((unsigned)a.rows);
-#define DMH_ROWS(THREADS, HELD)                                                             \
-  if (pieces <= THREADS * HELD) {                                                           \
-    hipLaunchKernelGGL((distill_row<T, THREADS, HELD, REST, GRAD>), rows, dim3(THREADS), 0, \
-                       stream, a);                                                          \
-    return;                                                                                 \
+#define DMH_ROWS(THREADS, HELD)                                                                   \
+  if (pieces <= THREADS * HELD) {                                                                 \
+    hipLaunchKernelGGL((distill_row<T, THREADS, HELD, REST, GRAD, PAST>), rows, dim3(THREADS), 0, \
+                       stream, a);                                                                \
+    return;                                                                                       \
   }
   DMH_ROWS(256, 8)
   DMH_ROWS(1024, 8)
@@ -436,19 +470,26 @@ static void launch_rows(hipStream_t stream, const DistillArgs& a) {
     DMH_ROWS(512, 48)
   }
 #undef DMH_ROWS
-  hipLaunchKernelGGL((distill_row<T, 1024, 0, REST, GRAD>), rows, dim3(1024), 0, stream, a);
+  hipLaunchKernelGGL((distill_row<T, 1024, 0, REST, GRAD, PAST>), rows, dim3(1024), 0, stream, a);
+}
+template <class T, bool REST, bool GRAD>
+static void launch_sized(hipStream_t stream, const DistillArgs& a) {
+  if (past_caches<T>(a.rows, a.classes))
+    launch_rows<T, REST, GRAD, true>(stream, a);
+  else
+    launch_rows<T, REST, GRAD, false>(stream, a);
 }
 template <class T>
 static void launch_distill(hipStream_t stream, const DistillArgs& a, bool rest) {
   if (rest)
-    a.dz ? launch_rows<T, true, true>(stream, a) : launch_rows<T, true, false>(stream, a);
+    a.dz ? launch_sized<T, true, true>(stream, a) : launch_sized<T, true, false>(stream, a);
   else
-    a.dz ? launch_rows<T, false, true>(stream, a) : launch_rows<T, false, false>(stream, a);
+    a.dz ? launch_sized<T, false, true>(stream, a) : launch_sized<T, false, false>(stream, a);
 }
 
 // The gradient from a forward pass's statistics, element by element, 256 threads for four pieces
 // each of a row; the listed classes are written again behind a barrier.
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;
   __shared__ int ids[LIST_MAX];
@@ -472,11 +513,11 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
     if (ec >= 0) dz[ec] = (T)0.f;
     return;
   }
-  type x[AHEAD];
+  i32x4 x[AHEAD];
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) {
     const int i = i0 + k * THREADS;
-    if (r.pieces) x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : 0));
+    if (r.pieces) x[k] = load_piece<T, PAST>(z + r.piece_class(i < r.pieces ? i : 0));
   }
   const float ex = ec >= 0 ? (float)z[ec] : 0.f;
   RowStats st;
@@ -494,10 +535,12 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
     twice = 0;
   }
   for (int j = t; j < K; j += THREADS) {
-    const long long c = load_index(a.ids, a.i64, row * K + j);
+    RawEntry e;
+    e.load(a, row * K + j);
+    const long long c = e.id(a);
     const bool in = c >= 0 && c < a.classes;
     ids[j] = in ? (int)c : -1;
-    qs[j] = in ? natural_exp(load_float(a.teacher, a.ttype, row * K + j) - st.tm) * st.qs : 0.f;
+    qs[j] = in ? natural_exp(e.value(a) - st.tm) * st.qs : 0.f;
   }
   const float coef = st.coef * g;
 #pragma unroll
@@ -506,8 +549,9 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
     type d;
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      d[j] = (T)(__builtin_amdgcn_exp2f(((float)x[k][j] - st.ref) * a.c2) * coef);
-    if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+      d[j] = (T)(__builtin_amdgcn_exp2f((element<T>(x[k], j) - st.ref) * a.c2) * coef);
+    if (i < r.pieces)
+      store_piece<T, PAST>(dz + r.piece_class(i), __builtin_bit_cast(i32x4, d));
   }
   if (ec >= 0) dz[ec] = (T)(__builtin_amdgcn_exp2f((ex - st.ref) * a.c2) * coef);
   __syncthreads();   // also: the list is written
@@ -539,9 +583,11 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
 template <class T>
 static void launch_distill_grad(hipStream_t stream, const DistillArgs& a) {
   const int whole = a.classes / Piece<T>::N;
-  hipLaunchKernelGGL((distill_grad<T>),
-                     dim3((unsigned)a.rows, (unsigned)(whole ? ceil_div(whole, 1024) : 1)),
-                     dim3(256), 0, stream, a);
+  const dim3 grid((unsigned)a.rows, (unsigned)(whole ? ceil_div(whole, 1024) : 1));
+  if (past_caches<T>(a.rows, a.classes))
+    hipLaunchKernelGGL((distill_grad<T, true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((distill_grad<T, false>), grid, dim3(256), 0, stream, a);
 }
 
 static bool distill_shape(long long rows, long long classes, long long k) {
@@ -587,7 +633,7 @@ int dmh_distill_workspace_size(long long rows, size_t* bytes) {
     set_error("dmh_distill_workspace_size: bad arguments (rows=%lld)", rows);
     return DMH_EINVAL;
   }
-  *bytes = 4 * (size_t)rows;
+  *bytes = 4 * (2 * (size_t)rows + COUNTS);
   return DMH_OK;
 }
 
@@ -617,26 +663,25 @@ int dmh_distill(hipStream_t stream, const void* logits, int dtype, long long row
   }
   const bool mean = reduction == RED_MEAN;
   DistillArgs a = distill_args(logits, rows, classes, z_rstride, ids, ids_64, k, teacher,
-                               teacher_dtype, ignore_index, temperature, stats,
-                               mean ? count : nullptr, dlogits, d_rstride);
+                               teacher_dtype, ignore_index, temperature, stats, nullptr, dlogits,
+                               d_rstride);
   a.row_loss = reduction == RED_NONE ? loss : (float*)ws;
   a.gscale *= grad_scale;
-  // a mean's gradient needs the count at the start, its loss in the end
-  const bool before = mean && dlogits && rows > 0;
-  if (before) {
-    hipLaunchKernelGGL(distill_count, dim3(1), dim3(1024), 0, stream, a, count);
+  if (mean) a.row_has = (float*)ws + rows;
+  if (mean && dlogits && rows > SELF_ROWS) {
+    float* counts = (float*)ws + 2 * rows;
+    hipLaunchKernelGGL(distill_count, dim3(COUNTS), dim3(256), 0, stream, a, counts);
     DMH_CHECK_LAUNCH("distill_count");
+    a.counts = counts;
   }
+  a.self_count = mean && dlogits && rows <= SELF_ROWS;
   if (rows > 0) {
     DMH_FOR_TYPE(dtype, T, (launch_distill<T>(stream, a, rest != 0)))
     DMH_CHECK_LAUNCH("distill_row");
   }
   if (reduction != RED_NONE) {
-    if (mean && !before)
-      hipLaunchKernelGGL(distill_reduce<true>, dim3(1), dim3(1024), 0, stream, a, count, loss);
-    else
-      hipLaunchKernelGGL(distill_reduce<false>, dim3(1), dim3(1024), 0, stream, a,
-                         mean ? count : nullptr, loss);
+    hipLaunchKernelGGL(distill_reduce, dim3(1), dim3(1024), 0, stream, a, loss,
+                       mean ? count : nullptr);
     DMH_CHECK_LAUNCH("distill_reduce");
   }
   return DMH_OK;

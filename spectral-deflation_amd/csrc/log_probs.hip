@@ -89,6 +89,7 @@ __device__ __forceinline__ float cut_value(uint32_t cut) {
   return cut < 0x007FFFFFu ? -INF : key_value(cut);
 }
 
+constexpr int SEGMENTS = 8;   // of a thread's part of a long row, whose maxima are kept
 constexpr int CANDS = 1024;   // what is sorted out in the end, K <= TOP_MAX of them kept
 
 struct TopLds {
@@ -254,12 +255,13 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
 
 // One row by THREADS threads that hold it in registers, HELD pieces each (packed between the
 // steps), or for HELD = 0 a workgroup that streams it.
-template <class T, int THREADS, int HELD, bool TOP>
+template <class T, int THREADS, int HELD, bool TOP, bool PAST>
 __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(LogProbArgs a) {
   __shared__ float maxes[16], sums[16], weights[16];   // of the waves
   __shared__ typename std::conditional<TOP, TopLds, char>::type top;
   __shared__ typename std::conditional<(TOP && HELD > 0), PieceList, char>::type
       lists[TOP && HELD ? THREADS / 64 : 1];
+  __shared__ float segments[TOP && !HELD ? SEGMENTS * THREADS : 1];
   constexpr int N = Piece<T>::N, AHEAD = 4;
   typedef typename Row<T>::type type;
   const long long row = blockIdx.x;
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int i = k * THREADS + t;
-    if (i < r.pieces) x[k] = __builtin_bit_cast(i32x4, *(const type*)(z + r.piece_class(i)));
+    if (i < r.pieces) x[k] = load_piece<T, PAST>(z + r.piece_class(i));
   }
   const int ec = r.edge(t);
   const float ex = ec >= 0 ? (float)z[ec] : -INF;
@@ -287,6 +289,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     }
     return;
   }
+  // a long row's rounds of AHEAD pieces a thread, by segment
+  const int segment_rounds = (r.pieces + AHEAD * THREADS * SEGMENTS - 1) / (AHEAD * THREADS * SEGMENTS);
   const bool known = a.tokens && y >= 0 && y < a.classes;
   const float zy = known ? (float)z[y] : __builtin_nanf("");
   Part3 p = {ex, 0.f, 0.f};
@@ -323,32 +327,44 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
       if (k * THREADS + t < r.pieces) {
-        const type v = __builtin_bit_cast(type, x[k]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) add((float)v[j], m0);
+        for (int j = 0; j < N; ++j) add(element<T>(x[k], j), m0);
       }
     }
     repack(x);
   } else {
     if (ec >= 0) add(ex, p.m == -INF ? 0.f : p.m);
+    int segment = t, left = segment_rounds;
+    if constexpr (TOP)
+      for (int s = 0; s < SEGMENTS; ++s) segments[s * THREADS + t] = -INF;
+    float of_segment = -INF;
     for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
-      type v[AHEAD];
+      i32x4 v[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int i = i0 + k * THREADS;
-        v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+        v[k] = load_piece<T, PAST>(z + r.piece_class(i < r.pieces ? i : i0));
       }
-      float most = p.m;
+      float most = -INF;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        most = maximum(most, piece_max<T>(__builtin_bit_cast(i32x4, v[k])));
+      for (int k = 0; k < AHEAD; ++k) most = maximum(most, piece_max<T>(v[k]));
+      if constexpr (TOP) {
+        of_segment = maximum(of_segment, most);
+        segments[segment] = of_segment;
+        if (--left == 0) {
+          segment += THREADS;
+          left = segment_rounds;
+          of_segment = -INF;
+        }
+      }
+      most = maximum(most, p.m);
       rescale(p, most, a.c2);
       const float m0 = most == -INF ? 0.f : most;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
         if (i0 + k * THREADS < r.pieces) {
 #pragma unroll
-          for (int j = 0; j < N; ++j) add((float)v[k][j], m0);
+          for (int j = 0; j < N; ++j) add(element<T>(v[k], j), m0);
         }
     }
     join_max();
@@ -445,13 +461,42 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       else if ((t & 63) == 0)
         atomicAdd(&top.n, CANDS + 1);   // more than this wave's list holds: search_top
     } else {
-      each(cut, [&](float v, int c) {
+      // every thread goes through those of its own segments that have a large class
+      auto put = [&](float v, int c) {
         const u64 k = rank_key(v, c);
         if (k >= from) {
           const int at = atomicAdd(&top.n, 1);
           if (at < CANDS) top.cand[at] = k;
         }
-      });
+      };
+      const float least = cut_value(cut);
+      if (r.edge(t) >= 0) put((float)z[r.edge(t)], r.edge(t));
+      uint32_t has = 0;
+#pragma unroll
+      for (int s = 0; s < SEGMENTS; ++s)
+        has |= (uint32_t)(segments[s * THREADS + t] >= least) << s;
+      while (has) {
+        const int s = __builtin_ctz(has);
+        has &= has - 1;
+        for (int n = 0; n < segment_rounds; ++n) {
+          const int i0 = t + (s * segment_rounds + n) * AHEAD * THREADS;
+          if (i0 >= r.pieces) break;
+          i32x4 v[AHEAD];
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const int i = i0 + k * THREADS;
+            v[k] = load_piece<T, false>(z + r.piece_class(i < r.pieces ? i : i0));
+          }
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const int i = i0 + k * THREADS;
+            if (i < r.pieces && piece_max<T>(v[k]) >= least) {
+#pragma unroll
+              for (int j = 0; j < N; ++j) put(element<T>(v[k], j), r.piece_class(i) + j);
+            }
+          }
+        }
+      }
     }
     __syncthreads();
     if (top.n > CANDS) search_top<THREADS>(K, a.classes, each, top);
@@ -462,20 +507,23 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
   }
 }
 
-template <class T, bool TOP>
+template <class T, bool TOP, bool PAST>
 static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
   const dim3 rows((unsigned)a.rows);
   if (pieces <= 256 * 8 && a.top <= 128)
-    hipLaunchKernelGGL((log_prob_row<T, 256, 8, TOP>), rows, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((log_prob_row<T, 256, 8, TOP, PAST>), rows, dim3(256), 0, stream, a);
   else if (pieces <= 1024 * 8)
-    hipLaunchKernelGGL((log_prob_row<T, 1024, 8, TOP>), rows, dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((log_prob_row<T, 1024, 8, TOP, PAST>), rows, dim3(1024), 0, stream, a);
   else
-    hipLaunchKernelGGL((log_prob_row<T, 1024, 0, TOP>), rows, dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((log_prob_row<T, 1024, 0, TOP, PAST>), rows, dim3(1024), 0, stream, a);
 }
 template <class T>
 static void launch_log_probs(hipStream_t stream, const LogProbArgs& a) {
-  a.top ? launch_rows<T, true>(stream, a) : launch_rows<T, false>(stream, a);
+  if (past_caches<T>(a.rows, a.classes))
+    a.top ? launch_rows<T, true, true>(stream, a) : launch_rows<T, false, true>(stream, a);
+  else
+    a.top ? launch_rows<T, true, false>(stream, a) : launch_rows<T, false, false>(stream, a);
 }
 
 // ---- gradient -----------------------------------------------------------------------------------
@@ -493,7 +541,7 @@ struct LogProbGradArgs {
 
 // Element by element, 256 threads for four pieces each of a row; the listed classes (the token and
 // the top ones) are written again behind a barrier, each by one thread with the sum of its terms.
-template <class T>
+template <class T, bool PAST>
 __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;
   __shared__ float lds[16];
@@ -519,11 +567,11 @@ __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
     if (ec >= 0) dz[ec] = (T)0.f;
     return;
   }
-  type x[AHEAD];
+  i32x4 x[AHEAD];
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) {
     const int i = i0 + k * THREADS;
-    if (r.pieces) x[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : 0));
+    if (r.pieces) x[k] = load_piece<T, PAST>(z + r.piece_class(i < r.pieces ? i : 0));
   }
   const float ex = ec >= 0 ? (float)z[ec] : 0.f;
   const float m = a.stats[row], s = a.stats[a.rows + row], ent = a.stats[2 * a.rows + row];
@@ -557,8 +605,9 @@ __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
     const int i = i0 + k * THREADS;
     type d;
 #pragma unroll
-    for (int j = 0; j < N; ++j) d[j] = (T)grad((float)x[k][j]);
-    if (i < r.pieces) *(type*)(dz + r.piece_class(i)) = d;
+    for (int j = 0; j < N; ++j) d[j] = (T)grad(element<T>(x[k], j));
+    if (i < r.pieces)
+      store_piece<T, PAST>(dz + r.piece_class(i), __builtin_bit_cast(i32x4, d));
   }
   if (ec >= 0) dz[ec] = (T)grad(ex);
   __syncthreads();   // also: the list is written
@@ -590,9 +639,11 @@ __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
 template <class T>
 static void launch_log_prob_grad(hipStream_t stream, const LogProbGradArgs& a) {
   const int whole = a.classes / Piece<T>::N;
-  hipLaunchKernelGGL((log_prob_grad<T>),
-                     dim3((unsigned)a.rows, (unsigned)(whole ? ceil_div(whole, 1024) : 1)),
-                     dim3(256), 0, stream, a);
+  const dim3 grid((unsigned)a.rows, (unsigned)(whole ? ceil_div(whole, 1024) : 1));
+  if (past_caches<T>(a.rows, a.classes))
+    hipLaunchKernelGGL((log_prob_grad<T, true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((log_prob_grad<T, false>), grid, dim3(256), 0, stream, a);
 }
 
 static bool log_prob_shape(long long rows, long long classes, long long top) {

@@ -145,6 +145,29 @@ struct Row {
   }
 };
 
+// Logits of much more than the last-level cache's 256 MB are read, and their gradient written, as what
+// no cache need keep: 8192 bf16 rows of 50257 with their gradient by distillation in 305 instead
+// of 321 us, in place 283 instead of 332.  (In 103 MB that a cache still holds, 48 instead of 43.)
+template <class T>
+inline bool past_caches(long long rows, long long classes) {
+  return rows * classes * (long long)sizeof(T) >= 384LL << 20;
+}
+// A piece of a row; with PAST as one that the caches need not keep.
+template <class T, bool PAST>
+__device__ __forceinline__ i32x4 load_piece(const T* at) {
+  typedef typename Piece<T>::type type;
+  return __builtin_bit_cast(i32x4, PAST ? __builtin_nontemporal_load((const type*)at)
+                                        : *(const type*)at);
+}
+template <class T, bool PAST>
+__device__ __forceinline__ void store_piece(T* at, i32x4 x) {
+  typedef typename Piece<T>::type type;
+  if (PAST)
+    __builtin_nontemporal_store(__builtin_bit_cast(type, x), (type*)at);
+  else
+    *(type*)at = __builtin_bit_cast(type, x);
+}
+
 // Element j of a piece.  bf16 by its bits: from converted values the compiler makes 16-bit maxima,
 // which it then has to convert back and forth.
 template <class T>

@@ -544,7 +544,7 @@ def _log_probs(logits, rows, tokens, top, tau, ignore_index, keep=False):
     entropy = torch.empty(shape, dtype=torch.float32, device=device)
     lp = top_lp = ids = stats = None
     if tokens is not None:
-        lp = torch.empty(shape, dtype=torch.float32, device=device)
+        lp = torch.empty_like(entropy)
         tokens = tokens.contiguous()
     if top:
         top_lp = torch.empty((*shape, top), dtype=torch.float32, device=device)

@@ -153,7 +153,7 @@ def test_entry_points_refuse_without_launching(lib):
     nb = ctypes.c_size_t()
     size = lib.dmh_distill_workspace_size
     assert size(-1, ctypes.byref(nb)) == 1 and size(1, None) == 1
-    assert size(1000, ctypes.byref(nb)) == 0 and nb.value == 4000
+    assert size(1000, ctypes.byref(nb)) == 0 and nb.value == 4 * (2 * 1000 + 64)
 
 
 def test_no_cpu_fallback():
