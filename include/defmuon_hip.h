@@ -319,8 +319,8 @@ int dmh_cross_entropy_grad_stats(dmh_stream_t stream, const void* logits, int dt
  *   top_log_probs, top_ids  (rows, top): the `top` largest, falling, of equal logits the lower
  *              class first; top <= 256 and <= classes, 0 for none
  *   stats      3 x rows floats for the gradient; may be NULL
- * A row whose token is ignore_index gives zeros, and ignore_index for top_ids; another token
- * outside [0, classes) gives NaN for its log probability.  A row without a softmax gives NaN, and
+ * A row whose token is ignore_index gives zeros, and ignore_index for top_ids (-100 if that is a
+ * class); another token outside [0, classes) gives NaN for its log probability.  A row without a softmax gives NaN, and
  * 0 .. top - 1 for top_ids.  1e-6 <= temperature <= 1e6, classes <= 2^27, rows < 2^22.
  * dmh_log_probs_grad: the logits' gradient from the outputs' (each may be NULL). */
 int dmh_log_probs(dmh_stream_t stream, const void* logits, int dtype, long long rows,

@@ -11,7 +11,7 @@
 // entropy is a sum of two parts that are not negative.
 //
 // The largest classes go by the logits themselves, ties by the lower class; -0 and 0 are equal.
-// A row whose token is `ignore` gives 0 everywhere and `ignore` for its classes.  A row without a
+// A row whose token is `ignore` gives 0 everywhere and `none` for its classes.  A row without a
 // softmax (a NaN, an infinity, -inf alone) gives NaN and the classes 0 to K - 1.
 #include "rows.h"
 
@@ -27,7 +27,7 @@ struct LogProbArgs {
   float* top_lp;         // (rows, top)
   long long* top_ids;    // (rows, top)
   float* stats;          // (3, rows): maximum, sum, entropy; or null
-  long long rows, zs, ignore;
+  long long rows, zs, ignore, none;   // none: what stands for no class
   int classes, t64, top;
   float itau, c2;        // 1 / tau; log2(e) / tau
 };
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     if (t < 3 && a.stats) a.stats[t * a.rows + row] = t == 1 ? 1.f : 0.f;
     for (int i = t; i < K; i += THREADS) {
       a.top_lp[row * K + i] = 0.f;
-      a.top_ids[row * K + i] = a.ignore;
+      a.top_ids[row * K + i] = a.none;
     }
     return;
   }
@@ -592,7 +592,7 @@ __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
     terms[j] = g * a.itau;
   }
   push = block_sum<THREADS>(push, lds);
-  const bool known = !a.tokens || (y >= 0 && y < a.classes);
+  const bool known = !a.glp || (y >= 0 && y < a.classes);
   const float scale = known ? -a.itau / s : __builtin_nanf("");
   const float log_s = __builtin_amdgcn_logf(s) * LN2;
   const float A = scale * (push + gh * (ent - log_s)), B = scale * gh * LN2;
@@ -684,6 +684,7 @@ int dmh_log_probs(hipStream_t stream, const void* logits, int dtype, long long r
   a.rows = rows;
   a.zs = z_rstride;
   a.ignore = ignore_index;
+  a.none = ignore_index < 0 || ignore_index >= classes ? ignore_index : -100;
   a.classes = (int)classes;
   a.t64 = tokens_64 != 0;
   a.top = top;

@@ -597,9 +597,10 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0, ignore_index=-1
 
     tokens: int64 or int32 (...); top up to 256.  The three log probabilities and entropies take
     part in autograd.  A row whose token is ignore_index gives zeros, and ignore_index for its
-    classes, which distillation skips in turn; another token outside the classes gives NaN for its
-    log probability (and for its row's gradient).  A row without a softmax (a NaN, an infinity,
-    -inf alone) gives NaN, and the classes 0, 1, ... for its top."""
+    classes (-100 where that is a class), which distillation skips in turn; another token outside
+    the classes gives NaN for its log probability (and its row's gradient, if that is wanted).  A
+    row without a softmax (a NaN, an infinity, -inf alone) gives NaN, and the classes 0, 1, ...
+    for its top."""
     what = "token_log_probs"
     _eager(what, function=True)
     _float(logits, what, "logits")
@@ -610,7 +611,7 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0, ignore_index=-1
         if tokens.shape != logits.shape[:-1]:
             raise NativeError(f"{what}: tokens {tuple(tokens.shape)} do not fit logits "
                               f"{tuple(logits.shape)}")
-    if not 0 <= top <= min(_MAX_TOP, logits.shape[-1]):
+    if not isinstance(top, int) or not 0 <= top <= min(_MAX_TOP, logits.shape[-1]):
         raise NativeError(f"{what}: top must be between 0 and {_MAX_TOP} and no more than the "
                           f"{logits.shape[-1]} classes, not {top}")
     _temperature(temperature, what)

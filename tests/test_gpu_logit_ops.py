@@ -651,3 +651,136 @@ def test_compiled_programs_run_the_calls(T):
     assert torch.equal(a, b)
     assert torch.equal(*(torch.autograd.grad(x, zg)[0] for x in (a, b)))
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_below_the_normal_ones_keep_their_order(T, dtype):
+    """Subnormal logits, and -0 among 0."""
+    g = torch.Generator().manual_seed(0)
+    z = torch.zeros(3, 4000)
+    z[0] = (torch.randn(4000, generator=g) * 1e-39)
+    z[1, ::2] = -0.0
+    z[2] = -(torch.randint(0, 4, (4000,), generator=g) * 2.0 ** -133)
+    z = z.to(dtype)
+    for k in (3, 100):
+        got = T.token_log_probs(z.to(DEV), top=k)
+        assert torch.equal(got.top_ids.cpu(), L.top(z, k))
+
+
+def test_an_ignored_token_that_is_a_class(T):
+    """The lists of its rows are marked by what is no class, and others may name it."""
+    z, _ = lp_case(6, 50, F32)
+    z[:, 0] += 9.0
+    y = torch.tensor([0, 3, 4, 0, 9, 1])
+    out = T.token_log_probs(z.to(DEV), y.to(DEV), top=3, ignore_index=0)
+    assert (out.top_ids == -100).all(1).tolist() == [True, False, False, True, False, False]
+    assert out.top_ids[1, 0] == 0 and not out.entropy[[0, 3]].any()
+    loss = T.distillation(z.to(DEV), out.top_ids, out.top_log_probs, rest=True, reduction="none")
+    assert torch.isfinite(loss).all() and loss[0] == loss[3] == 0
+
+
+def test_an_unknown_token_leaves_the_other_gradients(T):
+    z, _ = lp_case(4, 300, F32)
+    y = torch.tensor([5, 300, -1, 7])
+    leaf = z.to(DEV).requires_grad_()
+    out = T.token_log_probs(leaf, y.to(DEV), top=4)
+    gh, gt = normal(4), normal(4, 4, seed=1)
+    (dz,) = torch.autograd.grad([out.entropy, out.top_log_probs], leaf, [gh.to(DEV), gt.to(DEV)])
+    close(dz, *L.log_probs_grad(z, y, out.top_ids.cpu(), None, gh, gt, 1.0, F32))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_ids_beyond_32_bits(T, rest):
+    z, ids, t = kd_case(4, 300, 5, ragged=False)
+    ids[0, 2], ids[2, 1], ids[3, 4] = 2 ** 32 + 7, -2 ** 40, 2 ** 31
+    c = L.Distill(z, ids, t, 1.0, rest)
+    got = T.distillation(z.to(DEV), ids.to(DEV), t.to(DEV), rest=rest, reduction="none")
+    close(got, c.loss, c.loss_err)
+    assert torch.isnan(got).tolist() == [True, False, True, True]
+
+
+def test_as_many_classes_as_there_may_be(T, Err):
+    """2^27 classes: all zero but a few, of which the last is one."""
+    v = 1 << 27
+    z = torch.zeros(1, v, dtype=F16, device=DEV)
+    at = torch.tensor([v - 1, 12345, v // 2 + 3, v - 9])
+    z[0, at.to(DEV)] = torch.tensor([9.0, 7.0, 8.0, 6.0], dtype=F16, device=DEV)
+    total = float((v - 4) + torch.exp(torch.tensor([9.0, 8.0, 7.0, 6.0]).double()).sum())
+    lse = torch.log(torch.tensor(total).double())
+    y = torch.tensor([v - 1], device=DEV)
+    out = T.token_log_probs(z, y, top=6)
+    assert out.top_ids[0].tolist() == [v - 1, v // 2 + 3, 12345, v - 9, 0, 1]
+    # a thread adds 2^17 terms in sequence
+    bound = (v // 1024 + 100) * E32
+    close(out.top_log_probs[0], torch.tensor([9.0, 8.0, 7.0, 6.0, 0.0, 0.0]).double() - lse, bound)
+    close(out.log_probs, (9.0 - lse)[None], bound)
+    t = torch.log(torch.tensor([[0.5, 0.25]], device=DEV))
+    ids = at[None, :2].to(DEV)
+    loss, dz = T.distillation_step(z, ids, t, rest=True, reduction="sum")
+    p = torch.exp(torch.tensor([9.0, 7.0]).double() - lse)
+    q = torch.tensor([0.5, 0.25]).double()
+    rest = 1 - p.sum()
+    want = (q * (q.log() - p.log())).sum() + 0.25 * (torch.log(torch.tensor(0.25).double())
+                                                     - torch.log(rest))
+    close(loss, want, 3 * bound + 20 * E32)
+    got = dz[0, at[:2].to(DEV)].cpu().double()
+    assert float((got - (p - q)).abs().max()) <= 2 * bound + 2.0 ** -11
+    with pytest.raises(Err, match="bad arguments"):
+        T.token_log_probs(torch.zeros(1, dtype=F16, device=DEV).expand(v + 1)[None])
+
+
+def test_many_rows_of_few_classes(T):
+    n, v = (1 << 19) + 3, 9
+    z = normal(n, v, dtype=BF16, std=2.0)
+    y = torch.arange(n) % v
+    ids = torch.stack([y, (y + 4) % v], 1)
+    t = torch.log(torch.tensor([0.5, 0.2])).repeat(n, 1)
+    ids[5::7] = -100
+    some = torch.cat([torch.arange(500), torch.arange(n - 500, n)])
+    out = T.token_log_probs(z.to(DEV), y.to(DEV), top=2)
+    ref, top = L.log_probs(z[some], y[some], 2)
+    close(out.log_probs[some.to(DEV)], *ref["log_probs"])
+    assert torch.equal(out.top_ids.cpu(), L.top(z, 2))
+    c = L.Distill(z, ids, t, 1.0, True)
+    loss, err, count = c.mean()
+    got, dz = T.distillation_step(z.to(DEV), ids.to(DEV), t.to(DEV), rest=True)
+    close(got, loss, err)
+    close(dz, *c.grad_bound(1.0 / count, BF16))
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 700])
+def test_rows_with_a_teacher_are_counted(T, n):
+    """By the rows' own launch, or by one before it."""
+    z, ids, t = kd_case(n, 130, 3, ragged=False)
+    ids[::3, 0] = -100
+    c = L.Distill(z, ids, t, 1.0, False)
+    loss, err, count = c.mean()
+    got, dz = T.distillation_step(z.to(DEV), ids.int().to(DEV), t.to(DEV))
+    close(got, loss, err)
+    close(dz, *c.grad_bound(1.0 / count, F32))
+    close(T.distillation(z.to(DEV), ids.to(DEV), t.to(DEV)), loss, err)
+
+
+def test_logits_past_the_caches(T):
+    """The loads and stores of logits of 400 MB, a few rows of which are compared."""
+    n, v = 4300, 50257
+    z = torch.randn(n, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(BF16)
+    _, ids, t = kd_case(n, v, 6, ragged=False)
+    y = ids[:, 3].clamp(min=0)
+    some = torch.tensor([0, 1, 2, 777, n - 2, n - 1])
+    zs = z[some.to(DEV)].cpu()
+    c = L.Distill(zs, ids[some], t[some], 1.0, True)
+    ig, tg = ids.to(DEV), t.to(DEV)
+    leaf = z.clone().requires_grad_()
+    (g,) = torch.autograd.grad(T.distillation(leaf, ig, tg, rest=True, reduction="sum"), leaf)
+    close(g[some.to(DEV)], *c.grad_bound(1.0, BF16))
+    out = T.token_log_probs(leaf, y.to(DEV), top=10)
+    ref, top = L.log_probs(zs, y[some], 10)
+    close(out.entropy[some.to(DEV)], *ref["entropy"])
+    assert torch.equal(out.top_ids[some.to(DEV)].cpu(), top)
+    gy = normal(n)
+    (g,) = torch.autograd.grad(out.log_probs, leaf, gy.to(DEV))
+    close(g[some.to(DEV)], *L.log_probs_grad(zs, y[some], None, gy[some], None, None, 1.0, BF16))
+    close(T.distillation(z, ig, tg, rest=True, reduction="none")[some.to(DEV)], c.loss, c.loss_err)
+    _, dz = T.distillation_step(z, ig, tg, rest=True, reduction="sum", inplace=True)
+    close(dz[some.to(DEV)], *c.grad_bound(1.0, BF16))

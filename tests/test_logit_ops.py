@@ -329,3 +329,11 @@ def test_traces_record_the_call_or_refuse(stand_in):
             op(mode.from_tensor(z))
     with pytest.raises(NativeError, match="trace"):
         torch.jit.trace(step, z)
+
+
+def test_a_top_that_is_no_whole_number(stand_in):
+    from defmuon_amd._native import NativeError
+    T, _ = stand_in
+    for top in (2.0, 2.5, None, "3"):
+        with pytest.raises(NativeError, match="top"):
+            T.token_log_probs(torch.randn(3, 9), top=top)
