@@ -474,7 +474,7 @@ static void launch_rows(hipStream_t stream, const DistillArgs& a) {
 }
 template <class T, bool REST, bool GRAD>
 static void launch_sized(hipStream_t stream, const DistillArgs& a) {
-  if (past_caches<T>(a.rows, a.classes))
+  if (!a.stats && past_caches<T>(a.rows, a.classes))   // (with statistics, the gradient comes next)
     launch_rows<T, REST, GRAD, true>(stream, a);
   else
     launch_rows<T, REST, GRAD, false>(stream, a);

@@ -111,7 +111,7 @@ __device__ __forceinline__ void group_cut(int K, TopLds& l) {
     k[i] = l.keys[i * 64 + (threadIdx.x & 63)];
     most = k[i] > most ? k[i] : most;
   }
-  const int enough = K + K / 4 + 4;
+  const int enough = K + K / 16 + 1;
   uint32_t cut = 0;
   __builtin_amdgcn_s_setprio(3);   // the others wait for this one in the end
   for (int b = 31; b >= 0; --b) {
@@ -520,7 +520,9 @@ static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
 }
 template <class T>
 static void launch_log_probs(hipStream_t stream, const LogProbArgs& a) {
-  if (past_caches<T>(a.rows, a.classes))
+  // (the gradient's launch comes next, and finds a part of the logits still in the cache: both 215
+  // instead of 236 us for 4096 bf16 rows of 50257)
+  if (!a.stats && past_caches<T>(a.rows, a.classes))
     a.top ? launch_rows<T, true, true>(stream, a) : launch_rows<T, false, true>(stream, a);
   else
     a.top ? launch_rows<T, true, false>(stream, a) : launch_rows<T, false, false>(stream, a);
