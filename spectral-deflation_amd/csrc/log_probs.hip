@@ -46,6 +46,7 @@ __device__ __forceinline__ void rescale(Part3& p, float m, float c2) {
     p.m = m;
   }
 }
+
 // ---- the largest classes ----------------------------------------------------------------------
 typedef unsigned long long u64;
 
@@ -62,8 +63,9 @@ __device__ __forceinline__ u64 rank_key(float x, int c) {
   return (u64)order_key(x) << 32 | (uint32_t)~c;
 }
 
-// The largest of each of HELD pieces, for later: two 16-bit values a register, while fp32 ones are found again from
-// the piece, in three instructions.
+// The largest of each of HELD pieces, for later: two 16-bit values a register, while fp32 ones are
+// found again from the piece, in three instructions.  (A register for each piece made the compiler
+// spill a few others, whose reloads took the 8192 rows below from 176 to 280 us.)
 template <class T, int HELD>
 struct PieceMaxima {
   typedef T pair __attribute__((ext_vector_type(2)));
@@ -96,13 +98,15 @@ struct TopLds {
   uint32_t keys[512];   // of groups of threads
   u64 cand[CANDS];
   uint32_t cut, most;
-  int slots[64];         // a counter for each step of the search over all classes
+  int slots[128];        // a counter for each step of the search over all classes
   int n;
 };
 
 // A lower bound of the K-th largest of a row, by the first wave: the K-th largest of the maxima of
-// `groups` groups of threads, since K groups have a class that large.  A bit at a time, and no
-// further than to a few groups more than K.  The other waves go on with the row's sum.
+// 64 PER groups of threads, since K groups have a class that large.  A bit at a time, and no
+// further than to a few groups more than K: their classes are ranked by comparing all with all
+// (with K / 4 groups more, 256 of 50257 classes took 370 instead of 312 us).  The other waves go on
+// with the row's sum.
 template <int PER>
 __device__ __forceinline__ void group_cut(int K, TopLds& l) {
   uint32_t k[PER], most = 0;
@@ -136,7 +140,8 @@ __device__ __forceinline__ void group_cut(int K, TopLds& l) {
 }
 
 // The threads' maxima by groups: 256, or 512 for more than 64 classes.  (Of 256 and K = 64, about
-// 74 classes are as large as the 64th group's; of 512 and K = 256, about 355.)
+// 74 classes are as large as the 64th group's; of 512 and K = 256, about 355.)  Zeroes the counters
+// of what follows.
 template <int THREADS>
 __device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
   uint32_t k = order_key(largest), o;
@@ -153,7 +158,7 @@ __device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
   }
   l.keys[t] = k;   // the same from all threads of a group
   if (threadIdx.x == 0) l.n = 0;
-  if (threadIdx.x < 64) l.slots[threadIdx.x] = 0;
+  if (threadIdx.x < 128) l.slots[threadIdx.x] = 0;
 }
 template <int THREADS>
 __device__ __forceinline__ void find_cut(int K, TopLds& l) {
@@ -173,8 +178,8 @@ __device__ __forceinline__ void put_candidate(bool has, u64 key, TopLds& l) {
   if (has && at < CANDS) l.cand[at] = key;
 }
 
-// Pieces with a class that is large enough, gathered by a wave, 64 at most: their elements side by side in the
-// lanes, 64 at a time.
+// Pieces with a class that is large enough, gathered by a wave, 64 at most: their elements side by
+// side in the lanes, 64 at a time.
 struct PieceList {
   i32x4 data[64];
   int first[64];   // class of a piece's first element
@@ -194,44 +199,83 @@ __device__ __forceinline__ void put_pieces(int count, u64 from, const PieceList&
   __builtin_amdgcn_wave_barrier();
 }
 
-// Where more than CANDS classes are above the cut (many large ones in few groups, or many equal
-// ones): the candidates by a bit at a time over all classes.  The K-th largest is between cut and
-// the largest: the bits that these two share need no step, nor do a class's bits above those of the
-// last one.  each(cut, f) calls f(value, class) for all classes of the thread whose order_key is
-// at least cut, and may for others.
+// The candidates where more than CANDS classes are above the cut: many large ones in few groups, or
+// many equal ones.  each(cut, first, last, f) calls f(key, class) for the thread's classes from
+// first to last - 1 whose order_key is at least cut.
+//
+// First the K-th largest value.  The groups' is the row's where equal classes are the cause; else a
+// bit at a time between it and the largest, which only threads with such classes have to look at.
+// Then, if its classes are still too many, the first of them: twice as far each time, and the last
+// step halved.
 template <int THREADS, class Each>
 __device__ __forceinline__ void search_top(int K, int classes, const Each& each, TopLds& l) {
-  const uint32_t cut = l.cut, most = l.most;
-  const int high = cut == most ? -1 : 31 - __clz(cut ^ most);
-  const int low = 32 - __clz(classes);   // classes < 2^low
-  const uint32_t shared = ~((1u << low) - 1u);
-  u64 from = (u64)(high < 0 ? most : most & ~((2u << high) - 1u)) << 32;
-  if (high < 0) from |= shared;
+  uint32_t value = l.cut;
+  const uint32_t most = l.most;
   int step = 0;
-  for (int b = high < 0 ? low - 1 : 32 + high; b >= 0; --b) {
-    if (b == 31) {
-      from |= shared;
-      b = low - 1;
-    }
-    const u64 c = from | 1ull << b;
+  auto count = [&](uint32_t least, uint32_t up_to, int first, int last) {
     int n = 0;
-    each((uint32_t)(c >> 32), [&](float v, int i) { n += rank_key(v, i) >= c; });
-#pragma unroll
-    for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-    if ((threadIdx.x & 63) == 0 && n) atomicAdd(&l.slots[step], n);
+    each(least, first, last, [&](uint32_t k, int) { n += k <= up_to; });
+    const float s = wave_sum((float)n);   // exact: a wave has fewer than 2^24 classes
+    if ((threadIdx.x & 63) == 0 && s != 0.f) atomicAdd(&l.slots[step], (int)s);
     __syncthreads();
-    n = l.slots[step++];
-    if (n >= K) {
-      from = c;
-      if (n <= CANDS) break;
+    return l.slots[step++];
+  };
+  auto gather = [&](uint32_t least, int first, int last, uint32_t equal, int end) {
+    each(least, first, last, [&](uint32_t k, int c) {
+      if (k != equal || c < end) {
+        const int at = atomicAdd(&l.n, 1);
+        if (at < CANDS) l.cand[at] = (u64)k << 32 | (uint32_t)~c;
+      }
+    });
+  };
+  __syncthreads();   // everyone has seen that there are too many
+  if (threadIdx.x == 0) l.n = 0;
+  int above = value == most ? 0 : count(value + 1, most, 0, classes);
+  if (above >= K) {
+    int n = above;
+    value += 1;
+    if (n > CANDS) {
+      const int high = value == most ? -1 : 31 - __clz(value ^ most);
+      value = high < 0 ? most : most & ~((2u << high) - 1u);
+      for (int b = high; b >= 0; --b) {
+        const uint32_t c = value | 1u << b;
+        const int now = count(c, most, 0, classes);
+        if (now >= K) {
+          value = c;
+          n = now;
+          if (n <= CANDS) break;
+        }
+      }
+    }
+    if (n <= CANDS) {
+      gather(value, 0, classes, 0, 0);
+      __syncthreads();
+      return;
+    }
+    above = value == most ? 0 : count(value + 1, most, 0, classes);
+  }
+  int first = 0, last = classes < 512 ? classes : 512, before = 0, here;
+  // (both loops end, and all stores stay inside, also if someone writes to the row meanwhile)
+  while (before + (here = count(value, value, first, last)) < K - above && last < classes) {
+    before += here;
+    first = last;
+    last = last < classes / 2 ? 2 * last : classes;
+  }
+  while (above + before + here > CANDS && last - first > 1) {
+    const int middle = first + (last - first) / 2, n = count(value, value, first, middle);
+    if (before + n < K - above) {
+      before += n;
+      here -= n;
+      first = middle;
+    } else {
+      here = n;
+      last = middle;
     }
   }
-  if (threadIdx.x == 0) l.n = 0;
-  __syncthreads();
-  each((uint32_t)(from >> 32), [&](float v, int c) {
-    const u64 k = rank_key(v, c);
-    if (k >= from) l.cand[atomicAdd(&l.n, 1)] = k;
-  });
+  if (above > 0)
+    gather(value, 0, classes, value, last);
+  else
+    gather(value, 0, last, value, last);
   __syncthreads();
 }
 
@@ -239,7 +283,7 @@ __device__ __forceinline__ void search_top(int K, int classes, const Each& each,
 // number of larger ones, which as many threads as there are for each count together.
 template <int THREADS, class Put>
 __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) {
-  const int n = l.n;
+  const int n = l.n < CANDS ? l.n : CANDS;
   int share = 1;
   while (share < 64 && 2 * share * n <= THREADS) share *= 2;
   const int part = threadIdx.x & (share - 1);
@@ -255,6 +299,20 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
 
 // One row by THREADS threads that hold it in registers, HELD pieces each (packed between the
 // steps), or for HELD = 0 a workgroup that streams it.
+//
+// Without a top it reads each logit once and is bound by the memory, the vector units not far
+// behind: 8192 bf16 rows of 50257 take 138 us (5.9 TB/s), 1000 fp32 rows of 131072 80 (6.5).  Two
+// barriers and reductions by lane shifts, one for the maximum and one for the sums, take less of
+// them than one that joins parts of different maxima (176 us).
+//
+// Top classes: the threads' maxima, which the sums need anyway, give a lower bound of the K-th
+// largest class that few classes reach, whatever the distribution; those are gathered, piece by
+// piece, and ranked by comparing all with all.  The 64 largest take 173 us of the same rows, the
+// largest alone 154.  Where too many reach the bound (equal logits, or many large ones in one
+// thread's classes) the row is read again, as far as needed: 408 us for 8192 rows of zeros, 605
+// where a mask leaves 20 classes of them.  Long rows keep the maxima of SEGMENTS parts of each
+// thread's pieces, and read again only the parts that reach the bound (20 of 131072 classes: 85 us,
+// 105 with all parts of such threads).
 template <class T, int THREADS, int HELD, bool TOP, bool PAST>
 __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(LogProbArgs a) {
   __shared__ float maxes[16], sums[16], weights[16];   // of the waves
@@ -263,7 +321,6 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       lists[TOP && HELD ? THREADS / 64 : 1];
   __shared__ float segments[TOP && !HELD ? SEGMENTS * THREADS : 1];
   constexpr int N = Piece<T>::N, AHEAD = 4;
-  typedef typename Row<T>::type type;
   const long long row = blockIdx.x;
   const int t = threadIdx.x, K = a.top;
   const T* z = (const T*)a.z + row * a.zs;
@@ -290,7 +347,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     return;
   }
   // a long row's rounds of AHEAD pieces a thread, by segment
-  const int segment_rounds = (r.pieces + AHEAD * THREADS * SEGMENTS - 1) / (AHEAD * THREADS * SEGMENTS);
+  constexpr int ROUND = AHEAD * THREADS;
+  const int segment_rounds = (r.pieces + ROUND * SEGMENTS - 1) / (ROUND * SEGMENTS);
   const bool known = a.tokens && y >= 0 && y < a.classes;
   const float zy = known ? (float)z[y] : __builtin_nanf("");
   Part3 p = {ex, 0.f, 0.f};
@@ -379,10 +437,30 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       p.t = fmaf(e, fmaxf(d, LOWEST), p.t);
     };
     if (r.edge(t) >= 0) again((float)z[r.edge(t)]);
-    for (int i = t; i < r.pieces; i += THREADS) {
-      const type v = *(const type*)(z + r.piece_class(i));
+    if constexpr (HELD > 0) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) again((float)v[j]);
+      for (int k = 0; k < HELD; ++k) {
+        if (k * THREADS + t < r.pieces) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) again(element<T>(x[k], j));
+        }
+      }
+      repack(x);
+    } else {
+      for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
+        i32x4 v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int i = i0 + k * THREADS;
+          v[k] = load_piece<T, false>(z + r.piece_class(i < r.pieces ? i : i0));
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (i0 + k * THREADS < r.pieces) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) again(element<T>(v[k], j));
+          }
+      }
     }
   }
   const float ws = wave_sum(p.s), wt = wave_sum(p.t);
@@ -411,22 +489,31 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       return;
     }
     // (by value: what a lambda refers to may end in memory)
-    auto each = [=](uint32_t cut, auto f) {
+    auto each = [=](uint32_t cut, int first, int last, auto f) {
       if (order_key(largest) < cut) return;
-      if (r.edge(t) >= 0) f((float)z[r.edge(t)], r.edge(t));
-      for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {
-        type v[AHEAD];
+      auto visit = [&](float v, int c) {
+        const uint32_t k = order_key(v);
+        if (k >= cut && c >= first && c < last) f(k, c);
+      };
+      if (r.edge(t) >= 0) visit((float)z[r.edge(t)], r.edge(t));
+      const int begin = first > r.head ? (first - r.head) / N : 0;
+      const int end = last > r.head ? (last - r.head + N - 1) / N : 0;
+      const int stop = end < r.pieces ? end : r.pieces;
+      const float least = cut_value(cut);
+      // the thread's own pieces, which `largest` is of
+      for (int i0 = begin + ((t - begin) & (THREADS - 1)); i0 < stop; i0 += AHEAD * THREADS) {
+        i32x4 v[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          v[k] = *(const type*)(z + r.piece_class(i < r.pieces ? i : i0));
+          v[k] = load_piece<T, false>(z + r.piece_class(i < stop ? i : i0));
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           const int i = i0 + k * THREADS;
-          if (i < r.pieces && piece_max<T>(__builtin_bit_cast(i32x4, v[k])) >= cut_value(cut)) {
+          if (i < stop && piece_max<T>(v[k]) >= least) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) f((float)v[k][j], r.piece_class(i) + j);
+            for (int j = 0; j < N; ++j) visit(element<T>(v[k], j), r.piece_class(i) + j);
           }
         }
       }
@@ -507,6 +594,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
   }
 }
 
+// 256 threads where they hold a row (of 8009 bf16 classes, 64 largest: 92 us for 16384 rows) and
+// have groups enough, else 1024 (the 128 largest of those: 149 us, by 1024 threads 282).
 template <class T, bool TOP, bool PAST>
 static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
@@ -543,6 +632,7 @@ struct LogProbGradArgs {
 
 // Element by element, 256 threads for four pieces each of a row; the listed classes (the token and
 // the top ones) are written again behind a barrier, each by one thread with the sum of its terms.
+// Bound by the memory: 4096 bf16 rows of 50257 take 143 us (823 MB, 5.8 TB/s).
 template <class T, bool PAST>
 __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;

@@ -1,5 +1,5 @@
-// Rows of logits: the reductions, the exponentials and the pieces that the operators over the classes
-// of a vocabulary share.
+// Rows of logits: the reductions, the exponentials and the pieces that the operators over the
+// classes of a vocabulary share.
 #pragma once
 
 #include <type_traits>
@@ -71,7 +71,7 @@ __device__ __forceinline__ void rescale(Part& p, float m, float c2) {
   }
 }
 
-// ---- reductions by lane shifts: in the last lane of a row of 16, then of the wave -----------------
+// ---- reductions by lane shifts: in the last lane of a row of 16, then of the wave --------------
 template <int CTRL, int ROWS = 0xF>
 __device__ __forceinline__ float shifted(float v, float none) {
   return __builtin_bit_cast(
@@ -145,8 +145,8 @@ struct Row {
   }
 };
 
-// Logits of much more than the last-level cache's 256 MB are read, and their gradient written, as what
-// no cache need keep: 8192 bf16 rows of 50257 with their gradient by distillation in 305 instead
+// Logits of much more than the last-level cache's 256 MB are read, and their gradient written, as
+// what no cache need keep: 8192 bf16 rows of 50257 with their gradient by distillation in 305 instead
 // of 321 us, in place 283 instead of 332.  (In 103 MB that a cache still holds, 48 instead of 43.)
 template <class T>
 inline bool past_caches(long long rows, long long classes) {

@@ -1,15 +1,20 @@
 """The operators of a GPT-2 training step beside its matrix products and the optimizer: the
-embedding with its gradient, dropout, and the loss with its gradient.
+embedding with its gradient, dropout, and the loss with its gradient; and beside the loss, on the
+same rows of logits, log probabilities with entropy and top classes, and distillation from a
+teacher's, with their gradients.
 
     x = embedding(tokens, wte, wpe, dropout_p=0.1, rng=draw_rng())
     x = dropout(attn(x), 0.1, draw_rng(), residual=x)
     loss, dlogits = cross_entropy_step(logits, targets)
     logits.backward(dlogits)
 
+    top = token_log_probs(teacher(tokens), top=64, temperature=2.0)
+    loss, dlogits = distillation_step(logits, top.top_ids, top.top_log_probs, temperature=2.0)
+
 fp32, bf16 and fp16 tensors; everything is computed in fp32 and rounded once.  All functions
 run through the HIP library on the current stream and synchronise nothing; there is no CPU
-fallback.  embedding, dropout and cross_entropy take part in autograd; the *_backward
-functions and cross_entropy_step are for programs that call the gradients themselves.
+fallback.  embedding, dropout, cross_entropy, token_log_probs and distillation take part in
+autograd; the *_backward and *_step functions are for programs that call the gradients themselves.
 Arguments that do not fit raise NativeError, as do tensors that carry a forward-mode tangent:
 there is no such derivative.  So do traces that would record the results' allocation and not the
 launch behind it: make_fx and fake tensors for all functions, torch.jit.trace (which records
@@ -533,7 +538,7 @@ _MAX_TOP, _MAX_LIST = 256, 1024
 
 
 def _temperature(tau, what):
-    if not 1e-6 <= tau <= 1e6:
+    if not isinstance(tau, (int, float)) or not 1e-6 <= tau <= 1e6:
         raise NativeError(f"{what}: temperature must be between 1e-6 and 1e6, not {tau}")
 
 
@@ -696,7 +701,8 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
 
     token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is
     taken as it is, at the temperature already (raw logits go in divided by it, without `rest`).
-    k up to 1024.  An entry whose class is ignore_index is left out, and a row whose first entry
+    k up to 1024.  The loss carries the rounding of fp32 logarithms times temperature^2, about 1e-7
+    of it, and a divergence of zero may come out that far below.  An entry whose class is ignore_index is left out, and a row whose first entry
     is counts for nothing; another class outside the logits' makes its row NaN, as does a row
     without a softmax.  An entry of -inf adds nothing, whatever the logits say; a row of
     those alone is NaN, with `rest` it leaves all to the others.  The teacher takes no gradient."""

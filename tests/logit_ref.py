@@ -35,6 +35,8 @@ class Softmax:
         self.log_s = torch.logsumexp(-self.gap, -1, keepdim=True)
         self.lse = self.m + self.log_s
         self.log_p = -self.gap - self.log_s
+        # what lies half a last place beyond the largest fp32 value rounds to an infinity
+        self.log_p = torch.where(self.log_p <= -(2.0 ** 128 - 2.0 ** 103), -torch.inf, self.log_p)
         self.p = torch.exp(self.log_p)
         pd = _z0(self.p * self.gap)
         self.d1 = pd.sum(-1, keepdim=True)

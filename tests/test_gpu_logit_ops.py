@@ -784,3 +784,79 @@ def test_logits_past_the_caches(T):
     close(T.distillation(z, ig, tg, rest=True, reduction="none")[some.to(DEV)], c.loss, c.loss_err)
     _, dz = T.distillation_step(z, ig, tg, rest=True, reduction="sum", inplace=True)
     close(dz[some.to(DEV)], *c.grad_bound(1.0, BF16))
+
+
+def test_a_models_step_on_a_teacher(T):
+    """The benchmark's GPT-2 as a student of another one, in place, against torch's operators in
+    fp32.  As there, each gradient differs by the rounding of sums of some thousand fp32 terms
+    (2^-24 each, relative to its norm) at each of a dozen products on its way."""
+    import bench
+    tok = torch.randint(0, 517, (3, 41), generator=torch.Generator().manual_seed(0)).to(DEV)
+    x, y = tok[:, :-1], tok[:, 1:].clone()
+    y[2, 30:] = -100                        # padding
+    torch.manual_seed(1)
+    teacher = bench._gpt2(517, 64, 64, 2, 4).to(DEV)
+    with torch.no_grad():
+        zt = teacher.logits(x) * 3.0        # (of a random model, all classes are nearly alike)
+        top = T.token_log_probs(zt, y, top=16, temperature=2.0)
+    got = {}
+    for ops in ("torch", "hip"):
+        torch.manual_seed(0)
+        m = bench._gpt2(517, 64, 64, 2, 4, ops).to(DEV)
+        z = m.logits(x)
+        if ops == "hip":
+            loss, dz = T.distillation_step(z, top.top_ids, top.top_log_probs, temperature=2.0,
+                                           rest=True, inplace=True)
+            z.backward(dz)
+        else:
+            live = y != -100
+            lp = torch.log_softmax(zt / 2, -1)
+            at = torch.topk(lp, 16, -1)[1]
+            log_q, log_p = lp.gather(-1, at), torch.log_softmax(z / 2, -1)
+            q = log_q.exp()
+            inside = torch.zeros_like(lp, dtype=torch.bool).scatter_(-1, at, True)
+            left = lp.exp().masked_fill(inside, 0).sum(-1)
+            log_r = torch.logsumexp(log_p.masked_fill(inside, -torch.inf), -1)
+            kl = (q * (log_q - log_p.gather(-1, at))).sum(-1) + left * (left.log() - log_r)
+            loss = 4 * kl[live].mean()
+            loss.backward()
+        got[ops] = float(loss.detach()), {n: p.grad for n, p in m.named_parameters()}
+    (a, ga), (b, gb) = got["torch"], got["hip"]
+    assert abs(a - b) <= 1e-4 * a
+    assert ga.keys() == gb.keys()
+    for n in ga:
+        assert float((ga[n] - gb[n]).norm()) <= 12 * 2000 * E32 * float(ga[n].norm()), n
+
+
+@pytest.mark.parametrize("v", [1500, 9003, 50257, 66001, 131077])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_top_classes_among_equal_ones(T, v, dtype):
+    """Equal classes at the end, in the second half, behind a few larger ones, in lumps; masks that
+    leave fewer than are asked for."""
+    g = torch.Generator().manual_seed(v)
+    inf = float("inf")
+    z = torch.randn(12, v, generator=g).clamp(max=3.0)
+    z[0] = -1.0
+    z[0, -1100:] = 5.0
+    z[1, v // 2:] = 5.0
+    z[2, v // 2 + 7:] = torch.where(torch.rand(v - v // 2 - 7, generator=g) < 0.5, 5.0, -1.0)
+    z[3, v // 3:] = 4.0
+    z[3, torch.randperm(v, generator=g)[:60]] = torch.arange(60.0) + 5.0
+    z[4, :700] = 6.0 + torch.rand(min(v, 700), generator=g)
+    z[5, 20:] = -inf
+    z[6] = -inf
+    z[6, torch.randperm(v, generator=g)[:100]] = 2.0
+    z[7, :] = torch.arange(v).remainder(v // 7 + 1).float() / 64
+    z[8] = torch.arange(v).div(900, rounding_mode="floor").float()
+    z[9] = -torch.arange(v).div(900, rounding_mode="floor").float()
+    z[10, ::2] = -inf
+    z[11] = -torch.finfo(dtype).max
+    z[11, 3] = torch.finfo(dtype).max
+    z = z.to(dtype)
+    for k in (1, 20, 64, 65, 101, 256):
+        got = T.token_log_probs(z.to(DEV), top=k)
+        assert torch.equal(got.top_ids.cpu(), L.top(z, k)), k
+        check_log_probs(got, z, None, k, 1.0, k)
+    many = z.repeat(60, 1).to(DEV)          # more rows than fit at a time
+    got = T.token_log_probs(many, top=64)
+    assert torch.equal(got.top_ids.cpu(), L.top(z, 64).repeat(60, 1))

@@ -337,3 +337,15 @@ def test_a_top_that_is_no_whole_number(stand_in):
     for top in (2.0, 2.5, None, "3"):
         with pytest.raises(NativeError, match="top"):
             T.token_log_probs(torch.randn(3, 9), top=top)
+
+
+def test_a_temperature_that_is_no_number(stand_in):
+    """A tensor's value would have to be waited for."""
+    from defmuon_amd._native import NativeError
+    T, _ = stand_in
+    z, _, ids, t = _case()
+    for tau in (torch.tensor(1.0), "1", None):
+        with pytest.raises(NativeError, match="temperature"):
+            T.token_log_probs(z.float(), temperature=tau)
+        with pytest.raises(NativeError, match="temperature"):
+            T.distillation(z.float(), ids, t.float(), temperature=tau)
