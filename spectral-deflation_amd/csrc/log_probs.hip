@@ -371,11 +371,17 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     m = waves_max(maxes, THREADS / 64);
   };
   if constexpr (HELD > 0) {
+    // a small workgroup's waves pass over pieces behind the row (the 64 largest of 8009 classes,
+    // 16384 rows: 92 to 86 us; at 1024 threads the test is a register too many, 173 to 181 us)
+    const int wave = __builtin_amdgcn_readfirstlane(t);
 #pragma unroll
     for (int k = 0; k < HELD; k += 2) {
-      const float m0 = k * THREADS + t < r.pieces ? piece_max<T>(x[k]) : -INF;
-      const float m1 = (k + 1) * THREADS + t < r.pieces ? piece_max<T>(x[k + 1]) : -INF;
-      p.m = maximum(p.m, maximum(m0, m1));
+      float m0 = -INF, m1 = -INF;
+      if (THREADS > 256 || k * THREADS + wave < r.pieces) {
+        m0 = k * THREADS + t < r.pieces ? piece_max<T>(x[k]) : -INF;
+        m1 = (k + 1) * THREADS + t < r.pieces ? piece_max<T>(x[k + 1]) : -INF;
+        p.m = maximum(p.m, maximum(m0, m1));
+      }
       if constexpr (TOP) maxima.put(k, m0, m1);
     }
     repack(x);
