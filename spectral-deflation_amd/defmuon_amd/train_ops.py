@@ -701,11 +701,12 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
 
     token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is
     taken as it is, at the temperature already (raw logits go in divided by it, without `rest`).
-    k up to 1024.  The loss carries the rounding of fp32 logarithms times temperature^2, about 1e-7
-    of it, and a divergence of zero may come out that far below.  An entry whose class is ignore_index is left out, and a row whose first entry
-    is counts for nothing; another class outside the logits' makes its row NaN, as does a row
-    without a softmax.  An entry of -inf adds nothing, whatever the logits say; a row of
-    those alone is NaN, with `rest` it leaves all to the others.  The teacher takes no gradient."""
+    k up to 1024; a class named twice counts with both.  The loss carries the rounding of fp32
+    logarithms times temperature^2, about 1e-7 of it, and a divergence of zero may come out that far
+    below.  An entry whose class is ignore_index is left out, and a row whose first entry is counts
+    for nothing; another class outside the logits' makes its row NaN, as does a row without a
+    softmax.  An entry of -inf adds nothing, whatever the logits say; a row of those alone is NaN,
+    with `rest` it leaves all to the others.  The teacher takes no gradient."""
     _eager("distillation", function=True)
     _distill_args(logits, ids, teacher, temperature, reduction, "distillation")
     if _is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
