@@ -14,7 +14,9 @@
 //
 // The rest has a maximum and a sum of its own, m_R and s_R: p / p_R = exp(x - m_R) / s_R and
 // log p_R = m_R + log s_R - lse, where 1 - sum p would have lost all digits for a student that is
-// sure of the list.  Off the list, dz is one exponential times one factor of the row.
+// sure of the list.  Off the list, dz is one exponential times one factor of the row.  Where no
+// class is off the list, or only ones of -inf, there is no rest and r is 0: what rounding leaves of the
+// teacher's 1 would be infinitely far from such a student.
 //
 // An entry whose class is `ignore` is left out; a row whose first entry is has no teacher, loss 0
 // and gradient 0.  A class outside [0, V) makes its row NaN, as does a row without a softmax.  What
@@ -365,9 +367,10 @@ void distill_row(DistillArgs a) {
   }
   // coefficients
   const float log_s = natural_log(all.s);
-  const float left = REST ? fmaxf(1.f - qsum, 0.f) : 0.f;
-  float w = REST ? (qsum <= 1.f ? 1.f : qsum) : qsum / qsum;
-  if (!(all.s >= 0.5f)) w = __builtin_nanf("");
+  const bool others = REST && m != -INF;
+  const float left = others ? fmaxf(1.f - qsum, 0.f) : 0.f;
+  float w = !REST ? qsum / qsum : others && qsum <= 1.f ? 1.f : qsum;
+  if (!(all.s >= 0.5f) || (REST && !others && qsum == 0.f)) w = __builtin_nanf("");
   RowStats st;
   st.m = all.m;
   st.ws = w / all.s;
@@ -377,7 +380,7 @@ void distill_row(DistillArgs a) {
   st.coef = st.ws;
   if (REST) {
     st.coef = st.ws * (m == -INF ? 0.f : __builtin_amdgcn_exp2f((m - all.m) * a.c2));
-    if (left > 0.f && p.s > 0.f) st.coef -= left / p.s;
+    if (left > 0.f) st.coef -= left / p.s;
   }
   if (wave < list_waves) {
     float loss = 0.f;

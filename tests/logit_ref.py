@@ -138,7 +138,14 @@ class Distill:
         size = torch.where(q != 0, q * (log_q.abs() + log_p.abs()), zero)
         err = (_z0(q) * (lq_err + s.lp_err.gather(-1, at)) + _z0(q * eq * (log_q - log_p).abs())
                + 3 * E32 * _z0(size)).sum(-1) + k * E32 * _z0(terms.abs()).sum(-1)
-        w = q.sum(-1, keepdim=True) if not rest else torch.clamp(q.sum(-1, keepdim=True), min=1.0)
+        w = q.sum(-1, keepdim=True)
+        if rest:
+            listed = torch.zeros((*z.shape[:-1], v + 1), dtype=torch.bool)
+            listed.scatter_(-1, torch.where(inside, ids, v).long(), True)
+            o = Softmax(z, tau, ~listed[..., :v])
+            others = o.m != -torch.inf      # no class outside the list: nothing to leave it
+            left = torch.where(others, torch.clamp(1.0 - w, min=0.0), zero)
+            w = torch.where(others, torch.clamp(w, min=1.0), torch.where(w != 0, w, torch.nan))
         dense = torch.zeros_like(s.x).scatter_add_(-1, at, q)
         dense_err = torch.zeros_like(s.x).scatter_add_(-1, at, _z0(q * eq))
         dz = w * s.p - dense
@@ -146,15 +153,11 @@ class Distill:
         w_err = _z0(q * eq).sum(-1, keepdim=True) + (k + 8) * E32
         dz_err = w * s.p_err + s.p * w_err + dense_err + 6 * E32 * (w * s.p + _z0(dense))
         if rest:
-            listed = torch.zeros((*z.shape[:-1], v + 1), dtype=torch.bool)
-            listed.scatter_(-1, torch.where(inside, ids, v).long(), True)
-            o = Softmax(z, tau, ~listed[..., :v])
-            left = torch.clamp(1.0 - q.sum(-1, keepdim=True), min=0.0)
             log_r = (o.m - s.m) + (o.log_s - s.log_s)   # -inf where nothing is left
             log_r = torch.where(torch.isfinite(o.m), log_r, -torch.inf)
             part = torch.where(left != 0, left * (torch.log(left) - log_r), zero)[..., 0]
             loss = loss + part
-            left_err = w_err
+            left_err = torch.where(others, w_err, zero)
             log_left = torch.where(left > 0, torch.log(left), zero)
             err = err + (left_err * (_z0(log_left - log_r).abs() + 1)
                          + left * (o.rho + s.rho + 4 * E32 * (
@@ -163,7 +166,7 @@ class Distill:
             r = _z0(o.p)
             dz = dz - left * r
             dz_err = dz_err + r * left_err + left * (_z0(o.p_err)) + 6 * E32 * left * r
-        nan = bad | ~torch.isfinite(s.lse[..., 0])
+        nan = bad | ~torch.isfinite(s.lse[..., 0]) | torch.isnan(w[..., 0])
         self.loss = torch.where(self.live, torch.where(nan, torch.nan, loss * tau ** 2), zero)
         self.loss_err = 1.1 * _z0(err) * tau ** 2 + 4 * E32 * _z0(self.loss).abs()
         dz = torch.where(nan[..., None], torch.nan, dz * tau)

@@ -453,6 +453,34 @@ def test_masked_and_non_finite_rows(T, v, rest):
         assert torch.isnan(dz[nans]).all() and not dz[9].any()
 
 
+@pytest.mark.parametrize("v", [24, 600, 9001, 50257, 140001])
+def test_no_class_beside_the_list(T, v):
+    """A mask that leaves 20 classes to both, or a list of all: what rounding leaves of the
+    teacher's 1 belongs to no class and does not count."""
+    k, inf = 24, float("inf")
+    teacher, student = normal(40, v, std=3.0), normal(40, v, seed=1)
+    teacher[:30, v // 2 + 10:] = student[:30, v // 2 + 10:] = -inf
+    teacher[:30, :v // 2 - 10] = student[:30, :v // 2 - 10] = -inf
+    out = T.token_log_probs(teacher.to(DEV), top=k, temperature=1.5)
+    ids, t = out.top_ids.cpu(), out.top_log_probs.cpu()
+    assert (torch.exp(t[:30].double()).sum(1) < 1).any() and (t[:30, 20:] == -inf).all()
+    t[29] = -inf                         # ... and nothing on the list: no distribution at all
+    t[28] -= 1.0                         # less than 1 by far
+    c = L.Distill(student, ids, t, 1.5, True)
+    nans = torch.isnan(c.loss)
+    assert nans.nonzero().tolist() == [[29]] and torch.isfinite(c.loss[~nans]).all()
+    sg, ig, tg = student.to(DEV), ids.to(DEV), t.to(DEV)
+    kw = dict(temperature=1.5, rest=True)
+    close(T.distillation(sg, ig, tg, reduction="none", **kw), c.loss, c.loss_err)
+    want, bound = c.grad_bound(1.0, F32)
+    leaf = sg.clone().requires_grad_()
+    for dz in (T.distillation_step(sg, ig, tg, reduction="sum", **kw)[1],
+               torch.autograd.grad(T.distillation(leaf, ig, tg, reduction="sum", **kw), leaf)[0]):
+        dz = dz.cpu()
+        close(dz[~nans], want[~nans], bound[~nans])
+        assert torch.isnan(dz[nans]).all()
+
+
 def test_the_rest_of_a_student_without_doubt(T):
     """Off the list the student has less than the smallest fp32: the gradient there still has the
     rest's own shape, where p / (sum of p) is 0 / 0."""
