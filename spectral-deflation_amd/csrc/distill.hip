@@ -14,9 +14,11 @@
 //
 // The rest has a maximum and a sum of its own, m_R and s_R: p / p_R = exp(x - m_R) / s_R and
 // log p_R = m_R + log s_R - lse, where 1 - sum p would have lost all digits for a student that is
-// sure of the list.  Off the list, dz is one exponential times one factor of the row.  Where no
-// class is off the list, or only ones of -inf, there is no rest and r is 0: what rounding leaves of the
-// teacher's 1 would be infinitely far from such a student.
+// sure of the list.  Off the list, dz is one exponential times one factor of the row.
+//
+// Where no class is off the list, or only ones of -inf, there is no rest and r is 0.  So it is within
+// the rounding of sum q: what that leaves of a teacher's 1 would otherwise be infinitely far from a
+// student whose rest is masked, and count a million times over where the mask is -1e9.
 //
 // An entry whose class is `ignore` is left out; a row whose first entry is has no teacher, loss 0
 // and gradient 0.  A class outside [0, V) makes its row NaN, as does a row without a softmax.  What
@@ -45,6 +47,7 @@ struct DistillArgs {
   int classes, k, i64 /* 0 or 1 */, ttype, gout_rows;
   float itau, c2;        // 1 / tau; log2(e) / tau
   float lscale, gscale;  // tau^2; tau times the gradient's scale
+  float slack;           // a rest up to here is the list's rounding
 };
 
 // An entry of a list as it is in memory, of any of the types: loaded without a branch, which would
@@ -368,7 +371,7 @@ void distill_row(DistillArgs a) {
   // coefficients
   const float log_s = natural_log(all.s);
   const bool others = REST && m != -INF;
-  const float left = others ? fmaxf(1.f - qsum, 0.f) : 0.f;
+  const float left = others && 1.f - qsum > a.slack ? 1.f - qsum : 0.f;
   float w = !REST ? qsum / qsum : others && qsum <= 1.f ? 1.f : qsum;
   if (!(all.s >= 0.5f) || (REST && !others && qsum == 0.f)) w = __builtin_nanf("");
   RowStats st;
@@ -629,6 +632,9 @@ static DistillArgs distill_args(const void* logits, long long rows, long long cl
   a.c2 = (float)(1.4426950408889634 / temperature);
   a.lscale = temperature * temperature;
   a.gscale = temperature;
+  // Each of q's exponents t is off by half a last place and its product by another, 2^-24 |t| each,
+  // and sum q |t| is at most log k where sum q is 1; 8 for the exponentials and their sum.
+  a.slack = (float)(8.0 + 2.0 * log((double)k)) * 0x1p-24f;
   return a;
 }
 

@@ -696,8 +696,8 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
         temperature^2 sum over the list of q (log q - log p),    q = softmax(teacher)
 
     or, with `rest`, q = exp(teacher) and the classes outside the list as one more, whose q is
-    what the list's leave of 1 (nothing, if they sum to more, or if the logits outside the list are
-    all -inf or there are none) and whose p is the sum of theirs.
+    what the list's leave of 1 (nothing, if that is within the rounding of their fp32 sum, or if
+    there are no logits outside the list but -inf) and whose p is the sum of theirs.
     Reductions as in cross_entropy, a mean over the rows that have a teacher.
 
     token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is

@@ -8,6 +8,8 @@ Counted, in units of E32 = 2^-24, for x = z / tau, d = x - max x:
   a logarithm 3 of its value, a product or a sum 1
 Exponentials below 2^-126 are zero."""
 
+import math
+
 import torch
 
 from train_ref import E32, TINY, U
@@ -157,7 +159,8 @@ class Distill:
             log_r = torch.where(torch.isfinite(o.m), log_r, -torch.inf)
             part = torch.where(left != 0, left * (torch.log(left) - log_r), zero)[..., 0]
             loss = loss + part
-            left_err = torch.where(others, w_err, zero)
+            # up to the list's own rounding, a rest counts as none
+            left_err = torch.where(others, w_err + (8 + 2 * math.log(k)) * E32, zero)
             log_left = torch.where(left > 0, torch.log(left), zero)
             err = err + (left_err * (_z0(log_left - log_r).abs() + 1)
                          + left * (o.rho + s.rho + 4 * E32 * (

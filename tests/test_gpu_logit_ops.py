@@ -481,6 +481,29 @@ def test_no_class_beside_the_list(T, v):
         assert torch.isnan(dz[nans]).all()
 
 
+@pytest.mark.parametrize("mask", [-1e9, -1e4, torch.finfo(F32).min])
+@pytest.mark.parametrize("v", [600, 9001, 50257, 140001])
+def test_masks_beside_the_list(T, v, mask):
+    """Masks of finite values: what the rounding of the teacher's list leaves of its 1 is far from
+    the masked classes, but is none of theirs: the same as with masks of -inf."""
+    k, n = 24, 60
+    teacher, student = normal(n, v, std=3.0), normal(n, v, seed=1)
+    hidden = torch.ones(v, dtype=torch.bool)
+    hidden[v // 2:v // 2 + 20] = False
+    teacher[:, hidden] = student[:, hidden] = mask
+    out = T.token_log_probs(teacher.to(DEV), top=k)
+    ids, t = out.top_ids.cpu(), out.top_log_probs.cpu()
+    left = 1 - torch.exp(t.double()).sum(1)
+    assert (left > 0).any() and left.max() < 8 * L.E32
+    c = L.Distill(student.masked_fill(hidden, -float("inf")), ids,
+                  t.masked_fill(t < mask / 2, -float("inf")), 1.0, True)
+    got = T.distillation(student.to(DEV), ids.to(DEV), t.to(DEV), rest=True, reduction="none")
+    close(got, c.loss, c.loss_err)
+    _, dz = T.distillation_step(student.to(DEV), ids.to(DEV), t.to(DEV), rest=True,
+                                reduction="sum")
+    close(dz, *c.grad_bound(1.0, F32))
+
+
 def test_the_rest_of_a_student_without_doubt(T):
     """Off the list the student has less than the smallest fp32: the gradient there still has the
     rest's own shape, where p / (sum of p) is 0 / 0."""
