@@ -249,20 +249,24 @@ void distill_row(DistillArgs a) {
   auto edge_logit = [&]() {
     return r.edge(t) < 0 || (REST && edge_marks >> t & 1) ? -INF : edge_logits[t];
   };
+  // (with 48 pieces a thread 2% less, 293 us for 2048 bf16 rows of 151936; with fewer up to 1% more)
+  auto here = [&]() { return HELD > 16 ? anew(r.pieces) : r.pieces; };
   Part p = {edge_logit(), 0.f};
   if constexpr (HELD > 0) {
+    int pieces = here();
     if constexpr (REST) {
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
         const int i = k * THREADS + t;
-        const uint32_t listed = i < r.pieces ? byte_marks[i] : 0;
+        const uint32_t listed = i < pieces ? byte_marks[i] : 0;
         if (listed) x[k] = without_listed(x[k], listed);
       }
       repack(x);
+      pieces = here();
     }
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
-      if (k * THREADS + t < r.pieces) p.m = maximum(p.m, piece_max<T>(x[k]));
+      if (k * THREADS + t < pieces) p.m = maximum(p.m, piece_max<T>(x[k]));
     repack(x);
   } else {
     p.s = __builtin_amdgcn_exp2f((p.m - (p.m == -INF ? 0.f : p.m)) * a.c2);
@@ -324,9 +328,10 @@ void distill_row(DistillArgs a) {
   const float tm = REST ? 0.f : waves_max(teacher_max, list_waves);
   if constexpr (HELD > 0) {
     p.s = __builtin_amdgcn_exp2f((edge_logit() - m0) * a.c2);
+    const int pieces = here();
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
-      if (k * THREADS + t < r.pieces) {
+      if (k * THREADS + t < pieces) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
           p.s += __builtin_amdgcn_exp2f((element<T>(x[k], j) - m0) * a.c2);
@@ -410,10 +415,11 @@ void distill_row(DistillArgs a) {
       return __builtin_bit_cast(i32x4, d);
     };
     if constexpr (HELD > 0) {
+      const int pieces = here();
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
         const int i = k * THREADS + t;
-        if (i < r.pieces) store_piece<T, PAST>(dz + r.piece_class(i), gradient(x[k]));
+        if (i < pieces) store_piece<T, PAST>(dz + r.piece_class(i), gradient(x[k]));
       }
     } else {
       for (int i0 = t; i0 < r.pieces; i0 += AHEAD * THREADS) {

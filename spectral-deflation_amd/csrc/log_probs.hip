@@ -91,52 +91,58 @@ __device__ __forceinline__ float cut_value(uint32_t cut) {
   return cut < 0x007FFFFFu ? -INF : key_value(cut);
 }
 
+// The smallest of a wave's, in all lanes.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ uint32_t lesser(uint32_t v) {
+  const uint32_t o = __builtin_amdgcn_update_dpp(-1, (int)v, CTRL, ROWS, 0xF, false);
+  return o < v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+  v = lesser<0x118>(lesser<0x114>(lesser<0x112>(lesser<0x111>(v))));
+  return __builtin_amdgcn_readlane(lesser<0x143, 0xC>(lesser<0x142, 0xA>(v)), 63);
+}
+
 constexpr int SEGMENTS = 8;   // of a thread's part of a long row, whose maxima are kept
 constexpr int CANDS = 1024;   // what is sorted out in the end, K <= TOP_MAX of them kept
 
 struct TopLds {
   uint32_t keys[512];   // of groups of threads
   u64 cand[CANDS];
-  uint32_t cut, most;
+  uint32_t cut;
   int slots[128];        // a counter for each step of the search over all classes
   int n;
 };
 
 // A lower bound of the K-th largest of a row, by the first wave: the K-th largest of the maxima of
-// 64 PER groups of threads, since K groups have a class that large.  A bit at a time, and no
-// further than to a few groups more than K: their classes are ranked by comparing all with all
-// (with K / 4 groups more, 256 of 50257 classes took 370 instead of 312 us).  The other waves go on
-// with the row's sum.
+// 64 PER groups of threads, since K groups have a class that large.  Halving what lies between the
+// smallest of them and the largest (the 64 largest of 8009 classes, 16384 rows: 81 us; bit by bit from
+// the first one on 86, two bits at a time 95), and no further than to a few groups more than K: their
+// classes are ranked by comparing all with all (with K / 4 groups more, 256 of 50257 classes took 370
+// instead of 312 us).  The other waves go on with the row's sum.
 template <int PER>
-__device__ __forceinline__ void group_cut(int K, TopLds& l) {
-  uint32_t k[PER], most = 0;
+__device__ __forceinline__ void group_cut(int K, uint32_t high, TopLds& l) {
+  uint32_t k[PER], low = ~0u;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     k[i] = l.keys[i * 64 + (threadIdx.x & 63)];
-    most = k[i] > most ? k[i] : most;
+    low = k[i] < low ? k[i] : low;
   }
+  low = wave_min(low);
   const int enough = K + K / 16 + 1;
-  uint32_t cut = 0;
   __builtin_amdgcn_s_setprio(3);   // the others wait for this one in the end
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t c = cut | 1u << b;
+  while (low < high) {   // ends: low grows or high falls
+    const uint32_t c = low + (high - low) / 2 + 1;
     int n = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) n += __popcll(__ballot(k[i] >= c));
     if (n >= K) {
-      cut = c;
+      low = c;
       if (n <= enough) break;
+    } else {
+      high = c - 1;
     }
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t o = __shfl_xor(most, d);
-    most = o > most ? o : most;
-  }
-  if (threadIdx.x == 0) {
-    l.cut = cut;
-    l.most = most;
-  }
+  if (threadIdx.x == 0) l.cut = low;
 }
 
 // The threads' maxima by groups: 256, or 512 for more than 64 classes.  (Of 256 and K = 64, about
@@ -161,9 +167,10 @@ __device__ __forceinline__ void put_group(int K, float largest, TopLds& l) {
   if (threadIdx.x < 128) l.slots[threadIdx.x] = 0;
 }
 template <int THREADS>
-__device__ __forceinline__ void find_cut(int K, TopLds& l) {
-  if (THREADS == 256 || K <= 64) group_cut<4>(K, l);
-  else group_cut<8>(K, l);
+__device__ __forceinline__ void find_cut(int K, float largest, TopLds& l) {
+  const uint32_t high = __builtin_amdgcn_readfirstlane(order_key(largest));
+  if (THREADS == 256 || K <= 64) group_cut<4>(K, high, l);
+  else group_cut<8>(K, high, l);
 }
 
 // A candidate from each lane that has one; all lanes of the wave come here.
@@ -208,9 +215,9 @@ __device__ __forceinline__ void put_pieces(int count, u64 from, const PieceList&
 // Then, if its classes are still too many, the first of them: twice as far each time, and the last
 // step halved.
 template <int THREADS, class Each>
-__device__ __forceinline__ void search_top(int K, int classes, const Each& each, TopLds& l) {
+__device__ __forceinline__ void search_top(int K, int classes, uint32_t most, const Each& each,
+                                           TopLds& l) {
   uint32_t value = l.cut;
-  const uint32_t most = l.most;
   int step = 0;
   auto count = [&](uint32_t least, uint32_t up_to, int first, int last) {
     int n = 0;
@@ -309,7 +316,7 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
 // largest class that few classes reach, whatever the distribution; those are gathered, piece by
 // piece, and ranked by comparing all with all.  The 64 largest take 173 us of the same rows, the
 // largest alone 154.  Where too many reach the bound (equal logits, or many large ones in one
-// thread's classes) the row is read again, as far as needed: 408 us for 8192 rows of zeros, 605
+// thread's classes) the row is read again, as far as needed: 420 us for 8192 rows of zeros, 624
 // where a mask leaves 20 classes of them.  Long rows keep the maxima of SEGMENTS parts of each
 // thread's pieces, and read again only the parts that reach the bound (20 of 131072 classes: 85 us,
 // 105 with all parts of such threads).
@@ -366,20 +373,21 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     if ((t & 63) == 0) maxes[t >> 6] = w;
     if constexpr (TOP) put_group<THREADS>(K, p.m, top);
     __syncthreads();
-    if constexpr (TOP)
-      if (t < 64) find_cut<THREADS>(K, top);
     m = waves_max(maxes, THREADS / 64);
+    if constexpr (TOP)
+      if (t < 64) find_cut<THREADS>(K, m, top);
   };
   if constexpr (HELD > 0) {
     // a small workgroup's waves pass over pieces behind the row (the 64 largest of 8009 classes,
     // 16384 rows: 92 to 86 us; at 1024 threads the test is a register too many, 173 to 181 us)
     const int wave = __builtin_amdgcn_readfirstlane(t);
+    int pieces = anew(r.pieces);
 #pragma unroll
     for (int k = 0; k < HELD; k += 2) {
       float m0 = -INF, m1 = -INF;
-      if (THREADS > 256 || k * THREADS + wave < r.pieces) {
-        m0 = k * THREADS + t < r.pieces ? piece_max<T>(x[k]) : -INF;
-        m1 = (k + 1) * THREADS + t < r.pieces ? piece_max<T>(x[k + 1]) : -INF;
+      if (THREADS > 256 || k * THREADS + wave < pieces) {
+        m0 = k * THREADS + t < pieces ? piece_max<T>(x[k]) : -INF;
+        m1 = (k + 1) * THREADS + t < pieces ? piece_max<T>(x[k + 1]) : -INF;
         p.m = maximum(p.m, maximum(m0, m1));
       }
       if constexpr (TOP) maxima.put(k, m0, m1);
@@ -388,9 +396,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     join_max();
     const float m0 = m == -INF ? 0.f : m;
     if (ec >= 0) add(ex, m0);
+    pieces = anew(pieces);
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
-      if (k * THREADS + t < r.pieces) {
+      if (k * THREADS + t < pieces) {
 #pragma unroll
         for (int j = 0; j < N; ++j) add(element<T>(x[k], j), m0);
       }
@@ -444,9 +453,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
     };
     if (r.edge(t) >= 0) again((float)z[r.edge(t)]);
     if constexpr (HELD > 0) {
+      const int pieces = anew(r.pieces);
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
-        if (k * THREADS + t < r.pieces) {
+        if (k * THREADS + t < pieces) {
 #pragma unroll
           for (int j = 0; j < N; ++j) again(element<T>(x[k], j));
         }
@@ -535,9 +545,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
         put_candidate(key != 0 && key >= from, key, top);
       }
       int count = 0;
+      const int pieces = anew(r.pieces);
 #pragma unroll
       for (int k = 0; k < HELD; ++k) {
-        const bool has = k * THREADS + t < r.pieces && maxima.get(k, x[k]) >= least;
+        const bool has = k * THREADS + t < pieces && maxima.get(k, x[k]) >= least;
         const u64 who = __ballot(has);
         if (who) {
           const int at = count + __builtin_amdgcn_mbcnt_hi(
@@ -592,7 +603,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       }
     }
     __syncthreads();
-    if (top.n > CANDS) search_top<THREADS>(K, a.classes, each, top);
+    if (top.n > CANDS) search_top<THREADS>(K, a.classes, order_key(p.m), each, top);
     put_top<THREADS>(K, [&](int place, float v, int c) {
       a.top_lp[row * K + place] = (v - p.m) * a.itau - log_s;
       a.top_ids[row * K + place] = c;
@@ -600,8 +611,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
   }
 }
 
-// 256 threads where they hold a row (of 8009 bf16 classes, 64 largest: 92 us for 16384 rows) and
-// have groups enough, else 1024 (the 128 largest of those: 149 us, by 1024 threads 282).
+// 256 threads where they hold a row (of 8009 bf16 classes, 64 largest: 81 us for 16384 rows) and
+// have groups enough, else 1024 (the 128 largest of those: 140 us, by 1024 threads 282).
 template <class T, bool TOP, bool PAST>
 static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
