@@ -379,7 +379,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
   };
   if constexpr (HELD > 0) {
     // a small workgroup's waves pass over pieces behind the row (the 64 largest of 8009 classes,
-    // 16384 rows: 92 to 86 us; at 1024 threads the test is a register too many, 173 to 181 us)
+    // 16384 rows: 92 to 86 us; at 1024 threads up to 1% more)
     const int wave = __builtin_amdgcn_readfirstlane(t);
     int pieces = anew(r.pieces);
 #pragma unroll
