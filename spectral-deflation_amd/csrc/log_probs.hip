@@ -108,7 +108,7 @@ constexpr int CANDS = 1024;   // what is sorted out in the end, K <= TOP_MAX of 
 struct TopLds {
   uint32_t keys[512];   // of groups of threads
   u64 cand[CANDS];
-  uint32_t cut;
+  uint32_t cut, most;
   int slots[128];        // a counter for each step of the search over all classes
   int n;
 };
@@ -128,6 +128,7 @@ __device__ __forceinline__ void group_cut(int K, uint32_t high, TopLds& l) {
     low = k[i] < low ? k[i] : low;
   }
   low = wave_min(low);
+  if (threadIdx.x == 0) l.most = high;
   const int enough = K + K / 16 + 1;
   __builtin_amdgcn_s_setprio(3);   // the others wait for this one in the end
   while (low < high) {   // ends: low grows or high falls
@@ -215,9 +216,9 @@ __device__ __forceinline__ void put_pieces(int count, u64 from, const PieceList&
 // Then, if its classes are still too many, the first of them: twice as far each time, and the last
 // step halved.
 template <int THREADS, class Each>
-__device__ __forceinline__ void search_top(int K, int classes, uint32_t most, const Each& each,
-                                           TopLds& l) {
+__device__ __forceinline__ void search_top(int K, int classes, const Each& each, TopLds& l) {
   uint32_t value = l.cut;
+  const uint32_t most = l.most;
   int step = 0;
   auto count = [&](uint32_t least, uint32_t up_to, int first, int last) {
     int n = 0;
@@ -603,7 +604,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       }
     }
     __syncthreads();
-    if (top.n > CANDS) search_top<THREADS>(K, a.classes, order_key(p.m), each, top);
+    if (top.n > CANDS) search_top<THREADS>(K, a.classes, each, top);
     put_top<THREADS>(K, [&](int place, float v, int c) {
       a.top_lp[row * K + place] = (v - p.m) * a.itau - log_s;
       a.top_ids[row * K + place] = c;
