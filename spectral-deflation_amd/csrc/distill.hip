@@ -20,9 +20,11 @@
 // the rounding of sum q: what that leaves of a teacher's 1 would otherwise be infinitely far from a
 // student whose rest is masked, and count a million times over where the mask is -1e9.
 //
-// An entry whose class is `ignore` is left out; a row whose first entry is has no teacher, loss 0
-// and gradient 0.  A class outside [0, V) makes its row NaN, as does a row without a softmax.  What
-// has q_j = 0 (or r = 0) adds nothing, whatever p is.  A class that is listed twice has two terms.
+// An entry whose class is `ignore` is left out, also where that is one of the V classes (then `none`,
+// by which token_log_probs marks its lists, is left out too); a row whose first entry is has no
+// teacher, loss 0 and gradient 0.  Another class outside [0, V) makes its row NaN, as does a row
+// without a softmax.  What has q_j = 0 (or r = 0) adds nothing, whatever p is.  A class that is
+// listed twice has two terms.
 #include "rows.h"
 
 namespace dmh {
@@ -43,8 +45,9 @@ struct DistillArgs {
   int self_count;        // the rows' launch counts them itself
   const float* count;    // ... their sum (gradient kernel), or null
   const float* gout;     // gradient of the loss (gradient kernel): one, or one a row
-  long long rows, zs, ds, ignore;
+  long long rows, zs, ds, ignore, none;   // none: stands for no class
   int classes, k, i64 /* 0 or 1 */, ttype, gout_rows;
+  int skip;              // `ignore` where it is a class, else -1: one register in a comparison
   float itau, c2;        // 1 / tau; log2(e) / tau
   float lscale, gscale;  // tau^2; tau times the gradient's scale
   float slack;           // a rest up to here is the list's rounding
@@ -74,6 +77,10 @@ struct RawEntry {
   }
 };
 
+__device__ __forceinline__ bool left_out(const DistillArgs& a, long long id) {
+  return id == a.none || id == a.ignore;
+}
+
 // A mean's gradient needs the number of rows that have a teacher at the start.  Up to SELF_ROWS
 // every workgroup of the rows' launch counts them itself; else a launch does, by the rows' first
 // entries, which lie k apart: in COUNTS parts, of one workgroup each (8192 rows, k = 64: 16 us by
@@ -83,7 +90,7 @@ constexpr int COUNTS = 64, SELF_ROWS = 256;
 __device__ __forceinline__ bool has_teacher(const DistillArgs& a, long long row) {
   RawEntry e;
   e.load(a, row * a.k);
-  return e.id(a) != a.ignore;
+  return !left_out(a, e.id(a));
 }
 __global__ __launch_bounds__(256) void distill_count(DistillArgs a, float* counts) {
   __shared__ float lds[4];
@@ -182,7 +189,7 @@ void distill_row(DistillArgs a) {
     if (i < r.pieces) x[k] = load_piece<T, PAST>(z + r.piece_class(i));
   }
   if (edge >= 0) edge_logits[t] = (float)z[edge];   // (registers are few)
-  if (named.id(a) == a.ignore) {
+  if (left_out(a, named.id(a))) {
     if (t == 0) a.row_loss[row] = 0.f;
     if (t == 0 && a.row_has) a.row_has[row] = 0.f;
     if (t < 6 && a.stats) a.stats[t * a.rows + row] = 0.f;
@@ -206,8 +213,8 @@ void distill_row(DistillArgs a) {
   // the list; entries that are left out have no class
   float most_t = -INF, bad = 0.f;   // a NaN where a class is outside
   auto entry = [&](int j, long long c, float q) {
-    const bool in = c >= 0 && c < a.classes;
-    if (!in && c != a.ignore) bad = __builtin_nanf("");
+    const bool known = c >= 0 && c < a.classes, in = known && (int)c != a.skip;
+    if (!known && c != a.none) bad = __builtin_nanf("");
     ids[j] = in ? (int)c : -1;
     ts[j] = in ? q : -INF;
     if (!REST && in) most_t = maximum(most_t, q);
@@ -507,9 +514,10 @@ static void launch_distill(hipStream_t stream, const DistillArgs& a, bool rest) 
 
 // The gradient from a forward pass's statistics, element by element, 256 threads for four pieces
 // each of a row; the listed classes are written again behind a barrier.  Bound by the memory: 78 us
-// for 2000 fp32 rows of 32003 (512 MB, 6.6 TB/s; the logits are partly in the last-level cache still).
+// for 2000 fp32 rows of 32003 (512 MB, 6.6 TB/s; the logits are partly in the last-level cache still).  (64
+// registers at most: with two more only seven waves fit.)
 template <class T, bool PAST>
-__global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
+__global__ __launch_bounds__(256, 8) void distill_grad(DistillArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;
   __shared__ int ids[LIST_MAX];
   __shared__ float qs[LIST_MAX];
@@ -524,7 +532,7 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
   const Row<T> r(z, a.classes);
   const int first = blockIdx.y * THREADS * AHEAD, i0 = first + t;
   const int ec = blockIdx.y == 0 ? r.edge(t) : -1;
-  if (load_index(a.ids, a.i64, row * K) == a.ignore) {
+  if (left_out(a, load_index(a.ids, a.i64, row * K))) {
     const type zero = {};
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
@@ -557,7 +565,7 @@ __global__ __launch_bounds__(256) void distill_grad(DistillArgs a) {
     RawEntry e;
     e.load(a, row * K + j);
     const long long c = e.id(a);
-    const bool in = c >= 0 && c < a.classes;
+    const bool in = c >= 0 && c < a.classes && (int)c != a.skip;
     ids[j] = in ? (int)c : -1;
     qs[j] = in ? natural_exp(e.value(a) - st.tm) * st.qs : 0.f;
   }
@@ -629,7 +637,9 @@ static DistillArgs distill_args(const void* logits, long long rows, long long cl
   a.rows = rows;
   a.zs = z_rstride;
   a.ds = d_rstride;
+  a.none = no_class(ignore_index, classes);
   a.ignore = ignore_index;
+  a.skip = a.none == ignore_index ? -1 : (int)ignore_index;
   a.classes = (int)classes;
   a.k = k;
   a.i64 = ids_64 != 0;

@@ -794,7 +794,7 @@ int dmh_log_probs(hipStream_t stream, const void* logits, int dtype, long long r
   a.rows = rows;
   a.zs = z_rstride;
   a.ignore = ignore_index;
-  a.none = ignore_index < 0 || ignore_index >= classes ? ignore_index : -100;
+  a.none = no_class(ignore_index, classes);
   a.classes = (int)classes;
   a.t64 = tokens_64 != 0;
   a.top = top;

@@ -117,6 +117,11 @@ __device__ __forceinline__ float waves_sum(const float* lds, int waves) {
   return lane(row16_sum(i < waves ? lds[i] : 0.f), 15);
 }
 
+// What stands for no class in lists of classes: ignore_index, unless that is a class.
+inline long long no_class(long long ignore, long long classes) {
+  return ignore < 0 || ignore >= classes ? ignore : -100;
+}
+
 // A row in aligned pieces of 16 bytes, and the classes before the first and behind the last one,
 // up to seven on each side, which the first sixteen threads of a row take one by one.  Rows of an
 // odd number of classes start anywhere; with pieces from the row's start instead the loads

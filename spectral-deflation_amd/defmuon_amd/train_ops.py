@@ -602,10 +602,10 @@ def token_log_probs(logits, tokens=None, top=0, temperature=1.0, ignore_index=-1
 
     tokens: int64 or int32 (...); top up to 256.  The three log probabilities and entropies take
     part in autograd.  A row whose token is ignore_index gives zeros, and ignore_index for its
-    classes (-100 where that is a class), which distillation skips in turn; another token outside
-    the classes gives NaN for its log probability (and its row's gradient, if that is wanted).  A
-    row without a softmax (a NaN, an infinity, -inf alone) gives NaN, and the classes 0, 1, ...
-    for its top."""
+    classes (-100 where that is a class), which distillation leaves out in turn; another token
+    outside the classes gives NaN for its log probability (and its row's gradient, if that is
+    wanted).  A row without a softmax (a NaN, an infinity, -inf alone) gives NaN, and the classes
+    0, 1, ... for its top."""
     what = "token_log_probs"
     _eager(what, function=True)
     _float(logits, what, "logits")
@@ -705,8 +705,9 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
     k up to 1024; a class named twice counts with both.  The loss carries the rounding of fp32
     logarithms times temperature^2, about 1e-7 of it, and a divergence of zero may come out that far
     below.  An entry whose class is ignore_index is left out, and a row whose first entry is counts
-    for nothing; another class outside the logits' makes its row NaN, as does a row without a
-    softmax.  An entry of -inf adds nothing, whatever the logits say; a row of those alone is NaN,
+    for nothing.  (An ignore_index that is one of the classes leaves out that class and, as
+    token_log_probs marks its lists then, -100.)  Another class outside the logits' makes its row
+    NaN, as does a row without a softmax.  An entry of -inf adds nothing, whatever the logits say; a row of those alone is NaN,
     with `rest` it leaves all to the others.  The teacher takes no gradient."""
     _eager("distillation", function=True)
     _distill_args(logits, ids, teacher, temperature, reduction, "distillation")

@@ -911,3 +911,64 @@ def test_top_classes_among_equal_ones(T, v, dtype):
     many = z.repeat(60, 1).to(DEV)          # more rows than fit at a time
     got = T.token_log_probs(many, top=64)
     assert torch.equal(got.top_ids.cpu(), L.top(z, 64).repeat(60, 1))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("v,k", [(60, 20), (600, 3), (9001, 70), (50257, 64), (140001, 300)])
+def test_entries_left_out_by_a_class(T, v, k, rest):
+    """An ignore_index that is a class: its entries are left out wherever they stand, and so is
+    -100, by which token_log_probs then marks its lists."""
+    none = 11
+    z, ids, t = kd_case(12, v, k, cover=0.8, ragged=False)
+    z[:, none] += 6.0                       # a class that counts
+    ids = torch.where(ids == none, none + 1, ids)
+    ids[0, k // 2] = none                   # in the middle
+    ids[2, -1] = none                       # at the end
+    ids[3, 1:] = none                       # all but the first
+    ids[4, 0] = none                        # no teacher
+    ids[5, -1] = -100
+    ids[7, 1] = none
+    ids[7, -1] = -100
+    ids[8] = none
+    same = torch.where(ids == -100, none, ids)
+    c = L.Distill(z, same, t, 1.5, rest, none)
+    assert c.live.tolist() == [r not in (1, 4, 6, 8, 11) for r in range(12)]
+    assert torch.isfinite(c.loss).all()
+    loss, err, count = c.mean()
+    kw = dict(temperature=1.5, rest=rest, ignore_index=none)
+    zg, tg = z.to(DEV), t.to(DEV)
+    for ig in (ids.to(DEV), ids.int().to(DEV)):
+        close(T.distillation(zg, ig, tg, reduction="none", **kw), c.loss, c.loss_err)
+        close(T.distillation(zg, ig, tg, **kw), loss, err)
+        got, dz = T.distillation_step(zg, ig, tg, **kw)
+        close(got, loss, err)
+        close(dz, *c.grad_bound(1.0 / count, F32))
+        work = zg.clone()
+        got, dz = T.distillation_step(work, ig, tg, reduction="sum", inplace=True, **kw)
+        close(got, loss * count, err * count)
+        close(dz, *c.grad_bound(1.0, F32))
+        leaf = zg.clone().requires_grad_()
+        (dz,) = torch.autograd.grad(T.distillation(leaf, ig, tg, **kw), leaf)
+        close(dz, *c.grad_bound(1.0 / count, F32))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_a_teachers_padding_that_is_a_class(T, rest):
+    """The same ignore_index, a class, in the teacher's pass and in the student's."""
+    z, y = normal(300, 500, std=2.0), torch.arange(300) % 40
+    z[3::4, 0] += 9.0                       # class 0 at the head of some lists
+    student = normal(300, 500, seed=1)
+    out = T.token_log_probs(z.to(DEV), y.to(DEV), top=8, ignore_index=0)
+    ids = L.top(z, 8)
+    ids[y == 0] = 0
+    c = L.Distill(student, ids, out.top_log_probs.cpu(), 1.0, rest, 0)
+    loss, err, count = c.mean()
+    assert count == int(((y != 0) & (ids[:, 0] != 0)).sum()) and torch.isfinite(loss)
+    kw = dict(rest=rest, ignore_index=0)
+    got, dz = T.distillation_step(student.to(DEV), out.top_ids, out.top_log_probs, **kw)
+    close(got, loss, err)
+    close(dz, *c.grad_bound(1.0 / count, F32))
+    leaf = student.to(DEV).requires_grad_()
+    got = T.distillation(leaf, out.top_ids, out.top_log_probs, **kw)
+    close(got, loss, err)
+    close(torch.autograd.grad(got, leaf)[0], *c.grad_bound(1.0 / count, F32))
