@@ -200,7 +200,8 @@ void distill_row(DistillArgs a) {
     }
     return;
   }
-  // One wave of entries clears the marks that it sets itself, without a barrier.
+  // One wave of entries clears the marks that it sets itself, other lanes than set them: without a
+  // barrier, but in this order.
   if (t == 0) {
     edge_marks = 0;
     twice = 0;
@@ -209,7 +210,14 @@ void distill_row(DistillArgs a) {
   const int words = ((r.pieces < SPAN ? r.pieces : SPAN) + 15) / 16;
   if (t < marking)
     for (int i = t; i < words; i += marking) ((i32x4*)marks)[i] = i32x4{0, 0, 0, 0};
-  if ((REST || !HELD) && marking > 64) __syncthreads();
+  if (REST || !HELD) {
+    if (marking > 64) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
   // the list; entries that are left out have no class
   float most_t = -INF, bad = 0.f;   // a NaN where a class is outside
   auto entry = [&](int j, long long c, float q) {

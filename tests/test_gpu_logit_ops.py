@@ -972,3 +972,20 @@ def test_a_teachers_padding_that_is_a_class(T, rest):
     got = T.distillation(leaf, out.top_ids, out.top_log_probs, **kw)
     close(got, loss, err)
     close(torch.autograd.grad(got, leaf)[0], *c.grad_bound(1.0 / count, F32))
+
+
+@pytest.mark.parametrize("n,v,k", [(700, 300, 64), (700, 70, 64), (40, 9001, 33), (12, 140001, 64)])
+def test_lists_that_one_wave_marks(T, n, v, k):
+    """Up to 64 entries: one wave's lanes clear the marks of a row, and others of them set these;
+    classes in a lump, so that lanes share words, some of them twice."""
+    z, ids, t = kd_case(n, v, k, cover=0.7, ragged=False)
+    near = (torch.arange(k) + torch.arange(n)[:, None]) % min(v, 97)
+    near[::3, 1] = near[::3, 0]
+    near[::7, -1] = near[::7, k // 2]
+    ids = torch.where(ids >= 0, near, ids)
+    c = L.Distill(z, ids, t, 1.0, True)
+    zg, ig, tg = z.to(DEV), ids.to(DEV), t.to(DEV)
+    for _ in range(3):
+        close(T.distillation(zg, ig, tg, rest=True, reduction="none"), c.loss, c.loss_err)
+        close(T.distillation_step(zg, ig, tg, rest=True, reduction="sum")[1],
+              *c.grad_bound(1.0, F32))
