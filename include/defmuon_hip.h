@@ -322,7 +322,8 @@ int dmh_cross_entropy_grad_stats(dmh_stream_t stream, const void* logits, int dt
  * A row whose token is ignore_index gives zeros, and ignore_index for top_ids (-100 if that is a
  * class); another token outside [0, classes) gives NaN for its log probability.  A row without a
  * softmax gives NaN, and 0 .. top - 1 for top_ids.  1e-6 <= temperature <= 1e6, classes <= 2^27, rows < 2^22.
- * dmh_log_probs_grad: the logits' gradient from the outputs' (each may be NULL). */
+ * dmh_log_probs_grad: the logits' gradient, in other memory than theirs, from the outputs' (each
+ * may be NULL). */
 int dmh_log_probs(dmh_stream_t stream, const void* logits, int dtype, long long rows,
                   long long classes, long long z_rstride, const void* tokens, int tokens_64,
                   long long ignore_index, float temperature, int top, float* log_probs,
@@ -345,7 +346,7 @@ int dmh_log_probs_grad(dmh_stream_t stream, const void* logits, int dtype, long 
  * make their row NaN.  Reductions, loss, count, dlogits and grad_scale as for dmh_cross_entropy.
  * stats: 6 x rows floats for dmh_distill_grad; may be NULL.  dmh_distill_grad: the gradient from
  * these (and count, for a mean; NULL otherwise), times *grad_out, or grad_out[row] if
- * grad_out_rows.
+ * grad_out_rows, in other memory than the logits'.
  * 1 <= k <= 1024, 1e-6 <= temperature <= 1e6, classes <= 2^27, rows < 2^22. */
 int dmh_distill_workspace_size(long long rows, size_t* bytes);
 int dmh_distill(dmh_stream_t stream, const void* logits, int dtype, long long rows,

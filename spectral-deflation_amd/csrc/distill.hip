@@ -745,6 +745,10 @@ int dmh_distill_grad(hipStream_t stream, const void* logits, int dtype, long lon
     set_error("dmh_distill_grad: null tensor");
     return DMH_EINVAL;
   }
+  if (dlogits == logits) {   // the listed classes' are read again
+    set_error("dmh_distill_grad: the gradient cannot take the logits' place");
+    return DMH_EINVAL;
+  }
   DistillArgs a = distill_args(logits, rows, classes, z_rstride, ids, ids_64, k, teacher,
                                teacher_dtype, ignore_index, temperature, (float*)stats, count,
                                dlogits, d_rstride);

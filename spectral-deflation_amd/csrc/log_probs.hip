@@ -822,6 +822,10 @@ int dmh_log_probs_grad(hipStream_t stream, const void* logits, int dtype, long l
     set_error("dmh_log_probs_grad: null tensor");
     return DMH_EINVAL;
   }
+  if (dlogits == logits) {   // the listed classes' are read again
+    set_error("dmh_log_probs_grad: the gradient cannot take the logits' place");
+    return DMH_EINVAL;
+  }
   LogProbGradArgs a{};
   a.z = logits;
   a.tokens = tokens;

@@ -349,3 +349,14 @@ def test_a_temperature_that_is_no_number(stand_in):
             T.token_log_probs(z.float(), temperature=tau)
         with pytest.raises(NativeError, match="temperature"):
             T.distillation(z.float(), ids, t.float(), temperature=tau)
+
+
+def test_gradients_over_the_logits_are_refused(lib):
+    """The gradient kernels read the listed classes' logits again behind their row's gradient."""
+    z, other = ctypes.c_void_p(256), ctypes.c_void_p(4096)   # never read
+    assert lib.dmh_log_probs_grad(None, z, 0, 2, 9, 9, other, 1, -100, 1.0, 3, other, other, other,
+                                  None, other, z, 9) == 1
+    assert b"dmh_log_probs_grad" in lib.dmh_last_error()
+    assert lib.dmh_distill_grad(None, z, 0, 2, 9, 9, other, 1, 3, other, 0, -100, 1.0, other, None,
+                                other, 0, z, 9) == 1
+    assert b"dmh_distill_grad" in lib.dmh_last_error()
