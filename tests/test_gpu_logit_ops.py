@@ -989,3 +989,94 @@ def test_lists_that_one_wave_marks(T, n, v, k):
         close(T.distillation(zg, ig, tg, rest=True, reduction="none"), c.loss, c.loss_err)
         close(T.distillation_step(zg, ig, tg, rest=True, reduction="sum")[1],
               *c.grad_bound(1.0, F32))
+
+
+@pytest.mark.parametrize("n,v,dtype", [(4300, 50257, BF16), (3100, 33001, F32), (26000, 8009, BF16)])
+def test_log_probs_past_the_caches(T, n, v, dtype):
+    """Logits of more than 384 MiB without a gradient: rows held by a workgroup of either size, and
+    streamed ones; those whose top is searched for among them."""
+    assert n * v * dtype.itemsize >= 384 << 20
+    z = torch.randn(n, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    z = z.mul_(2.0).to(dtype)
+    z[1] = 0.0
+    z[2, 20:] = -float("inf")
+    z[3, v // 2:] = 9.0
+    y = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    y[4] = -100
+    some = torch.tensor([0, 1, 2, 3, 4, 5, n // 2, n - 2, n - 1])
+    y[2] = 7
+    zs, ys = z[some.to(DEV)].cpu(), y[some]
+    for k in (0, 1, 30, 200):
+        want, ids = L.log_probs(zs, ys, k)
+        got = T.token_log_probs(z, y.to(DEV), top=k)
+        for name, (value, bound) in want.items():
+            close(getattr(got, name)[some.to(DEV)], value, bound.nan_to_num(0.0, 0.0, 0.0),
+                  (k, name))
+        if k:
+            assert torch.equal(got.top_ids[some.to(DEV)].cpu(), ids), k
+
+
+def test_as_many_rows_as_there_may_be(T, Err):
+    n, v, k = (1 << 22) - 1, 130, 129
+    z = torch.randn(n, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).to(BF16)
+    some = torch.cat([torch.arange(50), torch.arange(n - 50, n)])
+    at = some.to(DEV)
+    zs = z[at].cpu()
+    y = torch.arange(n, device=DEV) % v
+    want, ids = L.log_probs(zs, y[at].cpu(), k)
+    out = T.token_log_probs(z, y, top=k)
+    for name, (value, bound) in want.items():
+        close(getattr(out, name)[at], value, bound, name)
+    assert torch.equal(out.top_ids[at].cpu(), ids)
+    leaf = z.requires_grad_()
+    gh = normal(100)
+    full = torch.zeros(n, device=DEV)
+    full[at] = gh.to(DEV)
+    del out
+    (dz,) = torch.autograd.grad(T.token_log_probs(leaf, y).entropy, leaf, full)
+    close(dz[at], *L.log_probs_grad(zs, None, None, None, gh, None, 1.0, BF16))
+    z = z.detach()
+    ids = torch.stack([y, (y + 4) % v], 1)
+    ids[5::7, 0] = -100
+    t = torch.log(torch.tensor([0.5, 0.2], device=DEV)).repeat(n, 1)
+    c = L.Distill(zs, ids[at].cpu(), t[at].cpu(), 1.0, True)
+    close(T.distillation(z, ids, t, rest=True, reduction="none")[at], c.loss, c.loss_err)
+    count = n - len(range(5, n, 7))
+    (dz,) = torch.autograd.grad(T.distillation(leaf, ids, t, rest=True), leaf)
+    close(dz[at], *c.grad_bound(1.0 / count, BF16))
+    dz = T.distillation_step(z, ids, t, rest=True, grad_scale=1e6, inplace=True)[1]
+    close(dz[at], *c.grad_bound(1e6 / count, BF16))
+    more = z[:1].expand(n + 1, v)
+    for call in (lambda: T.token_log_probs(more),
+                 lambda: T.distillation(more, ids[:1].expand(n + 1, 2), t[:1].expand(n + 1, 2))):
+        with pytest.raises(Err, match="bad arguments"):
+            call()
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("n,v,dtype", [(26000, 8009, BF16), (1700, 131077, BF16), (1600, 70001, F32),
+                                       (900, 120001, F32)])
+def test_distillation_past_the_caches(T, n, v, dtype, rest):
+    """Logits of more than 384 MiB: rows held by workgroups of each size, and streamed ones."""
+    assert n * v * dtype.itemsize >= 384 << 20
+    k = 40
+    z = torch.randn(n, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    z = z.mul_(2.0).to(dtype)
+    ids = (torch.arange(n)[:, None] * 37 + torch.arange(k) * (v // 41)) % v
+    ids[1::5] = -100
+    ids[0, 3] = ids[0, 2]
+    ids[2, 7:] = -100
+    t = torch.log_softmax(normal(n, k, std=2.0, seed=4), 1) - 0.1
+    some = torch.tensor([0, 1, 2, 3, 4, 7, n // 2, n - 3, n - 2, n - 1])
+    at = some.to(DEV)
+    c = L.Distill(z[at].cpu(), ids[some], t[some], 1.4, rest)
+    count = int((ids[:, 0] >= 0).sum())
+    ig, tg, kw = ids.to(DEV), t.to(DEV), dict(temperature=1.4, rest=rest)
+    close(T.distillation(z, ig, tg, reduction="none", **kw)[at], c.loss, c.loss_err)
+    dz = T.distillation_step(z, ig, tg, **kw)[1]
+    close(dz[at], *c.grad_bound(1.0 / count, dtype))
+    leaf = z.clone().requires_grad_()
+    (dz,) = torch.autograd.grad(T.distillation(leaf, ig, tg, **kw), leaf)
+    close(dz[at], *c.grad_bound(1.0 / count, dtype))
+    dz = T.distillation_step(z, ig, tg, reduction="sum", inplace=True, **kw)[1]
+    close(dz[at], *c.grad_bound(1.0, dtype))
