@@ -340,7 +340,8 @@ int dmh_log_probs_grad(dmh_stream_t stream, const void* logits, int dtype, long 
  * contiguous.  With p = softmax(logits / temperature):
  *   q = softmax(teacher):  loss = temperature^2 sum over the list of q (log q - log p)
  *   rest != 0:             q = exp(teacher), and the classes outside the list are one more, with
- *                          max(0, 1 - sum q) and the sum of their p
+ *                          max(0, 1 - sum q) and the sum of their p; what is within the rounding
+ *                          of an fp32 list's sum counts as 0, that of a 16-bit list is a rest
  * Entries whose class is ignore_index (where that is a class, also -100) are left out, rows whose
  * first entry is count for nothing and get a gradient of zero; other classes outside [0, classes)
  * make their row NaN.  Reductions, loss, count, dlogits and grad_scale as for dmh_cross_entropy.

@@ -697,7 +697,9 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
 
     or, with `rest`, q = exp(teacher) and the classes outside the list as one more, whose q is
     what the list's leave of 1 (nothing, if that is within the rounding of their fp32 sum, or if
-    there are no logits outside the list but -inf) and whose p is the sum of theirs.
+    there are no logits outside the list but -inf) and whose p is the sum of theirs.  The rounding
+    of a 16-bit list (up to 4e-3 of 1 for bf16) is a rest like any other: keep lists in fp32 where
+    the student's other classes are masked by finite values, from which it would be far.
     Reductions as in cross_entropy, a mean over the rows that have a teacher.
 
     token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is
