@@ -697,9 +697,10 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
 
     or, with `rest`, q = exp(teacher) and the classes outside the list as one more, whose q is
     what the list's leave of 1 (nothing, if that is within the rounding of their fp32 sum, or if
-    there are no logits outside the list but -inf) and whose p is the sum of theirs.  The rounding
-    of a 16-bit list (up to 4e-3 of 1 for bf16) is a rest like any other: keep lists in fp32 where
-    the student's other classes are masked by finite values, from which it would be far.
+    there are no logits outside the list but -inf) and whose p is the sum of theirs.  What
+    16-bit lists leave by their rounding (of bf16, 2^-8 of each logarithm) is a rest like any
+    other: keep lists in fp32 where the student's other classes are masked by finite values, from
+    which it would be far.
     Reductions as in cross_entropy, a mean over the rows that have a teacher.
 
     token_log_probs(teacher_logits, top=k, temperature=temperature) gives such lists: teacher is
@@ -709,8 +710,9 @@ def distillation(logits, ids, teacher, temperature=1.0, rest=False, ignore_index
     below.  An entry whose class is ignore_index is left out, and a row whose first entry is counts
     for nothing.  (An ignore_index that is one of the classes leaves out that class and, as
     token_log_probs marks its lists then, -100.)  Another class outside the logits' makes its row
-    NaN, as does a row without a softmax.  An entry of -inf adds nothing, whatever the logits say; a row of those alone is NaN,
-    with `rest` it leaves all to the others.  The teacher takes no gradient."""
+    NaN, as does a row without a softmax.  An entry of -inf adds nothing, whatever the logits say;
+    a row of those alone is NaN, with `rest` it leaves all to the others.  The teacher takes no
+    gradient."""
     _eager("distillation", function=True)
     _distill_args(logits, ids, teacher, temperature, reduction, "distillation")
     if _is_tracing() or torch.is_grad_enabled() and logits.requires_grad:
