@@ -148,11 +148,12 @@ __device__ __forceinline__ float natural_log(float x) { return __builtin_amdgcn_
 // sum, and the first writes the gradient), and with REST which logits are not the rest's: they
 // become -inf before the row is summed.
 //
-// Bound by the memory: 8192 bf16 rows of 50257 with gradient, lists of 64, take 292 us (5.6 TB/s) and
-// with REST 297, of an odd stride 306 and 317; the losses alone 128 and 150.  The listed classes'
-// second writes are 4 to 15 us of these.  (Put into their pieces before the first and only write they
-// cost as much in waiting for the list: 290 us, but 245 instead of 239 for 2048 rows of 131072, and
-// 10% more where rows are few or short.)
+// Bound by the memory: 8192 bf16 rows of 50257 with gradient, lists of 64, take 297 us (5.5 TB/s) and
+// with REST 307, of an odd stride 310 and 325; the losses alone 142 and 165, there the vector units
+// too (passes among others, their two small launches included; the shortest of five averages).  The
+// listed classes' second writes are 4 to 15 us of these.  (Put into their pieces before the first and
+// only write they cost as much in waiting for the list: 1% less, but 2% more for 2048 rows of 131072,
+// and 10% more where rows are few or short.)
 template <class T, int THREADS, int HELD, bool REST, bool GRAD, bool PAST>
 __global__ __launch_bounds__(THREADS, HELD > 16 ? 2 : HELD > 8 ? 4 : 8)
 void distill_row(DistillArgs a) {
@@ -264,7 +265,7 @@ void distill_row(DistillArgs a) {
   auto edge_logit = [&]() {
     return r.edge(t) < 0 || (REST && edge_marks >> t & 1) ? -INF : edge_logits[t];
   };
-  // (with 48 pieces a thread 2% less, 293 us for 2048 bf16 rows of 151936; with fewer up to 1% more)
+  // (with 48 pieces a thread 2% less, of 2048 bf16 rows of 151936; with fewer up to 1% more)
   auto here = [&]() { return HELD > 16 ? anew(r.pieces) : r.pieces; };
   Part p = {edge_logit(), 0.f};
   if constexpr (HELD > 0) {
@@ -485,7 +486,9 @@ void distill_row(DistillArgs a) {
 }
 
 // The fewest threads that hold a row; longer rows are held for the gradient as far as registers
-// go, and streamed for the loss alone.
+// go, and streamed for the loss alone.  (2048 bf16 rows with gradient: of 131072 233 us, of 151936 298,
+// of 200064, which are read twice, 440.)  Rows of few classes are bound by a workgroup's latency:
+// 16384 of 256 to 2000 bf16 classes take 30 us, with gradient 52 to 57.
 template <class T, bool REST, bool GRAD, bool PAST>
 static void launch_rows(hipStream_t stream, const DistillArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
@@ -522,8 +525,8 @@ static void launch_distill(hipStream_t stream, const DistillArgs& a, bool rest) 
 
 // The gradient from a forward pass's statistics, element by element, 256 threads for four pieces
 // each of a row; the listed classes are written again behind a barrier.  Bound by the memory: 78 us
-// for 2000 fp32 rows of 32003 (512 MB, 6.6 TB/s; the logits are partly in the last-level cache still).  (64
-// registers at most: with two more only seven waves fit.)
+// for 2000 fp32 rows of 32003 (512 MB, 6.6 TB/s; the logits are partly in the last-level cache
+// still).  Not more than 64 registers: with two more only seven waves fit.
 template <class T, bool PAST>
 __global__ __launch_bounds__(256, 8) void distill_grad(DistillArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;

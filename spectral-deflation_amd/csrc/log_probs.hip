@@ -65,7 +65,7 @@ __device__ __forceinline__ u64 rank_key(float x, int c) {
 
 // The largest of each of HELD pieces, for later: two 16-bit values a register, while fp32 ones are
 // found again from the piece, in three instructions.  (A register for each piece made the compiler
-// spill a few others, whose reloads took the 8192 rows below from 176 to 280 us.)
+// spill a few others, whose reloads made the 8192 rows below 60% slower.)
 template <class T, int HELD>
 struct PieceMaxima {
   typedef T pair __attribute__((ext_vector_type(2)));
@@ -115,10 +115,10 @@ struct TopLds {
 
 // A lower bound of the K-th largest of a row, by the first wave: the K-th largest of the maxima of
 // 64 PER groups of threads, since K groups have a class that large.  Halving what lies between the
-// smallest of them and the largest (the 64 largest of 8009 classes, 16384 rows: 81 us; bit by bit from
-// the first one on 86, two bits at a time 95), and no further than to a few groups more than K: their
-// classes are ranked by comparing all with all (with K / 4 groups more, 256 of 50257 classes took 370
-// instead of 312 us).  The other waves go on with the row's sum.
+// smallest of them and the largest (bit by bit from the first one on, the 64 largest of 8009 classes
+// took 6% longer, two bits at a time 17%), and no further than to a few groups more than K: their
+// classes are ranked by comparing all with all (with K / 4 groups more, 256 of 50257 classes took
+// 19% longer).  The other waves go on with the row's sum.
 template <int PER>
 __device__ __forceinline__ void group_cut(int K, uint32_t high, TopLds& l) {
   uint32_t k[PER], low = ~0u;
@@ -308,19 +308,23 @@ __device__ __forceinline__ void put_top(int K, const Put& put, const TopLds& l) 
 // One row by THREADS threads that hold it in registers, HELD pieces each (packed between the
 // steps), or for HELD = 0 a workgroup that streams it.
 //
+// (Figures: a pass among others, the shortest of five averages of 30, three sets of logits in turn.)
+//
 // Without a top it reads each logit once and is bound by the memory, the vector units not far
-// behind: 8192 bf16 rows of 50257 take 138 us (5.9 TB/s), 1000 fp32 rows of 131072 80 (6.5).  Two
+// behind: 8192 bf16 rows of 50257 take 143 us (5.8 TB/s), 1000 fp32 rows of 131072 82 (6.4).  Two
 // barriers and reductions by lane shifts, one for the maximum and one for the sums, take less of
-// them than one that joins parts of different maxima (176 us).
+// them than one that joins parts of different maxima (a fifth more).  Rows of few classes are bound
+// by the workgroups' own latency: 16384 of 256, 600, 1000 or 2000 bf16 classes all take 19 to 22 us.
 //
 // Top classes: the threads' maxima, which the sums need anyway, give a lower bound of the K-th
 // largest class that few classes reach, whatever the distribution; those are gathered, piece by
-// piece, and ranked by comparing all with all.  The 64 largest take 173 us of the same rows, the
-// largest alone 154.  Where too many reach the bound (equal logits, or many large ones in one
-// thread's classes) the row is read again, as far as needed: 420 us for 8192 rows of zeros, 624
-// where a mask leaves 20 classes of them.  Long rows keep the maxima of SEGMENTS parts of each
-// thread's pieces, and read again only the parts that reach the bound (20 of 131072 classes: 85 us,
-// 105 with all parts of such threads).
+// piece, and ranked by comparing all with all.  The 64 largest take 176 us of the same rows, the
+// largest alone 160, 256 of them 312.  Where too many reach the bound (equal logits, or many large
+// ones in one thread's classes) the row is read again, as far as needed: 426 us for 8192 rows of
+// zeros, 634 where a mask leaves 20 classes of them (181 without a top: such rows are summed twice).
+// Long rows keep the maxima of SEGMENTS parts of each thread's pieces, and read again only the parts
+// that reach the bound (20 of 131072 classes: 87 us, a fifth more with all parts of such threads).
+// Of few classes, 20 take 16384 rows to 57 us: a workgroup's latency again.
 template <class T, int THREADS, int HELD, bool TOP, bool PAST>
 __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(LogProbArgs a) {
   __shared__ float maxes[16], sums[16], weights[16];   // of the waves
@@ -379,8 +383,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
       if (t < 64) find_cut<THREADS>(K, m, top);
   };
   if constexpr (HELD > 0) {
-    // a small workgroup's waves pass over pieces behind the row (the 64 largest of 8009 classes,
-    // 16384 rows: 92 to 86 us; at 1024 threads up to 1% more)
+    // a small workgroup's waves pass over pieces behind the row (7% less for the 64 largest of 8009
+    // classes; at 1024 threads up to 1% more)
     const int wave = __builtin_amdgcn_readfirstlane(t);
     int pieces = anew(r.pieces);
 #pragma unroll
@@ -612,8 +616,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 6 : 8) void log_prob_row(
   }
 }
 
-// 256 threads where they hold a row (of 8009 bf16 classes, 64 largest: 81 us for 16384 rows) and
-// have groups enough, else 1024 (the 128 largest of those: 140 us, by 1024 threads 282).
+// 256 threads where they hold a row (of 8009 bf16 classes, 64 largest: 85 us for 16384 rows) and
+// have groups enough, else 1024 (the 128 largest of those: 142 us, by 1024 threads twice that; 256:
+// 464).  Rows of 17000 bf16 classes give 1024 threads two of their eight pieces each, and take 65 us
+// for 8192 (4.3 TB/s); workgroups between the two, or of less than 256, were not tried.
 template <class T, bool TOP, bool PAST>
 static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
   const int pieces = a.classes / Piece<T>::N;   // at most
@@ -627,8 +633,8 @@ static void launch_rows(hipStream_t stream, const LogProbArgs& a) {
 }
 template <class T>
 static void launch_log_probs(hipStream_t stream, const LogProbArgs& a) {
-  // (the gradient's launch comes next, and finds a part of the logits still in the cache: both 215
-  // instead of 236 us for 4096 bf16 rows of 50257)
+  // (the gradient's launch comes next, and finds a part of the logits still in the cache: both 206
+  // instead of 232 us for 4096 bf16 rows of 50257, 432 instead of 454 for 8192)
   if (!a.stats && past_caches<T>(a.rows, a.classes))
     a.top ? launch_rows<T, true, true>(stream, a) : launch_rows<T, false, true>(stream, a);
   else
@@ -650,7 +656,7 @@ struct LogProbGradArgs {
 
 // Element by element, 256 threads for four pieces each of a row; the listed classes (the token and
 // the top ones) are written again behind a barrier, each by one thread with the sum of its terms.
-// Bound by the memory: 4096 bf16 rows of 50257 take 143 us (823 MB, 5.8 TB/s).
+// Bound by the memory: 4096 bf16 rows of 50257 take 134 us (823 MB, 6.1 TB/s).
 template <class T, bool PAST>
 __global__ __launch_bounds__(256) void log_prob_grad(LogProbGradArgs a) {
   constexpr int N = Piece<T>::N, AHEAD = 4, THREADS = 256;

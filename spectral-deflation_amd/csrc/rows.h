@@ -151,8 +151,14 @@ struct Row {
 };
 
 // Logits of much more than the last-level cache's 256 MB are read, and their gradient written, as
-// what no cache need keep: 8192 bf16 rows of 50257 with their gradient by distillation in 305 instead
-// of 321 us, in place 283 instead of 332.  (In 103 MB that a cache still holds, 48 instead of 43.)
+// what no cache need keep.  Bf16 rows of 50257, a distilled step with the rest, us a pass through the
+// caches and by them, logits from memory:
+//   rows                      2000 (191 MiB)  3000       3800 (364 MiB)  4300       8192
+//   step                      91, 87          128, 123   158, 151        176, 169   322, 307
+//   ... in place              77, 76          140, 111   178, 141        201, 161   390, 304
+//   loss alone                47, 48          66, 66     80, 81          91, 91     164, 165
+// Below the switch it is the caches that may still hold the logits: 46 instead of 48 us for a step of
+// 1024 rows that they hold, 43 instead of 46 for the losses of 2000.
 template <class T>
 inline bool past_caches(long long rows, long long classes) {
   return rows * classes * (long long)sizeof(T) >= 384LL << 20;
