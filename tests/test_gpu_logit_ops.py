@@ -1080,3 +1080,92 @@ def test_distillation_past_the_caches(T, n, v, dtype, rest):
     close(dz[at], *c.grad_bound(1.0 / count, dtype))
     dz = T.distillation_step(z, ig, tg, reduction="sum", inplace=True, **kw)[1]
     close(dz[at], *c.grad_bound(1.0, dtype))
+
+
+def test_two_graphs_of_one_memory_pool(T):
+    """Rows counted by a launch of their own, in place and through autograd, in two graphs that
+    share their memory and are replayed in turn with eager work between."""
+    n, v, k = 700, 4099, 12
+    cases = []
+    for seed in (0, 1):
+        z, ids, t = kd_case(n, v, k, BF16, seed=seed)
+        cases.append([x.to(DEV) for x in (z, ids, t)])
+
+    def step(z, ids, t):
+        top = T.token_log_probs(z, top=5)
+        leaf = z.detach().requires_grad_()
+        loss = T.distillation(leaf, ids, t, rest=True)
+        (g,) = torch.autograd.grad(loss, leaf)
+        work = z.clone()
+        mean, dz = T.distillation_step(work, ids, t, inplace=True)
+        return (*top[1:], loss.detach(), g, mean, dz)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*cases[0])
+    torch.cuda.current_stream().wait_stream(side)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    outs = []
+    for graph in (first, second):
+        with torch.cuda.graph(graph, pool=first.pool() if graph is second else None):
+            outs.append(step(*cases[len(outs)]))
+    for turn in range(4):
+        for i, graph in enumerate((first, second)):
+            z, ids, t = kd_case(n, v, k, BF16, seed=10 + 2 * turn + i)
+            for a, b in zip(cases[i], (z, ids, t)):
+                a.copy_(b)
+            want = step(*cases[i])
+            torch.cuda.synchronize()
+            graph.replay()
+            got = [x.clone() for x in outs[i]]
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), (turn, i)
+
+
+def test_calls_on_two_streams_at_once(T):
+    """From two threads with a stream each."""
+    import threading
+    data, want, got = [], [], [None, None]
+    for seed in (0, 1):
+        z, ids, t = kd_case(900, 9003, 20, BF16, seed=seed)
+        data.append([x.to(DEV) for x in (z, ids, t)])
+
+    def calls(z, ids, t):
+        out = []
+        for _ in range(10):
+            out = [*T.token_log_probs(z, ids[:, 2].clamp(min=0), top=20),
+                   *T.distillation_step(z, ids, t, rest=True)]
+            leaf = z.detach().requires_grad_()
+            out.append(torch.autograd.grad(T.distillation(leaf, ids, t), leaf)[0])
+        return out
+    for d in data:
+        want.append(calls(*d))
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = calls(*data[i])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_a_repeated_forward_pass(T):
+    """Activation checkpointing runs the calls again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    h, w = normal(30, 16, seed=1).to(DEV).requires_grad_(), normal(16, 600, seed=2).to(DEV)
+    _, ids, t = kd_case(30, 600, 8)
+    y, ids, t = ids[:, 1].clamp(min=0).to(DEV), ids.to(DEV), t.to(DEV)
+
+    def f(h):
+        out = T.token_log_probs(h @ w, y, top=4)
+        return (out.log_probs.sum() + out.entropy.sum() + out.top_log_probs.sum()
+                + T.distillation(h @ w, ids, t, rest=True))
+    want = torch.autograd.grad(f(h), h)[0]
+    assert torch.equal(torch.autograd.grad(checkpoint(f, h, use_reentrant=False), h)[0], want)
